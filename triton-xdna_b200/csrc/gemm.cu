@@ -3490,6 +3490,10 @@ extern "C" int xb_matmul_sharded(const void* A, const void* B_shard, void* const
                                                                        err, errlen, 1, 0, &pa);
 }
 
+namespace xb {
+cudaError_t paged_status_take(int* status, cudaStream_t s);  // csrc/paged.cu
+}
+
 extern "C" int xb_device_status(void* stream, int* status, char* err, size_t errlen) {
   if (!status) {
     set_err(err, errlen, "xb_device_status: null output");
@@ -3501,6 +3505,9 @@ extern "C" int xb_device_status(void* stream, int* status, char* err, size_t err
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_gemm_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  int paged = 0;
+  if (e == cudaSuccess) e = xb::paged_status_take(&paged, s);
+  if (e == cudaSuccess && *status == 0) *status = paged;
   if (e != cudaSuccess) {
     set_err(err, errlen, "xb_device_status: %s", cudaGetErrorString(e));
     return XB_ERR_CUDA;

@@ -1,0 +1,1072 @@
+// Operators of a paged KV cache: RoPE of packed new tokens with the write of
+// their keys and values into pages, causal grouped-query attention of those
+// tokens over the pages, and page copies inside the pool.
+//
+// The contiguous counterparts are xb_rope_kv_bf16 and xb_attention_bf16
+// (csrc/llm.cu; examples/qwen2_5/model.py:851-889 and kernels/attention.py:
+// 27-122).  There every sequence of a batch has the same length; here a step
+// packs the new tokens of many sequences without padding:
+//
+//   q_start [B + 1]  tokens q_start[b] .. q_start[b + 1] - 1 belong to sequence b
+//   kv_len  [B]      positions sequence b holds, its new tokens included
+//   table   [B, max_pages]  the pages of each sequence, in order
+//   pages   [n_pages, KVH, page, D] bf16, any strides with unit last one
+//
+// All three live on the device and are read by the kernels, so a captured
+// graph serves every step of the same batch size.  Token i (0-based) of the
+// n_b = q_start[b + 1] - q_start[b] new ones sits at position
+// kv_len[b] - n_b + i and sees the keys 0 .. that position.
+//
+// Nothing the device holds can make a kernel leave its buffers: token ranges
+// are clamped to the rows given, lengths to what the table can hold, and a
+// page id outside the pool reads as zeros (attention) or is skipped (writes)
+// and sets the flag that xb_page_status reports.
+#include "common.cuh"
+#include "tc.cuh"
+
+namespace xb {
+namespace paged {
+
+using namespace tc;
+typedef __nv_bfloat16 bf16;
+
+__device__ int g_bad_page = 0;      // a page id outside the pool, or a position without a page
+__device__ int g_paged_status = 0;  // XB_ERR_TIMEOUT once a bounded wait ran out (xb_device_status)
+constexpr uint64_t kWaitLimit = 2000000000ull;  // 2 s per wait: far above any legitimate wait
+
+// ----------------------------------------------------------------------------- page copies
+
+// pages[o, dst[i]] = pages[o, src[i]] for every outer index o (layer, K or V):
+// a plain copy, 2 bytes moved per byte of page, HBM-bound.  The host has
+// checked that no destination is a source or named twice, so the pairs may
+// run in any order.  The pairs travel as kernel parameters: no upload, no
+// device buffer whose lifetime a captured graph would have to share.  A thread
+// moves four 16-byte vectors 256 apart (four loads in flight), a CTA 16 KB of
+// the outer slab's n * vpp vectors.
+constexpr int kCopyPairs = 500;  // 4000 bytes of parameters; larger lists take several launches
+template <int N>
+struct CopyPairs {
+  int32_t src[N], dst[N];
+};
+
+template <int N>
+__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyPairs<N> pairs, uint8_t* base,
+                                                         int64_t outer_stride, int64_t page_stride, uint32_t vpp,
+                                                         uint32_t total) {
+  pdl_wait();
+  pdl_trigger();
+  uint8_t* slab = base + (int64_t)blockIdx.y * outer_stride;
+  const uint32_t first = blockIdx.x * 1024u + threadIdx.x;
+  int4 v[4];
+  int64_t to[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint32_t i = first + u * 256u;
+    to[u] = -1;
+    if (i < total) {
+      const uint32_t p = i / vpp, at = i - p * vpp;
+      to[u] = (int64_t)pairs.dst[p] * page_stride + (int64_t)at * 16;
+      v[u] = __ldcs(reinterpret_cast<const int4*>(slab + (int64_t)pairs.src[p] * page_stride + (int64_t)at * 16));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (to[u] >= 0) *reinterpret_cast<int4*>(slab + to[u]) = v[u];
+}
+
+// ----------------------------------------------------------------------------- RoPE + page write
+
+struct Pages {  // K or V pages: element strides of page, head and row; rows of D contiguous elements
+  bf16* p;
+  int64_t page, head, row;
+};
+
+struct RopeArgs {
+  const bf16* qkv;
+  const float *cos_t, *sin_t;
+  bf16* q;
+  Pages k, v;
+  const int32_t *table, *q_start, *kv_len;
+  int64_t ld_qkv, ld_q, ld_table, rope_rows;
+  int T, B, H, KVH, D, page_size, max_pages, n_pages;
+};
+
+// One warp per packed token.  A lane keeps one group of 8 dims (and the 8 of
+// the other half they rotate with) and walks the head slots, so it reads its
+// 32 table values once; 16-byte loads and stores.  Products and sums are
+// rounded separately in fp32, as examples/qwen2_5/kernels/rope.py:63-66 and
+// the contiguous kernel do: the same bits.
+__global__ void __launch_bounds__(256) paged_rope_kv_kernel(const RopeArgs a, int* __restrict__ bad) {
+  pdl_wait();
+  pdl_trigger();
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (t >= a.T) return;
+  // the last b with q_start[b] <= t; empty sequences share their start with the next one
+  int lo = 0, hi = a.B + 1;  // q_start[lo - 1] <= t < q_start[hi]
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(a.q_start + mid) <= t) lo = mid + 1;
+    else hi = mid;
+  }
+  const int b = lo - 1;
+  if (b < 0 || b >= a.B) return;  // a row before the first or behind the last sequence
+  const int64_t pos = (int64_t)__ldg(a.kv_len + b) - ((int64_t)__ldg(a.q_start + b + 1) - t);
+  const int64_t slot_page = pos >= 0 ? pos / a.page_size : -1;
+  int id = -1;
+  if (pos >= 0 && slot_page < a.max_pages) id = __ldg(a.table + (int64_t)b * a.ld_table + slot_page);
+  const bool page_ok = id >= 0 && id < a.n_pages;
+  if (!page_ok && lane == 0) atomicExch(bad, 1);
+  if (pos < 0) return;
+  const bool rotate = a.cos_t != nullptr;
+  if (rotate && pos >= a.rope_rows) {
+    if (lane == 0) atomicExch(bad, 1);
+    return;
+  }
+  const int row = (int)(pos - slot_page * a.page_size);
+  const int half = a.D / 2, groups = half / 8;  // groups of 8 dims of a half; divides 32
+  const int c = (lane % groups) * 8;
+  float cl[8], ch[8], sl[8], sh[8];
+  if (rotate) {
+    const float* cr = a.cos_t + pos * a.D;
+    const float* sr = a.sin_t + pos * a.D;
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      *reinterpret_cast<float4*>(&cl[e]) = __ldg(reinterpret_cast<const float4*>(cr + c + e));
+      *reinterpret_cast<float4*>(&ch[e]) = __ldg(reinterpret_cast<const float4*>(cr + c + half + e));
+      *reinterpret_cast<float4*>(&sl[e]) = __ldg(reinterpret_cast<const float4*>(sr + c + e));
+      *reinterpret_cast<float4*>(&sh[e]) = __ldg(reinterpret_cast<const float4*>(sr + c + half + e));
+    }
+  }
+  const bf16* x = a.qkv + (int64_t)t * a.ld_qkv;
+  const int slots = a.H + 2 * a.KVH;
+  for (int slot = lane / groups; slot < slots; slot += 32 / groups) {
+    Vec16<bf16> u = ld16_stream(x + slot * a.D + c), w = ld16_stream(x + slot * a.D + half + c);
+    if (rotate && slot < a.H + a.KVH) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x0 = __bfloat162float(u.v[e]), x1 = __bfloat162float(w.v[e]);
+        u.v[e] = __float2bfloat16_rn(__fadd_rn(__fmul_rn(x0, cl[e]), __fmul_rn(-x1, sl[e])));
+        w.v[e] = __float2bfloat16_rn(__fadd_rn(__fmul_rn(x1, ch[e]), __fmul_rn(x0, sh[e])));
+      }
+    }
+    bf16* dst;
+    if (slot < a.H) {
+      dst = a.q + (int64_t)t * a.ld_q + slot * a.D;
+    } else {
+      if (!page_ok) continue;
+      const bool is_k = slot < a.H + a.KVH;
+      const Pages& pg = is_k ? a.k : a.v;
+      dst = pg.p + id * pg.page + (slot - a.H - (is_k ? 0 : a.KVH)) * pg.head + row * pg.row;
+    }
+    st16(dst + c, u);
+    st16(dst + half + c, w);
+  }
+}
+
+// ----------------------------------------------------------------------------- attention: the work and its split
+//
+// A unit of work is one (sequence, KV head, query tile): `tpt` consecutive
+// new tokens of a sequence times the n_rep query heads that share the KV head,
+// which are the rows of one matrix tile, so every key and value is read once
+// for all of them.  Query tile j of a sequence with `base` earlier positions
+// sees base + min(tpt (j + 1), n) keys.  All units laid end to end, weighted
+// by those keys, make one line of `total` keys; CTA c takes the piece
+// [c share, (c + 1) share) of it, whatever unit boundaries lie inside, so the
+// CTAs finish together however uneven the batch is.  A unit that one CTA
+// covers alone is written at once; one that spans several leaves a partial
+// (O, max, sum) per CTA in the workspace, and a second small kernel joins
+// them in CTA order (fixed order: repeatable bits).  The weights are a closed
+// form, so a CTA finds its piece with one scan over the sequences and a binary
+// search inside one, from lengths that only the device knows.
+
+struct AttnArgs {
+  const bf16* q;
+  bf16* out;
+  const int32_t *table, *q_start, *kv_len;
+  float* ws;  // [2 G] partials, then G Meta
+  int64_t ld_q, ld_out, ld_table;
+  int T, B, KVH, n_rep, tpt, page_size, max_pages, n_pages, box_rows;
+  int min_share;
+  float scale_log2;
+  int *bad, *status;
+};
+
+// What the joining kernel needs of CTA c: the unit that starts in c and goes on, and the CTA it ends in.
+struct Meta {
+  int last, token, rows, kvh;  // last < 0: no such unit
+};
+
+struct Seq {
+  int s0, n;          // first packed token, number of new tokens
+  int64_t len, base;  // keys held, keys before the new tokens (negative: the first tokens see none)
+  int nt;             // query tiles
+  int64_t perh;       // weight of one KV head
+};
+
+__device__ __forceinline__ int64_t cum_keys(const Seq& q, int tpt, int64_t j) {  // weight of query tiles 0 .. j - 1
+  const int64_t b = q.base > 0 ? q.base : 0;
+  return j * b + (j < q.nt ? tpt * j * (j + 1) / 2 : tpt * (int64_t)q.nt * (q.nt - 1) / 2 + q.n);
+}
+
+__device__ __forceinline__ Seq load_seq(const AttnArgs& a, int b) {
+  Seq q;
+  const int s0 = min(max(__ldg(a.q_start + b), 0), a.T);
+  const int s1 = min(max(__ldg(a.q_start + b + 1), s0), a.T);
+  q.s0 = s0;
+  q.n = s1 - s0;
+  const int64_t cap = (int64_t)a.max_pages * a.page_size;
+  const int64_t len = max(__ldg(a.kv_len + b), 0);
+  q.len = len < cap ? len : cap;
+  q.base = q.len - q.n;
+  q.nt = (q.n + a.tpt - 1) / a.tpt;
+  q.perh = cum_keys(q, a.tpt, q.nt);
+  return q;
+}
+
+// One CTA's walk over its piece of the line.
+struct Walk {
+  int64_t lo, hi;  // the CTA's piece
+  int64_t share;
+  int64_t u0;      // where the current unit starts
+  int b, kvh, j;
+  Seq q;
+};
+
+struct Segment {
+  int token, rows;     // first packed token and rows of the query tile
+  int kvh, b;
+  int64_t first_pos;   // position of the tile's first token
+  int64_t keys;        // keys the unit's last token sees (> 0 unless its rows are all empty)
+  int t0, t1;          // key tiles [t0, t1) of this CTA's part
+  bool starts, ends;   // the unit starts / ends in this CTA
+  int64_t u0, ulen;
+};
+
+// Every thread of the block calls this; `found` is shared.  False: no work for this CTA.
+template <int THREADS>
+__device__ __forceinline__ bool find_piece(const AttnArgs& a, Walk& w, int64_t (*warp_sum)[THREADS / 32],
+                                           int64_t* found, int ctas, int cta) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t total = 0;
+  // pass 0: the whole line's weight; pass 1: the sequence that holds `lo`
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t run = 0;
+    for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+      const int b = b0 + threadIdx.x;
+      const int64_t c = b < a.B ? load_seq(a, b).perh * a.KVH : 0;
+      int64_t s = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += v;
+      }
+      const int buf = (b0 / THREADS) & 1;
+      if (lane == 31) warp_sum[buf][warp] = s;
+      __syncthreads();
+      int64_t before = run, all = run;
+#pragma unroll
+      for (int i = 0; i < THREADS / 32; ++i) {
+        const int64_t v = warp_sum[buf][i];
+        if (i < warp) before += v;
+        all += v;
+      }
+      if (pass == 1) {
+        const int64_t excl = before + s - c;
+        if (c > 0 && excl <= w.lo && w.lo < excl + c) {
+          found[0] = b;
+          found[1] = excl;
+        }
+      }
+      run = all;
+    }
+    __syncthreads();
+    if (pass == 0) {
+      total = run;
+      w.share = (total + ctas - 1) / ctas;
+      if (w.share < a.min_share) w.share = a.min_share;
+      w.lo = (int64_t)cta * w.share;
+      w.hi = w.lo + w.share < total ? w.lo + w.share : total;
+      if (w.lo >= total) return false;  // the same for every thread of the CTA
+    }
+  }
+  w.b = (int)found[0];
+  w.q = load_seq(a, w.b);
+  const int64_t off = w.lo - found[1];
+  w.kvh = (int)(off / w.q.perh);
+  const int64_t in = off - w.kvh * w.q.perh;
+  int lo = 0, hi = w.q.nt - 1;  // the last tile j with cum(j) <= in
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cum_keys(w.q, a.tpt, mid) <= in) lo = mid;
+    else hi = mid - 1;
+  }
+  w.j = lo;
+  w.u0 = found[1] + w.kvh * w.q.perh + cum_keys(w.q, a.tpt, lo);
+  return true;
+}
+
+template <int TK>
+__device__ __forceinline__ Segment segment(const AttnArgs& a, const Walk& w) {
+  Segment g;
+  const int done = w.j * a.tpt;
+  const int tokens = min(a.tpt, w.q.n - done);
+  g.token = w.q.s0 + done;
+  g.rows = tokens * a.n_rep;
+  g.kvh = w.kvh;
+  g.b = w.b;
+  g.first_pos = w.q.base + done;
+  g.keys = g.first_pos + tokens;
+  if (g.keys < 0) g.keys = 0;
+  const int64_t b0 = w.q.base > 0 ? w.q.base : 0;
+  g.u0 = w.u0;
+  g.ulen = b0 + done + tokens;
+  const int64_t s = w.lo > w.u0 ? w.lo - w.u0 : 0;
+  const int64_t e = w.hi < w.u0 + g.ulen ? w.hi - w.u0 : g.ulen;
+  g.starts = w.lo <= w.u0;
+  g.ends = w.hi >= w.u0 + g.ulen;
+  const int nk = (int)((g.keys + TK - 1) / TK);
+  g.t0 = min((int)(s / TK), nk);  // cuts fall on tile boundaries, the same ones on both sides
+  g.t1 = g.ends ? nk : min((int)(e / TK), nk);
+  return g;
+}
+
+// Steps to the next unit of the CTA's piece; false at its end.
+__device__ __forceinline__ bool next_unit(const AttnArgs& a, Walk& w, const Segment& g) {
+  w.u0 = g.u0 + g.ulen;
+  if (w.u0 >= w.hi) return false;
+  if (++w.j < w.q.nt) return true;
+  w.j = 0;
+  if (++w.kvh < a.KVH) return true;
+  w.kvh = 0;
+  do {
+    if (++w.b >= a.B) return false;
+    w.q = load_seq(a, w.b);
+  } while (w.q.n == 0);
+  return true;
+}
+
+// ----------------------------------------------------------------------------- attention: few rows (mma.sync)
+//
+// For batches whose sequences bring few tokens each (decoding, verification
+// of drafted tokens): at most 16 rows per unit, the rows of an mma.sync
+// m16n8k16 tile (rows past n_rep * tokens are zero), so the kernel is bound by
+// reading K and V.  Each of the CTA's warps takes every kWarps-th 32-key tile
+// of the segment and is on its own: lanes issue the TMA loads of their tile's
+// page rows (128-byte swizzle) into one of the warp's three buffers, the warp
+// waits on that buffer's mbarrier, and keeps an online softmax (running max
+// and sum in fp32, P rounded to bf16 for P V as in the contiguous kernels).
+// 8 warps x 3 buffers x 8 KB keep up to 192 KB per SM in flight.  The warps'
+// (O, max, sum) meet in shared memory in warp order.
+constexpr int kHD = 64;
+constexpr int kWarps = 8, kBufs = 3, kTK = 32;
+constexpr int kTileBytes = kTK * kHD * 2;               // one K or V tile
+constexpr int kRingBytes = kWarps * kBufs * 2 * kTileBytes;
+constexpr int kMergeBytes = kWarps * 16 * kHD * 4;
+constexpr int kFewSmem = kRingBytes + kMergeBytes + 1024;
+constexpr int kFewRows = 16;
+
+struct alignas(64) KvMaps {
+  CUtensorMap k, v;  // [n_pages][KVH][page][64], box {64, box_rows, 1, 1}
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t c0,
+                                            int32_t c1, int32_t c2, int32_t c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// floats of one partial: O [rows][64], then max [rows], then sum [rows]
+__host__ __device__ constexpr int64_t part_floats(int rows) { return (int64_t)rows * (kHD + 2); }
+
+__global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __grid_constant__ KvMaps maps,
+                                                                        const AttnArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full[kWarps][kBufs];
+  __shared__ int64_t warp_sum[2][kWarps];
+  __shared__ int64_t found[2];
+  __shared__ float wm[kWarps][16], wl[kWarps][16];
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t base_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t ring = base_u32 + warp * (kBufs * 2 * kTileBytes);
+  float* red = reinterpret_cast<float*>(smem_raw + (base_u32 - smem_u32(smem_raw)) + kRingBytes);
+  if (lane == 0)
+    for (int i = 0; i < kBufs; ++i) mbar_init(&full[warp][i], 1);
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    prefetch_tmap(&maps.k);
+    prefetch_tmap(&maps.v);
+  }
+  mbar_fence_init();
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+
+  Meta* meta = reinterpret_cast<Meta*>(a.ws + 2 * (int64_t)gridDim.x * part_floats(kFewRows));
+  Walk w;
+  if (!find_piece<kWarps * 32>(a, w, warp_sum, found, gridDim.x, blockIdx.x)) {
+    if (threadIdx.x == 0) meta[blockIdx.x].last = -1;
+    return;
+  }
+  bool open_unit = false;
+  // tiles this warp has read / requested so far: buffer n % kBufs, parity (n / kBufs) & 1
+  uint32_t use = 0, issued = 0;
+  bool dead = false;  // a wait ran out: no more loads, the output is not valid
+  for (bool more = true; more;) {
+    const Segment s = segment<kTK>(a, w);
+    const int boxes = kTK / a.box_rows;
+    // lane 0 .. boxes - 1 load K rows, the next `boxes` lanes V rows of tile `tile` into buffer `buf`
+    auto issue = [&](int tile, uint32_t n) {
+      const uint32_t buf = n % kBufs;
+      const int64_t k0 = (int64_t)tile * kTK;
+      const int have = (int)min((int64_t)kTK, s.keys - k0);
+      const int nb = (have + a.box_rows - 1) / a.box_rows;
+      if (lane == 0) mbar_arrive_expect_tx(&full[warp][buf], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
+      __syncwarp();
+      const int box = lane < boxes ? lane : lane - boxes;
+      if (lane < 2 * boxes && box < nb) {
+        const uint32_t key = (uint32_t)(k0 + box * a.box_rows);
+        const uint32_t pi = key / (uint32_t)a.page_size;
+        int id = __ldg(a.table + s.b * a.ld_table + pi);
+        if (id < 0 || id >= a.n_pages) {  // reads as zeros: a coordinate past the pool
+          atomicExch(a.bad, 1);
+          id = a.n_pages;
+        }
+        const bool is_v = lane >= boxes;
+        tma_load_4d(ring + buf * 2 * kTileBytes + (is_v ? kTileBytes : 0) + box * a.box_rows * kHD * 2,
+                    is_v ? &maps.v : &maps.k, &full[warp][buf], 0, (int)(key - pi * a.page_size), s.kvh, id);
+      }
+    };
+    issued = use;
+    int next = dead ? s.t1 : s.t0 + warp;  // next tile to issue
+    for (; next < s.t1 && issued < use + kBufs; next += kWarps) issue(next, issued++);
+
+    uint32_t qa[4][4];
+    {
+      const int r0 = g, r1 = g + 8;
+      const bool ok0 = r0 < s.rows, ok1 = r1 < s.rows;
+      const bf16* p0 = a.q + (int64_t)(s.token + r0 / a.n_rep) * a.ld_q + (s.kvh * a.n_rep + r0 % a.n_rep) * kHD;
+      const bf16* p1 = a.q + (int64_t)(s.token + r1 / a.n_rep) * a.ld_q + (s.kvh * a.n_rep + r1 % a.n_rep) * kHD;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        const int c = kk * 16 + 2 * t;
+        qa[kk][0] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c) : 0u;
+        qa[kk][1] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c) : 0u;
+        qa[kk][2] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c + 8) : 0u;
+        qa[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c + 8) : 0u;
+      }
+    }
+    const int64_t pos0 = s.first_pos + g / a.n_rep, pos1 = s.first_pos + (g + 8) / a.n_rep;
+    float o[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    for (int tile = s.t0 + warp; tile < s.t1 && !dead; tile += kWarps) {
+      const uint32_t buf = use % kBufs;
+      const bool landed = mbar_wait(&full[warp][buf], (use / kBufs) & 1, kWaitLimit, &abort_flag);
+      if (__any_sync(0xffffffffu, !landed)) {
+        atomicExch(a.status, XB_ERR_TIMEOUT);
+        abort_flag = 1;
+        dead = true;
+        break;
+      }
+      const int64_t k0 = (int64_t)tile * kTK;
+      const uint32_t sk = ring + buf * 2 * kTileBytes, sv = sk + kTileBytes;
+      const int have = (int)min((int64_t)kTK, s.keys - k0);
+      if (have < kTK) {
+        // values behind the last key hold whatever the page or buffer held: a
+        // NaN there would survive its zero weight
+        for (int i = have * 8 + lane; i < kTK * 8; i += 32)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + i * 16), "r"(0) : "memory");
+        __syncwarp();
+      }
+      float sc[4][4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // dims 32 h .. 32 h + 31: four 16-byte chunks of the key rows
+          const int r = nt * 8 + (lane & 7), c = 4 * h + (lane >> 3);
+          uint32_t kb[4];
+          ldsm4(kb, sk + r * 128 + ((c ^ (r & 7)) << 4));
+          mma_16816(sc[nt], qa[2 * h], kb[0], kb[1]);
+          mma_16816(sc[nt], qa[2 * h + 1], kb[2], kb[3]);
+        }
+      }
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t key = k0 + nt * 8 + 2 * t + (e & 1);
+          sc[nt][e] = key <= (e < 2 ? pos0 : pos1) && key < s.keys ? sc[nt][e] * a.scale_log2 : -INFINITY;
+          if (e < 2) mx0 = fmaxf(mx0, sc[nt][e]);
+          else mx1 = fmaxf(mx1, sc[nt][e]);
+        }
+#pragma unroll
+      for (int o_ = 1; o_ <= 2; o_ <<= 1) {
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o_));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o_));
+      }
+      const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
+      const float base0 = mn0 == -INFINITY ? 0.0f : mn0, base1 = mn1 == -INFINITY ? 0.0f : mn1;
+      const float al0 = ex2_approx(m0 - base0), al1 = ex2_approx(m1 - base1);
+      m0 = mn0;
+      m1 = mn1;
+      float rs0 = 0.0f, rs1 = 0.0f;
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        sc[nt][0] = ex2_approx(sc[nt][0] - base0);
+        sc[nt][1] = ex2_approx(sc[nt][1] - base0);
+        sc[nt][2] = ex2_approx(sc[nt][2] - base1);
+        sc[nt][3] = ex2_approx(sc[nt][3] - base1);
+        rs0 += sc[nt][0] + sc[nt][1];
+        rs1 += sc[nt][2] + sc[nt][3];
+      }
+      l0 = l0 * al0 + rs0;
+      l1 = l1 * al1 + rs1;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) {
+        o[dt][0] *= al0;
+        o[dt][1] *= al0;
+        o[dt][2] *= al1;
+        o[dt][3] *= al1;
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        uint32_t pa[4];
+        pa[0] = pack2(sc[2 * kk][0], sc[2 * kk][1]);
+        pa[1] = pack2(sc[2 * kk][2], sc[2 * kk][3]);
+        pa[2] = pack2(sc[2 * kk + 1][0], sc[2 * kk + 1][1]);
+        pa[3] = pack2(sc[2 * kk + 1][2], sc[2 * kk + 1][3]);
+#pragma unroll
+        for (int dt = 0; dt < 8; dt += 2) {
+          const int mi = lane >> 3, r = kk * 16 + (mi & 1) * 8 + (lane & 7), c = dt + (mi >> 1);
+          uint32_t vb[4];
+          ldsm4_t(vb, sv + r * 128 + ((c ^ (r & 7)) << 4));
+          mma_16816(o[dt], pa, vb[0], vb[1]);
+          mma_16816(o[dt + 1], pa, vb[2], vb[3]);
+        }
+      }
+      ++use;
+      __syncwarp();  // the buffer is read: it takes the warp's tile kBufs steps ahead
+      if (have < kTK) {  // the unit's last tile
+        fence_proxy_async_smem();  // the zeros, before a later unit's TMA write to the buffer
+      } else if (next < s.t1) {
+        issue(next, issued++);
+        next += kWarps;
+      }
+    }
+#pragma unroll
+    for (int o_ = 1; o_ <= 2; o_ <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, o_);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, o_);
+    }
+    __syncthreads();  // the previous segment's merge has been read
+    if (t == 0) {
+      wm[warp][g] = m0;
+      wm[warp][g + 8] = m1;
+      wl[warp][g] = l0;
+      wl[warp][g + 8] = l1;
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {
+      const int d = dt * 8 + 2 * t;
+      *reinterpret_cast<float2*>(&red[(warp * 16 + g) * kHD + d]) = make_float2(o[dt][0], o[dt][1]);
+      *reinterpret_cast<float2*>(&red[(warp * 16 + g + 8) * kHD + d]) = make_float2(o[dt][2], o[dt][3]);
+    }
+    __syncthreads();
+    const bool whole = s.starts && s.ends;
+    float* part = a.ws + (2 * (int64_t)blockIdx.x + (s.starts ? 1 : 0)) * part_floats(kFewRows);
+    for (int i = threadIdx.x; i < s.rows * (kHD / 4); i += kWarps * 32) {
+      const int r = i / (kHD / 4), d = (i % (kHD / 4)) * 4;
+      float M = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) M = fmaxf(M, wm[k][r]);
+      const float base = M == -INFINITY ? 0.0f : M;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float f = ex2_approx(wm[k][r] - base);
+        const float4 v = *reinterpret_cast<const float4*>(&red[(k * 16 + r) * kHD + d]);
+        acc.x += v.x * f;
+        acc.y += v.y * f;
+        acc.z += v.z * f;
+        acc.w += v.w * f;
+        l += wl[k][r] * f;
+      }
+      if (whole) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+        bf16* op = a.out + (int64_t)(s.token + r / a.n_rep) * a.ld_out + (s.kvh * a.n_rep + r % a.n_rep) * kHD + d;
+        uint2 pk;
+        pk.x = pack2(acc.x * inv, acc.y * inv);
+        pk.y = pack2(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2*>(op) = pk;
+      } else {
+        *reinterpret_cast<float4*>(part + r * kHD + d) = acc;
+        if (d == 0) {
+          part[kFewRows * kHD + r] = M;
+          part[kFewRows * kHD + kFewRows + r] = l;
+        }
+      }
+    }
+    if (s.starts && !s.ends) {
+      open_unit = true;
+      if (threadIdx.x == 0)
+        meta[blockIdx.x] = Meta{(int)((s.u0 + s.ulen - 1) / w.share), s.token, s.rows, s.kvh};
+    }
+    more = next_unit(a, w, s);
+  }
+  if (!open_unit && threadIdx.x == 0) meta[blockIdx.x].last = -1;
+  if (dead) {  // loads still in flight land before the CTA's shared memory is given up
+    uint64_t deadline = 0;
+    for (; use < issued; ++use)
+      mbar_wait_deadline(&full[warp][use % kBufs], (use / kBufs) & 1, &deadline, kWaitLimit);
+  }
+}
+
+// Joins the partials of the unit that starts in CTA blockIdx.x and goes on in
+// the next ones: o = sum_c o_c 2^(m_c - M), l likewise, in CTA order.
+template <int ROWS>
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, int ctas) {
+  pdl_wait();
+  pdl_trigger();
+  const Meta m = reinterpret_cast<const Meta*>(a.ws + 2 * (int64_t)ctas * part_floats(ROWS))[blockIdx.x];
+  if (m.last < 0) return;
+  for (int i = threadIdx.x; i < m.rows * (kHD / 4); i += 256) {
+    const int r = i / (kHD / 4), d = (i % (kHD / 4)) * 4;
+    float M = -INFINITY;
+    for (int c = blockIdx.x; c <= m.last; ++c) {
+      const float* p = a.ws + (2 * (int64_t)c + (c == blockIdx.x)) * part_floats(ROWS);
+      M = fmaxf(M, p[ROWS * kHD + r]);
+    }
+    const float base = M == -INFINITY ? 0.0f : M;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.0f;
+    for (int c = blockIdx.x; c <= m.last; ++c) {
+      const float* p = a.ws + (2 * (int64_t)c + (c == blockIdx.x)) * part_floats(ROWS);
+      const float f = ex2_approx(p[ROWS * kHD + r] - base);
+      const float4 v = *reinterpret_cast<const float4*>(p + r * kHD + d);
+      acc.x += v.x * f;
+      acc.y += v.y * f;
+      acc.z += v.z * f;
+      acc.w += v.w * f;
+      l += p[ROWS * kHD + ROWS + r] * f;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    bf16* op = a.out + (int64_t)(m.token + r / a.n_rep) * a.ld_out + (m.kvh * a.n_rep + r % a.n_rep) * kHD + d;
+    uint2 pk;
+    pk.x = pack2(acc.x * inv, acc.y * inv);
+    pk.y = pack2(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(op) = pk;
+  }
+}
+
+// ----------------------------------------------------------------------------- host side
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encoder() {
+  static std::atomic<EncodeTiledFn> fn{nullptr};
+  EncodeTiledFn f = fn.load(std::memory_order_acquire);
+  if (f) return f;
+  void* p = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
+  if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !p) return nullptr;
+  f = reinterpret_cast<EncodeTiledFn>(p);
+  fn.store(f, std::memory_order_release);
+  return f;
+}
+
+int page_map(CUtensorMap* map, const void* p, int64_t n_pages, int64_t heads, int64_t page_size, int64_t page_ld,
+             int64_t head_ld, int64_t row_ld, int box_rows, const char* what, char* err, size_t errlen) {
+  EncodeTiledFn enc = encoder();
+  if (!enc) {
+    set_err(err, errlen, "%s: cuTensorMapEncodeTiled unavailable", what);
+    return XB_ERR_CUDA;
+  }
+  cuuint64_t dims[4] = {(cuuint64_t)kHD, (cuuint64_t)page_size, (cuuint64_t)heads, (cuuint64_t)n_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)row_ld * 2, (cuuint64_t)head_ld * 2, (cuuint64_t)page_ld * 2};
+  cuuint32_t box[4] = {(cuuint32_t)kHD, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_err(err, errlen, "%s: cuTensorMapEncodeTiled failed (%d) for pages [%lld][%lld][%lld][64]", what, (int)r,
+            (long long)n_pages, (long long)heads, (long long)page_size);
+    return XB_ERR_CUDA;
+  }
+  return XB_OK;
+}
+
+// Addresses of the two status words on the current device.
+int status_words(int** bad, int** status, const char* what, char* err, size_t errlen) {
+  if (cudaGetSymbolAddress((void**)bad, g_bad_page) != cudaSuccess ||
+      cudaGetSymbolAddress((void**)status, g_paged_status) != cudaSuccess) {
+    set_err(err, errlen, "%s: status words unavailable: %s", what, cudaGetErrorString(cudaGetLastError()));
+    return XB_ERR_CUDA;
+  }
+  return XB_OK;
+}
+
+// What every page operand has to satisfy, device contents aside.
+int check_pages(int64_t n_pages, int64_t page_size, int64_t kv_heads, int64_t batch, int64_t max_pages,
+                int64_t table_ld, int64_t k_page, int64_t k_head, int64_t k_row, int64_t v_page, int64_t v_head,
+                int64_t v_row, const char* what, char* err, size_t errlen) {
+  if (n_pages <= 0 || page_size <= 0 || kv_heads <= 0 || batch < 0 || max_pages <= 0 || table_ld < max_pages) {
+    set_err(err, errlen, "%s: bad shape", what);
+    return XB_ERR_INVALID;
+  }
+  if (page_size % 8) {
+    set_err(err, errlen, "%s: page_size %lld is not a multiple of 8", what, (long long)page_size);
+    return XB_ERR_UNSUPPORTED;
+  }
+  const int64_t lds[6] = {k_page, k_head, k_row, v_page, v_head, v_row};
+  for (int64_t ld : lds)
+    if (ld <= 0 || ld % 8 || ld >= (1LL << 38)) {
+      set_err(err, errlen, "%s: page strides must be positive multiples of 8 elements", what);
+      return XB_ERR_UNSUPPORTED;
+    }
+  if (n_pages > 0x7ffffffeLL || max_pages > 0x7fffffffLL || max_pages * page_size > 0x7fffffffLL ||
+      batch > 0x7ffffffeLL || kv_heads > 65535) {
+    set_err(err, errlen, "%s: more than 2^31 - 1 pages, positions or sequences", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  return XB_OK;
+}
+
+template <int N>
+cudaError_t launch_copy(const int32_t* src, const int32_t* dst, int n, uint8_t* base, int64_t outer,
+                        int64_t outer_stride, int64_t page_stride, uint32_t vpp, cudaStream_t s) {
+  CopyPairs<N> pairs;
+  memset(&pairs, 0, sizeof(pairs));
+  memcpy(pairs.src, src, n * sizeof(int32_t));
+  memcpy(pairs.dst, dst, n * sizeof(int32_t));
+  const uint32_t total = (uint32_t)n * vpp;
+  return launch_k<false>(copy_pages_kernel<N>, dim3((total + 1023u) / 1024u, (unsigned)outer), 256, 0, s, pairs, base,
+                         outer_stride, page_stride, vpp, total);
+}
+
+}  // namespace paged
+
+// The timeout flag of this file's kernels, read and cleared by xb_device_status.
+cudaError_t paged_status_take(int* status, cudaStream_t s) {
+  int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(status, paged::g_paged_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess)
+    e = cudaMemcpyToSymbolAsync(paged::g_paged_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  return e;
+}
+
+}  // namespace xb
+
+using namespace xb::paged;
+using xb::aligned16;
+using xb::check_launch;
+using xb::launch_k;
+using xb::set_err;
+
+extern "C" int xb_copy_pages(void* pages, int64_t outer, int64_t outer_bytes, int64_t n_pages, int64_t page_bytes,
+                             const int32_t* src, const int32_t* dst, int64_t n, void* stream, char* err,
+                             size_t errlen) {
+  const char* what = "xb_copy_pages";
+  if (outer < 0 || n_pages < 0 || page_bytes < 0 || n < 0) {
+    set_err(err, errlen, "%s: negative size", what);
+    return XB_ERR_INVALID;
+  }
+  if (n == 0) return XB_OK;
+  if (!src || !dst) {
+    set_err(err, errlen, "%s: null page list", what);
+    return XB_ERR_INVALID;
+  }
+  if (n > n_pages || n_pages > 0x7fffffffLL) {
+    set_err(err, errlen, "%s: %lld copies in a pool of %lld pages", what, (long long)n, (long long)n_pages);
+    return XB_ERR_INVALID;
+  }
+  // one bit per page: destinations are distinct and none is a source
+  uint64_t* seen = static_cast<uint64_t*>(calloc((size_t)(n_pages + 63) / 64, 8));
+  if (!seen) {
+    set_err(err, errlen, "%s: out of host memory", what);
+    return XB_ERR_INVALID;
+  }
+  const char* wrong = nullptr;
+  int64_t at = 0;
+  for (int64_t i = 0; i < n && !wrong; ++i) {
+    if (src[i] < 0 || src[i] >= n_pages) wrong = "source outside the pool", at = src[i];
+    else if (dst[i] < 0 || dst[i] >= n_pages) wrong = "destination outside the pool", at = dst[i];
+    else if (seen[dst[i] >> 6] >> (dst[i] & 63) & 1) wrong = "destination given twice", at = dst[i];
+    else seen[dst[i] >> 6] |= 1ull << (dst[i] & 63);
+  }
+  for (int64_t i = 0; i < n && !wrong; ++i)
+    if (seen[src[i] >> 6] >> (src[i] & 63) & 1) wrong = "page is both a source and a destination", at = src[i];
+  free(seen);
+  if (wrong) {
+    set_err(err, errlen, "%s: %s (page %lld)", what, wrong, (long long)at);
+    return XB_ERR_INVALID;
+  }
+  if (outer == 0 || page_bytes == 0) return XB_OK;
+  if (!pages) {
+    set_err(err, errlen, "%s: null pointer", what);
+    return XB_ERR_INVALID;
+  }
+  if (page_bytes % 16 || outer_bytes % 16 || !aligned16(pages) || (outer > 1 && outer_bytes < n_pages * page_bytes)) {
+    set_err(err, errlen, "%s: pages must be whole 16-byte vectors in slabs that do not overlap", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  if (outer > 65535 || page_bytes / 16 * kCopyPairs > 0xffff0000LL) {
+    set_err(err, errlen, "%s: %lld slabs of %lld-byte pages not supported", what, (long long)outer,
+            (long long)page_bytes);
+    return XB_ERR_UNSUPPORTED;
+  }
+  const uint32_t vpp = (uint32_t)(page_bytes / 16);
+  uint8_t* base = static_cast<uint8_t*>(pages);
+  for (int64_t i = 0; i < n; i += kCopyPairs) {
+    const int c = (int)(n - i < kCopyPairs ? n - i : kCopyPairs);
+    cudaError_t e = c <= 28 ? launch_copy<28>(src + i, dst + i, c, base, outer, outer_bytes, page_bytes, vpp,
+                                              (cudaStream_t)stream)
+                            : launch_copy<kCopyPairs>(src + i, dst + i, c, base, outer, outer_bytes, page_bytes, vpp,
+                                                      (cudaStream_t)stream);
+    if (e != cudaSuccess) {
+      set_err(err, errlen, "%s: %s", what, cudaGetErrorString(e));
+      return XB_ERR_CUDA;
+    }
+  }
+  return check_launch(what, err, errlen);
+}
+
+extern "C" int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t, const float* sin_t, void* q_out,
+                                     void* k_pages, void* v_pages, const int32_t* page_table, const int32_t* q_start,
+                                     const int32_t* kv_len, int64_t tokens, int64_t batch, int64_t n_head,
+                                     int64_t n_kv_head, int64_t head_dim, int64_t n_pages, int64_t page_size,
+                                     int64_t max_pages, int64_t rope_rows, int64_t ld_qkv, int64_t ld_q,
+                                     int64_t ld_table, int64_t k_page, int64_t k_head, int64_t k_row, int64_t v_page,
+                                     int64_t v_head, int64_t v_row, void* stream, char* err, size_t errlen) {
+  const char* what = "xb_paged_rope_kv_bf16";
+  if (tokens < 0 || n_head <= 0 || head_dim <= 0 || n_head > 65535) {
+    set_err(err, errlen, "%s: bad shape", what);
+    return XB_ERR_INVALID;
+  }
+  int rc = check_pages(n_pages, page_size, n_kv_head, batch, max_pages, ld_table, k_page, k_head, k_row, v_page,
+                       v_head, v_row, what, err, errlen);
+  if (rc) return rc;
+  if (head_dim % 16 || head_dim > 512 || 32 % (head_dim / 16)) {
+    set_err(err, errlen, "%s: head_dim %lld not supported (16, 32, 64, 128, 256, 512)", what, (long long)head_dim);
+    return XB_ERR_UNSUPPORTED;
+  }
+  if (tokens == 0 || batch == 0) return XB_OK;
+  if (!qkv || !q_out || !k_pages || !v_pages || !page_table || !q_start || !kv_len || (!cos_t) != (!sin_t)) {
+    set_err(err, errlen, "%s: null pointer", what);
+    return XB_ERR_INVALID;
+  }
+  if (ld_qkv < (n_head + 2 * n_kv_head) * head_dim || ld_q < n_head * head_dim) {
+    set_err(err, errlen, "%s: row pitch shorter than the row", what);
+    return XB_ERR_INVALID;
+  }
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_pages) || !aligned16(v_pages) || ld_qkv % 8 || ld_q % 8 ||
+      (cos_t && (!aligned16(cos_t) || !aligned16(sin_t)))) {
+    set_err(err, errlen, "%s: rows must be whole 16-byte vectors", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  if (tokens > 0x7ffffff0LL) {
+    set_err(err, errlen, "%s: too many tokens", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  RopeArgs a;
+  a.qkv = static_cast<const bf16*>(qkv);
+  a.cos_t = cos_t;
+  a.sin_t = sin_t;
+  a.q = static_cast<bf16*>(q_out);
+  a.k = Pages{static_cast<bf16*>(k_pages), k_page, k_head, k_row};
+  a.v = Pages{static_cast<bf16*>(v_pages), v_page, v_head, v_row};
+  a.table = page_table;
+  a.q_start = q_start;
+  a.kv_len = kv_len;
+  a.ld_qkv = ld_qkv;
+  a.ld_q = ld_q;
+  a.ld_table = ld_table;
+  a.rope_rows = rope_rows;
+  a.T = (int)tokens;
+  a.B = (int)batch;
+  a.H = (int)n_head;
+  a.KVH = (int)n_kv_head;
+  a.D = (int)head_dim;
+  a.page_size = (int)page_size;
+  a.max_pages = (int)max_pages;
+  a.n_pages = (int)n_pages;
+  int *bad = nullptr, *status = nullptr;
+  rc = status_words(&bad, &status, what, err, errlen);
+  if (rc) return rc;
+  launch_k<false>(paged_rope_kv_kernel, (unsigned)((tokens + 7) / 8), 256, 0, (cudaStream_t)stream, a, bad);
+  return check_launch(what, err, errlen);
+}
+
+extern "C" int xb_paged_attention_workspace_size(int64_t tokens, int64_t batch, int64_t n_head, int64_t n_kv_head,
+                                                 size_t* bytes, char* err, size_t errlen) {
+  const char* what = "xb_paged_attention_workspace_size";
+  if (!bytes || tokens < 0 || batch < 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head) {
+    set_err(err, errlen, "%s: bad arguments", what);
+    return XB_ERR_INVALID;
+  }
+  int sms = 148;
+  xb::sm_count(&sms);
+  *bytes = (size_t)sms * (2 * part_floats(kFewRows) * sizeof(float) + sizeof(Meta));
+  return XB_OK;
+}
+
+extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const void* v_pages, void* out,
+                                       const int32_t* page_table, const int32_t* q_start, const int32_t* kv_len,
+                                       int64_t tokens, int64_t batch, int64_t n_head, int64_t n_kv_head,
+                                       int64_t head_dim, int64_t n_pages, int64_t page_size, int64_t max_pages,
+                                       int64_t ld_q, int64_t ld_out, int64_t ld_table, int64_t k_page, int64_t k_head,
+                                       int64_t k_row, int64_t v_page, int64_t v_head, int64_t v_row, float scale,
+                                       void* workspace, size_t workspace_bytes, void* stream, char* err,
+                                       size_t errlen) {
+  const char* what = "xb_paged_attention_bf16";
+  if (tokens < 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head || n_head > 65535) {
+    set_err(err, errlen, "%s: bad shape", what);
+    return XB_ERR_INVALID;
+  }
+  int rc = check_pages(n_pages, page_size, n_kv_head, batch, max_pages, ld_table, k_page, k_head, k_row, v_page,
+                       v_head, v_row, what, err, errlen);
+  if (rc) return rc;
+  if (head_dim != kHD) {
+    set_err(err, errlen, "%s: head_dim %lld not supported (64)", what, (long long)head_dim);
+    return XB_ERR_UNSUPPORTED;
+  }
+  const int n_rep = (int)(n_head / n_kv_head);
+  if (n_rep > 16) {
+    set_err(err, errlen, "%s: %d query heads per KV head not supported (1..16)", what, n_rep);
+    return XB_ERR_UNSUPPORTED;
+  }
+  if (!(scale > 0.0f)) {
+    set_err(err, errlen, "%s: the scale must be positive", what);
+    return XB_ERR_INVALID;
+  }
+  if (tokens == 0 || batch == 0) return XB_OK;
+  if (!q || !k_pages || !v_pages || !out || !page_table || !q_start || !kv_len) {
+    set_err(err, errlen, "%s: null pointer", what);
+    return XB_ERR_INVALID;
+  }
+  if (ld_q < n_head * kHD || ld_out < n_head * kHD) {
+    set_err(err, errlen, "%s: row pitch shorter than the row", what);
+    return XB_ERR_INVALID;
+  }
+  if (!aligned16(q) || !aligned16(out) || !aligned16(k_pages) || !aligned16(v_pages) || ld_q % 8 || ld_out % 8) {
+    set_err(err, errlen, "%s: rows must be whole 16-byte vectors", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  if (tokens > 0x7fffffffLL) {
+    set_err(err, errlen, "%s: too many tokens", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  size_t need = 0;
+  rc = xb_paged_attention_workspace_size(tokens, batch, n_head, n_kv_head, &need, err, errlen);
+  if (rc) return rc;
+  if (!workspace || workspace_bytes < need || !aligned16(workspace)) {
+    set_err(err, errlen, "%s: needs a 16-byte aligned workspace of %zu bytes (%zu given)", what, need,
+            workspace_bytes);
+    return XB_ERR_INVALID;
+  }
+  AttnArgs a;
+  a.q = static_cast<const bf16*>(q);
+  a.out = static_cast<bf16*>(out);
+  a.table = page_table;
+  a.q_start = q_start;
+  a.kv_len = kv_len;
+  a.ws = static_cast<float*>(workspace);
+  a.ld_q = ld_q;
+  a.ld_out = ld_out;
+  a.ld_table = ld_table;
+  a.T = (int)tokens;
+  a.B = (int)batch;
+  a.KVH = (int)n_kv_head;
+  a.n_rep = n_rep;
+  a.tpt = kFewRows / n_rep;
+  a.page_size = (int)page_size;
+  a.max_pages = (int)max_pages;
+  a.n_pages = (int)n_pages;
+  a.min_share = 128;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  rc = status_words(&a.bad, &a.status, what, err, errlen);
+  if (rc) return rc;
+  int box = 8;  // rows of one load: the largest power of two that divides a page, at most a tile
+  while (box < kTK && page_size % (2 * box) == 0) box *= 2;
+  a.box_rows = box;
+  KvMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  rc = page_map(&maps.k, k_pages, n_pages, n_kv_head, page_size, k_page, k_head, k_row, box, what, err, errlen);
+  if (!rc) rc = page_map(&maps.v, v_pages, n_pages, n_kv_head, page_size, v_page, v_head, v_row, box, what, err, errlen);
+  if (rc) return rc;
+  cudaError_t e = xb::once_per_device(reinterpret_cast<const void*>(paged_attn_few_kernel), xb::kOnceSmem, [](int*) {
+    return cudaFuncSetAttribute(paged_attn_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+  });
+  if (e != cudaSuccess) {
+    set_err(err, errlen, "%s: kernel setup: %s", what, cudaGetErrorString(e));
+    return XB_ERR_CUDA;
+  }
+  int sms = 148;
+  xb::sm_count(&sms);
+  cudaStream_t s = (cudaStream_t)stream;
+  e = launch_k(paged_attn_few_kernel, (unsigned)sms, kWarps * 32, kFewSmem, s, maps, a);
+  if (e == cudaSuccess) e = launch_k(paged_attn_join_kernel<kFewRows>, (unsigned)sms, 256, 0, s, a, sms);
+  if (e != cudaSuccess) {
+    set_err(err, errlen, "%s: %s", what, cudaGetErrorString(e));
+    return XB_ERR_CUDA;
+  }
+  return check_launch(what, err, errlen);
+}
+
+extern "C" int xb_page_status(void* stream, int* status, char* err, size_t errlen) {
+  if (!status) {
+    set_err(err, errlen, "xb_page_status: null output");
+    return XB_ERR_INVALID;
+  }
+  cudaStream_t s = (cudaStream_t)stream;
+  int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(status, g_bad_page, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_bad_page, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) {
+    set_err(err, errlen, "xb_page_status: %s", cudaGetErrorString(e));
+    return XB_ERR_CUDA;
+  }
+  return XB_OK;
+}

@@ -55,6 +55,7 @@ _CTYPES = {
     # device pointers travel as plain addresses
     "int64_t*": ctypes.c_void_p,
     "const int64_t*": ctypes.c_void_p,
+    "const int32_t*": ctypes.c_void_p,  # device arrays (paged cache) or host page lists (xb_copy_pages)
     "float*": ctypes.c_void_p,
     "const float*": ctypes.c_void_p,
     "size_t": ctypes.c_size_t,

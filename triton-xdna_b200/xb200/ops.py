@@ -10,6 +10,7 @@ raises.  For the reference's host-tensor launch semantics see
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -1001,3 +1002,179 @@ def argmax(x, out=None):
         out = torch.empty(x.shape[0], dtype=torch.int64, device=x.device)
     _lib.call("xb_argmax_f32", x.data_ptr(), x.shape[0], x.shape[1], x.stride(0), out.data_ptr(), _stream())
     return out
+
+
+# --------------------------------------------------------------------------- paged KV cache
+#
+# A step packs the new tokens of many sequences: tokens q_start[b] ..
+# q_start[b + 1] - 1 are the last ones of sequence b, which with them holds
+# kv_len[b] positions, in the pages page_table[b, :].  All three are int32
+# device tensors that the kernels read, so captured graphs replay with other
+# lengths.  xb200.paged.PagedKVCache keeps them and the pool.
+
+
+class _on_device:
+    """Makes `device` the current one for a call (tensors of another device
+    than the current one are enqueued on their own device's current stream)."""
+
+    def __init__(self, device):
+        self.prev, self.dev = torch.cuda.current_device(), device.index
+
+    def __enter__(self):
+        if self.dev != self.prev:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc):
+        if self.dev != self.prev:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+def _page_args(k_pages, v_pages, page_table, q_start, kv_len):
+    """Checks what the host can see of a paged batch: (batch, max_pages, table pitch, the six page strides)."""
+    if k_pages.dtype != torch.bfloat16 or v_pages.dtype != torch.bfloat16:
+        raise TypeError("k_pages and v_pages must be bf16")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must share a shape [n_pages, n_kv_head, page_size, head_dim]")
+    for t, n in ((page_table, "page_table"), (q_start, "q_start"), (kv_len, "kv_len")):
+        if t.dtype != torch.int32:
+            raise TypeError(f"{n} must be int32")
+    B = kv_len.shape[0] if kv_len.dim() == 1 else -1
+    if B < 0 or tuple(q_start.shape) != (B + 1,) or page_table.dim() != 2 or page_table.shape[0] != B:
+        raise ValueError("a batch of B sequences has kv_len [B], q_start [B + 1] and page_table [B, max_pages]")
+    if not (q_start.is_contiguous() and kv_len.is_contiguous()) or (page_table.stride(1) != 1
+                                                                   and page_table.shape[1] > 1):
+        raise ValueError("q_start, kv_len and the rows of page_table must be contiguous")
+    if page_table.shape[1] == 0:
+        raise ValueError("page_table needs at least one column")
+    n, h, p, d = k_pages.shape
+    lds = []
+    for t in (k_pages, v_pages):
+        if t.stride(3) != 1 and d > 1:
+            raise ValueError("page rows must be contiguous")
+        # the stride of a dimension of one is arbitrary: any multiple of 8 stands for it
+        lds += [t.stride(i) if size > 1 else h * p * d for i, size in ((0, n), (1, h), (2, p))]
+    return B, page_table.shape[1], page_table.stride(0) if B > 1 else page_table.shape[1], lds
+
+
+def _token_rows(t, name, tokens, row) -> int:
+    """Row pitch of a [tokens, row] (or [tokens, heads, dim]) tensor whose rows are contiguous."""
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be bf16")
+    inner = t.numel() // t.shape[0] if t.dim() > 1 and t.shape[0] else row
+    if t.dim() not in (2, 3) or t.shape[0] != tokens or inner != row:
+        raise ValueError(f"{name} must have {tokens} rows of {row} elements")
+    if tokens and (t.stride(-1) != 1 or (t.dim() == 3 and t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+        raise ValueError(f"the rows of {name} must be contiguous")
+    return t.stride(0) if tokens > 1 else row
+
+
+def _overlap(a, b) -> bool:
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len):
+    """RoPE of the packed QKV projection [T, (H + 2 KVH) * D] (none when the
+    tables are None) into q_out [T, H, D], and the write of its keys and values
+    into the pages at their positions: rope_kv() for a paged cache, the same
+    bits.  Tokens outside the sequences are left alone; page_status() tells of
+    positions without a page or table row."""
+    _cuda(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len)
+    if (cos_t is None) != (sin_t is None):
+        raise ValueError("give both RoPE tables or neither")
+    B, max_pages, ld_table, lds = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
+    n, KVH, P, D = k_pages.shape
+    if q_out.dim() != 3 or q_out.shape[2] != D:
+        raise ValueError(f"q_out must be [tokens, n_head, {D}]")
+    T, H = q_out.shape[0], q_out.shape[1]
+    rows = 0
+    if cos_t is not None:
+        for t in (cos_t, sin_t):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != D or not t.is_contiguous():
+                raise ValueError(f"RoPE tables must be contiguous float32 [positions, {D}]")
+        rows = min(cos_t.shape[0], sin_t.shape[0])
+    ld_qkv, ld_q = _token_rows(qkv, "qkv", T, (H + 2 * KVH) * D), _token_rows(q_out, "q_out", T, H * D)
+    if _overlap(qkv, q_out):
+        raise ValueError("q_out must not share memory with qkv")
+    with _on_device(q_out.device):
+        _lib.call("xb_paged_rope_kv_bf16", qkv.data_ptr(), cos_t.data_ptr() if rows else None,
+                  sin_t.data_ptr() if rows else None, q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                  page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), T, B, H, KVH, D, n, P, max_pages,
+                  rows, ld_qkv, ld_q, ld_table, *lds, _stream())
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale):
+    """Causal GQA attention of packed new tokens over a paged cache: q [T, H,
+    64], out [T, H * 64] (or [T, H, 64]); the token at position p of its
+    sequence sees keys 0 .. p.  attention() for sequences of different lengths,
+    from single tokens to whole prompts in one batch.  Rows outside the
+    sequences are left as they are; a token that sees no key gets zeros."""
+    _cuda(q, k_pages, v_pages, out, page_table, q_start, kv_len)
+    B, max_pages, ld_table, lds = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
+    n, KVH, P, D = k_pages.shape
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"q must be [tokens, n_head, {D}]")
+    T, H = q.shape[0], q.shape[1]
+    ld_q, ld_out = _token_rows(q, "q", T, H * D), _token_rows(out, "out", T, H * D)
+    if _overlap(q, out):
+        raise ValueError("out must not share memory with q")
+    with _on_device(q.device):
+        need = ctypes.c_size_t(0)
+        _lib.call("xb_paged_attention_workspace_size", T, B, H, KVH, ctypes.byref(need))
+        # of this call alone: the caching allocator orders its reuse on the
+        # stream, and a captured graph keeps its own
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        _lib.call("xb_paged_attention_bf16", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
+                  page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), T, B, H, KVH, D, n, P, max_pages,
+                  ld_q, ld_out, ld_table, *lds, float(scale), ws.data_ptr(), ws.numel(), _stream())
+    return out
+
+
+def _page_list(ids, name) -> torch.Tensor:
+    t = torch.as_tensor(ids)
+    if t.device.type != "cpu" or t.dim() != 1 or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        if t.numel() or t.device.type != "cpu" or t.dim() != 1:
+            raise TypeError(f"{name} must be a sequence of page numbers on the host")
+    if t.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8) and t.numel():
+        lo, hi = t.aminmax()
+        if int(lo) < 0 or int(hi) > 0x7FFFFFFF:
+            raise ValueError(f"{name} holds page numbers outside the pool")
+    return t.to(torch.int32).contiguous()
+
+
+def copy_pages(pages, src, dst, dim: int = 2):
+    """pages[.., dst[i], ..] = pages[.., src[i], ..] along dimension `dim` of a
+    contiguous pool (PagedKVCache.pages: [n_layer, 2, n_pages, n_kv_head,
+    page_size, head_dim]): all layers' keys and values in one launch.  src and
+    dst are page numbers on the host (lists or CPU integer tensors); no page
+    may be a destination twice, or both a source and a destination."""
+    _cuda(pages)
+    if not -pages.dim() <= dim < pages.dim():
+        raise ValueError(f"pages has no dimension {dim}")
+    dim %= pages.dim()
+    if not pages.is_contiguous():
+        raise ValueError("pages must be contiguous")
+    src, dst = _page_list(src, "src"), _page_list(dst, "dst")
+    if src.numel() != dst.numel():
+        raise ValueError(f"{src.numel()} sources for {dst.numel()} destinations")
+    outer = math.prod(pages.shape[:dim])
+    page_bytes = math.prod(pages.shape[dim + 1:]) * pages.element_size()
+    with _on_device(pages.device):
+        _lib.call("xb_copy_pages", pages.data_ptr(), outer, pages.shape[dim] * page_bytes, pages.shape[dim],
+                  page_bytes, src.data_ptr(), dst.data_ptr(), src.numel(), _stream())
+    return pages
+
+
+def page_status() -> int:
+    """1 if a paged operator met a page number outside its pool, or a position
+    without a page or RoPE row, since the last call, else 0."""
+    st = ctypes.c_int(0)
+    _lib.call("xb_page_status", _stream(), ctypes.byref(st))
+    return st.value
