@@ -170,15 +170,18 @@ __global__ void __launch_bounds__(256) paged_rope_kv_kernel(const RopeArgs a, in
 // new tokens of a sequence times the n_rep query heads that share the KV head,
 // which are the rows of one matrix tile, so every key and value is read once
 // for all of them.  Query tile j of a sequence with `base` earlier positions
-// sees base + min(tpt (j + 1), n) keys.  All units laid end to end, weighted
-// by those keys, make one line of `total` keys; CTA c takes the piece
-// [c share, (c + 1) share) of it, whatever unit boundaries lie inside, so the
-// CTAs finish together however uneven the batch is.  A unit that one CTA
-// covers alone is written at once; one that spans several leaves a partial
-// (O, max, sum) per CTA in the workspace, and a second small kernel joins
-// them in CTA order (fixed order: repeatable bits).  The weights are a closed
-// form, so a CTA finds its piece with one scan over the sequences and a binary
-// search inside one, from lengths that only the device knows.
+// sees base + min(tpt (j + 1), n) keys; its weight is those keys plus `over`,
+// what starting and finishing a unit costs in keys.  All units laid end to end
+// are one line of weight `total`; CTA c takes the piece [c share, (c + 1) share)
+// of it, whatever unit boundaries lie inside, so the CTAs finish together
+// however uneven the batch is.  A cut closer than `snap` keys to a unit's
+// first or last key moves to the unit's boundary (both neighbours move it the
+// same way).  A unit that one CTA covers alone is written at once; one that
+// spans several leaves a partial (O, max, sum) per CTA in the workspace, and a
+// second small kernel joins them in CTA order (fixed order: repeatable bits).
+// The weights are a closed form, so a CTA finds its piece with one scan over
+// the sequences and a binary search inside one, from lengths that only the
+// device knows.
 
 struct AttnArgs {
   const bf16* q;
@@ -187,7 +190,7 @@ struct AttnArgs {
   float* ws;  // [2 G] partials, then G Meta
   int64_t ld_q, ld_out, ld_table;
   int T, B, KVH, n_rep, tpt, page_size, max_pages, n_pages, box_rows;
-  int min_share;
+  int min_share, over, snap;
   float scale_log2;
   int *bad, *status;
 };
@@ -204,9 +207,9 @@ struct Seq {
   int64_t perh;       // weight of one KV head
 };
 
-__device__ __forceinline__ int64_t cum_keys(const Seq& q, int tpt, int64_t j) {  // weight of query tiles 0 .. j - 1
-  const int64_t b = q.base > 0 ? q.base : 0;
-  return j * b + (j < q.nt ? tpt * j * (j + 1) / 2 : tpt * (int64_t)q.nt * (q.nt - 1) / 2 + q.n);
+__device__ __forceinline__ int64_t cum_keys(const AttnArgs& a, const Seq& q, int64_t j) {  // weight of tiles 0 .. j - 1
+  const int64_t b = (q.base > 0 ? q.base : 0) + a.over;
+  return j * b + (j < q.nt ? a.tpt * j * (j + 1) / 2 : a.tpt * (int64_t)q.nt * (q.nt - 1) / 2 + q.n);
 }
 
 __device__ __forceinline__ Seq load_seq(const AttnArgs& a, int b) {
@@ -220,27 +223,27 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs& a, int b) {
   q.len = len < cap ? len : cap;
   q.base = q.len - q.n;
   q.nt = (q.n + a.tpt - 1) / a.tpt;
-  q.perh = cum_keys(q, a.tpt, q.nt);
+  q.perh = cum_keys(a, q, q.nt);
   return q;
 }
 
-// One CTA's walk over its piece of the line.
+// One CTA's walk over its piece [lo, hi) of the line.
 struct Walk {
-  int64_t lo, hi;  // the CTA's piece
-  int64_t share;
-  int64_t u0;      // where the current unit starts
+  int64_t lo, hi, share;
+  int64_t u0;  // where the current unit starts
   int b, kvh, j;
-  Seq q;
 };
 
+// The CTA's part of one unit.
 struct Segment {
-  int token, rows;     // first packed token and rows of the query tile
-  int kvh, b;
-  int64_t first_pos;   // position of the tile's first token
-  int64_t keys;        // keys the unit's last token sees (> 0 unless its rows are all empty)
-  int t0, t1;          // key tiles [t0, t1) of this CTA's part
-  bool starts, ends;   // the unit starts / ends in this CTA
-  int64_t u0, ulen;
+  int b, kvh;
+  int token, rows;    // first packed token and rows of the query tile
+  int first_pos;      // position of the tile's first token (may be negative)
+  int keys;           // keys the unit's last token sees; 0 when none of its tokens sees any
+  int t0, t1;         // key tiles of this part
+  int last;           // the CTA in which the unit ends
+  bool starts, ends;  // the unit starts / ends in this CTA
+  int64_t next;       // where the next unit starts
 };
 
 // Every thread of the block calls this; `found` is shared.  False: no work for this CTA.
@@ -291,59 +294,69 @@ __device__ __forceinline__ bool find_piece(const AttnArgs& a, Walk& w, int64_t (
     }
   }
   w.b = (int)found[0];
-  w.q = load_seq(a, w.b);
+  const Seq q = load_seq(a, w.b);
   const int64_t off = w.lo - found[1];
-  w.kvh = (int)(off / w.q.perh);
-  const int64_t in = off - w.kvh * w.q.perh;
-  int lo = 0, hi = w.q.nt - 1;  // the last tile j with cum(j) <= in
+  w.kvh = (int)(off / q.perh);
+  const int64_t in = off - w.kvh * q.perh;
+  int lo = 0, hi = q.nt - 1;  // the last tile j with cum(j) <= in
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (cum_keys(w.q, a.tpt, mid) <= in) lo = mid;
+    if (cum_keys(a, q, mid) <= in) lo = mid;
     else hi = mid - 1;
   }
   w.j = lo;
-  w.u0 = found[1] + w.kvh * w.q.perh + cum_keys(w.q, a.tpt, lo);
+  w.u0 = found[1] + w.kvh * q.perh + cum_keys(a, q, lo);
   return true;
 }
 
-template <int TK>
-__device__ __forceinline__ Segment segment(const AttnArgs& a, const Walk& w) {
-  Segment g;
-  const int done = w.j * a.tpt;
-  const int tokens = min(a.tpt, w.q.n - done);
-  g.token = w.q.s0 + done;
-  g.rows = tokens * a.n_rep;
-  g.kvh = w.kvh;
-  g.b = w.b;
-  g.first_pos = w.q.base + done;
-  g.keys = g.first_pos + tokens;
-  if (g.keys < 0) g.keys = 0;
-  const int64_t b0 = w.q.base > 0 ? w.q.base : 0;
-  g.u0 = w.u0;
-  g.ulen = b0 + done + tokens;
-  const int64_t s = w.lo > w.u0 ? w.lo - w.u0 : 0;
-  const int64_t e = w.hi < w.u0 + g.ulen ? w.hi - w.u0 : g.ulen;
-  g.starts = w.lo <= w.u0;
-  g.ends = w.hi >= w.u0 + g.ulen;
-  const int nk = (int)((g.keys + TK - 1) / TK);
-  g.t0 = min((int)(s / TK), nk);  // cuts fall on tile boundaries, the same ones on both sides
-  g.t1 = g.ends ? nk : min((int)(e / TK), nk);
-  return g;
-}
-
-// Steps to the next unit of the CTA's piece; false at its end.
-__device__ __forceinline__ bool next_unit(const AttnArgs& a, Walk& w, const Segment& g) {
-  w.u0 = g.u0 + g.ulen;
-  if (w.u0 >= w.hi) return false;
-  if (++w.j < w.q.nt) return true;
+// Steps to the next unit; false behind the last one.
+__device__ __forceinline__ bool next_unit(const AttnArgs& a, Walk& w, int64_t u0) {
+  w.u0 = u0;
+  if (u0 >= w.hi) return false;
+  if (++w.j < load_seq(a, w.b).nt) return true;
   w.j = 0;
   if (++w.kvh < a.KVH) return true;
   w.kvh = 0;
   do {
     if (++w.b >= a.B) return false;
-    w.q = load_seq(a, w.b);
-  } while (w.q.n == 0);
+  } while (load_seq(a, w.b).n == 0);
   return true;
+}
+
+// The part of the current unit that belongs to this CTA, stepping over one
+// whose cut was moved away; false when nothing is left.
+template <int TK>
+__device__ __forceinline__ bool segment(const AttnArgs& a, Walk& w, Segment& g) {
+  for (;;) {
+    const Seq q = load_seq(a, w.b);
+    const int done = w.j * a.tpt;
+    const int tokens = min(a.tpt, q.n - done);
+    const int keys = (int)max(q.base + done + tokens, (int64_t)0);
+    const int64_t ulen = a.over + (q.base > 0 ? q.base : 0) + done + tokens;
+    const int64_t cut0 = w.lo - w.u0, cut1 = w.hi - w.u0;  // the piece's ends inside the unit
+    g.next = w.u0 + ulen;
+    g.starts = cut0 < a.over + a.snap;
+    if (!g.starts && ulen - cut0 < a.snap) {  // only at the piece's start: the unit ended in the CTA before
+      if (!next_unit(a, w, g.next)) return false;
+      continue;
+    }
+    if (cut1 < a.over + a.snap && cut1 < ulen) return false;  // the unit starts in the next CTA
+    g.ends = cut1 >= ulen || ulen - cut1 < a.snap;
+    const int nk = (keys + TK - 1) / TK;
+    g.t0 = g.starts ? 0 : min((int)((cut0 - a.over) / TK), nk);  // cuts fall on tile boundaries
+    g.t1 = g.ends ? nk : min((int)((cut1 - a.over) / TK), nk);
+    // the CTA that holds the unit's last key, or the one before it if that cut was moved to the unit's end
+    int64_t last = (g.next - 1) / w.share;
+    if (last * w.share > w.u0 && g.next - last * w.share < a.snap) --last;
+    g.last = (int)last;
+    g.b = w.b;
+    g.kvh = w.kvh;
+    g.token = q.s0 + done;
+    g.rows = tokens * a.n_rep;
+    g.first_pos = (int)(q.base + done);
+    g.keys = keys;
+    return true;
+  }
 }
 
 // ----------------------------------------------------------------------------- attention: few rows (mma.sync)
@@ -442,14 +455,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
   // tiles this warp has read / requested so far: buffer n % kBufs, parity (n / kBufs) & 1
   uint32_t use = 0, issued = 0;
   bool dead = false;  // a wait ran out: no more loads, the output is not valid
-  for (bool more = true; more;) {
-    const Segment s = segment<kTK>(a, w);
+  Segment s;
+  for (bool more = segment<kTK>(a, w, s); more; more = next_unit(a, w, s.next) && segment<kTK>(a, w, s)) {
     const int boxes = kTK / a.box_rows;
     // lane 0 .. boxes - 1 load K rows, the next `boxes` lanes V rows of tile `tile` into buffer `buf`
     auto issue = [&](int tile, uint32_t n) {
       const uint32_t buf = n % kBufs;
-      const int64_t k0 = (int64_t)tile * kTK;
-      const int have = (int)min((int64_t)kTK, s.keys - k0);
+      const int k0 = tile * kTK;
+      const int have = min(kTK, s.keys - k0);
       const int nb = (have + a.box_rows - 1) / a.box_rows;
       if (lane == 0) mbar_arrive_expect_tx(&full[warp][buf], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
       __syncwarp();
@@ -486,7 +499,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
         qa[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c + 8) : 0u;
       }
     }
-    const int64_t pos0 = s.first_pos + g / a.n_rep, pos1 = s.first_pos + (g + 8) / a.n_rep;
+    // the last key each of this thread's rows sees
+    const int pos0 = min(s.first_pos + g / a.n_rep, s.keys - 1), pos1 = min(s.first_pos + (g + 8) / a.n_rep, s.keys - 1);
     float o[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -500,9 +514,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
         dead = true;
         break;
       }
-      const int64_t k0 = (int64_t)tile * kTK;
+      const int k0 = tile * kTK;
       const uint32_t sk = ring + buf * 2 * kTileBytes, sv = sk + kTileBytes;
-      const int have = (int)min((int64_t)kTK, s.keys - k0);
+      const int have = min(kTK, s.keys - k0);
       if (have < kTK) {
         // values behind the last key hold whatever the page or buffer held: a
         // NaN there would survive its zero weight
@@ -528,8 +542,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
       for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int64_t key = k0 + nt * 8 + 2 * t + (e & 1);
-          sc[nt][e] = key <= (e < 2 ? pos0 : pos1) && key < s.keys ? sc[nt][e] * a.scale_log2 : -INFINITY;
+          const int key = k0 + nt * 8 + 2 * t + (e & 1);
+          sc[nt][e] = key <= (e < 2 ? pos0 : pos1) ? sc[nt][e] * a.scale_log2 : -INFINITY;
           if (e < 2) mx0 = fmaxf(mx0, sc[nt][e]);
           else mx1 = fmaxf(mx1, sc[nt][e]);
         }
@@ -644,15 +658,419 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
     if (s.starts && !s.ends) {
       open_unit = true;
       if (threadIdx.x == 0)
-        meta[blockIdx.x] = Meta{(int)((s.u0 + s.ulen - 1) / w.share), s.token, s.rows, s.kvh};
+        meta[blockIdx.x] = Meta{s.last, s.token, s.rows, s.kvh};
     }
-    more = next_unit(a, w, s);
   }
   if (!open_unit && threadIdx.x == 0) meta[blockIdx.x].last = -1;
   if (dead) {  // loads still in flight land before the CTA's shared memory is given up
     uint64_t deadline = 0;
     for (; use < issued; ++use)
       mbar_wait_deadline(&full[warp][use % kBufs], (use / kBufs) & 1, &deadline, kWaitLimit);
+  }
+}
+
+// ----------------------------------------------------------------------------- attention: many rows (tcgen05)
+//
+// For batches whose sequences bring many tokens (prompts, chunks, mixed
+// steps): units of up to 128 rows (tpt = 128 / n_rep tokens), key tiles of 64.
+// Two persistent CTAs per SM, each walking its piece of the line:
+//   warp 0     loads each unit's Q and streams K / V page rows into a ring of
+//              five tiles (one lane per page piece, TMA, 128-byte swizzle);
+//   warp 1     issues S_g = Q K_g^T into one of two 64-column TMEM buffers and
+//              O += P_g V_g; P_g is the MMA's A operand straight from TMEM;
+//   warps 2-5  softmax, one query row per thread: scores from TMEM, bf16(P)
+//              back into the first half of the same TMEM buffer.
+// Keeping P in TMEM takes its write and its 16 KB operand read per tile off
+// shared memory, whose 128 bytes a clock would otherwise be the first limit
+// (Q, K, V and P reads, P writes and the TMA's writes: 640 of them a tile,
+// against 512 clocks of exponentials).  S_{g+1} is issued before P_g V_g, so
+// the softmax always has the next scores waiting.  O accumulates in TMEM
+// relative to a per-row base that moves only when a tile's maximum exceeds it
+// by more than 2^8 (bf16 keeps its 8 bits at any scale), and only then is O
+// rescaled.  Warps whose 32 rows are all past the unit's (a single token of a
+// decoding sequence in a mixed batch) skip the arithmetic.  Every wait is
+// bounded; a timeout sets the status word, drains what is in flight and ends.
+constexpr int kTcRows = 128;
+constexpr int kTcTK = 64;
+constexpr int kTcStages = 5;
+constexpr int kTcQBytes = kTcRows * kHD * 2;
+constexpr int kTcTileBytes = kTcTK * kHD * 2;  // one K or V tile
+constexpr int kTcSmem = kTcQBytes + kTcStages * 2 * kTcTileBytes + 1024;
+constexpr int kTcThreads = 192;
+
+struct alignas(64) TcMaps {
+  CUtensorMap q;  // [T][n_head][64], box {64, n_rep, tpt}
+  CUtensorMap k, v;
+};
+
+// D[tmem] (+)= A[tmem] x B[smem desc], kind::f16; A: lane = row, 32-bit column = two consecutive K elements
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(
+          d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __grid_constant__ TcMaps maps,
+                                                                      const AttnArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t q_full, q_empty, drain_bar, o_full, o_empty;
+  __shared__ __align__(8) uint64_t s_full[2], p_full[2];
+  __shared__ __align__(8) uint64_t kv_full[kTcStages], kv_empty[kTcStages];
+  __shared__ int64_t warp_sum[2][kTcThreads / 32];
+  __shared__ int64_t found[2];
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ volatile int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t sQ = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t sKV = sQ + kTcQBytes;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 1);
+    mbar_init(&drain_bar, 1);
+    mbar_init(&o_full, 1);     // one P V accumulated into O
+    mbar_init(&o_empty, 128);  // a unit's O read by the softmax warps
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+    }
+    for (int i = 0; i < kTcStages; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    abort_flag = 0;
+    mbar_fence_init();
+    prefetch_tmap(&maps.q);
+    prefetch_tmap(&maps.k);
+    prefetch_tmap(&maps.v);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_base_sh, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;  // S / P buffers at columns 0 and 64, O at 128
+  pdl_wait();
+  pdl_trigger();
+
+  auto fail = [&]() {
+    atomicExch(a.status, XB_ERR_TIMEOUT);
+    abort_flag = 1;
+  };
+  Walk w;
+  Segment s;
+  const bool any_work = find_piece<kTcThreads>(a, w, warp_sum, found, gridDim.x, blockIdx.x);
+  bool more = any_work && segment<kTcTK>(a, w, s);
+  auto advance = [&]() { more = next_unit(a, w, s.next) && segment<kTcTK>(a, w, s); };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    uint32_t issued[kTcStages];
+#pragma unroll
+    for (int i = 0; i < kTcStages; ++i) issued[i] = 0;
+    const int boxes = kTcTK / a.box_rows;  // 1 .. 8 page pieces per tile; lane < boxes: K, the next ones: V
+    const bool is_v = lane >= boxes;
+    const int box = is_v ? lane - boxes : lane;
+    const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+    const uint32_t q_bytes = (uint32_t)(a.tpt * a.n_rep * kHD * 2);
+    int g = 0, lu = 0;  // tiles and units (with tiles) so far
+    bool ok = true;
+    for (; more && ok; advance()) {
+      if (s.t0 >= s.t1) continue;
+      // this lane's page of the first tile, fetched while Q's buffer may still be in use
+      auto page_of = [&](int tile) -> int {
+        const int key = tile * kTcTK + box * a.box_rows;
+        return lane < 2 * boxes && key < s.keys ? __ldg(a.table + s.b * a.ld_table + (uint32_t)key / (uint32_t)a.page_size)
+                                                : 0;
+      };
+      int id = page_of(s.t0);
+      if (lu > 0) ok = mbar_wait(&q_empty, (lu - 1) & 1, kWaitLimit, &abort_flag);
+      if (__any_sync(0xffffffffu, !ok)) {
+        fail();
+        ok = false;
+        break;
+      }
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&q_full, q_bytes);
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+            "[%2];" ::"r"(sQ),
+            "l"(reinterpret_cast<uint64_t>(&maps.q)), "r"(smem_u32(&q_full)), "r"(0), "r"(s.kvh * a.n_rep),
+            "r"(s.token)
+            : "memory");
+      }
+      ++lu;
+      for (int j = s.t0; j < s.t1; ++j, ++g) {
+        const int st = g % kTcStages;
+        const int here = id;
+        if (j + 1 < s.t1) id = page_of(j + 1);
+        ok = mbar_wait(&kv_empty[st], ((g / kTcStages) & 1) ^ 1, kWaitLimit, &abort_flag);
+        if (__any_sync(0xffffffffu, !ok)) {
+          fail();
+          ok = false;
+          break;
+        }
+        const int have = min(kTcTK, s.keys - j * kTcTK);
+        const int nb = (have + a.box_rows - 1) / a.box_rows;
+        if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
+        __syncwarp();
+        if (lane < 2 * boxes && box < nb) {
+          int page = here;
+          if (page < 0 || page >= a.n_pages) {  // reads as zeros: a coordinate past the pool
+            atomicExch(a.bad, 1);
+            page = a.n_pages;
+          }
+          const uint32_t row = (uint32_t)(j * kTcTK + box * a.box_rows) % (uint32_t)a.page_size;
+          tma_load_4d(sKV + st * 2 * kTcTileBytes + (is_v ? kTcTileBytes : 0) + box * a.box_rows * kHD * 2, map,
+                      &kv_full[st], 0, (int)row, s.kvh, page);
+        }
+        issued[st] = g / kTcStages + 1;
+      }
+    }
+    // every load issued must have landed before the CTA exits (also after an abort)
+    if (lane == 0) {
+      uint64_t deadline = 0;
+      if (lu > 0 && !mbar_wait_deadline(&q_full, (lu - 1) & 1, &deadline, kWaitLimit)) fail();
+#pragma unroll
+      for (int st = 0; st < kTcStages; ++st)
+        if (issued[st] && !mbar_wait_deadline(&kv_full[st], (issued[st] - 1) & 1, &deadline, kWaitLimit)) fail();
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t kIdS = umma_idesc(1, 1, 1, 0, 0, kTcRows, kTcTK);  // Q (K-major) x K tile (K-major)
+      constexpr uint32_t kIdO = umma_idesc(1, 1, 1, 0, 1, kTcRows, kHD);    // P (TMEM) x V tile (MN-major)
+      bool any = false, ok = true;
+      int g = 0, lu = 0;
+      int pend = -1, pend_lu = 0;  // the tile whose P V is still to issue
+      bool pend_first = false;
+      // P_g V_g accumulated into O once P_g is written (and O rescaled where
+      // its base moved); a unit's first tile starts O afresh, after the
+      // softmax has read the previous unit's
+      auto pv = [&]() -> bool {
+        if (!mbar_wait(&p_full[pend & 1], (pend >> 1) & 1, kWaitLimit, &abort_flag)) return false;
+        if (pend_first && pend_lu > 0 && !mbar_wait(&o_empty, (pend_lu - 1) & 1, kWaitLimit, &abort_flag)) return false;
+        tc_fence_after();
+        const uint32_t sv = sKV + (pend % kTcStages) * 2 * kTcTileBytes + kTcTileBytes;
+        const uint32_t p = tmem + (pend & 1) * 64;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)  // keys in steps of 16: 8 columns of P
+          mma_f16_ts(tmem + 128, p + ks * 8, umma_desc_sw128(sv + ks * 16 * 128, kTcTileBytes, 1024), kIdO,
+                     (!pend_first || ks > 0) ? 1u : 0u);
+        tc_commit(&o_full);
+        tc_commit(&kv_empty[pend % kTcStages]);
+        return true;
+      };
+      for (; more && ok; advance()) {
+        if (s.t0 >= s.t1) continue;
+        if (!mbar_wait(&q_full, lu & 1, kWaitLimit, &abort_flag)) {
+          fail();
+          break;
+        }
+        for (int j = s.t0; j < s.t1; ++j, ++g) {
+          // S_g over P_{g-2}, whose P V has completed
+          const int st = g % kTcStages;
+          if (!mbar_wait(&kv_full[st], (g / kTcStages) & 1, kWaitLimit, &abort_flag) ||
+              (g >= 2 && !mbar_wait(&o_full, (g - 2) & 1, kWaitLimit, &abort_flag))) {
+            fail();
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sk = sKV + st * 2 * kTcTileBytes;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)  // head dim in steps of 16
+            mma_f16(tmem + (g & 1) * 64, umma_desc_sw128(sQ + ks * 32, 16, 1024),
+                    umma_desc_sw128(sk + ks * 32, 16, 1024), kIdS, ks > 0 ? 1u : 0u);
+          any = true;
+          tc_commit(&s_full[g & 1]);
+          if (j == s.t1 - 1) tc_commit(&q_empty);  // the unit's last S: Q may be replaced
+          if (pend >= 0 && !pv()) {
+            fail();
+            ok = false;
+            break;
+          }
+          pend = g;
+          pend_first = j == s.t0;
+          pend_lu = lu;
+        }
+        ++lu;
+      }
+      if (ok && pend >= 0 && !pv()) fail();
+      if (any) {  // every issued MMA completes before TMEM is released (also after an abort)
+        tc_commit(&drain_bar);
+        uint64_t deadline = 0;
+        if (!mbar_wait_deadline(&drain_bar, 0, &deadline, kWaitLimit)) fail();
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax: one query row per thread
+    const int q4 = warp & 3;  // TMEM lane quarter
+    const int r = q4 * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+    constexpr float kRebase = 8.0f;  // log2 of the largest P kept without rescaling
+    Meta* meta = reinterpret_cast<Meta*>(a.ws + 2 * (int64_t)gridDim.x * part_floats(kTcRows));
+    bool open_unit = false, ok = true;
+    int g = 0;
+    for (; more && ok; advance()) {
+      const bool valid = r < s.rows;
+      const bool warp_valid = q4 * 32 < s.rows;  // uniform: some row of this warp is the unit's
+      const int tok = r / a.n_rep;
+      const int seen = min(s.first_pos + tok, s.keys - 1);  // the last key this row sees
+      float m = -INFINITY, l = 0.0f;                        // m: the base of P (log2 units)
+      for (int j = s.t0; j < s.t1; ++j, ++g) {
+        const int sb = g & 1;
+        if (!mbar_wait(&s_full[sb], (g >> 1) & 1, kWaitLimit, &abort_flag)) {
+          fail();
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int k0 = j * kTcTK;
+        if (s.keys - k0 < kTcTK) {
+          // values behind the last key hold whatever the page or ring held: a
+          // NaN there would survive its zero weight
+          const int st = g % kTcStages;
+          mbar_wait(&kv_full[st], (g / kTcStages) & 1, kWaitLimit, &abort_flag);  // (landed: S_g has read K)
+          const uint32_t sv = sKV + st * 2 * kTcTileBytes + kTcTileBytes;
+          for (int i = (s.keys - k0) * 8 + (int)threadIdx.x - 64; i < kTcTK * 8; i += 128)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + i * 16), "r"(0) : "memory");
+          fence_proxy_async_smem();
+        }
+        if (warp_valid) {
+          uint32_t sv[64];
+          tmem_ld_32x32b_x32(tmem + sb * 64 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
+          tmem_ld_32x32b_x32(tmem + sb * 64 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+          tmem_ld_wait();
+          float p[64], mx8[8];
+          // raw scores (the scale is positive: their maximum scales to the scaled ones')
+          const bool whole = __all_sync(0xffffffffu, !valid || k0 + kTcTK - 1 <= seen);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mx8[i] = -INFINITY;
+          if (whole) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c) {
+              p[c] = __uint_as_float(sv[c]);
+              mx8[c & 7] = fmaxf(mx8[c & 7], p[c]);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 64; ++c) {
+              p[c] = k0 + c <= seen ? __uint_as_float(sv[c]) : -INFINITY;
+              mx8[c & 7] = fmaxf(mx8[c & 7], p[c]);
+            }
+          }
+          const float mxr = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                                  fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+          const float mn = fmaxf(m, mxr * a.scale_log2);
+          const bool first = j == s.t0;
+          // rows past the unit's hold leftovers: they have no say
+          const bool rebase = first || __any_sync(0xffffffffu, valid && mn > m + kRebase);
+          float alpha = 1.0f;
+          if (rebase) {
+            alpha = m == -INFINITY ? 0.0f : ex2_approx(m - mn);
+            m = mn;
+          }
+          const float base = m == -INFINITY ? 0.0f : m;
+          float rs8[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) rs8[i] = 0.0f;
+#pragma unroll
+          for (int c = 0; c < 64; ++c) {  // P = exp2(S * scale - base): one FMA and one exponential
+            p[c] = ex2_approx(fmaf(p[c], a.scale_log2, -base));
+            rs8[c & 7] += p[c];
+          }
+          l = l * alpha + (((rs8[0] + rs8[1]) + (rs8[2] + rs8[3])) + ((rs8[4] + rs8[5]) + (rs8[6] + rs8[7])));
+          uint32_t pk[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) pk[c] = pack2(p[2 * c], p[2 * c + 1]);
+          tmem_st_32x32b_x32(tmem + sb * 64 + lane_off, pk);
+          // P_{g-1} V is in O (waited for in every tile: the barrier's parity
+          // tells neighbouring phases apart, no more)
+          if (!first && !mbar_wait(&o_full, (g - 1) & 1, kWaitLimit, &abort_flag)) {
+            fail();
+            ok = false;
+            break;
+          }
+          if (rebase && !first) {  // rescale O's rows to the new bases before P_g V adds to them
+            tc_fence_after();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t ov[32];
+              tmem_ld_32x32b_x32(tmem + 128 + h * 32 + lane_off, ov);
+              tmem_ld_wait();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+              tmem_st_32x32b_x32(tmem + 128 + h * 32 + lane_off, ov);
+            }
+          }
+          tmem_st_wait();
+        } else if (j > s.t0 && !mbar_wait(&o_full, (g - 1) & 1, kWaitLimit, &abort_flag)) {
+          fail();
+          ok = false;
+          break;
+        }
+        tc_fence_before();
+        mbar_arrive(&p_full[sb]);
+      }
+      if (!ok) break;
+      uint32_t ov[64];
+      if (s.t0 < s.t1) {  // the unit's last P V, then O: read and released for the next unit
+        if (!mbar_wait(&o_full, (g - 1) & 1, kWaitLimit, &abort_flag)) {
+          fail();
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (warp_valid) {
+          tmem_ld_32x32b_x32(tmem + 128 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[0]));
+          tmem_ld_32x32b_x32(tmem + 128 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[32]));
+          tmem_ld_wait();
+        }
+        tc_fence_before();
+        mbar_arrive(&o_empty);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) ov[c] = 0u;
+      }
+      if (valid && s.starts && s.ends) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+        bf16* op = a.out + (int64_t)(s.token + tok) * a.ld_out + (s.kvh * a.n_rep + r - tok * a.n_rep) * kHD;
+#pragma unroll
+        for (int c8 = 0; c8 < 8; ++c8) {
+          uint4 x;
+          x.x = pack2(__uint_as_float(ov[c8 * 8 + 0]) * inv, __uint_as_float(ov[c8 * 8 + 1]) * inv);
+          x.y = pack2(__uint_as_float(ov[c8 * 8 + 2]) * inv, __uint_as_float(ov[c8 * 8 + 3]) * inv);
+          x.z = pack2(__uint_as_float(ov[c8 * 8 + 4]) * inv, __uint_as_float(ov[c8 * 8 + 5]) * inv);
+          x.w = pack2(__uint_as_float(ov[c8 * 8 + 6]) * inv, __uint_as_float(ov[c8 * 8 + 7]) * inv);
+          *reinterpret_cast<uint4*>(op + c8 * 8) = x;
+        }
+      } else if (valid) {
+        float* part = a.ws + (2 * (int64_t)blockIdx.x + (s.starts ? 1 : 0)) * part_floats(kTcRows);
+#pragma unroll
+        for (int c4 = 0; c4 < 16; ++c4)
+          *reinterpret_cast<uint4*>(part + r * kHD + c4 * 4) = *reinterpret_cast<const uint4*>(&ov[c4 * 4]);
+        part[kTcRows * kHD + r] = m;
+        part[kTcRows * kHD + kTcRows + r] = l;
+      }
+      if (s.starts && !s.ends) {
+        open_unit = true;
+        if (threadIdx.x == 64) meta[blockIdx.x] = Meta{s.last, s.token, s.rows, s.kvh};
+      }
+    }
+    if (!open_unit && threadIdx.x == 64) meta[blockIdx.x].last = -1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
   }
 }
 
@@ -734,6 +1152,29 @@ int page_map(CUtensorMap* map, const void* p, int64_t n_pages, int64_t heads, in
   return XB_OK;
 }
 
+// Q as [tokens][n_head][64]; a box is the rows of one unit: n_rep heads of tpt tokens.
+int query_map(CUtensorMap* map, const void* q, int64_t tokens, int64_t heads, int64_t ld, int n_rep, int tpt,
+              const char* what, char* err, size_t errlen) {
+  EncodeTiledFn enc = encoder();
+  if (!enc) {
+    set_err(err, errlen, "%s: cuTensorMapEncodeTiled unavailable", what);
+    return XB_ERR_CUDA;
+  }
+  cuuint64_t dims[3] = {(cuuint64_t)kHD, (cuuint64_t)heads, (cuuint64_t)tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)kHD * 2, (cuuint64_t)ld * 2};
+  cuuint32_t box[3] = {(cuuint32_t)kHD, (cuuint32_t)n_rep, (cuuint32_t)tpt};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_err(err, errlen, "%s: cuTensorMapEncodeTiled failed (%d) for q [%lld][%lld][64]", what, (int)r,
+            (long long)tokens, (long long)heads);
+    return XB_ERR_CUDA;
+  }
+  return XB_OK;
+}
+
 // Addresses of the two status words on the current device.
 int status_words(int** bad, int** status, const char* what, char* err, size_t errlen) {
   if (cudaGetSymbolAddress((void**)bad, g_bad_page) != cudaSuccess ||
@@ -768,6 +1209,13 @@ int check_pages(int64_t n_pages, int64_t page_size, int64_t kv_heads, int64_t ba
     return XB_ERR_UNSUPPORTED;
   }
   return XB_OK;
+}
+
+// Which attention kernel: the mma.sync one while the batch's rows per (sequence,
+// KV head) fill at most one of its 16-row tiles on average, so K and V are
+// read about once; the host knows this much without the lengths.
+bool few_rows(int64_t tokens, int64_t batch, int64_t n_rep) {
+  return n_rep <= kFewRows && tokens * n_rep <= kFewRows * batch;
 }
 
 template <int N>
@@ -946,7 +1394,8 @@ extern "C" int xb_paged_attention_workspace_size(int64_t tokens, int64_t batch, 
   }
   int sms = 148;
   xb::sm_count(&sms);
-  *bytes = (size_t)sms * (2 * part_floats(kFewRows) * sizeof(float) + sizeof(Meta));
+  const bool few = few_rows(tokens, batch, n_head / n_kv_head);
+  *bytes = (size_t)(few ? sms : 2 * sms) * (2 * part_floats(few ? kFewRows : kTcRows) * sizeof(float) + sizeof(Meta));
   return XB_OK;
 }
 
@@ -971,8 +1420,8 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
     return XB_ERR_UNSUPPORTED;
   }
   const int n_rep = (int)(n_head / n_kv_head);
-  if (n_rep > 16) {
-    set_err(err, errlen, "%s: %d query heads per KV head not supported (1..16)", what, n_rep);
+  if (n_rep > kTcRows) {
+    set_err(err, errlen, "%s: %d query heads per KV head not supported (1..128)", what, n_rep);
     return XB_ERR_UNSUPPORTED;
   }
   if (!(scale > 0.0f)) {
@@ -1018,24 +1467,31 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
   a.B = (int)batch;
   a.KVH = (int)n_kv_head;
   a.n_rep = n_rep;
-  a.tpt = kFewRows / n_rep;
   a.page_size = (int)page_size;
   a.max_pages = (int)max_pages;
   a.n_pages = (int)n_pages;
-  a.min_share = 128;
   a.scale_log2 = scale * 1.4426950408889634f;
   rc = status_words(&a.bad, &a.status, what, err, errlen);
   if (rc) return rc;
+  const bool few = few_rows(tokens, batch, n_rep);
+  const int rows = few ? kFewRows : kTcRows, tile = few ? kTK : kTcTK;
+  a.tpt = rows / n_rep;
+  a.over = 96;
+  a.snap = few ? 64 : 128;
+  a.min_share = few ? 256 : 512;  // at least over + 2 snap: no piece may lie between two moved cuts
   int box = 8;  // rows of one load: the largest power of two that divides a page, at most a tile
-  while (box < kTK && page_size % (2 * box) == 0) box *= 2;
+  while (box < tile && page_size % (2 * box) == 0) box *= 2;
   a.box_rows = box;
-  KvMaps maps;
+  TcMaps maps;
   memset(&maps, 0, sizeof(maps));
   rc = page_map(&maps.k, k_pages, n_pages, n_kv_head, page_size, k_page, k_head, k_row, box, what, err, errlen);
   if (!rc) rc = page_map(&maps.v, v_pages, n_pages, n_kv_head, page_size, v_page, v_head, v_row, box, what, err, errlen);
+  if (!rc && !few) rc = query_map(&maps.q, q, tokens, n_head, ld_q, n_rep, a.tpt, what, err, errlen);
   if (rc) return rc;
-  cudaError_t e = xb::once_per_device(reinterpret_cast<const void*>(paged_attn_few_kernel), xb::kOnceSmem, [](int*) {
-    return cudaFuncSetAttribute(paged_attn_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+  const void* kernel = few ? reinterpret_cast<const void*>(paged_attn_few_kernel)
+                           : reinterpret_cast<const void*>(paged_attn_tc_kernel);
+  cudaError_t e = xb::once_per_device(kernel, xb::kOnceSmem, [&](int*) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, few ? kFewSmem : kTcSmem);
   });
   if (e != cudaSuccess) {
     set_err(err, errlen, "%s: kernel setup: %s", what, cudaGetErrorString(e));
@@ -1043,9 +1499,18 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
   }
   int sms = 148;
   xb::sm_count(&sms);
+  const int ctas = few ? sms : 2 * sms;
   cudaStream_t s = (cudaStream_t)stream;
-  e = launch_k(paged_attn_few_kernel, (unsigned)sms, kWarps * 32, kFewSmem, s, maps, a);
-  if (e == cudaSuccess) e = launch_k(paged_attn_join_kernel<kFewRows>, (unsigned)sms, 256, 0, s, a, sms);
+  if (few) {
+    KvMaps kv;
+    kv.k = maps.k;
+    kv.v = maps.v;
+    e = launch_k(paged_attn_few_kernel, (unsigned)ctas, kWarps * 32, kFewSmem, s, kv, a);
+    if (e == cudaSuccess) e = launch_k(paged_attn_join_kernel<kFewRows>, (unsigned)ctas, 256, 0, s, a, ctas);
+  } else {
+    e = launch_k(paged_attn_tc_kernel, (unsigned)ctas, kTcThreads, kTcSmem, s, maps, a);
+    if (e == cudaSuccess) e = launch_k(paged_attn_join_kernel<kTcRows>, (unsigned)ctas, 256, 0, s, a, ctas);
+  }
   if (e != cudaSuccess) {
     set_err(err, errlen, "%s: %s", what, cudaGetErrorString(e));
     return XB_ERR_CUDA;
