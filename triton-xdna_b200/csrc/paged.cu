@@ -227,32 +227,34 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs& a, int b) {
   return q;
 }
 
-// One CTA's walk over its piece [lo, hi) of the line.
+// A walk over one piece [lo, hi) of the line.
 struct Walk {
   int64_t lo, hi, share;
   int64_t u0;  // where the current unit starts
   int b, kvh, j;
+  Seq q;
 };
 
-// The CTA's part of one unit.
+// The part of one unit that belongs to a piece.
 struct Segment {
   int b, kvh;
-  int token, rows;    // first packed token and rows of the query tile
-  int first_pos;      // position of the tile's first token (may be negative)
-  int keys;           // keys the unit's last token sees; 0 when none of its tokens sees any
-  int t0, t1;         // key tiles of this part
-  int last;           // the CTA in which the unit ends
-  bool starts, ends;  // the unit starts / ends in this CTA
-  int64_t next;       // where the next unit starts
+  int token, rows;   // first packed token and rows of the query tile
+  int first_pos;     // position of the tile's first token (may be negative)
+  int keys;          // keys the unit's last token sees; 0 when none of its tokens sees any
+  int t0, t1;        // key tiles of this part
+  int starts, ends;  // the unit starts / ends in this piece
 };
 
-// Every thread of the block calls this; `found` is shared.  False: no work for this CTA.
-template <int THREADS>
-__device__ __forceinline__ bool find_piece(const AttnArgs& a, Walk& w, int64_t (*warp_sum)[THREADS / 32],
-                                           int64_t* found, int ctas, int cta) {
+// Weight of the whole line and, for the piece that starts at `first` + i times
+// the share (i < N), the sequence that holds its start: one scan each.  Every
+// thread of the block calls this; sums and found[N][2] are shared.  Returns
+// the share; found[i][0] < 0: piece i is empty.
+template <int THREADS, int N>
+__device__ __forceinline__ int64_t find_pieces(const AttnArgs& a, int64_t pieces, int64_t first,
+                                               int64_t (*sums)[THREADS / 32], int64_t (*found)[2], int64_t* total_out) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int64_t total = 0;
-  // pass 0: the whole line's weight; pass 1: the sequence that holds `lo`
+  if (threadIdx.x < N) found[threadIdx.x][0] = -1;
+  int64_t total = 0, share = 0;
   for (int pass = 0; pass < 2; ++pass) {
     int64_t run = 0;
     for (int b0 = 0; b0 < a.B; b0 += THREADS) {
@@ -265,20 +267,24 @@ __device__ __forceinline__ bool find_piece(const AttnArgs& a, Walk& w, int64_t (
         if (lane >= o) s += v;
       }
       const int buf = (b0 / THREADS) & 1;
-      if (lane == 31) warp_sum[buf][warp] = s;
+      if (lane == 31) sums[buf][warp] = s;
       __syncthreads();
       int64_t before = run, all = run;
 #pragma unroll
       for (int i = 0; i < THREADS / 32; ++i) {
-        const int64_t v = warp_sum[buf][i];
+        const int64_t v = sums[buf][i];
         if (i < warp) before += v;
         all += v;
       }
-      if (pass == 1) {
-        const int64_t excl = before + s - c;
-        if (c > 0 && excl <= w.lo && w.lo < excl + c) {
-          found[0] = b;
-          found[1] = excl;
+      if (pass == 1 && c > 0) {
+        const int64_t e = before + s - c;  // this sequence's start
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int64_t lo = (first + i) * share;
+          if (e <= lo && lo < e + c) {
+            found[i][0] = b;
+            found[i][1] = e;
+          }
         }
       }
       run = all;
@@ -286,77 +292,94 @@ __device__ __forceinline__ bool find_piece(const AttnArgs& a, Walk& w, int64_t (
     __syncthreads();
     if (pass == 0) {
       total = run;
-      w.share = (total + ctas - 1) / ctas;
-      if (w.share < a.min_share) w.share = a.min_share;
-      w.lo = (int64_t)cta * w.share;
-      w.hi = w.lo + w.share < total ? w.lo + w.share : total;
-      if (w.lo >= total) return false;  // the same for every thread of the CTA
+      share = (total + pieces - 1) / pieces;
+      if (share < a.min_share) share = a.min_share;
     }
   }
+  *total_out = total;
+  return share;
+}
+
+// Places a walk at piece `piece`'s start, inside sequence found[0] that begins at found[1].
+__device__ __forceinline__ void place(const AttnArgs& a, Walk& w, int64_t piece, int64_t share, int64_t total,
+                                      const int64_t* found) {
+  w.share = share;
+  w.lo = piece * share;
+  w.hi = w.lo + share < total ? w.lo + share : total;
   w.b = (int)found[0];
-  const Seq q = load_seq(a, w.b);
-  const int64_t off = w.lo - found[1];
-  w.kvh = (int)(off / q.perh);
-  const int64_t in = off - w.kvh * q.perh;
-  int lo = 0, hi = q.nt - 1;  // the last tile j with cum(j) <= in
+  w.q = load_seq(a, w.b);
+  int64_t in = w.lo - found[1];
+  w.kvh = 0;
+  if (in >= w.q.perh) {
+    w.kvh = (int)(in / w.q.perh);
+    in -= w.kvh * w.q.perh;
+  }
+  int lo = 0, hi = w.q.nt - 1;  // the last tile j with cum(j) <= in
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (cum_keys(a, q, mid) <= in) lo = mid;
+    if (cum_keys(a, w.q, mid) <= in) lo = mid;
     else hi = mid - 1;
   }
   w.j = lo;
-  w.u0 = found[1] + w.kvh * q.perh + cum_keys(a, q, lo);
-  return true;
+  w.u0 = found[1] + w.kvh * w.q.perh + cum_keys(a, w.q, lo);
 }
 
-// Steps to the next unit; false behind the last one.
-__device__ __forceinline__ bool next_unit(const AttnArgs& a, Walk& w, int64_t u0) {
-  w.u0 = u0;
-  if (u0 >= w.hi) return false;
-  if (++w.j < load_seq(a, w.b).nt) return true;
+__device__ __forceinline__ int64_t unit_weight(const AttnArgs& a, const Walk& w) {
+  return a.over + (w.q.base > 0 ? w.q.base : 0) + min(a.tpt * (w.j + 1), w.q.n);
+}
+
+// Steps to the next unit; false behind the piece's last one.
+__device__ __forceinline__ bool next_unit(const AttnArgs& a, Walk& w) {
+  w.u0 += unit_weight(a, w);
+  if (w.u0 >= w.hi) return false;
+  if (++w.j < w.q.nt) return true;
   w.j = 0;
   if (++w.kvh < a.KVH) return true;
   w.kvh = 0;
   do {
     if (++w.b >= a.B) return false;
-  } while (load_seq(a, w.b).n == 0);
+    w.q = load_seq(a, w.b);
+  } while (w.q.n == 0);
   return true;
 }
 
-// The part of the current unit that belongs to this CTA, stepping over one
-// whose cut was moved away; false when nothing is left.
+// The part of the current unit that belongs to this piece, stepping over a
+// unit whose cut was moved away; false when nothing is left.
 template <int TK>
 __device__ __forceinline__ bool segment(const AttnArgs& a, Walk& w, Segment& g) {
   for (;;) {
-    const Seq q = load_seq(a, w.b);
     const int done = w.j * a.tpt;
-    const int tokens = min(a.tpt, q.n - done);
-    const int keys = (int)max(q.base + done + tokens, (int64_t)0);
-    const int64_t ulen = a.over + (q.base > 0 ? q.base : 0) + done + tokens;
+    const int tokens = min(a.tpt, w.q.n - done);
+    const int keys = (int)max(w.q.base + done + tokens, (int64_t)0);
+    const int64_t ulen = unit_weight(a, w);
     const int64_t cut0 = w.lo - w.u0, cut1 = w.hi - w.u0;  // the piece's ends inside the unit
-    g.next = w.u0 + ulen;
     g.starts = cut0 < a.over + a.snap;
-    if (!g.starts && ulen - cut0 < a.snap) {  // only at the piece's start: the unit ended in the CTA before
-      if (!next_unit(a, w, g.next)) return false;
+    if (!g.starts && ulen - cut0 < a.snap) {  // only at the piece's start: the unit ended in the piece before
+      if (!next_unit(a, w)) return false;
       continue;
     }
-    if (cut1 < a.over + a.snap && cut1 < ulen) return false;  // the unit starts in the next CTA
+    if (cut1 < a.over + a.snap && cut1 < ulen) return false;  // the unit starts in the next piece
     g.ends = cut1 >= ulen || ulen - cut1 < a.snap;
     const int nk = (keys + TK - 1) / TK;
     g.t0 = g.starts ? 0 : min((int)((cut0 - a.over) / TK), nk);  // cuts fall on tile boundaries
     g.t1 = g.ends ? nk : min((int)((cut1 - a.over) / TK), nk);
-    // the CTA that holds the unit's last key, or the one before it if that cut was moved to the unit's end
-    int64_t last = (g.next - 1) / w.share;
-    if (last * w.share > w.u0 && g.next - last * w.share < a.snap) --last;
-    g.last = (int)last;
     g.b = w.b;
     g.kvh = w.kvh;
-    g.token = q.s0 + done;
+    g.token = w.q.s0 + done;
     g.rows = tokens * a.n_rep;
-    g.first_pos = (int)(q.base + done);
+    g.first_pos = (int)(w.q.base + done);
     g.keys = keys;
     return true;
   }
+}
+
+// The piece in which the current unit ends: the one that holds its last key,
+// or the one before it if that cut was moved to the unit's end.
+__device__ __forceinline__ int64_t unit_last(const AttnArgs& a, const Walk& w) {
+  const int64_t end = w.u0 + unit_weight(a, w);
+  int64_t last = (end - 1) / w.share;
+  if (last * w.share > w.u0 && end - last * w.share < a.snap) --last;
+  return last;
 }
 
 // ----------------------------------------------------------------------------- attention: few rows (mma.sync)
@@ -364,20 +387,24 @@ __device__ __forceinline__ bool segment(const AttnArgs& a, Walk& w, Segment& g) 
 // For batches whose sequences bring few tokens each (decoding, verification
 // of drafted tokens): at most 16 rows per unit, the rows of an mma.sync
 // m16n8k16 tile (rows past n_rep * tokens are zero), so the kernel is bound by
-// reading K and V.  Each of the CTA's warps takes every kWarps-th 32-key tile
-// of the segment and is on its own: lanes issue the TMA loads of their tile's
-// page rows (128-byte swizzle) into one of the warp's three buffers, the warp
-// waits on that buffer's mbarrier, and keeps an online softmax (running max
-// and sum in fp32, P rounded to bf16 for P V as in the contiguous kernels).
-// 8 warps x 3 buffers x 8 KB keep up to 192 KB per SM in flight.  The warps'
-// (O, max, sum) meet in shared memory in warp order.
+// reading K and V.  Every warp of the grid has a piece of the line of its own
+// and runs through it alone: its lanes issue the TMA loads of a 32-key tile's
+// page rows (128-byte swizzle) into one of the warp's two buffers, the next
+// unit's tiles while the present one is computed, and the warp keeps an online
+// softmax (running max and sum in fp32, P rounded to bf16 for P V as in the
+// contiguous kernels).  8 warps x 2 buffers x 8 KB keep up to 128 KB per SM in
+// flight.  A unit inside one warp's piece goes straight to the output; parts
+// of one that spans warps of the CTA meet in shared memory after the CTA's
+// only barrier, and what spans CTAs goes on to the joining kernel.
 constexpr int kHD = 64;
-constexpr int kWarps = 8, kBufs = 3, kTK = 32;
-constexpr int kTileBytes = kTK * kHD * 2;               // one K or V tile
-constexpr int kRingBytes = kWarps * kBufs * 2 * kTileBytes;
-constexpr int kMergeBytes = kWarps * 16 * kHD * 4;
-constexpr int kFewSmem = kRingBytes + kMergeBytes + 1024;
+constexpr int kWarps = 8, kBufs = 2, kTK = 32;
+constexpr int kTileBytes = kTK * kHD * 2;  // one K or V tile
+constexpr int kWarpRing = kBufs * 2 * kTileBytes;
 constexpr int kFewRows = 16;
+constexpr int kPartLd = kHD + 8;  // row pitch of a partial in shared memory: conflict-free 8-byte stores
+constexpr int kHeadBytes = kFewRows * kPartLd * 4;
+constexpr int kFewSmem = kWarps * (kWarpRing + kHeadBytes) + 1024;
+static_assert(kHeadBytes <= kWarpRing, "a warp's last partial goes into its own ring");
 
 struct alignas(64) KvMaps {
   CUtensorMap k, v;  // [n_pages][KVH][page][64], box {64, box_rows, 1, 1}
@@ -420,253 +447,312 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 // floats of one partial: O [rows][64], then max [rows], then sum [rows]
 __host__ __device__ constexpr int64_t part_floats(int rows) { return (int64_t)rows * (kHD + 2); }
 
+// A warp's part of a unit that it does not cover alone.
+struct Part {
+  int token, rows, kvh;
+  int ends;   // the unit ends in this warp's piece
+  int last;   // (parts that start a unit) the piece in which it ends
+  int valid;
+};
+
+__device__ __forceinline__ void store_out4(const AttnArgs& a, int token, int kvh, int r, int d, float4 v) {
+  bf16* op = a.out + (int64_t)(token + r / a.n_rep) * a.ld_out + (kvh * a.n_rep + r % a.n_rep) * kHD + d;
+  uint2 pk;
+  pk.x = pack2(v.x, v.y);
+  pk.y = pack2(v.z, v.w);
+  *reinterpret_cast<uint2*>(op) = pk;
+}
+
 __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __grid_constant__ KvMaps maps,
                                                                         const AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kWarps][kBufs];
-  __shared__ int64_t warp_sum[2][kWarps];
-  __shared__ int64_t found[2];
-  __shared__ float wm[kWarps][16], wl[kWarps][16];
+  __shared__ int64_t sums[2][kWarps];
+  __shared__ int64_t found[kWarps][2];
+  __shared__ Part part[2][kWarps];  // [0]: of a unit that started before, [1]: of one that goes on
+  __shared__ float part_m[2][kWarps][kFewRows], part_l[2][kWarps][kFewRows];
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t base_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t ring = base_u32 + warp * (kBufs * 2 * kTileBytes);
-  float* red = reinterpret_cast<float*>(smem_raw + (base_u32 - smem_u32(smem_raw)) + kRingBytes);
-  if (lane == 0)
+  uint8_t* smem = smem_raw + (base_u32 - smem_u32(smem_raw));
+  const uint32_t ring = base_u32 + warp * kWarpRing;
+  // O of the two kinds of parts: the first beside the ring, the second, the
+  // last thing a warp does, in its ring
+  auto part_o = [&](int kind, int w_) -> float* {
+    return reinterpret_cast<float*>(kind == 0 ? smem + kWarps * kWarpRing + w_ * kHeadBytes : smem + w_ * kWarpRing);
+  };
+  if (lane == 0) {
     for (int i = 0; i < kBufs; ++i) mbar_init(&full[warp][i], 1);
+    mbar_fence_init();
+    part[0][warp].valid = part[1][warp].valid = 0;
+  }
   if (threadIdx.x == 0) {
     abort_flag = 0;
     prefetch_tmap(&maps.k);
     prefetch_tmap(&maps.v);
   }
-  mbar_fence_init();
-  __syncthreads();
   pdl_wait();
   pdl_trigger();
-
+  int64_t total;
+  const int64_t share = find_pieces<kWarps * 32, kWarps>(a, (int64_t)gridDim.x * kWarps, (int64_t)blockIdx.x * kWarps,
+                                                         sums, found, &total);
   Meta* meta = reinterpret_cast<Meta*>(a.ws + 2 * (int64_t)gridDim.x * part_floats(kFewRows));
-  Walk w;
-  if (!find_piece<kWarps * 32>(a, w, warp_sum, found, gridDim.x, blockIdx.x)) {
+  if (found[0][0] < 0) {  // no warp of this CTA has work
     if (threadIdx.x == 0) meta[blockIdx.x].last = -1;
     return;
   }
-  bool open_unit = false;
-  // tiles this warp has read / requested so far: buffer n % kBufs, parity (n / kBufs) & 1
-  uint32_t use = 0, issued = 0;
-  bool dead = false;  // a wait ran out: no more loads, the output is not valid
-  Segment s;
-  for (bool more = segment<kTK>(a, w, s); more; more = next_unit(a, w, s.next) && segment<kTK>(a, w, s)) {
+  if (found[warp][0] >= 0) {
     const int boxes = kTK / a.box_rows;
-    // lane 0 .. boxes - 1 load K rows, the next `boxes` lanes V rows of tile `tile` into buffer `buf`
-    auto issue = [&](int tile, uint32_t n) {
-      const uint32_t buf = n % kBufs;
-      const int k0 = tile * kTK;
-      const int have = min(kTK, s.keys - k0);
-      const int nb = (have + a.box_rows - 1) / a.box_rows;
+    const bool is_v = lane >= boxes;
+    const int box = is_v ? lane - boxes : lane;
+    const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+    // two walks over the piece: one requests tiles, one computes them
+    Walk wi, wc;
+    Segment si, sc;
+    place(a, wi, (int64_t)blockIdx.x * kWarps + warp, share, total, found[warp]);
+    wc = wi;
+    bool more = segment<kTK>(a, wi, si);
+    wc = wi;
+    sc = si;
+    bool more_i = more;
+    int ni = si.t0;  // next tile to request
+    uint32_t use = 0, issued = 0;  // tiles read / requested: buffer n % kBufs, parity (n / kBufs) & 1
+    bool dead = false;  // a wait ran out: no more loads, the output is not valid
+    auto settle = [&]() {  // the request walk on a tile, if any is left
+      while (more_i && ni >= si.t1) {
+        more_i = next_unit(a, wi) && segment<kTK>(a, wi, si);
+        ni = si.t0;
+      }
+    };
+    settle();
+    // lanes 0 .. boxes - 1 load K rows, the next `boxes` lanes V rows
+    auto request = [&]() {
+      const uint32_t buf = issued % kBufs;
+      const int k0 = ni * kTK;
+      const int nb = (min(kTK, si.keys - k0) + a.box_rows - 1) / a.box_rows;
       if (lane == 0) mbar_arrive_expect_tx(&full[warp][buf], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
       __syncwarp();
-      const int box = lane < boxes ? lane : lane - boxes;
       if (lane < 2 * boxes && box < nb) {
         const uint32_t key = (uint32_t)(k0 + box * a.box_rows);
         const uint32_t pi = key / (uint32_t)a.page_size;
-        int id = __ldg(a.table + s.b * a.ld_table + pi);
+        int id = __ldg(a.table + si.b * a.ld_table + pi);
         if (id < 0 || id >= a.n_pages) {  // reads as zeros: a coordinate past the pool
           atomicExch(a.bad, 1);
           id = a.n_pages;
         }
-        const bool is_v = lane >= boxes;
-        tma_load_4d(ring + buf * 2 * kTileBytes + (is_v ? kTileBytes : 0) + box * a.box_rows * kHD * 2,
-                    is_v ? &maps.v : &maps.k, &full[warp][buf], 0, (int)(key - pi * a.page_size), s.kvh, id);
+        tma_load_4d(ring + buf * 2 * kTileBytes + (is_v ? kTileBytes : 0) + box * a.box_rows * kHD * 2, map,
+                    &full[warp][buf], 0, (int)(key - pi * a.page_size), si.kvh, id);
       }
+      ++issued;
+      ++ni;
+      settle();
     };
-    issued = use;
-    int next = dead ? s.t1 : s.t0 + warp;  // next tile to issue
-    for (; next < s.t1 && issued < use + kBufs; next += kWarps) issue(next, issued++);
+    while (more_i && issued < kBufs) request();
 
-    uint32_t qa[4][4];
-    {
-      const int r0 = g, r1 = g + 8;
-      const bool ok0 = r0 < s.rows, ok1 = r1 < s.rows;
-      const bf16* p0 = a.q + (int64_t)(s.token + r0 / a.n_rep) * a.ld_q + (s.kvh * a.n_rep + r0 % a.n_rep) * kHD;
-      const bf16* p1 = a.q + (int64_t)(s.token + r1 / a.n_rep) * a.ld_q + (s.kvh * a.n_rep + r1 % a.n_rep) * kHD;
+    for (; more; more = next_unit(a, wc) && segment<kTK>(a, wc, sc)) {
+      uint32_t qa[4][4];
+      {
+        const int r0 = g, r1 = g + 8;
+        const bool ok0 = r0 < sc.rows, ok1 = r1 < sc.rows;
+        const bf16* p0 = a.q + (int64_t)(sc.token + r0 / a.n_rep) * a.ld_q + (sc.kvh * a.n_rep + r0 % a.n_rep) * kHD;
+        const bf16* p1 = a.q + (int64_t)(sc.token + r1 / a.n_rep) * a.ld_q + (sc.kvh * a.n_rep + r1 % a.n_rep) * kHD;
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const int c = kk * 16 + 2 * t;
-        qa[kk][0] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c) : 0u;
-        qa[kk][1] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c) : 0u;
-        qa[kk][2] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c + 8) : 0u;
-        qa[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c + 8) : 0u;
-      }
-    }
-    // the last key each of this thread's rows sees
-    const int pos0 = min(s.first_pos + g / a.n_rep, s.keys - 1), pos1 = min(s.first_pos + (g + 8) / a.n_rep, s.keys - 1);
-    float o[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-    for (int tile = s.t0 + warp; tile < s.t1 && !dead; tile += kWarps) {
-      const uint32_t buf = use % kBufs;
-      const bool landed = mbar_wait(&full[warp][buf], (use / kBufs) & 1, kWaitLimit, &abort_flag);
-      if (__any_sync(0xffffffffu, !landed)) {
-        atomicExch(a.status, XB_ERR_TIMEOUT);
-        abort_flag = 1;
-        dead = true;
-        break;
-      }
-      const int k0 = tile * kTK;
-      const uint32_t sk = ring + buf * 2 * kTileBytes, sv = sk + kTileBytes;
-      const int have = min(kTK, s.keys - k0);
-      if (have < kTK) {
-        // values behind the last key hold whatever the page or buffer held: a
-        // NaN there would survive its zero weight
-        for (int i = have * 8 + lane; i < kTK * 8; i += 32)
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + i * 16), "r"(0) : "memory");
-        __syncwarp();
-      }
-      float sc[4][4];
-#pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {  // dims 32 h .. 32 h + 31: four 16-byte chunks of the key rows
-          const int r = nt * 8 + (lane & 7), c = 4 * h + (lane >> 3);
-          uint32_t kb[4];
-          ldsm4(kb, sk + r * 128 + ((c ^ (r & 7)) << 4));
-          mma_16816(sc[nt], qa[2 * h], kb[0], kb[1]);
-          mma_16816(sc[nt], qa[2 * h + 1], kb[2], kb[3]);
+        for (int kk = 0; kk < 4; ++kk) {
+          const int c = kk * 16 + 2 * t;
+          qa[kk][0] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c) : 0u;
+          qa[kk][1] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c) : 0u;
+          qa[kk][2] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c + 8) : 0u;
+          qa[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c + 8) : 0u;
         }
       }
-      float mx0 = -INFINITY, mx1 = -INFINITY;
+      // the last key each of this thread's rows sees
+      const int pos0 = min(sc.first_pos + g / a.n_rep, sc.keys - 1);
+      const int pos1 = min(sc.first_pos + (g + 8) / a.n_rep, sc.keys - 1);
+      float o[8][4];
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = k0 + nt * 8 + 2 * t + (e & 1);
-          sc[nt][e] = key <= (e < 2 ? pos0 : pos1) ? sc[nt][e] * a.scale_log2 : -INFINITY;
-          if (e < 2) mx0 = fmaxf(mx0, sc[nt][e]);
-          else mx1 = fmaxf(mx1, sc[nt][e]);
+      for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+      for (int tile = sc.t0; tile < sc.t1 && !dead; ++tile) {
+        const uint32_t buf = use % kBufs;
+        const bool landed = mbar_wait(&full[warp][buf], (use / kBufs) & 1, kWaitLimit, &abort_flag);
+        if (__any_sync(0xffffffffu, !landed)) {
+          atomicExch(a.status, XB_ERR_TIMEOUT);
+          abort_flag = 1;
+          dead = true;
+          break;
         }
+        const int k0 = tile * kTK;
+        const uint32_t sk = ring + buf * 2 * kTileBytes, sv = sk + kTileBytes;
+        const int have = min(kTK, sc.keys - k0);
+        if (have < kTK) {
+          // values behind the last key hold whatever the page or buffer held: a
+          // NaN there would survive its zero weight
+          for (int i = have * 8 + lane; i < kTK * 8; i += 32)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + i * 16), "r"(0) : "memory");
+          fence_proxy_async_smem();  // before a later TMA write to the buffer
+          __syncwarp();
+        }
+        float s[4][4];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+          s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // dims 32 h .. 32 h + 31: four 16-byte chunks of the key rows
+            const int r = nt * 8 + (lane & 7), c = 4 * h + (lane >> 3);
+            uint32_t kb[4];
+            ldsm4(kb, sk + r * 128 + ((c ^ (r & 7)) << 4));
+            mma_16816(s[nt], qa[2 * h], kb[0], kb[1]);
+            mma_16816(s[nt], qa[2 * h + 1], kb[2], kb[3]);
+          }
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = k0 + nt * 8 + 2 * t + (e & 1);
+            s[nt][e] = key <= (e < 2 ? pos0 : pos1) ? s[nt][e] * a.scale_log2 : -INFINITY;
+            if (e < 2) mx0 = fmaxf(mx0, s[nt][e]);
+            else mx1 = fmaxf(mx1, s[nt][e]);
+          }
+#pragma unroll
+        for (int o_ = 1; o_ <= 2; o_ <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o_));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o_));
+        }
+        const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
+        const float base0 = mn0 == -INFINITY ? 0.0f : mn0, base1 = mn1 == -INFINITY ? 0.0f : mn1;
+        const float al0 = ex2_approx(m0 - base0), al1 = ex2_approx(m1 - base1);
+        m0 = mn0;
+        m1 = mn1;
+        float rs0 = 0.0f, rs1 = 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+          s[nt][0] = ex2_approx(s[nt][0] - base0);
+          s[nt][1] = ex2_approx(s[nt][1] - base0);
+          s[nt][2] = ex2_approx(s[nt][2] - base1);
+          s[nt][3] = ex2_approx(s[nt][3] - base1);
+          rs0 += s[nt][0] + s[nt][1];
+          rs1 += s[nt][2] + s[nt][3];
+        }
+        l0 = l0 * al0 + rs0;
+        l1 = l1 * al1 + rs1;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+          o[dt][0] *= al0;
+          o[dt][1] *= al0;
+          o[dt][2] *= al1;
+          o[dt][3] *= al1;
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          uint32_t pa[4];
+          pa[0] = pack2(s[2 * kk][0], s[2 * kk][1]);
+          pa[1] = pack2(s[2 * kk][2], s[2 * kk][3]);
+          pa[2] = pack2(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+          pa[3] = pack2(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+#pragma unroll
+          for (int dt = 0; dt < 8; dt += 2) {
+            const int mi = lane >> 3, r = kk * 16 + (mi & 1) * 8 + (lane & 7), c = dt + (mi >> 1);
+            uint32_t vb[4];
+            ldsm4_t(vb, sv + r * 128 + ((c ^ (r & 7)) << 4));
+            mma_16816(o[dt], pa, vb[0], vb[1]);
+            mma_16816(o[dt + 1], pa, vb[2], vb[3]);
+          }
+        }
+        ++use;
+        __syncwarp();  // the buffer is read: it takes a tile further on
+        if (more_i) request();
+      }
 #pragma unroll
       for (int o_ = 1; o_ <= 2; o_ <<= 1) {
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o_));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o_));
+        l0 += __shfl_xor_sync(0xffffffffu, l0, o_);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, o_);
       }
-      const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
-      const float base0 = mn0 == -INFINITY ? 0.0f : mn0, base1 = mn1 == -INFINITY ? 0.0f : mn1;
-      const float al0 = ex2_approx(m0 - base0), al1 = ex2_approx(m1 - base1);
-      m0 = mn0;
-      m1 = mn1;
-      float rs0 = 0.0f, rs1 = 0.0f;
+      if (sc.starts && sc.ends) {
+        const float i0 = l0 == 0.0f ? 0.0f : 1.0f / l0, i1 = l1 == 0.0f ? 0.0f : 1.0f / l1;  // no key: zeros
+        bf16* p0 = a.out + (int64_t)(sc.token + g / a.n_rep) * a.ld_out + (sc.kvh * a.n_rep + g % a.n_rep) * kHD;
+        bf16* p1 = a.out + (int64_t)(sc.token + (g + 8) / a.n_rep) * a.ld_out +
+                   (sc.kvh * a.n_rep + (g + 8) % a.n_rep) * kHD;
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        sc[nt][0] = ex2_approx(sc[nt][0] - base0);
-        sc[nt][1] = ex2_approx(sc[nt][1] - base0);
-        sc[nt][2] = ex2_approx(sc[nt][2] - base1);
-        sc[nt][3] = ex2_approx(sc[nt][3] - base1);
-        rs0 += sc[nt][0] + sc[nt][1];
-        rs1 += sc[nt][2] + sc[nt][3];
-      }
-      l0 = l0 * al0 + rs0;
-      l1 = l1 * al1 + rs1;
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) {
-        o[dt][0] *= al0;
-        o[dt][1] *= al0;
-        o[dt][2] *= al1;
-        o[dt][3] *= al1;
-      }
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        uint32_t pa[4];
-        pa[0] = pack2(sc[2 * kk][0], sc[2 * kk][1]);
-        pa[1] = pack2(sc[2 * kk][2], sc[2 * kk][3]);
-        pa[2] = pack2(sc[2 * kk + 1][0], sc[2 * kk + 1][1]);
-        pa[3] = pack2(sc[2 * kk + 1][2], sc[2 * kk + 1][3]);
-#pragma unroll
-        for (int dt = 0; dt < 8; dt += 2) {
-          const int mi = lane >> 3, r = kk * 16 + (mi & 1) * 8 + (lane & 7), c = dt + (mi >> 1);
-          uint32_t vb[4];
-          ldsm4_t(vb, sv + r * 128 + ((c ^ (r & 7)) << 4));
-          mma_16816(o[dt], pa, vb[0], vb[1]);
-          mma_16816(o[dt + 1], pa, vb[2], vb[3]);
+        for (int dt = 0; dt < 8; ++dt) {
+          const int d = dt * 8 + 2 * t;
+          if (g < sc.rows) *reinterpret_cast<uint32_t*>(p0 + d) = pack2(o[dt][0] * i0, o[dt][1] * i0);
+          if (g + 8 < sc.rows) *reinterpret_cast<uint32_t*>(p1 + d) = pack2(o[dt][2] * i1, o[dt][3] * i1);
         }
-      }
-      ++use;
-      __syncwarp();  // the buffer is read: it takes the warp's tile kBufs steps ahead
-      if (have < kTK) {  // the unit's last tile
-        fence_proxy_async_smem();  // the zeros, before a later unit's TMA write to the buffer
-      } else if (next < s.t1) {
-        issue(next, issued++);
-        next += kWarps;
-      }
-    }
+      } else {
+        const int kind = sc.starts ? 1 : 0;
+        float* po = part_o(kind, warp);
 #pragma unroll
-    for (int o_ = 1; o_ <= 2; o_ <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, o_);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, o_);
+        for (int dt = 0; dt < 8; ++dt) {
+          const int d = dt * 8 + 2 * t;
+          *reinterpret_cast<float2*>(po + g * kPartLd + d) = make_float2(o[dt][0], o[dt][1]);
+          *reinterpret_cast<float2*>(po + (g + 8) * kPartLd + d) = make_float2(o[dt][2], o[dt][3]);
+        }
+        if (t == 0) {
+          part_m[kind][warp][g] = m0;
+          part_m[kind][warp][g + 8] = m1;
+          part_l[kind][warp][g] = l0;
+          part_l[kind][warp][g + 8] = l1;
+        }
+        if (lane == 0)
+          part[kind][warp] = Part{sc.token, sc.rows, sc.kvh, sc.ends, kind ? (int)unit_last(a, wc) : 0, 1};
+      }
     }
-    __syncthreads();  // the previous segment's merge has been read
-    if (t == 0) {
-      wm[warp][g] = m0;
-      wm[warp][g + 8] = m1;
-      wl[warp][g] = l0;
-      wl[warp][g + 8] = l1;
+    if (dead) {  // loads still in flight land before the CTA's shared memory is given up
+      uint64_t deadline = 0;
+      for (; use < issued; ++use)
+        mbar_wait_deadline(&full[warp][use % kBufs], (use / kBufs) & 1, &deadline, kWaitLimit);
     }
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) {
-      const int d = dt * 8 + 2 * t;
-      *reinterpret_cast<float2*>(&red[(warp * 16 + g) * kHD + d]) = make_float2(o[dt][0], o[dt][1]);
-      *reinterpret_cast<float2*>(&red[(warp * 16 + g + 8) * kHD + d]) = make_float2(o[dt][2], o[dt][3]);
+  }
+  __syncthreads();
+  // Chains of parts: one that came in from the CTA before (its parts start with
+  // warp 0's first kind), and one from every warp whose piece starts a unit
+  // that goes on.  They go on through the first kind of the next warps until
+  // one ends the unit, or leave the CTA.
+  bool open_unit = false;
+  for (int c = -1; c < kWarps; ++c) {
+    const Part p = c < 0 ? part[0][0] : part[1][c];
+    if (!p.valid) continue;
+    int end = c < 0 ? 0 : c;  // last warp of the chain
+    bool ends = p.ends;
+    while (!ends && end + 1 < kWarps) ends = part[0][++end].ends;
+    const bool whole = c >= 0 && ends;
+    if (c >= 0 && !ends) {
+      open_unit = true;
+      if (threadIdx.x == 0) meta[blockIdx.x] = Meta{p.last / kWarps, p.token, p.rows, p.kvh};
     }
-    __syncthreads();
-    const bool whole = s.starts && s.ends;
-    float* part = a.ws + (2 * (int64_t)blockIdx.x + (s.starts ? 1 : 0)) * part_floats(kFewRows);
-    for (int i = threadIdx.x; i < s.rows * (kHD / 4); i += kWarps * 32) {
+    float* out_part = a.ws + (2 * (int64_t)blockIdx.x + (c < 0 ? 0 : 1)) * part_floats(kFewRows);
+    for (int i = threadIdx.x; i < p.rows * (kHD / 4); i += kWarps * 32) {
       const int r = i / (kHD / 4), d = (i % (kHD / 4)) * 4;
       float M = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) M = fmaxf(M, wm[k][r]);
+      for (int k = max(c, 0); k <= end; ++k) M = fmaxf(M, part_m[k == c][k][r]);
       const float base = M == -INFINITY ? 0.0f : M;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       float l = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        const float f = ex2_approx(wm[k][r] - base);
-        const float4 v = *reinterpret_cast<const float4*>(&red[(k * 16 + r) * kHD + d]);
+      for (int k = max(c, 0); k <= end; ++k) {
+        const float f = ex2_approx(part_m[k == c][k][r] - base);
+        const float4 v = *reinterpret_cast<const float4*>(part_o(k == c, k) + r * kPartLd + d);
         acc.x += v.x * f;
         acc.y += v.y * f;
         acc.z += v.z * f;
         acc.w += v.w * f;
-        l += wl[k][r] * f;
+        l += part_l[k == c][k][r] * f;
       }
       if (whole) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
-        bf16* op = a.out + (int64_t)(s.token + r / a.n_rep) * a.ld_out + (s.kvh * a.n_rep + r % a.n_rep) * kHD + d;
-        uint2 pk;
-        pk.x = pack2(acc.x * inv, acc.y * inv);
-        pk.y = pack2(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>(op) = pk;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        store_out4(a, p.token, p.kvh, r, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
       } else {
-        *reinterpret_cast<float4*>(part + r * kHD + d) = acc;
+        *reinterpret_cast<float4*>(out_part + r * kHD + d) = acc;
         if (d == 0) {
-          part[kFewRows * kHD + r] = M;
-          part[kFewRows * kHD + kFewRows + r] = l;
+          out_part[kFewRows * kHD + r] = M;
+          out_part[kFewRows * kHD + kFewRows + r] = l;
         }
       }
     }
-    if (s.starts && !s.ends) {
-      open_unit = true;
-      if (threadIdx.x == 0)
-        meta[blockIdx.x] = Meta{s.last, s.token, s.rows, s.kvh};
-    }
   }
   if (!open_unit && threadIdx.x == 0) meta[blockIdx.x].last = -1;
-  if (dead) {  // loads still in flight land before the CTA's shared memory is given up
-    uint64_t deadline = 0;
-    for (; use < issued; ++use)
-      mbar_wait_deadline(&full[warp][use % kBufs], (use / kBufs) & 1, &deadline, kWaitLimit);
-  }
 }
 
 // ----------------------------------------------------------------------------- attention: many rows (tcgen05)
@@ -674,8 +760,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
 // For batches whose sequences bring many tokens (prompts, chunks, mixed
 // steps): units of up to 128 rows (tpt = 128 / n_rep tokens), key tiles of 64.
 // Two persistent CTAs per SM, each walking its piece of the line:
-//   warp 0     loads each unit's Q and streams K / V page rows into a ring of
-//              five tiles (one lane per page piece, TMA, 128-byte swizzle);
+//   warp 0     walks the piece, tells the others its segments through a small
+//              ring, loads each unit's Q (two buffers) and streams K / V page
+//              rows into a ring of four tiles (one lane per page piece, TMA,
+//              128-byte swizzle);
 //   warp 1     issues S_g = Q K_g^T into one of two 64-column TMEM buffers and
 //              O += P_g V_g; P_g is the MMA's A operand straight from TMEM;
 //   warps 2-5  softmax, one query row per thread: scores from TMEM, bf16(P)
@@ -692,10 +780,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
 // bounded; a timeout sets the status word, drains what is in flight and ends.
 constexpr int kTcRows = 128;
 constexpr int kTcTK = 64;
-constexpr int kTcStages = 5;
+constexpr int kTcStages = 4;
+constexpr int kTcSegs = 4;  // segments published ahead
 constexpr int kTcQBytes = kTcRows * kHD * 2;
 constexpr int kTcTileBytes = kTcTK * kHD * 2;  // one K or V tile
-constexpr int kTcSmem = kTcQBytes + kTcStages * 2 * kTcTileBytes + 1024;
+constexpr int kTcSmem = 2 * kTcQBytes + kTcStages * 2 * kTcTileBytes + 1024;
 constexpr int kTcThreads = 192;
 
 struct alignas(64) TcMaps {
@@ -716,25 +805,31 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
 __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __grid_constant__ TcMaps maps,
                                                                       const AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full, q_empty, drain_bar, o_full, o_empty;
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], drain_bar, o_full, o_empty;
   __shared__ __align__(8) uint64_t s_full[2], p_full[2];
   __shared__ __align__(8) uint64_t kv_full[kTcStages], kv_empty[kTcStages];
-  __shared__ int64_t warp_sum[2][kTcThreads / 32];
-  __shared__ int64_t found[2];
+  __shared__ __align__(8) uint64_t seg_full[kTcSegs], seg_empty[kTcSegs];
+  __shared__ Segment segs[kTcSegs];  // rows == 0: the end
+  __shared__ int64_t sums[2][kTcThreads / 32];
+  __shared__ int64_t found[1][2];
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t sQ = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t sKV = sQ + kTcQBytes;
+  const uint32_t sKV = sQ + 2 * kTcQBytes;
 
   if (threadIdx.x == 0) {
-    mbar_init(&q_full, 1);
-    mbar_init(&q_empty, 1);
     mbar_init(&drain_bar, 1);
     mbar_init(&o_full, 1);     // one P V accumulated into O
     mbar_init(&o_empty, 128);  // a unit's O read by the softmax warps
+    for (int i = 0; i < kTcSegs; ++i) {
+      mbar_init(&seg_full[i], 1);
+      mbar_init(&seg_empty[i], 5);  // the MMA warp and the four softmax warps
+    }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
     }
@@ -763,14 +858,26 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     atomicExch(a.status, XB_ERR_TIMEOUT);
     abort_flag = 1;
   };
-  Walk w;
-  Segment s;
-  const bool any_work = find_piece<kTcThreads>(a, w, warp_sum, found, gridDim.x, blockIdx.x);
-  bool more = any_work && segment<kTcTK>(a, w, s);
-  auto advance = [&]() { more = next_unit(a, w, s.next) && segment<kTcTK>(a, w, s); };
+  Meta* meta = reinterpret_cast<Meta*>(a.ws + 2 * (int64_t)gridDim.x * part_floats(kTcRows));
+  int64_t total;
+  const int64_t share = find_pieces<kTcThreads, 1>(a, gridDim.x, blockIdx.x, sums, found, &total);
+  // A wait of a whole warp: the same answer in every lane (false: it ran out)
+  auto wait_all = [&](uint64_t* bar, int phase) -> bool {
+    if (__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, kWaitLimit, &abort_flag))) return true;
+    fail();
+    return false;
+  };
+  // Segment number n for a consumer warp (all its lanes); false at the end or after a timeout
+  auto take = [&](int n, Segment& s) -> bool {
+    if (!wait_all(&seg_full[n % kTcSegs], n / kTcSegs)) return false;
+    s = segs[n % kTcSegs];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&seg_empty[n % kTcSegs]);
+    return s.rows > 0;
+  };
 
   if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
+    // ------------------------------------------------------------ walk and TMA producer
     uint32_t issued[kTcStages];
 #pragma unroll
     for (int i = 0; i < kTcStages; ++i) issued[i] = 0;
@@ -779,9 +886,33 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     const int box = is_v ? lane - boxes : lane;
     const CUtensorMap* map = is_v ? &maps.v : &maps.k;
     const uint32_t q_bytes = (uint32_t)(a.tpt * a.n_rep * kHD * 2);
-    int g = 0, lu = 0;  // tiles and units (with tiles) so far
-    bool ok = true;
-    for (; more && ok; advance()) {
+    int g = 0, lu = 0, n = 0;  // tiles, units (with tiles) and segments so far
+    bool ok = true, open_unit = false;
+    Walk w;
+    Segment s;
+    bool more = found[0][0] >= 0;
+    if (more) {
+      place(a, w, blockIdx.x, share, total, found[0]);
+      more = segment<kTcTK>(a, w, s);
+    }
+    auto publish = [&](int rows) -> bool {
+      if (!wait_all(&seg_empty[n % kTcSegs], n / kTcSegs + 1)) return false;
+      if (lane == 0) {
+        segs[n % kTcSegs] = s;
+        segs[n % kTcSegs].rows = rows;
+        mbar_arrive(&seg_full[n % kTcSegs]);
+      }
+      __syncwarp();
+      ++n;
+      return true;
+    };
+    for (; more && ok; more = next_unit(a, w) && segment<kTcTK>(a, w, s)) {
+      if (s.starts && !s.ends) {
+        open_unit = true;
+        if (lane == 0) meta[blockIdx.x] = Meta{(int)unit_last(a, w), s.token, s.rows, s.kvh};
+      }
+      ok = publish(s.rows);
+      if (!ok) break;
       if (s.t0 >= s.t1) continue;
       // this lane's page of the first tile, fetched while Q's buffer may still be in use
       auto page_of = [&](int tile) -> int {
@@ -790,18 +921,14 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
                                                 : 0;
       };
       int id = page_of(s.t0);
-      if (lu > 0) ok = mbar_wait(&q_empty, (lu - 1) & 1, kWaitLimit, &abort_flag);
-      if (__any_sync(0xffffffffu, !ok)) {
-        fail();
-        ok = false;
-        break;
-      }
+      ok = wait_all(&q_empty[lu & 1], (lu >> 1) + 1);
+      if (!ok) break;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&q_full, q_bytes);
+        mbar_arrive_expect_tx(&q_full[lu & 1], q_bytes);
         asm volatile(
             "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
-            "[%2];" ::"r"(sQ),
-            "l"(reinterpret_cast<uint64_t>(&maps.q)), "r"(smem_u32(&q_full)), "r"(0), "r"(s.kvh * a.n_rep),
+            "[%2];" ::"r"(sQ + (lu & 1) * kTcQBytes),
+            "l"(reinterpret_cast<uint64_t>(&maps.q)), "r"(smem_u32(&q_full[lu & 1])), "r"(0), "r"(s.kvh * a.n_rep),
             "r"(s.token)
             : "memory");
       }
@@ -810,12 +937,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
         const int st = g % kTcStages;
         const int here = id;
         if (j + 1 < s.t1) id = page_of(j + 1);
-        ok = mbar_wait(&kv_empty[st], ((g / kTcStages) & 1) ^ 1, kWaitLimit, &abort_flag);
-        if (__any_sync(0xffffffffu, !ok)) {
-          fail();
-          ok = false;
-          break;
-        }
+        ok = wait_all(&kv_empty[st], g / kTcStages + 1);
+        if (!ok) break;
         const int have = min(kTcTK, s.keys - j * kTcTK);
         const int nb = (have + a.box_rows - 1) / a.box_rows;
         if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
@@ -833,52 +956,53 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
         issued[st] = g / kTcStages + 1;
       }
     }
+    if (ok) publish(0);
+    if (!open_unit && lane == 0) meta[blockIdx.x].last = -1;
     // every load issued must have landed before the CTA exits (also after an abort)
     if (lane == 0) {
       uint64_t deadline = 0;
-      if (lu > 0 && !mbar_wait_deadline(&q_full, (lu - 1) & 1, &deadline, kWaitLimit)) fail();
+      for (int i = lu > 2 ? lu - 2 : 0; i < lu; ++i)
+        if (!mbar_wait_deadline(&q_full[i & 1], (i >> 1) & 1, &deadline, kWaitLimit)) fail();
 #pragma unroll
       for (int st = 0; st < kTcStages; ++st)
         if (issued[st] && !mbar_wait_deadline(&kv_full[st], (issued[st] - 1) & 1, &deadline, kWaitLimit)) fail();
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t kIdS = umma_idesc(1, 1, 1, 0, 0, kTcRows, kTcTK);  // Q (K-major) x K tile (K-major)
-      constexpr uint32_t kIdO = umma_idesc(1, 1, 1, 0, 1, kTcRows, kHD);    // P (TMEM) x V tile (MN-major)
-      bool any = false, ok = true;
-      int g = 0, lu = 0;
-      int pend = -1, pend_lu = 0;  // the tile whose P V is still to issue
-      bool pend_first = false;
-      // P_g V_g accumulated into O once P_g is written (and O rescaled where
-      // its base moved); a unit's first tile starts O afresh, after the
-      // softmax has read the previous unit's
-      auto pv = [&]() -> bool {
-        if (!mbar_wait(&p_full[pend & 1], (pend >> 1) & 1, kWaitLimit, &abort_flag)) return false;
-        if (pend_first && pend_lu > 0 && !mbar_wait(&o_empty, (pend_lu - 1) & 1, kWaitLimit, &abort_flag)) return false;
-        tc_fence_after();
-        const uint32_t sv = sKV + (pend % kTcStages) * 2 * kTcTileBytes + kTcTileBytes;
-        const uint32_t p = tmem + (pend & 1) * 64;
+    constexpr uint32_t kIdS = umma_idesc(1, 1, 1, 0, 0, kTcRows, kTcTK);  // Q (K-major) x K tile (K-major)
+    constexpr uint32_t kIdO = umma_idesc(1, 1, 1, 0, 1, kTcRows, kHD);    // P (TMEM) x V tile (MN-major)
+    bool any = false, ok = true;
+    int g = 0, lu = 0;
+    int pend = -1, pend_lu = 0;  // the tile whose P V is still to issue
+    bool pend_first = false;
+    // P_g V_g accumulated into O once P_g is written (and O rescaled where its
+    // base moved); a unit's first tile starts O afresh, after the softmax has
+    // read the previous unit's
+    auto pv = [&]() -> bool {
+      if (!mbar_wait(&p_full[pend & 1], (pend >> 1) & 1, kWaitLimit, &abort_flag)) return false;
+      if (pend_first && pend_lu > 0 && !mbar_wait(&o_empty, (pend_lu - 1) & 1, kWaitLimit, &abort_flag)) return false;
+      tc_fence_after();
+      const uint32_t sv = sKV + (pend % kTcStages) * 2 * kTcTileBytes + kTcTileBytes;
+      const uint32_t p = tmem + (pend & 1) * 64;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)  // keys in steps of 16: 8 columns of P
-          mma_f16_ts(tmem + 128, p + ks * 8, umma_desc_sw128(sv + ks * 16 * 128, kTcTileBytes, 1024), kIdO,
-                     (!pend_first || ks > 0) ? 1u : 0u);
-        tc_commit(&o_full);
-        tc_commit(&kv_empty[pend % kTcStages]);
-        return true;
-      };
-      for (; more && ok; advance()) {
-        if (s.t0 >= s.t1) continue;
-        if (!mbar_wait(&q_full, lu & 1, kWaitLimit, &abort_flag)) {
-          fail();
-          break;
-        }
-        for (int j = s.t0; j < s.t1; ++j, ++g) {
+      for (int ks = 0; ks < 4; ++ks)  // keys in steps of 16: 8 columns of P
+        mma_f16_ts(tmem + 128, p + ks * 8, umma_desc_sw128(sv + ks * 16 * 128, kTcTileBytes, 1024), kIdO,
+                   (!pend_first || ks > 0) ? 1u : 0u);
+      tc_commit(&o_full);
+      tc_commit(&kv_empty[pend % kTcStages]);
+      return true;
+    };
+    Segment s;
+    for (int n = 0; ok && take(n, s); ++n) {
+      if (s.t0 >= s.t1) continue;
+      if (lane == 0) {
+        if (!mbar_wait(&q_full[lu & 1], (lu >> 1) & 1, kWaitLimit, &abort_flag)) ok = false;
+        const uint32_t q = sQ + (lu & 1) * kTcQBytes;
+        for (int j = s.t0; j < s.t1 && ok; ++j, ++g) {
           // S_g over P_{g-2}, whose P V has completed
           const int st = g % kTcStages;
           if (!mbar_wait(&kv_full[st], (g / kTcStages) & 1, kWaitLimit, &abort_flag) ||
               (g >= 2 && !mbar_wait(&o_full, (g - 2) & 1, kWaitLimit, &abort_flag))) {
-            fail();
             ok = false;
             break;
           }
@@ -886,13 +1010,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
           const uint32_t sk = sKV + st * 2 * kTcTileBytes;
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)  // head dim in steps of 16
-            mma_f16(tmem + (g & 1) * 64, umma_desc_sw128(sQ + ks * 32, 16, 1024),
+            mma_f16(tmem + (g & 1) * 64, umma_desc_sw128(q + ks * 32, 16, 1024),
                     umma_desc_sw128(sk + ks * 32, 16, 1024), kIdS, ks > 0 ? 1u : 0u);
           any = true;
           tc_commit(&s_full[g & 1]);
-          if (j == s.t1 - 1) tc_commit(&q_empty);  // the unit's last S: Q may be replaced
+          if (j == s.t1 - 1) tc_commit(&q_empty[lu & 1]);  // the unit's last S: Q may be replaced
           if (pend >= 0 && !pv()) {
-            fail();
             ok = false;
             break;
           }
@@ -900,8 +1023,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
           pend_first = j == s.t0;
           pend_lu = lu;
         }
-        ++lu;
+        if (!ok) fail();
       }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ++lu;
+    }
+    if (lane == 0) {
       if (ok && pend >= 0 && !pv()) fail();
       if (any) {  // every issued MMA completes before TMEM is released (also after an abort)
         tc_commit(&drain_bar);
@@ -909,16 +1036,17 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
         if (!mbar_wait_deadline(&drain_bar, 0, &deadline, kWaitLimit)) fail();
       }
     }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax: one query row per thread
     const int q4 = warp & 3;  // TMEM lane quarter
     const int r = q4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
     constexpr float kRebase = 8.0f;  // log2 of the largest P kept without rescaling
-    Meta* meta = reinterpret_cast<Meta*>(a.ws + 2 * (int64_t)gridDim.x * part_floats(kTcRows));
-    bool open_unit = false, ok = true;
+    bool ok = true;
     int g = 0;
-    for (; more && ok; advance()) {
+    Segment s;
+    for (int n = 0; ok && take(n, s); ++n) {
       const bool valid = r < s.rows;
       const bool warp_valid = q4 * 32 < s.rows;  // uniform: some row of this warp is the unit's
       const int tok = r / a.n_rep;
@@ -926,18 +1054,16 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
       float m = -INFINITY, l = 0.0f;                        // m: the base of P (log2 units)
       for (int j = s.t0; j < s.t1; ++j, ++g) {
         const int sb = g & 1;
-        if (!mbar_wait(&s_full[sb], (g >> 1) & 1, kWaitLimit, &abort_flag)) {
-          fail();
-          ok = false;
-          break;
-        }
+        ok = wait_all(&s_full[sb], g >> 1);
+        if (!ok) break;
         tc_fence_after();
         const int k0 = j * kTcTK;
         if (s.keys - k0 < kTcTK) {
           // values behind the last key hold whatever the page or ring held: a
           // NaN there would survive its zero weight
           const int st = g % kTcStages;
-          mbar_wait(&kv_full[st], (g / kTcStages) & 1, kWaitLimit, &abort_flag);  // (landed: S_g has read K)
+          ok = wait_all(&kv_full[st], g / kTcStages);  // (landed: S_g has read K)
+          if (!ok) break;
           const uint32_t sv = sKV + st * 2 * kTcTileBytes + kTcTileBytes;
           for (int i = (s.keys - k0) * 8 + (int)threadIdx.x - 64; i < kTcTK * 8; i += 128)
             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + i * 16), "r"(0) : "memory");
@@ -993,11 +1119,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
           tmem_st_32x32b_x32(tmem + sb * 64 + lane_off, pk);
           // P_{g-1} V is in O (waited for in every tile: the barrier's parity
           // tells neighbouring phases apart, no more)
-          if (!first && !mbar_wait(&o_full, (g - 1) & 1, kWaitLimit, &abort_flag)) {
-            fail();
-            ok = false;
-            break;
-          }
+          if (!first) ok = wait_all(&o_full, g - 1);
+          if (!ok) break;
           if (rebase && !first) {  // rescale O's rows to the new bases before P_g V adds to them
             tc_fence_after();
 #pragma unroll
@@ -1011,10 +1134,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
             }
           }
           tmem_st_wait();
-        } else if (j > s.t0 && !mbar_wait(&o_full, (g - 1) & 1, kWaitLimit, &abort_flag)) {
-          fail();
-          ok = false;
-          break;
+        } else if (j > s.t0) {
+          ok = wait_all(&o_full, g - 1);
+          if (!ok) break;
         }
         tc_fence_before();
         mbar_arrive(&p_full[sb]);
@@ -1022,11 +1144,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
       if (!ok) break;
       uint32_t ov[64];
       if (s.t0 < s.t1) {  // the unit's last P V, then O: read and released for the next unit
-        if (!mbar_wait(&o_full, (g - 1) & 1, kWaitLimit, &abort_flag)) {
-          fail();
-          ok = false;
-          break;
-        }
+        ok = wait_all(&o_full, g - 1);
+        if (!ok) break;
         tc_fence_after();
         if (warp_valid) {
           tmem_ld_32x32b_x32(tmem + 128 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[0]));
@@ -1059,12 +1178,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
         part[kTcRows * kHD + r] = m;
         part[kTcRows * kHD + kTcRows + r] = l;
       }
-      if (s.starts && !s.ends) {
-        open_unit = true;
-        if (threadIdx.x == 64) meta[blockIdx.x] = Meta{s.last, s.token, s.rows, s.kvh};
-      }
     }
-    if (!open_unit && threadIdx.x == 64) meta[blockIdx.x].last = -1;
   }
   tc_fence_before();
   __syncthreads();
@@ -1075,39 +1189,64 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
 }
 
 // Joins the partials of the unit that starts in CTA blockIdx.x and goes on in
-// the next ones: o = sum_c o_c 2^(m_c - M), l likewise, in CTA order.
-template <int ROWS>
+// the next ones: o = sum_c o_c 2^(m_c - M), l likewise.  A CTA takes 256 / (16
+// LANES) rows; LANES threads share a row's 16-byte column, each with every
+// LANES-th partial, and meet by shuffles in a fixed order.
+template <int ROWS, int LANES>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, int ctas) {
   pdl_wait();
   pdl_trigger();
   const Meta m = reinterpret_cast<const Meta*>(a.ws + 2 * (int64_t)ctas * part_floats(ROWS))[blockIdx.x];
-  if (m.last < 0) return;
-  for (int i = threadIdx.x; i < m.rows * (kHD / 4); i += 256) {
-    const int r = i / (kHD / 4), d = (i % (kHD / 4)) * 4;
-    float M = -INFINITY;
-    for (int c = blockIdx.x; c <= m.last; ++c) {
-      const float* p = a.ws + (2 * (int64_t)c + (c == blockIdx.x)) * part_floats(ROWS);
-      M = fmaxf(M, p[ROWS * kHD + r]);
+  constexpr int kRows = 256 / (16 * LANES);
+  const int ln = threadIdx.x % LANES, col = (threadIdx.x / LANES) % 16;
+  const int r = blockIdx.y * kRows + threadIdx.x / (16 * LANES), d = col * 4;
+  if (m.last < 0 || (int)blockIdx.y * kRows >= m.rows) return;
+  const int c0 = blockIdx.x, n = m.last - c0 + 1;
+  float M = -INFINITY, l = 0.0f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = ln; i0 < n; i0 += 4 * LANES) {  // four partials in flight
+    float pm[4], pl[4];
+    float4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * LANES;
+      const float* p = a.ws + (2 * (int64_t)(c0 + i) + (i == 0)) * part_floats(ROWS);
+      const bool in = i < n;
+      pm[u] = in ? p[ROWS * kHD + r] : -INFINITY;
+      pl[u] = in ? p[ROWS * kHD + ROWS + r] : 0.0f;
+      v[u] = in ? *reinterpret_cast<const float4*>(p + r * kHD + d) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const float base = M == -INFINITY ? 0.0f : M;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.0f;
-    for (int c = blockIdx.x; c <= m.last; ++c) {
-      const float* p = a.ws + (2 * (int64_t)c + (c == blockIdx.x)) * part_floats(ROWS);
-      const float f = ex2_approx(p[ROWS * kHD + r] - base);
-      const float4 v = *reinterpret_cast<const float4*>(p + r * kHD + d);
-      acc.x += v.x * f;
-      acc.y += v.y * f;
-      acc.z += v.z * f;
-      acc.w += v.w * f;
-      l += p[ROWS * kHD + ROWS + r] * f;
+    const float mn = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), M);
+    const float base = mn == -INFINITY ? 0.0f : mn;
+    const float f0 = ex2_approx(M - base);
+    acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
+    l *= f0;
+    M = mn;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float f = ex2_approx(pm[u] - base);
+      acc.x += v[u].x * f;
+      acc.y += v[u].y * f;
+      acc.z += v[u].z * f;
+      acc.w += v[u].w * f;
+      l += pl[u] * f;
     }
+  }
+#pragma unroll
+  for (int o = 1; o < LANES; o <<= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, M, o);
+    const float mn = fmaxf(M, om), base = mn == -INFINITY ? 0.0f : mn;
+    const float f = ex2_approx(M - base), fo = ex2_approx(om - base);
+    acc.x = acc.x * f + __shfl_xor_sync(0xffffffffu, acc.x, o) * fo;
+    acc.y = acc.y * f + __shfl_xor_sync(0xffffffffu, acc.y, o) * fo;
+    acc.z = acc.z * f + __shfl_xor_sync(0xffffffffu, acc.z, o) * fo;
+    acc.w = acc.w * f + __shfl_xor_sync(0xffffffffu, acc.w, o) * fo;
+    l = l * f + __shfl_xor_sync(0xffffffffu, l, o) * fo;
+    M = mn;
+  }
+  if (ln == 0 && r < m.rows) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    bf16* op = a.out + (int64_t)(m.token + r / a.n_rep) * a.ld_out + (m.kvh * a.n_rep + r % a.n_rep) * kHD + d;
-    uint2 pk;
-    pk.x = pack2(acc.x * inv, acc.y * inv);
-    pk.y = pack2(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(op) = pk;
+    store_out4(a, m.token, m.kvh, r, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   }
 }
 
@@ -1476,9 +1615,9 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
   const bool few = few_rows(tokens, batch, n_rep);
   const int rows = few ? kFewRows : kTcRows, tile = few ? kTK : kTcTK;
   a.tpt = rows / n_rep;
-  a.over = 96;
-  a.snap = few ? 64 : 128;
-  a.min_share = few ? 256 : 512;  // at least over + 2 snap: no piece may lie between two moved cuts
+  a.over = few ? 32 : 96;
+  a.snap = few ? 16 : 64;
+  a.min_share = few ? 64 : 224;  // over + 2 snap: no piece may lie between two moved cuts
   int box = 8;  // rows of one load: the largest power of two that divides a page, at most a tile
   while (box < tile && page_size % (2 * box) == 0) box *= 2;
   a.box_rows = box;
@@ -1506,10 +1645,10 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
     kv.k = maps.k;
     kv.v = maps.v;
     e = launch_k(paged_attn_few_kernel, (unsigned)ctas, kWarps * 32, kFewSmem, s, kv, a);
-    if (e == cudaSuccess) e = launch_k(paged_attn_join_kernel<kFewRows>, (unsigned)ctas, 256, 0, s, a, ctas);
+    if (e == cudaSuccess) e = launch_k(paged_attn_join_kernel<kFewRows, 4>, dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
   } else {
     e = launch_k(paged_attn_tc_kernel, (unsigned)ctas, kTcThreads, kTcSmem, s, maps, a);
-    if (e == cudaSuccess) e = launch_k(paged_attn_join_kernel<kTcRows>, (unsigned)ctas, 256, 0, s, a, ctas);
+    if (e == cudaSuccess) e = launch_k(paged_attn_join_kernel<kTcRows, 1>, dim3((unsigned)ctas, kTcRows / 16), 256, 0, s, a, ctas);
   }
   if (e != cudaSuccess) {
     set_err(err, errlen, "%s: %s", what, cudaGetErrorString(e));
