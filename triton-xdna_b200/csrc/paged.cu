@@ -174,9 +174,8 @@ __global__ void __launch_bounds__(256) paged_rope_kv_kernel(const RopeArgs a, in
 // what starting and finishing a unit costs in keys.  All units laid end to end
 // are one line of weight `total`; CTA c takes the piece [c share, (c + 1) share)
 // of it, whatever unit boundaries lie inside, so the CTAs finish together
-// however uneven the batch is.  A cut closer than `snap` keys to a unit's
-// first or last key moves to the unit's boundary (both neighbours move it the
-// same way).  A unit that one CTA covers alone is written at once; one that
+// however uneven the batch is.  A cut close to a unit's first or last key moves
+// to the unit's boundary (both neighbours move it the same way).  A unit that one CTA covers alone is written at once; one that
 // spans several leaves a partial (O, max, sum) per CTA in the workspace, and a
 // second small kernel joins them in CTA order (fixed order: repeatable bits).
 // The weights are a closed form, so a CTA finds its piece with one scan over
@@ -191,6 +190,7 @@ struct AttnArgs {
   int64_t ld_q, ld_out, ld_table;
   int T, B, KVH, n_rep, tpt, page_size, max_pages, n_pages, box_rows;
   int min_share, over, snap;
+  uint32_t rep_magic;  // ceil(2^16 / n_rep)
   float scale_log2;
   int *bad, *status;
 };
@@ -200,39 +200,63 @@ struct Meta {
   int last, token, rows, kvh;  // last < 0: no such unit
 };
 
+// r / n_rep for a row r < 128: the product is above the quotient by less than r / 2^16 < 1 / n_rep.
+__device__ __forceinline__ int row_token(const AttnArgs& a, int r) { return (int)(((uint32_t)r * a.rep_magic) >> 16); }
+
+// I: int where the host has seen that the line's weight stays below 2^31
+// whatever the lengths, else int64_t (the walks are a good part of a short
+// call's instructions).
+template <typename I>
 struct Seq {
-  int s0, n;          // first packed token, number of new tokens
-  int64_t len, base;  // keys held, keys before the new tokens (negative: the first tokens see none)
-  int nt;             // query tiles
-  int64_t perh;       // weight of one KV head
+  int s0, n;      // first packed token, number of new tokens
+  int len, base;  // keys held, keys before the new tokens (negative: the first tokens see none)
+  int nt;         // query tiles
+  I perh;         // weight of one KV head
 };
 
-__device__ __forceinline__ int64_t cum_keys(const AttnArgs& a, const Seq& q, int64_t j) {  // weight of tiles 0 .. j - 1
-  const int64_t b = (q.base > 0 ? q.base : 0) + a.over;
-  return j * b + (j < q.nt ? a.tpt * j * (j + 1) / 2 : a.tpt * (int64_t)q.nt * (q.nt - 1) / 2 + q.n);
+template <typename I>
+__device__ __forceinline__ I cum_keys(const AttnArgs& a, const Seq<I>& q, int j) {  // weight of tiles 0 .. j - 1
+  const I b = max(q.base, 0) + a.over;
+  if (sizeof(I) == 4)  // the product of two tile numbers may pass 2^31 before it is halved
+    return j * b + (j < q.nt ? (I)((int64_t)a.tpt * j * (j + 1) / 2) : (I)((int64_t)a.tpt * q.nt * (q.nt - 1) / 2) + q.n);
+  return j * b + (j < q.nt ? (I)a.tpt * j * (j + 1) / 2 : (I)a.tpt * q.nt * (q.nt - 1) / 2 + q.n);
 }
 
-__device__ __forceinline__ Seq load_seq(const AttnArgs& a, int b) {
-  Seq q;
-  const int s0 = min(max(__ldg(a.q_start + b), 0), a.T);
-  const int s1 = min(max(__ldg(a.q_start + b + 1), s0), a.T);
+template <typename I>
+__device__ __forceinline__ Seq<I> make_seq(const AttnArgs& a, int s0, int n, int len) {
+  Seq<I> q;
   q.s0 = s0;
-  q.n = s1 - s0;
-  const int64_t cap = (int64_t)a.max_pages * a.page_size;
-  const int64_t len = max(__ldg(a.kv_len + b), 0);
-  q.len = len < cap ? len : cap;
-  q.base = q.len - q.n;
-  q.nt = (q.n + a.tpt - 1) / a.tpt;
-  q.perh = cum_keys(a, q, q.nt);
+  q.n = n;
+  q.len = len;
+  q.base = len - n;
+  q.nt = n <= a.tpt ? (n > 0) : (n + a.tpt - 1) / a.tpt;
+  q.perh = q.nt == 0 ? (I)0 : q.nt == 1 ? (I)(max(q.base, 0) + a.over + n) : cum_keys(a, q, q.nt);
   return q;
 }
 
+template <typename I>
+__device__ __forceinline__ Seq<I> load_seq(const AttnArgs& a, int b) {
+  const int s0 = min(max(__ldg(a.q_start + b), 0), a.T);
+  const int s1 = min(max(__ldg(a.q_start + b + 1), s0), a.T);
+  return make_seq<I>(a, s0, s1 - s0, min(max(__ldg(a.kv_len + b), 0), a.max_pages * a.page_size));
+}
+
+// Where a piece starts: a sequence, its first point on the line and its numbers.
+template <typename I>
+struct Found {
+  I start;
+  int b, s0, n, len;  // b < 0: the piece is empty
+};
+
 // A walk over one piece [lo, hi) of the line.
+template <typename I>
 struct Walk {
-  int64_t lo, hi, share;
-  int64_t u0;  // where the current unit starts
+  I lo, hi;
+  int snap;  // cuts this close to a unit's end or first key move there
+  I u0;    // where the current unit starts
+  I ulen;  // its weight
   int b, kvh, j;
-  Seq q;
+  Seq<I> q;
 };
 
 // The part of one unit that belongs to a piece.
@@ -245,149 +269,177 @@ struct Segment {
   int starts, ends;  // the unit starts / ends in this piece
 };
 
+// Share of `pieces` equal pieces of the line: at least total / pieces (the
+// product is rounded up by more than the float error; every thread of the grid
+// computes the same value).
+template <typename I>
+__device__ __forceinline__ I share_of(const AttnArgs& a, I total, int pieces) {
+  const I share = (I)((float)total * __frcp_rn((float)pieces) * 1.000001f) + 1;
+  return share < a.min_share ? a.min_share : share;
+}
+
+// How far a cut moves to a unit's boundary: a part of one costs a warp or CTA
+// as much as `snap` keys (starting the second unit, merging the parts), but no
+// piece may grow by more than two thirds, nor lie between two moved cuts.
+template <typename I>
+__device__ __forceinline__ int cut_snap(const AttnArgs& a, I share) {
+  return (int)min((I)a.snap, (share - a.over) / 3);
+}
+
 // Weight of the whole line and, for the piece that starts at `first` + i times
-// the share (i < N), the sequence that holds its start: one scan each.  Every
-// thread of the block calls this; sums and found[N][2] are shared.  Returns
-// the share; found[i][0] < 0: piece i is empty.
-template <int THREADS, int N>
-__device__ __forceinline__ int64_t find_pieces(const AttnArgs& a, int64_t pieces, int64_t first,
-                                               int64_t (*sums)[THREADS / 32], int64_t (*found)[2], int64_t* total_out) {
+// the share (i < N), the sequence that holds its start.  Every thread of the
+// block calls this; sums and found[N] are shared.  One scan over the sequences
+// when the block has a thread for each, two otherwise.  Returns the share.
+template <int THREADS, int N, typename I>
+__device__ __forceinline__ I find_pieces(const AttnArgs& a, int pieces, int first, I (*sums)[THREADS / 32],
+                                         Found<I>* found, I* total_out) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x < N) found[threadIdx.x][0] = -1;
-  int64_t total = 0, share = 0;
+  if (threadIdx.x < N) found[threadIdx.x].b = -1;
+  I total = 0, share = 0, start = 0, c = 0;
+  Seq<I> q;
   for (int pass = 0; pass < 2; ++pass) {
-    int64_t run = 0;
+    I run = 0;
     for (int b0 = 0; b0 < a.B; b0 += THREADS) {
       const int b = b0 + threadIdx.x;
-      const int64_t c = b < a.B ? load_seq(a, b).perh * a.KVH : 0;
-      int64_t s = c;
+      if (pass == 0 || a.B > THREADS) {
+        c = 0;
+        if (b < a.B) {
+          q = load_seq<I>(a, b);
+          c = q.perh * a.KVH;
+        }
+        I s = c;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += v;
-      }
-      const int buf = (b0 / THREADS) & 1;
-      if (lane == 31) sums[buf][warp] = s;
-      __syncthreads();
-      int64_t before = run, all = run;
+        for (int o = 1; o < 32; o <<= 1) {
+          const I v = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += v;
+        }
+        const int buf = (b0 / THREADS) & 1;
+        if (lane == 31) sums[buf][warp] = s;
+        __syncthreads();
+        start = run + s - c;  // this sequence's first point
 #pragma unroll
-      for (int i = 0; i < THREADS / 32; ++i) {
-        const int64_t v = sums[buf][i];
-        if (i < warp) before += v;
-        all += v;
-      }
-      if (pass == 1 && c > 0) {
-        const int64_t e = before + s - c;  // this sequence's start
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int64_t lo = (first + i) * share;
-          if (e <= lo && lo < e + c) {
-            found[i][0] = b;
-            found[i][1] = e;
-          }
+        for (int i = 0; i < THREADS / 32; ++i) {
+          const I v = sums[buf][i];
+          if (i < warp) start += v;
+          run += v;
         }
       }
-      run = all;
+      if (pass == 1 && c > 0) {
+        I lo = first * share;
+#pragma unroll
+        for (int i = 0; i < N; ++i, lo += share)
+          if (start <= lo && lo - start < c) found[i] = Found<I>{start, b, q.s0, q.n, q.len};
+      }
     }
-    __syncthreads();
     if (pass == 0) {
+      if (a.B > THREADS) __syncthreads();
       total = run;
-      share = (total + pieces - 1) / pieces;
-      if (share < a.min_share) share = a.min_share;
+      share = share_of(a, total, pieces);
     }
   }
+  __syncthreads();
   *total_out = total;
   return share;
 }
 
-// Places a walk at piece `piece`'s start, inside sequence found[0] that begins at found[1].
-__device__ __forceinline__ void place(const AttnArgs& a, Walk& w, int64_t piece, int64_t share, int64_t total,
-                                      const int64_t* found) {
-  w.share = share;
+template <typename I>
+__device__ __forceinline__ I unit_weight(const AttnArgs& a, const Walk<I>& w) {
+  return a.over + max(w.q.base, 0) + min(a.tpt * (w.j + 1), w.q.n);
+}
+
+// Places a walk at piece `piece`'s start.
+template <typename I>
+__device__ __forceinline__ void place(const AttnArgs& a, Walk<I>& w, int piece, I share, I total, const Found<I>& f) {
+  w.snap = cut_snap(a, share);
   w.lo = piece * share;
-  w.hi = w.lo + share < total ? w.lo + share : total;
-  w.b = (int)found[0];
-  w.q = load_seq(a, w.b);
-  int64_t in = w.lo - found[1];
+  w.hi = total - w.lo < share ? total : w.lo + share;
+  w.b = f.b;
+  w.q = make_seq<I>(a, f.s0, f.n, f.len);
+  I in = w.lo - f.start;
   w.kvh = 0;
   if (in >= w.q.perh) {
     w.kvh = (int)(in / w.q.perh);
     in -= w.kvh * w.q.perh;
   }
-  int lo = 0, hi = w.q.nt - 1;  // the last tile j with cum(j) <= in
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cum_keys(a, w.q, mid) <= in) lo = mid;
-    else hi = mid - 1;
+  w.j = 0;
+  w.u0 = f.start + w.kvh * w.q.perh;
+  if (w.q.nt > 1) {
+    int lo = 0, hi = w.q.nt - 1;  // the last tile j with cum(j) <= in
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cum_keys(a, w.q, mid) <= in) lo = mid;
+      else hi = mid - 1;
+    }
+    w.j = lo;
+    w.u0 += cum_keys(a, w.q, lo);
   }
-  w.j = lo;
-  w.u0 = found[1] + w.kvh * w.q.perh + cum_keys(a, w.q, lo);
-}
-
-__device__ __forceinline__ int64_t unit_weight(const AttnArgs& a, const Walk& w) {
-  return a.over + (w.q.base > 0 ? w.q.base : 0) + min(a.tpt * (w.j + 1), w.q.n);
+  w.ulen = unit_weight(a, w);
 }
 
 // Steps to the next unit; false behind the piece's last one.
-__device__ __forceinline__ bool next_unit(const AttnArgs& a, Walk& w) {
-  w.u0 += unit_weight(a, w);
+template <typename I>
+__device__ __forceinline__ bool next_unit(const AttnArgs& a, Walk<I>& w) {
+  w.u0 += w.ulen;
   if (w.u0 >= w.hi) return false;
-  if (++w.j < w.q.nt) return true;
-  w.j = 0;
-  if (++w.kvh < a.KVH) return true;
-  w.kvh = 0;
-  do {
-    if (++w.b >= a.B) return false;
-    w.q = load_seq(a, w.b);
-  } while (w.q.n == 0);
+  if (++w.j >= w.q.nt) {
+    w.j = 0;
+    if (++w.kvh >= a.KVH) {
+      w.kvh = 0;
+      do {
+        if (++w.b >= a.B) return false;
+        w.q = load_seq<I>(a, w.b);
+      } while (w.q.n == 0);
+    }
+  }
+  w.ulen = unit_weight(a, w);
   return true;
 }
 
 // The part of the current unit that belongs to this piece, stepping over a
 // unit whose cut was moved away; false when nothing is left.
-template <int TK>
-__device__ __forceinline__ bool segment(const AttnArgs& a, Walk& w, Segment& g) {
+template <int TK, typename I>
+__device__ __forceinline__ bool segment(const AttnArgs& a, Walk<I>& w, Segment& g) {
   for (;;) {
-    const int done = w.j * a.tpt;
-    const int tokens = min(a.tpt, w.q.n - done);
-    const int keys = (int)max(w.q.base + done + tokens, (int64_t)0);
-    const int64_t ulen = unit_weight(a, w);
-    const int64_t cut0 = w.lo - w.u0, cut1 = w.hi - w.u0;  // the piece's ends inside the unit
-    g.starts = cut0 < a.over + a.snap;
-    if (!g.starts && ulen - cut0 < a.snap) {  // only at the piece's start: the unit ended in the piece before
+    const I cut0 = w.lo - w.u0, cut1 = w.hi - w.u0;  // the piece's ends inside the unit
+    g.starts = cut0 < a.over + w.snap;
+    if (!g.starts && w.ulen - cut0 < w.snap) {  // only at the piece's start: the unit ended in the piece before
       if (!next_unit(a, w)) return false;
       continue;
     }
-    if (cut1 < a.over + a.snap && cut1 < ulen) return false;  // the unit starts in the next piece
-    g.ends = cut1 >= ulen || ulen - cut1 < a.snap;
-    const int nk = (keys + TK - 1) / TK;
-    g.t0 = g.starts ? 0 : min((int)((cut0 - a.over) / TK), nk);  // cuts fall on tile boundaries
-    g.t1 = g.ends ? nk : min((int)((cut1 - a.over) / TK), nk);
+    if (cut1 < a.over + w.snap && cut1 < w.ulen) return false;  // the unit starts in the next piece
+    g.ends = w.ulen - cut1 < w.snap;
+    const int done = w.j * a.tpt;
+    const int tokens = min(a.tpt, w.q.n - done);
     g.b = w.b;
     g.kvh = w.kvh;
     g.token = w.q.s0 + done;
     g.rows = tokens * a.n_rep;
-    g.first_pos = (int)(w.q.base + done);
-    g.keys = keys;
+    g.first_pos = w.q.base + done;
+    g.keys = max(g.first_pos + tokens, 0);
+    const int nk = (int)(((unsigned)g.keys + TK - 1) / TK);
+    g.t0 = g.starts ? 0 : min((int)((unsigned)(cut0 - a.over) / TK), nk);  // cuts fall on tile boundaries
+    g.t1 = g.ends ? nk : min((int)((unsigned)(cut1 - a.over) / TK), nk);
     return true;
   }
 }
 
 // The piece in which the current unit ends: the one that holds its last key,
 // or the one before it if that cut was moved to the unit's end.
-__device__ __forceinline__ int64_t unit_last(const AttnArgs& a, const Walk& w) {
-  const int64_t end = w.u0 + unit_weight(a, w);
-  int64_t last = (end - 1) / w.share;
-  if (last * w.share > w.u0 && end - last * w.share < a.snap) --last;
-  return last;
+template <typename I>
+__device__ __forceinline__ int unit_last(const AttnArgs& a, const Walk<I>& w, I share) {
+  const I end = w.u0 + w.ulen;
+  I last = (end - 1) / share;
+  if (last * share > w.u0 && end - last * share < w.snap) --last;
+  return (int)last;
 }
 
 // ----------------------------------------------------------------------------- attention: few rows (mma.sync)
 //
 // For batches whose sequences bring few tokens each (decoding, verification
 // of drafted tokens): at most 16 rows per unit, the rows of an mma.sync
-// m16n8k16 tile (rows past n_rep * tokens are zero), so the kernel is bound by
-// reading K and V.  Every warp of the grid has a piece of the line of its own
+// m16n8k16 tile (rows past n_rep * tokens are zero; with 8 rows at most, ROWS
+// leaves out the other half of the softmax), so the kernel is bound by reading K
+// and V.  Every warp of the grid has a piece of the line of its own
 // and runs through it alone: its lanes issue the TMA loads of a 32-key tile's
 // page rows (128-byte swizzle) into one of the warp's two buffers, the next
 // unit's tiles while the present one is computed, and the warp keeps an online
@@ -456,19 +508,21 @@ struct Part {
 };
 
 __device__ __forceinline__ void store_out4(const AttnArgs& a, int token, int kvh, int r, int d, float4 v) {
-  bf16* op = a.out + (int64_t)(token + r / a.n_rep) * a.ld_out + (kvh * a.n_rep + r % a.n_rep) * kHD + d;
+  const int tok = row_token(a, r);
+  bf16* op = a.out + (int64_t)(token + tok) * a.ld_out + (kvh * a.n_rep + r - tok * a.n_rep) * kHD + d;
   uint2 pk;
   pk.x = pack2(v.x, v.y);
   pk.y = pack2(v.z, v.w);
   *reinterpret_cast<uint2*>(op) = pk;
 }
 
+template <int ROWS, typename I>
 __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __grid_constant__ KvMaps maps,
                                                                         const AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kWarps][kBufs];
-  __shared__ int64_t sums[2][kWarps];
-  __shared__ int64_t found[kWarps][2];
+  __shared__ I sums[2][kWarps];
+  __shared__ Found<I> found[kWarps];
   __shared__ Part part[2][kWarps];  // [0]: of a unit that started before, [1]: of one that goes on
   __shared__ float part_m[2][kWarps][kFewRows], part_l[2][kWarps][kFewRows];
   __shared__ volatile int abort_flag;
@@ -494,24 +548,24 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
   }
   pdl_wait();
   pdl_trigger();
-  int64_t total;
-  const int64_t share = find_pieces<kWarps * 32, kWarps>(a, (int64_t)gridDim.x * kWarps, (int64_t)blockIdx.x * kWarps,
-                                                         sums, found, &total);
+  I total;
+  const I share =
+      find_pieces<kWarps * 32, kWarps, I>(a, gridDim.x * kWarps, blockIdx.x * kWarps, sums, found, &total);
   Meta* meta = reinterpret_cast<Meta*>(a.ws + 2 * (int64_t)gridDim.x * part_floats(kFewRows));
-  if (found[0][0] < 0) {  // no warp of this CTA has work
+  if (found[0].b < 0) {  // no warp of this CTA has work
     if (threadIdx.x == 0) meta[blockIdx.x].last = -1;
     return;
   }
-  if (found[warp][0] >= 0) {
+  if (found[warp].b >= 0) {
     const int boxes = kTK / a.box_rows;
     const bool is_v = lane >= boxes;
     const int box = is_v ? lane - boxes : lane;
     const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+    const int tok0 = row_token(a, g), tok1 = row_token(a, g + 8);  // the tokens of this thread's two rows
     // two walks over the piece: one requests tiles, one computes them
-    Walk wi, wc;
+    Walk<I> wi, wc;
     Segment si, sc;
-    place(a, wi, (int64_t)blockIdx.x * kWarps + warp, share, total, found[warp]);
-    wc = wi;
+    place(a, wi, (int)blockIdx.x * kWarps + warp, share, total, found[warp]);
     bool more = segment<kTK>(a, wi, si);
     wc = wi;
     sc = si;
@@ -519,24 +573,35 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
     int ni = si.t0;  // next tile to request
     uint32_t use = 0, issued = 0;  // tiles read / requested: buffer n % kBufs, parity (n / kBufs) & 1
     bool dead = false;  // a wait ran out: no more loads, the output is not valid
-    auto settle = [&]() {  // the request walk on a tile, if any is left
+    // 32 entries of the page table row from page `win` on, one per lane: one
+    // latency for many tiles
+    uint32_t win = 0;
+    int win_id = 0;
+    auto window = [&](uint32_t first) {
+      win = first;
+      const uint32_t pi = first + lane;
+      win_id = pi * (uint64_t)a.page_size < (uint32_t)si.keys ? __ldg(a.table + si.b * a.ld_table + pi) : -1;
+    };
+    auto settle = [&](bool fresh) {  // the request walk on a tile, if any is left
       while (more_i && ni >= si.t1) {
         more_i = next_unit(a, wi) && segment<kTK>(a, wi, si);
         ni = si.t0;
+        fresh = true;
       }
+      if (more_i && fresh) window((uint32_t)(ni * kTK) / (uint32_t)a.page_size);
     };
-    settle();
     // lanes 0 .. boxes - 1 load K rows, the next `boxes` lanes V rows
     auto request = [&]() {
       const uint32_t buf = issued % kBufs;
-      const int k0 = ni * kTK;
-      const int nb = (min(kTK, si.keys - k0) + a.box_rows - 1) / a.box_rows;
+      const int k0 = ni * kTK, have = min(kTK, si.keys - k0);
+      const int nb = (have + a.box_rows - 1) / a.box_rows;
+      const uint32_t key = (uint32_t)(k0 + min(box, nb - 1) * a.box_rows);
+      const uint32_t pi = key / (uint32_t)a.page_size;
+      if (__any_sync(0xffffffffu, pi - win >= 32u)) window((uint32_t)k0 / (uint32_t)a.page_size);
+      int id = __shfl_sync(0xffffffffu, win_id, (int)(pi - win));
       if (lane == 0) mbar_arrive_expect_tx(&full[warp][buf], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
       __syncwarp();
       if (lane < 2 * boxes && box < nb) {
-        const uint32_t key = (uint32_t)(k0 + box * a.box_rows);
-        const uint32_t pi = key / (uint32_t)a.page_size;
-        int id = __ldg(a.table + si.b * a.ld_table + pi);
         if (id < 0 || id >= a.n_pages) {  // reads as zeros: a coordinate past the pool
           atomicExch(a.bad, 1);
           id = a.n_pages;
@@ -546,29 +611,30 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
       }
       ++issued;
       ++ni;
-      settle();
+      settle(false);
     };
+    uint32_t qa[4][4];
+    auto load_q = [&]() {
+      const bool ok0 = g < sc.rows, ok1 = g + 8 < sc.rows;
+      const bf16* p0 = a.q + (int64_t)(sc.token + tok0) * a.ld_q + (sc.kvh * a.n_rep + g - tok0 * a.n_rep) * kHD;
+      const bf16* p1 = a.q + (int64_t)(sc.token + tok1) * a.ld_q + (sc.kvh * a.n_rep + g + 8 - tok1 * a.n_rep) * kHD;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        const int c = kk * 16 + 2 * t;
+        qa[kk][0] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c) : 0u;
+        qa[kk][1] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c) : 0u;
+        qa[kk][2] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c + 8) : 0u;
+        qa[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c + 8) : 0u;
+      }
+    };
+    settle(true);
+    if (more) load_q();
     while (more_i && issued < kBufs) request();
 
-    for (; more; more = next_unit(a, wc) && segment<kTK>(a, wc, sc)) {
-      uint32_t qa[4][4];
-      {
-        const int r0 = g, r1 = g + 8;
-        const bool ok0 = r0 < sc.rows, ok1 = r1 < sc.rows;
-        const bf16* p0 = a.q + (int64_t)(sc.token + r0 / a.n_rep) * a.ld_q + (sc.kvh * a.n_rep + r0 % a.n_rep) * kHD;
-        const bf16* p1 = a.q + (int64_t)(sc.token + r1 / a.n_rep) * a.ld_q + (sc.kvh * a.n_rep + r1 % a.n_rep) * kHD;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const int c = kk * 16 + 2 * t;
-          qa[kk][0] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c) : 0u;
-          qa[kk][1] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c) : 0u;
-          qa[kk][2] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c + 8) : 0u;
-          qa[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c + 8) : 0u;
-        }
-      }
+    while (more) {
       // the last key each of this thread's rows sees
-      const int pos0 = min(sc.first_pos + g / a.n_rep, sc.keys - 1);
-      const int pos1 = min(sc.first_pos + (g + 8) / a.n_rep, sc.keys - 1);
+      const int pos0 = min(sc.first_pos + tok0, sc.keys - 1), pos1 = min(sc.first_pos + tok1, sc.keys - 1);
+      const int first_pos = min(sc.first_pos, sc.keys - 1);  // the last one that every row sees
       float o[8][4];
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -606,52 +672,61 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
             mma_16816(s[nt], qa[2 * h + 1], kb[2], kb[3]);
           }
         }
-        float mx0 = -INFINITY, mx1 = -INFINITY;
+        if (k0 + kTK - 1 > first_pos) {  // some row does not see the whole tile
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
+          for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = k0 + nt * 8 + 2 * t + (e & 1);
-            s[nt][e] = key <= (e < 2 ? pos0 : pos1) ? s[nt][e] * a.scale_log2 : -INFINITY;
-            if (e < 2) mx0 = fmaxf(mx0, s[nt][e]);
-            else mx1 = fmaxf(mx1, s[nt][e]);
-          }
+            for (int e = 0; e < ROWS / 4; ++e) {
+              const int key = k0 + nt * 8 + 2 * t + (e & 1);
+              if (key > (e < 2 ? pos0 : pos1)) s[nt][e] = -INFINITY;
+            }
+        }
+        // raw scores: the scale is positive, so their maximum scales to the scaled ones'
+        float mx0 = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])),
+                          fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
+        float mx1 = -INFINITY;
+        if (ROWS > 8)
+          mx1 = fmaxf(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])),
+                      fmaxf(fmaxf(s[2][2], s[2][3]), fmaxf(s[3][2], s[3][3])));
 #pragma unroll
         for (int o_ = 1; o_ <= 2; o_ <<= 1) {
           mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o_));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o_));
+          if (ROWS > 8) mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o_));
         }
-        const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
+        const float mn0 = fmaxf(m0, mx0 * a.scale_log2), mn1 = ROWS > 8 ? fmaxf(m1, mx1 * a.scale_log2) : m1;
         const float base0 = mn0 == -INFINITY ? 0.0f : mn0, base1 = mn1 == -INFINITY ? 0.0f : mn1;
-        const float al0 = ex2_approx(m0 - base0), al1 = ex2_approx(m1 - base1);
+        if (__any_sync(0xffffffffu, mn0 > m0 || mn1 > m1)) {  // some row's maximum moved
+          const float al0 = ex2_approx(m0 - base0), al1 = ex2_approx(m1 - base1);
+          l0 *= al0;
+          l1 *= al1;
+#pragma unroll
+          for (int dt = 0; dt < 8; ++dt) {
+            o[dt][0] *= al0;
+            o[dt][1] *= al0;
+            if (ROWS > 8) o[dt][2] *= al1;
+            if (ROWS > 8) o[dt][3] *= al1;
+          }
+        }
         m0 = mn0;
         m1 = mn1;
-        float rs0 = 0.0f, rs1 = 0.0f;
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
-          s[nt][0] = ex2_approx(s[nt][0] - base0);
-          s[nt][1] = ex2_approx(s[nt][1] - base0);
-          s[nt][2] = ex2_approx(s[nt][2] - base1);
-          s[nt][3] = ex2_approx(s[nt][3] - base1);
-          rs0 += s[nt][0] + s[nt][1];
-          rs1 += s[nt][2] + s[nt][3];
-        }
-        l0 = l0 * al0 + rs0;
-        l1 = l1 * al1 + rs1;
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-          o[dt][0] *= al0;
-          o[dt][1] *= al0;
-          o[dt][2] *= al1;
-          o[dt][3] *= al1;
+          s[nt][0] = ex2_approx(fmaf(s[nt][0], a.scale_log2, -base0));
+          s[nt][1] = ex2_approx(fmaf(s[nt][1], a.scale_log2, -base0));
+          l0 += s[nt][0] + s[nt][1];
+          if (ROWS > 8) {
+            s[nt][2] = ex2_approx(fmaf(s[nt][2], a.scale_log2, -base1));
+            s[nt][3] = ex2_approx(fmaf(s[nt][3], a.scale_log2, -base1));
+            l1 += s[nt][2] + s[nt][3];
+          }
         }
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
           uint32_t pa[4];
           pa[0] = pack2(s[2 * kk][0], s[2 * kk][1]);
-          pa[1] = pack2(s[2 * kk][2], s[2 * kk][3]);
+          pa[1] = ROWS > 8 ? pack2(s[2 * kk][2], s[2 * kk][3]) : 0u;
           pa[2] = pack2(s[2 * kk + 1][0], s[2 * kk + 1][1]);
-          pa[3] = pack2(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+          pa[3] = ROWS > 8 ? pack2(s[2 * kk + 1][2], s[2 * kk + 1][3]) : 0u;
 #pragma unroll
           for (int dt = 0; dt < 8; dt += 2) {
             const int mi = lane >> 3, r = kk * 16 + (mi & 1) * 8 + (lane & 7), c = dt + (mi >> 1);
@@ -668,18 +743,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
 #pragma unroll
       for (int o_ = 1; o_ <= 2; o_ <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, o_);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, o_);
+        if (ROWS > 8) l1 += __shfl_xor_sync(0xffffffffu, l1, o_);
       }
       if (sc.starts && sc.ends) {
         const float i0 = l0 == 0.0f ? 0.0f : 1.0f / l0, i1 = l1 == 0.0f ? 0.0f : 1.0f / l1;  // no key: zeros
-        bf16* p0 = a.out + (int64_t)(sc.token + g / a.n_rep) * a.ld_out + (sc.kvh * a.n_rep + g % a.n_rep) * kHD;
-        bf16* p1 = a.out + (int64_t)(sc.token + (g + 8) / a.n_rep) * a.ld_out +
-                   (sc.kvh * a.n_rep + (g + 8) % a.n_rep) * kHD;
+        bf16* p0 = a.out + (int64_t)(sc.token + tok0) * a.ld_out + (sc.kvh * a.n_rep + g - tok0 * a.n_rep) * kHD;
+        bf16* p1 = a.out + (int64_t)(sc.token + tok1) * a.ld_out + (sc.kvh * a.n_rep + g + 8 - tok1 * a.n_rep) * kHD;
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
           const int d = dt * 8 + 2 * t;
           if (g < sc.rows) *reinterpret_cast<uint32_t*>(p0 + d) = pack2(o[dt][0] * i0, o[dt][1] * i0);
-          if (g + 8 < sc.rows) *reinterpret_cast<uint32_t*>(p1 + d) = pack2(o[dt][2] * i1, o[dt][3] * i1);
+          if (ROWS > 8 && g + 8 < sc.rows) *reinterpret_cast<uint32_t*>(p1 + d) = pack2(o[dt][2] * i1, o[dt][3] * i1);
         }
       } else {
         const int kind = sc.starts ? 1 : 0;
@@ -688,17 +762,21 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
         for (int dt = 0; dt < 8; ++dt) {
           const int d = dt * 8 + 2 * t;
           *reinterpret_cast<float2*>(po + g * kPartLd + d) = make_float2(o[dt][0], o[dt][1]);
-          *reinterpret_cast<float2*>(po + (g + 8) * kPartLd + d) = make_float2(o[dt][2], o[dt][3]);
+          if (ROWS > 8) *reinterpret_cast<float2*>(po + (g + 8) * kPartLd + d) = make_float2(o[dt][2], o[dt][3]);
         }
         if (t == 0) {
           part_m[kind][warp][g] = m0;
-          part_m[kind][warp][g + 8] = m1;
           part_l[kind][warp][g] = l0;
-          part_l[kind][warp][g + 8] = l1;
+          if (ROWS > 8) {
+            part_m[kind][warp][g + 8] = m1;
+            part_l[kind][warp][g + 8] = l1;
+          }
         }
         if (lane == 0)
-          part[kind][warp] = Part{sc.token, sc.rows, sc.kvh, sc.ends, kind ? (int)unit_last(a, wc) : 0, 1};
+          part[kind][warp] = Part{sc.token, sc.rows, sc.kvh, sc.ends, kind ? unit_last(a, wc, share) : 0, 1};
       }
+      more = next_unit(a, wc) && segment<kTK>(a, wc, sc);
+      if (more) load_q();
     }
     if (dead) {  // loads still in flight land before the CTA's shared memory is given up
       uint64_t deadline = 0;
@@ -711,45 +789,59 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
   // warp 0's first kind), and one from every warp whose piece starts a unit
   // that goes on.  They go on through the first kind of the next warps until
   // one ends the unit, or leave the CTA.
-  bool open_unit = false;
-  for (int c = -1; c < kWarps; ++c) {
-    const Part p = c < 0 ? part[0][0] : part[1][c];
-    if (!p.valid) continue;
-    int end = c < 0 ? 0 : c;  // last warp of the chain
-    bool ends = p.ends;
-    while (!ends && end + 1 < kWarps) ends = part[0][++end].ends;
+  // The warp that starts a chain joins it; the one that came in is the job of
+  // the warp it ends in.
+  const uint32_t mine = lane < kWarps ? 1u : 0u;
+  const uint32_t in0 = __ballot_sync(0xffffffffu, mine && part[0][lane & (kWarps - 1)].valid);
+  const uint32_t end0 = __ballot_sync(0xffffffffu, mine && part[0][lane & (kWarps - 1)].valid &&
+                                                       part[0][lane & (kWarps - 1)].ends);
+  const uint32_t open1 = __ballot_sync(0xffffffffu, mine && part[1][lane & (kWarps - 1)].valid);
+  const int last_end = 31 - __clz((int)(end0 | 1u));  // the last warp in which a unit ends (or 0)
+  const bool open_unit = open1 != 0 && (end0 == 0 || (open1 >> last_end) != 0);
+  for (int job = 0; job < 2; ++job) {
+    // job 0: the chain that came in, if it ends (or leaves the CTA) in this warp; job 1: the one this warp starts
+    const int c = job == 0 ? -1 : warp;
+    const uint32_t ahead = job == 0 ? end0 : end0 & (0xfffffffeu << warp);
+    const bool ends = ahead != 0;
+    const int end = ends ? __ffs((int)ahead) - 1 : kWarps - 1;
+    if (job == 0 ? !(in0 & 1u) || warp != end : !(open1 >> warp & 1u)) continue;
+    const Part p = part[c >= 0][max(c, 0)];
     const bool whole = c >= 0 && ends;
-    if (c >= 0 && !ends) {
-      open_unit = true;
-      if (threadIdx.x == 0) meta[blockIdx.x] = Meta{p.last / kWarps, p.token, p.rows, p.kvh};
-    }
-    float* out_part = a.ws + (2 * (int64_t)blockIdx.x + (c < 0 ? 0 : 1)) * part_floats(kFewRows);
-    for (int i = threadIdx.x; i < p.rows * (kHD / 4); i += kWarps * 32) {
-      const int r = i / (kHD / 4), d = (i % (kHD / 4)) * 4;
-      float M = -INFINITY;
-      for (int k = max(c, 0); k <= end; ++k) M = fmaxf(M, part_m[k == c][k][r]);
+    if (c >= 0 && !ends && lane == 0) meta[blockIdx.x] = Meta{p.last / kWarps, p.token, p.rows, p.kvh};
+    float* out_part = a.ws + (2 * (int64_t)blockIdx.x + (c >= 0)) * part_floats(kFewRows);
+    const int first = max(c, 0);
+    if (lane < p.rows) {  // the factor of each part for this lane's row, in the place of its max
+      float M = -INFINITY, l = 0.0f;
+      for (int k = first; k <= end; ++k) M = fmaxf(M, part_m[k == c][k][lane]);
       const float base = M == -INFINITY ? 0.0f : M;
+      for (int k = first; k <= end; ++k) {
+        const float f = ex2_approx(part_m[k == c][k][lane] - base);
+        part_m[k == c][k][lane] = f;
+        l += part_l[k == c][k][lane] * f;
+      }
+      if (whole) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int k = first; k <= end; ++k) part_m[k == c][k][lane] *= inv;
+      } else {
+        out_part[kFewRows * kHD + lane] = M;
+        out_part[kFewRows * kHD + kFewRows + lane] = l;
+      }
+    }
+    __syncwarp();
+    for (int i = lane; i < p.rows * (kHD / 4); i += 32) {
+      const int r = i / (kHD / 4), d = (i % (kHD / 4)) * 4;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float l = 0.0f;
-      for (int k = max(c, 0); k <= end; ++k) {
-        const float f = ex2_approx(part_m[k == c][k][r] - base);
+#pragma unroll 2
+      for (int k = first; k <= end; ++k) {
+        const float f = part_m[k == c][k][r];
         const float4 v = *reinterpret_cast<const float4*>(part_o(k == c, k) + r * kPartLd + d);
         acc.x += v.x * f;
         acc.y += v.y * f;
         acc.z += v.z * f;
         acc.w += v.w * f;
-        l += part_l[k == c][k][r] * f;
       }
-      if (whole) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        store_out4(a, p.token, p.kvh, r, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-      } else {
-        *reinterpret_cast<float4*>(out_part + r * kHD + d) = acc;
-        if (d == 0) {
-          out_part[kFewRows * kHD + r] = M;
-          out_part[kFewRows * kHD + kFewRows + r] = l;
-        }
-      }
+      if (whole) store_out4(a, p.token, p.kvh, r, d, acc);
+      else *reinterpret_cast<float4*>(out_part + r * kHD + d) = acc;
     }
   }
   if (!open_unit && threadIdx.x == 0) meta[blockIdx.x].last = -1;
@@ -802,6 +894,7 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+template <typename I>
 __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __grid_constant__ TcMaps maps,
                                                                       const AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -810,8 +903,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
   __shared__ __align__(8) uint64_t kv_full[kTcStages], kv_empty[kTcStages];
   __shared__ __align__(8) uint64_t seg_full[kTcSegs], seg_empty[kTcSegs];
   __shared__ Segment segs[kTcSegs];  // rows == 0: the end
-  __shared__ int64_t sums[2][kTcThreads / 32];
-  __shared__ int64_t found[1][2];
+  __shared__ I sums[2][kTcThreads / 32];
+  __shared__ Found<I> found[1];
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile int abort_flag;
 
@@ -859,8 +952,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     abort_flag = 1;
   };
   Meta* meta = reinterpret_cast<Meta*>(a.ws + 2 * (int64_t)gridDim.x * part_floats(kTcRows));
-  int64_t total;
-  const int64_t share = find_pieces<kTcThreads, 1>(a, gridDim.x, blockIdx.x, sums, found, &total);
+  I total;
+  const I share = find_pieces<kTcThreads, 1, I>(a, gridDim.x, blockIdx.x, sums, found, &total);
   // A wait of a whole warp: the same answer in every lane (false: it ran out)
   auto wait_all = [&](uint64_t* bar, int phase) -> bool {
     if (__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, kWaitLimit, &abort_flag))) return true;
@@ -888,11 +981,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     const uint32_t q_bytes = (uint32_t)(a.tpt * a.n_rep * kHD * 2);
     int g = 0, lu = 0, n = 0;  // tiles, units (with tiles) and segments so far
     bool ok = true, open_unit = false;
-    Walk w;
+    Walk<I> w;
     Segment s;
-    bool more = found[0][0] >= 0;
+    bool more = found[0].b >= 0;
     if (more) {
-      place(a, w, blockIdx.x, share, total, found[0]);
+      place(a, w, (int)blockIdx.x, share, total, found[0]);
       more = segment<kTcTK>(a, w, s);
     }
     auto publish = [&](int rows) -> bool {
@@ -909,7 +1002,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     for (; more && ok; more = next_unit(a, w) && segment<kTcTK>(a, w, s)) {
       if (s.starts && !s.ends) {
         open_unit = true;
-        if (lane == 0) meta[blockIdx.x] = Meta{(int)unit_last(a, w), s.token, s.rows, s.kvh};
+        if (lane == 0) meta[blockIdx.x] = Meta{unit_last(a, w, share), s.token, s.rows, s.kvh};
       }
       ok = publish(s.rows);
       if (!ok) break;
@@ -1049,7 +1142,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     for (int n = 0; ok && take(n, s); ++n) {
       const bool valid = r < s.rows;
       const bool warp_valid = q4 * 32 < s.rows;  // uniform: some row of this warp is the unit's
-      const int tok = r / a.n_rep;
+      const int tok = row_token(a, r);
       const int seen = min(s.first_pos + tok, s.keys - 1);  // the last key this row sees
       float m = -INFINITY, l = 0.0f;                        // m: the base of P (log2 units)
       for (int j = s.t0; j < s.t1; ++j, ++g) {
@@ -1357,6 +1450,16 @@ bool few_rows(int64_t tokens, int64_t batch, int64_t n_rep) {
   return n_rep <= kFewRows && tokens * n_rep <= kFewRows * batch;
 }
 
+// Launch of an attention kernel, its shared-memory limit raised once per device.
+template <typename M>
+cudaError_t launch_main(void (*kernel)(M, AttnArgs), int ctas, int threads, int smem, cudaStream_t s, const M& maps,
+                        const AttnArgs& a) {
+  cudaError_t e = once_per_device(reinterpret_cast<const void*>(kernel), kOnceSmem, [&](int*) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  });
+  return e != cudaSuccess ? e : launch_k(kernel, (unsigned)ctas, threads, smem, s, maps, a);
+}
+
 template <int N>
 cudaError_t launch_copy(const int32_t* src, const int32_t* dst, int n, uint8_t* base, int64_t outer,
                         int64_t outer_stride, int64_t page_stride, uint32_t vpp, cudaStream_t s) {
@@ -1613,11 +1716,13 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
   rc = status_words(&a.bad, &a.status, what, err, errlen);
   if (rc) return rc;
   const bool few = few_rows(tokens, batch, n_rep);
-  const int rows = few ? kFewRows : kTcRows, tile = few ? kTK : kTcTK;
+  const bool eight = few && n_rep <= 8 && tokens * n_rep <= 8 * batch;  // the same rule for half a tile
+  const int rows = few ? (eight ? 8 : kFewRows) : kTcRows, tile = few ? kTK : kTcTK;
   a.tpt = rows / n_rep;
-  a.over = few ? 32 : 96;
-  a.snap = few ? 16 : 64;
-  a.min_share = few ? 64 : 224;  // over + 2 snap: no piece may lie between two moved cuts
+  a.rep_magic = (65536u + (uint32_t)n_rep - 1u) / (uint32_t)n_rep;
+  a.over = few ? 16 : 96;
+  a.snap = few ? 32 : 128;
+  a.min_share = few ? 32 : 192;
   int box = 8;  // rows of one load: the largest power of two that divides a page, at most a tile
   while (box < tile && page_size % (2 * box) == 0) box *= 2;
   a.box_rows = box;
@@ -1627,28 +1732,31 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
   if (!rc) rc = page_map(&maps.v, v_pages, n_pages, n_kv_head, page_size, v_page, v_head, v_row, box, what, err, errlen);
   if (!rc && !few) rc = query_map(&maps.q, q, tokens, n_head, ld_q, n_rep, a.tpt, what, err, errlen);
   if (rc) return rc;
-  const void* kernel = few ? reinterpret_cast<const void*>(paged_attn_few_kernel)
-                           : reinterpret_cast<const void*>(paged_attn_tc_kernel);
-  cudaError_t e = xb::once_per_device(kernel, xb::kOnceSmem, [&](int*) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, few ? kFewSmem : kTcSmem);
-  });
-  if (e != cudaSuccess) {
-    set_err(err, errlen, "%s: kernel setup: %s", what, cudaGetErrorString(e));
-    return XB_ERR_CUDA;
-  }
   int sms = 148;
   xb::sm_count(&sms);
   const int ctas = few ? sms : 2 * sms;
+  // The line's weight whatever the lengths are: at most tokens / tpt + batch
+  // query tiles per KV head, each of at most the table's positions.  With the
+  // pieces' rounding it stays an int below 2^30.
+  const double most = ((double)tokens / a.tpt + batch) * n_kv_head * ((double)max_pages * page_size + a.over + a.tpt);
+  const bool wide = most + (double)a.min_share * ctas * kWarps >= (double)(1 << 30);
   cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t e;
   if (few) {
     KvMaps kv;
     kv.k = maps.k;
     kv.v = maps.v;
-    e = launch_k(paged_attn_few_kernel, (unsigned)ctas, kWarps * 32, kFewSmem, s, kv, a);
-    if (e == cudaSuccess) e = launch_k(paged_attn_join_kernel<kFewRows, 4>, dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
+    e = eight ? (wide ? launch_main(paged_attn_few_kernel<8, int64_t>, ctas, kWarps * 32, kFewSmem, s, kv, a)
+                      : launch_main(paged_attn_few_kernel<8, int>, ctas, kWarps * 32, kFewSmem, s, kv, a))
+              : (wide ? launch_main(paged_attn_few_kernel<16, int64_t>, ctas, kWarps * 32, kFewSmem, s, kv, a)
+                      : launch_main(paged_attn_few_kernel<16, int>, ctas, kWarps * 32, kFewSmem, s, kv, a));
+    if (e == cudaSuccess)
+      e = launch_k(paged_attn_join_kernel<kFewRows, 4>, dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
   } else {
-    e = launch_k(paged_attn_tc_kernel, (unsigned)ctas, kTcThreads, kTcSmem, s, maps, a);
-    if (e == cudaSuccess) e = launch_k(paged_attn_join_kernel<kTcRows, 1>, dim3((unsigned)ctas, kTcRows / 16), 256, 0, s, a, ctas);
+    e = wide ? launch_main(paged_attn_tc_kernel<int64_t>, ctas, kTcThreads, kTcSmem, s, maps, a)
+             : launch_main(paged_attn_tc_kernel<int>, ctas, kTcThreads, kTcSmem, s, maps, a);
+    if (e == cudaSuccess)
+      e = launch_k(paged_attn_join_kernel<kTcRows, 1>, dim3((unsigned)ctas, kTcRows / 16), 256, 0, s, a, ctas);
   }
   if (e != cudaSuccess) {
     set_err(err, errlen, "%s: %s", what, cudaGetErrorString(e));
