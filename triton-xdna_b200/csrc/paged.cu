@@ -251,7 +251,7 @@ struct Found {
 // A walk over one piece [lo, hi) of the line.
 template <typename I>
 struct Walk {
-  I lo, hi;
+  I lo, hi, share;
   int snap;  // cuts this close to a unit's end or first key move there
   I u0;    // where the current unit starts
   I ulen;  // its weight
@@ -267,6 +267,7 @@ struct Segment {
   int keys;          // keys the unit's last token sees; 0 when none of its tokens sees any
   int t0, t1;        // key tiles of this part
   int starts, ends;  // the unit starts / ends in this piece
+  int last;          // where it starts and goes on: the piece in which it ends
 };
 
 // Share of `pieces` equal pieces of the line: at least total / pieces (the
@@ -350,6 +351,7 @@ __device__ __forceinline__ I unit_weight(const AttnArgs& a, const Walk<I>& w) {
 // Places a walk at piece `piece`'s start.
 template <typename I>
 __device__ __forceinline__ void place(const AttnArgs& a, Walk<I>& w, int piece, I share, I total, const Found<I>& f) {
+  w.share = share;
   w.snap = cut_snap(a, share);
   w.lo = piece * share;
   w.hi = total - w.lo < share ? total : w.lo + share;
@@ -419,44 +421,54 @@ __device__ __forceinline__ bool segment(const AttnArgs& a, Walk<I>& w, Segment& 
     const int nk = (int)(((unsigned)g.keys + TK - 1) / TK);
     g.t0 = g.starts ? 0 : min((int)((unsigned)(cut0 - a.over) / TK), nk);  // cuts fall on tile boundaries
     g.t1 = g.ends ? nk : min((int)((unsigned)(cut1 - a.over) / TK), nk);
+    if (g.starts && !g.ends) {
+      // the piece that holds the unit's last key, or the one before it if that cut was moved to the unit's end
+      const I end = w.u0 + w.ulen;
+      I last = (end - 1) / w.share;
+      if (last * w.share > w.u0 && end - last * w.share < w.snap) --last;
+      g.last = (int)last;
+    }
     return true;
   }
 }
 
-// The piece in which the current unit ends: the one that holds its last key,
-// or the one before it if that cut was moved to the unit's end.
-template <typename I>
-__device__ __forceinline__ int unit_last(const AttnArgs& a, const Walk<I>& w, I share) {
-  const I end = w.u0 + w.ulen;
-  I last = (end - 1) / share;
-  if (last * share > w.u0 && end - last * share < w.snap) --last;
-  return (int)last;
-}
-
 // ----------------------------------------------------------------------------- attention: few rows (mma.sync)
 //
-// For batches whose sequences bring few tokens each (decoding, verification
-// of drafted tokens): at most 16 rows per unit, the rows of an mma.sync
-// m16n8k16 tile (rows past n_rep * tokens are zero; with 8 rows at most, ROWS
-// leaves out the other half of the softmax), so the kernel is bound by reading K
-// and V.  Every warp of the grid has a piece of the line of its own
+// For batches whose sequences bring few tokens each (decoding, verification of
+// drafted tokens): at most 8 or 16 rows per unit, so the kernel is bound by
+// reading K and V.  Every warp of the grid has a piece of the line of its own
 // and runs through it alone: its lanes issue the TMA loads of a 32-key tile's
 // page rows (128-byte swizzle) into one of the warp's two buffers, the next
 // unit's tiles while the present one is computed, and the warp keeps an online
 // softmax (running max and sum in fp32, P rounded to bf16 for P V as in the
 // contiguous kernels).  8 warps x 2 buffers x 8 KB keep up to 128 KB per SM in
-// flight.  A unit inside one warp's piece goes straight to the output; parts
-// of one that spans warps of the CTA meet in shared memory after the CTA's
-// only barrier, and what spans CTAs goes on to the joining kernel.
+// flight.  The products run transposed on mma.sync m16n8k16, S^T = K Q^T and
+// O^T = V^T P^T: keys and dims fill the 16 rows and the query rows the 8
+// columns, so 8 rows take 16 MMAs a tile; with the query rows in the 16-row
+// place they took 32, and those were the longest part of a short call (0.7 of
+// the 1.4 us of two tiles).  A unit inside one warp's piece goes straight to
+// the output; parts of one that spans warps of the CTA meet in shared memory
+// after the CTA's only barrier, and what spans CTAs goes on to the joining
+// kernel.  Calls of few keys are bound by latency and by fetching instructions
+// (each line is cold in a new launch): every long piece of code is there once.
 constexpr int kHD = 64;
-constexpr int kWarps = 8, kBufs = 2, kTK = 32;
+constexpr int kTK = 32;
 constexpr int kTileBytes = kTK * kHD * 2;  // one K or V tile
-constexpr int kWarpRing = kBufs * 2 * kTileBytes;
-constexpr int kFewRows = 16;
-constexpr int kPartLd = kHD + 8;  // row pitch of a partial in shared memory: conflict-free 8-byte stores
-constexpr int kHeadBytes = kFewRows * kPartLd * 4;
-constexpr int kFewSmem = kWarps * (kWarpRing + kHeadBytes) + 1024;
-static_assert(kHeadBytes <= kWarpRing, "a warp's last partial goes into its own ring");
+constexpr int kFewRows = 16;               // rows of a partial in the workspace
+constexpr int kQueue = 4;                  // segments a warp's requests may be ahead of its computation
+constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared memory: conflict-free stores
+// 12 warps x 2 buffers and 8 x 3 of the 8-row kernel measured no faster
+// (64 sequences of 576 keys: 12.1 and 11.0 us, 8 x 2 11.0; 160 long ones 87.4
+// and 90.2, 8 x 2 86.1).
+template <int ROWS>
+struct FewCfg {
+  static constexpr int kWarps = 8, kBufs = 2;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kRing = kBufs * 2 * kTileBytes;  // of one warp
+  static constexpr int kHead = ROWS * kPartLd * 4;      // a warp's kind 0 partial; kind 1 goes into its own ring
+  static constexpr int kSmem = kWarps * (kRing + kHead) + 1024;
+  static_assert(kHead <= kRing && kSmem <= 224 * 1024, "shared memory");
+};
 
 struct alignas(64) KvMaps {
   CUtensorMap k, v;  // [n_pages][KVH][page][64], box {64, box_rows, 1, 1}
@@ -496,16 +508,15 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                : "memory");
 }
 
+// transposes an 8 x 8 matrix of 16-bit elements held one row per four lanes
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 // floats of one partial: O [rows][64], then max [rows], then sum [rows]
 __host__ __device__ constexpr int64_t part_floats(int rows) { return (int64_t)rows * (kHD + 2); }
-
-// A warp's part of a unit that it does not cover alone.
-struct Part {
-  int token, rows, kvh;
-  int ends;   // the unit ends in this warp's piece
-  int last;   // (parts that start a unit) the piece in which it ends
-  int valid;
-};
 
 __device__ __forceinline__ void store_out4(const AttnArgs& a, int token, int kvh, int r, int d, float4 v) {
   const int tok = row_token(a, r);
@@ -517,32 +528,39 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int token, int kvh
 }
 
 template <int ROWS, typename I>
-__global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __grid_constant__ KvMaps maps,
+__global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kernel(const __grid_constant__ KvMaps maps,
                                                                         const AttnArgs a) {
+  using C = FewCfg<ROWS>;
+  constexpr int kWarps = C::kWarps, kBufs = C::kBufs;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kWarps][kBufs];
   __shared__ I sums[2][kWarps];
   __shared__ Found<I> found[kWarps];
-  __shared__ Part part[2][kWarps];  // [0]: of a unit that started before, [1]: of one that goes on
-  __shared__ float part_m[2][kWarps][kFewRows], part_l[2][kWarps][kFewRows];
+  // A warp's parts of units that it does not cover alone: kind 0 of one that
+  // started before its piece, kind 1 of one that goes on behind it.
+  __shared__ Segment part[2][kWarps];
+  __shared__ float part_m[2][kWarps][ROWS], part_l[2][kWarps][ROWS];
+  __shared__ uint32_t comes, ends0, opens;  // one bit per warp: has a kind 0, its unit ends there, has a kind 1
+  __shared__ Segment queue[kWarps][kQueue];
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
+  constexpr int NT = ROWS / 8;  // 8-row column tiles
   const uint32_t base_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base_u32 - smem_u32(smem_raw));
-  const uint32_t ring = base_u32 + warp * kWarpRing;
+  const uint32_t ring = base_u32 + warp * C::kRing;
   // O of the two kinds of parts: the first beside the ring, the second, the
   // last thing a warp does, in its ring
   auto part_o = [&](int kind, int w_) -> float* {
-    return reinterpret_cast<float*>(kind == 0 ? smem + kWarps * kWarpRing + w_ * kHeadBytes : smem + w_ * kWarpRing);
+    return reinterpret_cast<float*>(kind == 0 ? smem + kWarps * C::kRing + w_ * C::kHead : smem + w_ * C::kRing);
   };
   if (lane == 0) {
     for (int i = 0; i < kBufs; ++i) mbar_init(&full[warp][i], 1);
     mbar_fence_init();
-    part[0][warp].valid = part[1][warp].valid = 0;
   }
   if (threadIdx.x == 0) {
     abort_flag = 0;
+    comes = ends0 = opens = 0;
     prefetch_tmap(&maps.k);
     prefetch_tmap(&maps.v);
   }
@@ -550,7 +568,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
   pdl_trigger();
   I total;
   const I share =
-      find_pieces<kWarps * 32, kWarps, I>(a, gridDim.x * kWarps, blockIdx.x * kWarps, sums, found, &total);
+      find_pieces<C::kThreads, kWarps, I>(a, gridDim.x * kWarps, blockIdx.x * kWarps, sums, found, &total);
   Meta* meta = reinterpret_cast<Meta*>(a.ws + 2 * (int64_t)gridDim.x * part_floats(kFewRows));
   if (found[0].b < 0) {  // no warp of this CTA has work
     if (threadIdx.x == 0) meta[blockIdx.x].last = -1;
@@ -559,45 +577,53 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
   if (found[warp].b >= 0) {
     const int boxes = kTK / a.box_rows;
     const bool is_v = lane >= boxes;
-    const int box = is_v ? lane - boxes : lane;
+    const int box = lane & (boxes - 1);  // boxes: a power of two
     const CUtensorMap* map = is_v ? &maps.v : &maps.k;
-    const int tok0 = row_token(a, g), tok1 = row_token(a, g + 8);  // the tokens of this thread's two rows
-    // two walks over the piece: one requests tiles, one computes them
-    Walk<I> wi, wc;
+    // This thread's rows: 8 n + 2 t and the next one, and the tokens they belong to
+    int tok[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) tok[n][e] = row_token(a, 8 * n + 2 * t + e);
+    // The walk runs with the requests; the computation follows through a small
+    // queue of segments.
+    Walk<I> wi;
     Segment si, sc;
     place(a, wi, (int)blockIdx.x * kWarps + warp, share, total, found[warp]);
-    bool more = segment<kTK>(a, wi, si);
-    wc = wi;
-    sc = si;
-    bool more_i = more;
-    int ni = si.t0;  // next tile to request
+    bool fresh = true, more_i = true;
+    si.t1 = 0;
+    sc.t1 = 0;
+    int ni = 0;  // next tile to request
+    uint32_t pushed = 0, popped = 0;
     uint32_t use = 0, issued = 0;  // tiles read / requested: buffer n % kBufs, parity (n / kBufs) & 1
     bool dead = false;  // a wait ran out: no more loads, the output is not valid
     // 32 entries of the page table row from page `win` on, one per lane: one
     // latency for many tiles
     uint32_t win = 0;
     int win_id = 0;
+    int pi = 0, row = 0;  // page index and row of this lane's box of the next tile
     auto window = [&](uint32_t first) {
       win = first;
-      const uint32_t pi = first + lane;
-      win_id = pi * (uint64_t)a.page_size < (uint32_t)si.keys ? __ldg(a.table + si.b * a.ld_table + pi) : -1;
+      const uint32_t p = first + lane;
+      win_id = p * (uint64_t)a.page_size < (uint32_t)si.keys ? __ldg(a.table + si.b * a.ld_table + p) : -1;
     };
-    auto settle = [&](bool fresh) {  // the request walk on a tile, if any is left
-      while (more_i && ni >= si.t1) {
-        more_i = next_unit(a, wi) && segment<kTK>(a, wi, si);
-        ni = si.t0;
-        fresh = true;
+    auto enter = [&]() {  // the first tile of a segment
+      const uint32_t key = (uint32_t)(ni * kTK);
+      const uint32_t p = key / (uint32_t)a.page_size;
+      window(p);
+      pi = (int)p;
+      row = (int)(key - p * (uint32_t)a.page_size) + box * a.box_rows;
+      while (row >= a.page_size) {
+        row -= a.page_size;
+        ++pi;
       }
-      if (more_i && fresh) window((uint32_t)(ni * kTK) / (uint32_t)a.page_size);
     };
     // lanes 0 .. boxes - 1 load K rows, the next `boxes` lanes V rows
     auto request = [&]() {
       const uint32_t buf = issued % kBufs;
       const int k0 = ni * kTK, have = min(kTK, si.keys - k0);
       const int nb = (have + a.box_rows - 1) / a.box_rows;
-      const uint32_t key = (uint32_t)(k0 + min(box, nb - 1) * a.box_rows);
-      const uint32_t pi = key / (uint32_t)a.page_size;
-      if (__any_sync(0xffffffffu, pi - win >= 32u)) window((uint32_t)k0 / (uint32_t)a.page_size);
+      if (__any_sync(0xffffffffu, box < nb && pi - win >= 32u)) window(__shfl_sync(0xffffffffu, (uint32_t)pi, 0));
       int id = __shfl_sync(0xffffffffu, win_id, (int)(pi - win));
       if (lane == 0) mbar_arrive_expect_tx(&full[warp][buf], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
       __syncwarp();
@@ -607,39 +633,52 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
           id = a.n_pages;
         }
         tma_load_4d(ring + buf * 2 * kTileBytes + (is_v ? kTileBytes : 0) + box * a.box_rows * kHD * 2, map,
-                    &full[warp][buf], 0, (int)(key - pi * a.page_size), si.kvh, id);
+                    &full[warp][buf], 0, row, si.kvh, id);
+      }
+      row += kTK;
+      while (row >= a.page_size) {
+        row -= a.page_size;
+        ++pi;
       }
       ++issued;
       ++ni;
-      settle(false);
     };
-    uint32_t qa[4][4];
+    uint32_t qb[NT][4][2];
     auto load_q = [&]() {
-      const bool ok0 = g < sc.rows, ok1 = g + 8 < sc.rows;
-      const bf16* p0 = a.q + (int64_t)(sc.token + tok0) * a.ld_q + (sc.kvh * a.n_rep + g - tok0 * a.n_rep) * kHD;
-      const bf16* p1 = a.q + (int64_t)(sc.token + tok1) * a.ld_q + (sc.kvh * a.n_rep + g + 8 - tok1 * a.n_rep) * kHD;
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const int c = kk * 16 + 2 * t;
-        qa[kk][0] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c) : 0u;
-        qa[kk][1] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c) : 0u;
-        qa[kk][2] = ok0 ? *reinterpret_cast<const uint32_t*>(p0 + c + 8) : 0u;
-        qa[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(p1 + c + 8) : 0u;
+      for (int n = 0; n < NT; ++n) {
+        const int r = 8 * n + g, tk = row_token(a, r);
+        const bf16* p = a.q + (int64_t)(sc.token + tk) * a.ld_q + (sc.kvh * a.n_rep + r - tk * a.n_rep) * kHD + 2 * t;
+        const bool in = r < sc.rows;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          qb[n][kk][0] = in ? *reinterpret_cast<const uint32_t*>(p + kk * 16) : 0u;
+          qb[n][kk][1] = in ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 8) : 0u;
+        }
       }
     };
-    settle(true);
-    if (more) load_q();
-    while (more_i && issued < kBufs) request();
-
-    while (more) {
-      // the last key each of this thread's rows sees
-      const int pos0 = min(sc.first_pos + tok0, sc.keys - 1), pos1 = min(sc.first_pos + tok1, sc.keys - 1);
-      const int first_pos = min(sc.first_pos, sc.keys - 1);  // the last one that every row sees
-      float o[8][4];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-      for (int tile = sc.t0; tile < sc.t1 && !dead; ++tile) {
+    int pos[NT][2], first_pos = 0;  // the last keys that this thread's rows see, and that every row sees
+    int tile = 0;
+    float o[NT][4][4], m[NT][2], l[NT][2];
+    for (;;) {
+      while (more_i) {
+        if (ni < si.t1) {
+          if (issued - use == kBufs) break;
+          request();
+        } else {
+          if (pushed - popped == kQueue) break;
+          more_i = (fresh || next_unit(a, wi)) && segment<kTK>(a, wi, si);
+          fresh = false;
+          if (!more_i) break;
+          if (lane == 0) queue[warp][pushed % kQueue] = si;
+          __syncwarp();
+          ++pushed;
+          ni = si.t0;
+          if (ni < si.t1) enter();
+          if (tile < sc.t1) break;  // compute meanwhile
+        }
+      }
+      if (tile < sc.t1) {
         const uint32_t buf = use % kBufs;
         const bool landed = mbar_wait(&full[warp][buf], (use / kBufs) & 1, kWaitLimit, &abort_flag);
         if (__any_sync(0xffffffffu, !landed)) {
@@ -659,124 +698,156 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
           fence_proxy_async_smem();  // before a later TMA write to the buffer
           __syncwarp();
         }
-        float s[4][4];
+        // S^T = K Q^T: keys are the MMA's 16 rows, query rows its 8 columns
+        float s[NT][2][4];
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+        for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {  // dims 32 h .. 32 h + 31: four 16-byte chunks of the key rows
-            const int r = nt * 8 + (lane & 7), c = 4 * h + (lane >> 3);
-            uint32_t kb[4];
-            ldsm4(kb, sk + r * 128 + ((c ^ (r & 7)) << 4));
-            mma_16816(s[nt], qa[2 * h], kb[0], kb[1]);
-            mma_16816(s[nt], qa[2 * h + 1], kb[2], kb[3]);
+          for (int n = 0; n < NT; ++n) s[n][mt][0] = s[n][mt][1] = s[n][mt][2] = s[n][mt][3] = 0.0f;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const int mi = lane >> 3, r = mt * 16 + (mi & 1) * 8 + (lane & 7), c = 2 * kk + (mi >> 1);
+            uint32_t ka[4];
+            ldsm4(ka, sk + r * 128 + ((c ^ (r & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816(s[n][mt], ka, qb[n][kk][0], qb[n][kk][1]);
           }
         }
         if (k0 + kTK - 1 > first_pos) {  // some row does not see the whole tile
 #pragma unroll
-          for (int nt = 0; nt < 4; ++nt)
+          for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-            for (int e = 0; e < ROWS / 4; ++e) {
-              const int key = k0 + nt * 8 + 2 * t + (e & 1);
-              if (key > (e < 2 ? pos0 : pos1)) s[nt][e] = -INFINITY;
+            for (int e = 0; e < 4; ++e) {
+              const int key = k0 + mt * 16 + g + (e >> 1) * 8;
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                if (key > pos[n][e & 1]) s[n][mt][e] = -INFINITY;
             }
         }
-        // raw scores: the scale is positive, so their maximum scales to the scaled ones'
-        float mx0 = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])),
-                          fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
-        float mx1 = -INFINITY;
-        if (ROWS > 8)
-          mx1 = fmaxf(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])),
-                      fmaxf(fmaxf(s[2][2], s[2][3]), fmaxf(s[3][2], s[3][3])));
+        uint32_t pb[NT][4];  // P as the B operand of O^T = V^T P^T, 8 keys each
 #pragma unroll
-        for (int o_ = 1; o_ <= 2; o_ <<= 1) {
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o_));
-          if (ROWS > 8) mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o_));
-        }
-        const float mn0 = fmaxf(m0, mx0 * a.scale_log2), mn1 = ROWS > 8 ? fmaxf(m1, mx1 * a.scale_log2) : m1;
-        const float base0 = mn0 == -INFINITY ? 0.0f : mn0, base1 = mn1 == -INFINITY ? 0.0f : mn1;
-        if (__any_sync(0xffffffffu, mn0 > m0 || mn1 > m1)) {  // some row's maximum moved
-          const float al0 = ex2_approx(m0 - base0), al1 = ex2_approx(m1 - base1);
-          l0 *= al0;
-          l1 *= al1;
+        for (int n = 0; n < NT; ++n) {
+          float base[2], al[2];
+          bool moved = false;
 #pragma unroll
-          for (int dt = 0; dt < 8; ++dt) {
-            o[dt][0] *= al0;
-            o[dt][1] *= al0;
-            if (ROWS > 8) o[dt][2] *= al1;
-            if (ROWS > 8) o[dt][3] *= al1;
+          for (int e = 0; e < 2; ++e) {
+            // raw scores: the scale is positive, so their maximum scales to the scaled ones'
+            float mx = fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2]));
+#pragma unroll
+            for (int o_ = 4; o_ <= 16; o_ <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o_));
+            const float mn = fmaxf(m[n][e], mx * a.scale_log2);
+            base[e] = mn == -INFINITY ? 0.0f : mn;
+            al[e] = ex2_approx(m[n][e] - base[e]);
+            moved |= mn > m[n][e];
+            m[n][e] = mn;
+          }
+          if (__any_sync(0xffffffffu, moved)) {
+            l[n][0] *= al[0];
+            l[n][1] *= al[1];
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+              o[n][mt][0] *= al[0];
+              o[n][mt][1] *= al[1];
+              o[n][mt][2] *= al[0];
+              o[n][mt][3] *= al[1];
+            }
+          }
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[n][mt][e] = ex2_approx(fmaf(s[n][mt][e], a.scale_log2, -base[e & 1]));
+              l[n][e & 1] += s[n][mt][e];
+            }
+            pb[n][2 * mt] = transpose8(pack2(s[n][mt][0], s[n][mt][1]));
+            pb[n][2 * mt + 1] = transpose8(pack2(s[n][mt][2], s[n][mt][3]));
           }
         }
-        m0 = mn0;
-        m1 = mn1;
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          s[nt][0] = ex2_approx(fmaf(s[nt][0], a.scale_log2, -base0));
-          s[nt][1] = ex2_approx(fmaf(s[nt][1], a.scale_log2, -base0));
-          l0 += s[nt][0] + s[nt][1];
-          if (ROWS > 8) {
-            s[nt][2] = ex2_approx(fmaf(s[nt][2], a.scale_log2, -base1));
-            s[nt][3] = ex2_approx(fmaf(s[nt][3], a.scale_log2, -base1));
-            l1 += s[nt][2] + s[nt][3];
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {  // dims 16 mt .. 16 mt + 15
+            const int mi = lane >> 3, r = ks * 16 + (mi >> 1) * 8 + (lane & 7), c = 2 * mt + (mi & 1);
+            uint32_t va[4];
+            ldsm4_t(va, sv + r * 128 + ((c ^ (r & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816(o[n][mt], va, pb[n][2 * ks], pb[n][2 * ks + 1]);
           }
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          uint32_t pa[4];
-          pa[0] = pack2(s[2 * kk][0], s[2 * kk][1]);
-          pa[1] = ROWS > 8 ? pack2(s[2 * kk][2], s[2 * kk][3]) : 0u;
-          pa[2] = pack2(s[2 * kk + 1][0], s[2 * kk + 1][1]);
-          pa[3] = ROWS > 8 ? pack2(s[2 * kk + 1][2], s[2 * kk + 1][3]) : 0u;
-#pragma unroll
-          for (int dt = 0; dt < 8; dt += 2) {
-            const int mi = lane >> 3, r = kk * 16 + (mi & 1) * 8 + (lane & 7), c = dt + (mi >> 1);
-            uint32_t vb[4];
-            ldsm4_t(vb, sv + r * 128 + ((c ^ (r & 7)) << 4));
-            mma_16816(o[dt], pa, vb[0], vb[1]);
-            mma_16816(o[dt + 1], pa, vb[2], vb[3]);
-          }
-        }
         ++use;
+        ++tile;
         __syncwarp();  // the buffer is read: it takes a tile further on
-        if (more_i) request();
+        if (tile < sc.t1) continue;
+      } else {
+        // the next segment
+        if (popped == pushed) break;
+        sc = queue[warp][popped % kQueue];
+        ++popped;
+        __syncwarp();
+        load_q();
+        tile = sc.t0;
+        first_pos = min(sc.first_pos, sc.keys - 1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            pos[n][e] = min(sc.first_pos + tok[n][e], sc.keys - 1);
+            m[n][e] = -INFINITY;
+            l[n][e] = 0.0f;
+          }
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) o[n][mt][0] = o[n][mt][1] = o[n][mt][2] = o[n][mt][3] = 0.0f;
+        }
+        if (tile < sc.t1) continue;
       }
 #pragma unroll
-      for (int o_ = 1; o_ <= 2; o_ <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, o_);
-        if (ROWS > 8) l1 += __shfl_xor_sync(0xffffffffu, l1, o_);
-      }
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int o_ = 4; o_ <= 16; o_ <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o_);
       if (sc.starts && sc.ends) {
-        const float i0 = l0 == 0.0f ? 0.0f : 1.0f / l0, i1 = l1 == 0.0f ? 0.0f : 1.0f / l1;  // no key: zeros
-        bf16* p0 = a.out + (int64_t)(sc.token + tok0) * a.ld_out + (sc.kvh * a.n_rep + g - tok0 * a.n_rep) * kHD;
-        bf16* p1 = a.out + (int64_t)(sc.token + tok1) * a.ld_out + (sc.kvh * a.n_rep + g + 8 - tok1 * a.n_rep) * kHD;
+        // neighbours in g swap a row each, so that a thread stores two dims of one row
+        const int odd = g & 1;
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-          const int d = dt * 8 + 2 * t;
-          if (g < sc.rows) *reinterpret_cast<uint32_t*>(p0 + d) = pack2(o[dt][0] * i0, o[dt][1] * i0);
-          if (ROWS > 8 && g + 8 < sc.rows) *reinterpret_cast<uint32_t*>(p1 + d) = pack2(o[dt][2] * i1, o[dt][3] * i1);
+        for (int n = 0; n < NT; ++n) {
+          const float i0 = l[n][0] == 0.0f ? 0.0f : 1.0f / l[n][0];  // no key: zeros
+          const float i1 = l[n][1] == 0.0f ? 0.0f : 1.0f / l[n][1];
+          const int r = 8 * n + 2 * t + odd, tk = odd ? tok[n][1] : tok[n][0];
+          bf16* p = a.out + (int64_t)(sc.token + tk) * a.ld_out + (sc.kvh * a.n_rep + r - tk * a.n_rep) * kHD + (g & 6);
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float x0 = o[n][mt][2 * h] * i0, x1 = o[n][mt][2 * h + 1] * i1;
+              const float got = __shfl_xor_sync(0xffffffffu, odd ? x0 : x1, 4);
+              const uint32_t pk = odd ? pack2(got, x1) : pack2(x0, got);
+              if (r < sc.rows) *reinterpret_cast<uint32_t*>(p + mt * 16 + h * 8) = pk;
+            }
         }
       } else {
         const int kind = sc.starts ? 1 : 0;
         float* po = part_o(kind, warp);
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-          const int d = dt * 8 + 2 * t;
-          *reinterpret_cast<float2*>(po + g * kPartLd + d) = make_float2(o[dt][0], o[dt][1]);
-          if (ROWS > 8) *reinterpret_cast<float2*>(po + (g + 8) * kPartLd + d) = make_float2(o[dt][2], o[dt][3]);
-        }
-        if (t == 0) {
-          part_m[kind][warp][g] = m0;
-          part_l[kind][warp][g] = l0;
-          if (ROWS > 8) {
-            part_m[kind][warp][g + 8] = m1;
-            part_l[kind][warp][g + 8] = l1;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = 8 * n + 2 * t + e;
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+              po[r * kPartLd + mt * 16 + g] = o[n][mt][e];
+              po[r * kPartLd + mt * 16 + g + 8] = o[n][mt][e + 2];
+            }
+            if (g == 0) {
+              part_m[kind][warp][r] = m[n][e];
+              part_l[kind][warp][r] = l[n][e];
+            }
           }
+        if (lane == 0) {
+          part[kind][warp] = sc;
+          atomicOr(kind ? &opens : &comes, 1u << warp);
+          if (!kind && sc.ends) atomicOr(&ends0, 1u << warp);
         }
-        if (lane == 0)
-          part[kind][warp] = Part{sc.token, sc.rows, sc.kvh, sc.ends, kind ? unit_last(a, wc, share) : 0, 1};
       }
-      more = next_unit(a, wc) && segment<kTK>(a, wc, sc);
-      if (more) load_q();
     }
     if (dead) {  // loads still in flight land before the CTA's shared memory is given up
       uint64_t deadline = 0;
@@ -786,62 +857,49 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_few_kernel(const __
   }
   __syncthreads();
   // Chains of parts: one that came in from the CTA before (its parts start with
-  // warp 0's first kind), and one from every warp whose piece starts a unit
-  // that goes on.  They go on through the first kind of the next warps until
-  // one ends the unit, or leave the CTA.
-  // The warp that starts a chain joins it; the one that came in is the job of
-  // the warp it ends in.
-  const uint32_t mine = lane < kWarps ? 1u : 0u;
-  const uint32_t in0 = __ballot_sync(0xffffffffu, mine && part[0][lane & (kWarps - 1)].valid);
-  const uint32_t end0 = __ballot_sync(0xffffffffu, mine && part[0][lane & (kWarps - 1)].valid &&
-                                                       part[0][lane & (kWarps - 1)].ends);
-  const uint32_t open1 = __ballot_sync(0xffffffffu, mine && part[1][lane & (kWarps - 1)].valid);
-  const int last_end = 31 - __clz((int)(end0 | 1u));  // the last warp in which a unit ends (or 0)
-  const bool open_unit = open1 != 0 && (end0 == 0 || (open1 >> last_end) != 0);
-  for (int job = 0; job < 2; ++job) {
-    // job 0: the chain that came in, if it ends (or leaves the CTA) in this warp; job 1: the one this warp starts
-    const int c = job == 0 ? -1 : warp;
-    const uint32_t ahead = job == 0 ? end0 : end0 & (0xfffffffeu << warp);
-    const bool ends = ahead != 0;
-    const int end = ends ? __ffs((int)ahead) - 1 : kWarps - 1;
-    if (job == 0 ? !(in0 & 1u) || warp != end : !(open1 >> warp & 1u)) continue;
-    const Part p = part[c >= 0][max(c, 0)];
-    const bool whole = c >= 0 && ends;
-    if (c >= 0 && !ends && lane == 0) meta[blockIdx.x] = Meta{p.last / kWarps, p.token, p.rows, p.kvh};
-    float* out_part = a.ws + (2 * (int64_t)blockIdx.x + (c >= 0)) * part_floats(kFewRows);
-    const int first = max(c, 0);
-    if (lane < p.rows) {  // the factor of each part for this lane's row, in the place of its max
+  // warp 0's kind 0), and one from every warp with a kind 1.  A chain goes on
+  // through the kind 0 of the next warps until one ends the unit, or leaves
+  // the CTA.  The CTA's threads form a team per chain (2, 4 or 8 of them when
+  // there are several); a thread has one row's 16-byte column at a time.
+  uint32_t chains = (opens << 1) | (comes & 1u);
+  const int count = __popc(chains), teams = count <= 1 ? 1 : count == 2 ? 2 : count <= 4 ? 4 : 8;
+  const int size = C::kThreads / teams, team = threadIdx.x / size;
+  bool open_unit = false;
+  for (int n = 0; chains; chains &= chains - 1, ++n) {
+    const int c = __ffs((int)chains) - 2;  // the warp of the kind 1, or -1
+    const uint32_t ahead = ends0 & (0xffffffffu << (c + 1));
+    const int first = max(c, 0), end = ahead ? __ffs((int)ahead) - 1 : kWarps - 1;
+    const Segment& p = part[c >= 0][first];
+    const bool whole = c >= 0 && ahead;
+    open_unit |= c >= 0 && !ahead;
+    if ((n & (teams - 1)) != team) continue;
+    for (int i = threadIdx.x % size; i < p.rows * 16; i += size) {
+      const int r = i / 16, d = (i % 16) * 4;
       float M = -INFINITY, l = 0.0f;
-      for (int k = first; k <= end; ++k) M = fmaxf(M, part_m[k == c][k][lane]);
-      const float base = M == -INFINITY ? 0.0f : M;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = first; k <= end; ++k) {
-        const float f = ex2_approx(part_m[k == c][k][lane] - base);
-        part_m[k == c][k][lane] = f;
-        l += part_l[k == c][k][lane] * f;
+        const float m = part_m[k == c][k][r], mn = fmaxf(M, m), base = mn == -INFINITY ? 0.0f : mn;
+        const float f0 = ex2_approx(M - base), f = ex2_approx(m - base);
+        const float4 v = *reinterpret_cast<const float4*>(part_o(k == c, k) + r * kPartLd + d);
+        acc.x = acc.x * f0 + v.x * f;
+        acc.y = acc.y * f0 + v.y * f;
+        acc.z = acc.z * f0 + v.z * f;
+        acc.w = acc.w * f0 + v.w * f;
+        l = l * f0 + part_l[k == c][k][r] * f;
+        M = mn;
       }
       if (whole) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        for (int k = first; k <= end; ++k) part_m[k == c][k][lane] *= inv;
+        store_out4(a, p.token, p.kvh, r, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
       } else {
-        out_part[kFewRows * kHD + lane] = M;
-        out_part[kFewRows * kHD + kFewRows + lane] = l;
+        float* out_part = a.ws + (2 * (int64_t)blockIdx.x + (c >= 0)) * part_floats(kFewRows);
+        *reinterpret_cast<float4*>(out_part + r * kHD + d) = acc;
+        if (d == 0) {
+          out_part[kFewRows * kHD + r] = M;
+          out_part[kFewRows * kHD + kFewRows + r] = l;
+          if (r == 0 && c >= 0) meta[blockIdx.x] = Meta{p.last / kWarps, p.token, p.rows, p.kvh};
+        }
       }
-    }
-    __syncwarp();
-    for (int i = lane; i < p.rows * (kHD / 4); i += 32) {
-      const int r = i / (kHD / 4), d = (i % (kHD / 4)) * 4;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-      for (int k = first; k <= end; ++k) {
-        const float f = part_m[k == c][k][r];
-        const float4 v = *reinterpret_cast<const float4*>(part_o(k == c, k) + r * kPartLd + d);
-        acc.x += v.x * f;
-        acc.y += v.y * f;
-        acc.z += v.z * f;
-        acc.w += v.w * f;
-      }
-      if (whole) store_out4(a, p.token, p.kvh, r, d, acc);
-      else *reinterpret_cast<float4*>(out_part + r * kHD + d) = acc;
     }
   }
   if (!open_unit && threadIdx.x == 0) meta[blockIdx.x].last = -1;
@@ -1002,7 +1060,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     for (; more && ok; more = next_unit(a, w) && segment<kTcTK>(a, w, s)) {
       if (s.starts && !s.ends) {
         open_unit = true;
-        if (lane == 0) meta[blockIdx.x] = Meta{unit_last(a, w, share), s.token, s.rows, s.kvh};
+        if (lane == 0) meta[blockIdx.x] = Meta{s.last, s.token, s.rows, s.kvh};
       }
       ok = publish(s.rows);
       if (!ok) break;
@@ -1460,6 +1518,12 @@ cudaError_t launch_main(void (*kernel)(M, AttnArgs), int ctas, int threads, int 
   return e != cudaSuccess ? e : launch_k(kernel, (unsigned)ctas, threads, smem, s, maps, a);
 }
 
+template <int ROWS, typename I>
+cudaError_t launch_few(int ctas, cudaStream_t s, const KvMaps& maps, const AttnArgs& a) {
+  using C = FewCfg<ROWS>;
+  return launch_main(paged_attn_few_kernel<ROWS, I>, ctas, C::kThreads, C::kSmem, s, maps, a);
+}
+
 template <int N>
 cudaError_t launch_copy(const int32_t* src, const int32_t* dst, int n, uint8_t* base, int64_t outer,
                         int64_t outer_stride, int64_t page_stride, uint32_t vpp, cudaStream_t s) {
@@ -1739,17 +1803,17 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
   // query tiles per KV head, each of at most the table's positions.  With the
   // pieces' rounding it stays an int below 2^30.
   const double most = ((double)tokens / a.tpt + batch) * n_kv_head * ((double)max_pages * page_size + a.over + a.tpt);
-  const bool wide = most + (double)a.min_share * ctas * kWarps >= (double)(1 << 30);
+  const bool wide = most + (double)a.min_share * ctas * 16 >= (double)(1 << 30);
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
   if (few) {
     KvMaps kv;
     kv.k = maps.k;
     kv.v = maps.v;
-    e = eight ? (wide ? launch_main(paged_attn_few_kernel<8, int64_t>, ctas, kWarps * 32, kFewSmem, s, kv, a)
-                      : launch_main(paged_attn_few_kernel<8, int>, ctas, kWarps * 32, kFewSmem, s, kv, a))
-              : (wide ? launch_main(paged_attn_few_kernel<16, int64_t>, ctas, kWarps * 32, kFewSmem, s, kv, a)
-                      : launch_main(paged_attn_few_kernel<16, int>, ctas, kWarps * 32, kFewSmem, s, kv, a));
+    e = eight ? (wide ? launch_few<8, int64_t>(ctas, s, kv, a)
+                      : launch_few<8, int>(ctas, s, kv, a))
+              : (wide ? launch_few<16, int64_t>(ctas, s, kv, a)
+                      : launch_few<16, int>(ctas, s, kv, a));
     if (e == cudaSuccess)
       e = launch_k(paged_attn_join_kernel<kFewRows, 4>, dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
   } else {
