@@ -952,11 +952,48 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+// 16 columns of the warp's TMEM lanes
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Two fp32 at a time: one instruction for a pair, each rounded as on its own.
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n"
+      " mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return d;
+}
+
 template <typename I>
 __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __grid_constant__ TcMaps maps,
                                                                       const AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], drain_bar, o_full, o_empty;
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], drain_bar, o_full[2], o_empty;
   __shared__ __align__(8) uint64_t s_full[2], p_full[2];
   __shared__ __align__(8) uint64_t kv_full[kTcStages], kv_empty[kTcStages];
   __shared__ __align__(8) uint64_t seg_full[kTcSegs], seg_empty[kTcSegs];
@@ -972,15 +1009,15 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
 
   if (threadIdx.x == 0) {
     mbar_init(&drain_bar, 1);
-    mbar_init(&o_full, 1);     // one P V accumulated into O
     mbar_init(&o_empty, 128);  // a unit's O read by the softmax warps
     for (int i = 0; i < kTcSegs; ++i) {
       mbar_init(&seg_full[i], 1);
       mbar_init(&seg_empty[i], 5);  // the MMA warp and the four softmax warps
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&o_full[i], 1);  // P V of an even / odd tile accumulated into O
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
+      mbar_init(&q_empty[i], 128);  // Q's buffer, which the output passes through, free
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
     }
@@ -1139,7 +1176,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
       for (int ks = 0; ks < 4; ++ks)  // keys in steps of 16: 8 columns of P
         mma_f16_ts(tmem + 128, p + ks * 8, umma_desc_sw128(sv + ks * 16 * 128, kTcTileBytes, 1024), kIdO,
                    (!pend_first || ks > 0) ? 1u : 0u);
-      tc_commit(&o_full);
+      tc_commit(&o_full[pend & 1]);
       tc_commit(&kv_empty[pend % kTcStages]);
       return true;
     };
@@ -1153,7 +1190,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
           // S_g over P_{g-2}, whose P V has completed
           const int st = g % kTcStages;
           if (!mbar_wait(&kv_full[st], (g / kTcStages) & 1, kWaitLimit, &abort_flag) ||
-              (g >= 2 && !mbar_wait(&o_full, (g - 2) & 1, kWaitLimit, &abort_flag))) {
+              (g >= 2 && !mbar_wait(&o_full[g & 1], ((g - 2) >> 1) & 1, kWaitLimit, &abort_flag))) {
             ok = false;
             break;
           }
@@ -1165,7 +1202,6 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
                     umma_desc_sw128(sk + ks * 32, 16, 1024), kIdS, ks > 0 ? 1u : 0u);
           any = true;
           tc_commit(&s_full[g & 1]);
-          if (j == s.t1 - 1) tc_commit(&q_empty[lu & 1]);  // the unit's last S: Q may be replaced
           if (pend >= 0 && !pv()) {
             ok = false;
             break;
@@ -1194,8 +1230,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     const int r = q4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
     constexpr float kRebase = 8.0f;  // log2 of the largest P kept without rescaling
+    const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
     bool ok = true;
-    int g = 0;
+    int g = 0, lu = 0;
     Segment s;
     for (int n = 0; ok && take(n, s); ++n) {
       const bool valid = r < s.rows;
@@ -1221,114 +1258,148 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
           fence_proxy_async_smem();
         }
         if (warp_valid) {
-          uint32_t sv[64];
-          tmem_ld_32x32b_x32(tmem + sb * 64 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
-          tmem_ld_32x32b_x32(tmem + sb * 64 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+          float2 p[32];  // raw scores (the scale is positive: their maximum scales to the scaled ones')
+          tmem_ld_32x32b_x32(tmem + sb * 64 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
+          tmem_ld_32x32b_x32(tmem + sb * 64 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&p[16]));
           tmem_ld_wait();
-          float p[64], mx8[8];
-          // raw scores (the scale is positive: their maximum scales to the scaled ones')
-          const bool whole = __all_sync(0xffffffffu, !valid || k0 + kTcTK - 1 <= seen);
+          if (!__all_sync(0xffffffffu, !valid || k0 + kTcTK - 1 <= seen)) {  // some row does not see the whole tile
 #pragma unroll
-          for (int i = 0; i < 8; ++i) mx8[i] = -INFINITY;
-          if (whole) {
-#pragma unroll
-            for (int c = 0; c < 64; ++c) {
-              p[c] = __uint_as_float(sv[c]);
-              mx8[c & 7] = fmaxf(mx8[c & 7], p[c]);
-            }
-          } else {
-#pragma unroll
-            for (int c = 0; c < 64; ++c) {
-              p[c] = k0 + c <= seen ? __uint_as_float(sv[c]) : -INFINITY;
-              mx8[c & 7] = fmaxf(mx8[c & 7], p[c]);
+            for (int c = 0; c < 32; ++c) {
+              if (k0 + 2 * c > seen) p[c].x = -INFINITY;
+              if (k0 + 2 * c + 1 > seen) p[c].y = -INFINITY;
             }
           }
-          const float mxr = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                                  fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-          const float mn = fmaxf(m, mxr * a.scale_log2);
+          float mx[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(p[i].x, p[i].y);
+#pragma unroll
+          for (int c = 4; c < 32; ++c) mx[c & 3] = fmaxf(fmaxf(mx[c & 3], p[c].x), p[c].y);
+          const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2);
           const bool first = j == s.t0;
           // rows past the unit's hold leftovers: they have no say
           const bool rebase = first || __any_sync(0xffffffffu, valid && mn > m + kRebase);
-          float alpha = 1.0f;
           if (rebase) {
-            alpha = m == -INFINITY ? 0.0f : ex2_approx(m - mn);
+            const float alpha = m == -INFINITY ? 0.0f : ex2_approx(m - mn);
+            l *= alpha;
             m = mn;
-          }
-          const float base = m == -INFINITY ? 0.0f : m;
-          float rs8[8];
+            if (!first) {  // O, with P_{g-1} V in it, to the new bases before P_g V adds to it
+              ok = wait_all(&o_full[sb ^ 1], (g - 1) >> 1);
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) rs8[i] = 0.0f;
+              for (int h = 0; h < 4; ++h) {
+                uint32_t ov[16];
+                tmem_ld_x16(tmem + 128 + h * 16 + lane_off, ov);
+                tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 64; ++c) {  // P = exp2(S * scale - base): one FMA and one exponential
-            p[c] = ex2_approx(fmaf(p[c], a.scale_log2, -base));
-            rs8[c & 7] += p[c];
-          }
-          l = l * alpha + (((rs8[0] + rs8[1]) + (rs8[2] + rs8[3])) + ((rs8[4] + rs8[5]) + (rs8[6] + rs8[7])));
-          uint32_t pk[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) pk[c] = pack2(p[2 * c], p[2 * c + 1]);
-          tmem_st_32x32b_x32(tmem + sb * 64 + lane_off, pk);
-          // P_{g-1} V is in O (waited for in every tile: the barrier's parity
-          // tells neighbouring phases apart, no more)
-          if (!first) ok = wait_all(&o_full, g - 1);
-          if (!ok) break;
-          if (rebase && !first) {  // rescale O's rows to the new bases before P_g V adds to them
-            tc_fence_after();
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t ov[32];
-              tmem_ld_32x32b_x32(tmem + 128 + h * 32 + lane_off, ov);
-              tmem_ld_wait();
-#pragma unroll
-              for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
-              tmem_st_32x32b_x32(tmem + 128 + h * 32 + lane_off, ov);
+                for (int c = 0; c < 16; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+                tmem_st_x16(tmem + 128 + h * 16 + lane_off, ov);
+              }
             }
           }
+          const float base = m == -INFINITY ? 0.0f : m;
+          const float2 base2 = make_float2(-base, -base);
+          float2 sum[2] = {make_float2(l, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {  // P = exp2(S * scale - base)
+              float2 e = fma2(p[16 * h + c], scale2, base2);
+              e.x = ex2_approx(e.x);
+              e.y = ex2_approx(e.y);
+              sum[c & 1] = add2(sum[c & 1], e);
+              pk[c] = pack2(e.x, e.y);
+            }
+            tmem_st_x16(tmem + sb * 64 + h * 16 + lane_off, pk);
+          }
+          l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_st_wait();
-        } else if (j > s.t0) {
-          ok = wait_all(&o_full, g - 1);
-          if (!ok) break;
         }
         tc_fence_before();
         mbar_arrive(&p_full[sb]);
       }
       if (!ok) break;
-      uint32_t ov[64];
-      if (s.t0 < s.t1) {  // the unit's last P V, then O: read and released for the next unit
-        ok = wait_all(&o_full, g - 1);
-        if (!ok) break;
-        tc_fence_after();
-        if (warp_valid) {
-          tmem_ld_32x32b_x32(tmem + 128 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[0]));
-          tmem_ld_32x32b_x32(tmem + 128 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[32]));
-          tmem_ld_wait();
-        }
-        tc_fence_before();
-        mbar_arrive(&o_empty);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 64; ++c) ov[c] = 0u;
-      }
-      if (valid && s.starts && s.ends) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
-        bf16* op = a.out + (int64_t)(s.token + tok) * a.ld_out + (s.kvh * a.n_rep + r - tok * a.n_rep) * kHD;
-#pragma unroll
-        for (int c8 = 0; c8 < 8; ++c8) {
-          uint4 x;
-          x.x = pack2(__uint_as_float(ov[c8 * 8 + 0]) * inv, __uint_as_float(ov[c8 * 8 + 1]) * inv);
-          x.y = pack2(__uint_as_float(ov[c8 * 8 + 2]) * inv, __uint_as_float(ov[c8 * 8 + 3]) * inv);
-          x.z = pack2(__uint_as_float(ov[c8 * 8 + 4]) * inv, __uint_as_float(ov[c8 * 8 + 5]) * inv);
-          x.w = pack2(__uint_as_float(ov[c8 * 8 + 6]) * inv, __uint_as_float(ov[c8 * 8 + 7]) * inv);
-          *reinterpret_cast<uint4*>(op + c8 * 8) = x;
-        }
-      } else if (valid) {
-        float* part = a.ws + (2 * (int64_t)blockIdx.x + (s.starts ? 1 : 0)) * part_floats(kTcRows);
-#pragma unroll
-        for (int c4 = 0; c4 < 16; ++c4)
-          *reinterpret_cast<uint4*>(part + r * kHD + c4 * 4) = *reinterpret_cast<const uint4*>(&ov[c4 * 4]);
+      const bool whole = s.starts && s.ends;
+      float* part = a.ws + (2 * (int64_t)blockIdx.x + (s.starts ? 1 : 0)) * part_floats(kTcRows);
+      if (valid && !whole) {
         part[kTcRows * kHD + r] = m;
         part[kTcRows * kHD + kTcRows + r] = l;
       }
+      auto out_row = [&](int row) -> bf16* {
+        const int tk = row_token(a, row);
+        return a.out + (int64_t)(s.token + tk) * a.ld_out + (s.kvh * a.n_rep + row - tk * a.n_rep) * kHD;
+      };
+      if (s.t0 >= s.t1) {  // no key in this part: zeros
+        if (valid)
+          for (int c = 0; c < 16; ++c) {
+            if (!whole) *reinterpret_cast<float4*>(part + r * kHD + c * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+            else *reinterpret_cast<uint2*>(out_row(r) + c * 4) = make_uint2(0u, 0u);
+          }
+        continue;
+      }
+      // the unit's last P V, then O: read and released for the next unit
+      ok = wait_all(&o_full[(g - 1) & 1], (g - 1) >> 1);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t ov[64];
+      if (warp_valid) {
+        tmem_ld_32x32b_x32(tmem + 128 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[0]));
+        tmem_ld_32x32b_x32(tmem + 128 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[32]));
+        tmem_ld_wait();
+      }
+      tc_fence_before();
+      mbar_arrive(&o_empty);
+      if (warp_valid) {
+        // Rows pass through the unit's own Q buffer (its scores are done), so
+        // that a store instruction writes whole 128-byte rows: a row per
+        // thread took 1.6 us a unit.  16-byte chunk c of row i at c ^ (i & 7).
+        const uint32_t rows_base = sQ + (lu & 1) * kTcQBytes + q4 * 32 * 128;
+        const uint32_t mine = rows_base + lane * 128;
+        auto put = [&](int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((c ^ (lane & 7)) << 4)), "r"(x), "r"(y),
+                       "r"(z), "r"(w)
+                       : "memory");
+        };
+        auto get = [&](int row) -> uint4 {
+          uint4 v;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(rows_base + row * 128 + (((lane & 7) ^ (row & 7)) << 4))
+                       : "memory");
+          return v;
+        };
+        if (whole) {
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            put(c, pack2(__uint_as_float(ov[8 * c + 0]) * inv, __uint_as_float(ov[8 * c + 1]) * inv),
+                pack2(__uint_as_float(ov[8 * c + 2]) * inv, __uint_as_float(ov[8 * c + 3]) * inv),
+                pack2(__uint_as_float(ov[8 * c + 4]) * inv, __uint_as_float(ov[8 * c + 5]) * inv),
+                pack2(__uint_as_float(ov[8 * c + 6]) * inv, __uint_as_float(ov[8 * c + 7]) * inv));
+          __syncwarp();
+          for (int i = lane >> 3; i < 32; i += 4) {
+            const int row = q4 * 32 + i;
+            if (row < s.rows) *reinterpret_cast<uint4*>(out_row(row) + (lane & 7) * 8) = get(i);
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              put(c, ov[32 * h + 4 * c], ov[32 * h + 4 * c + 1], ov[32 * h + 4 * c + 2], ov[32 * h + 4 * c + 3]);
+            __syncwarp();
+            for (int i = lane >> 3; i < 32; i += 4) {
+              const int row = q4 * 32 + i;
+              if (row < s.rows) *reinterpret_cast<uint4*>(part + row * kHD + h * 32 + (lane & 7) * 4) = get(i);
+            }
+            __syncwarp();
+          }
+        }
+        fence_proxy_async_smem();  // before the next Q's TMA write to the buffer
+      }
+      mbar_arrive(&q_empty[lu & 1]);
+      ++lu;
     }
   }
   tc_fence_before();
