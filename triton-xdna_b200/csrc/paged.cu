@@ -1378,8 +1378,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
                 pack2(__uint_as_float(ov[8 * c + 4]) * inv, __uint_as_float(ov[8 * c + 5]) * inv),
                 pack2(__uint_as_float(ov[8 * c + 6]) * inv, __uint_as_float(ov[8 * c + 7]) * inv));
           __syncwarp();
-          for (int i = lane >> 3; i < 32; i += 4) {
-            const int row = q4 * 32 + i;
+#pragma unroll
+          for (int i0 = 0; i0 < 32; i0 += 4) {
+            const int i = i0 + (lane >> 3), row = q4 * 32 + i;
             if (row < s.rows) *reinterpret_cast<uint4*>(out_row(row) + (lane & 7) * 8) = get(i);
           }
         } else {
@@ -1389,8 +1390,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
             for (int c = 0; c < 8; ++c)
               put(c, ov[32 * h + 4 * c], ov[32 * h + 4 * c + 1], ov[32 * h + 4 * c + 2], ov[32 * h + 4 * c + 3]);
             __syncwarp();
-            for (int i = lane >> 3; i < 32; i += 4) {
-              const int row = q4 * 32 + i;
+#pragma unroll
+            for (int i0 = 0; i0 < 32; i0 += 4) {
+              const int i = i0 + (lane >> 3), row = q4 * 32 + i;
               if (row < s.rows) *reinterpret_cast<uint4*>(part + row * kHD + h * 32 + (lane & 7) * 4) = get(i);
             }
             __syncwarp();
@@ -1855,9 +1857,9 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
   const int rows = few ? (eight ? 8 : kFewRows) : kTcRows, tile = few ? kTK : kTcTK;
   a.tpt = rows / n_rep;
   a.rep_magic = (65536u + (uint32_t)n_rep - 1u) / (uint32_t)n_rep;
-  a.over = few ? 16 : 96;
+  a.over = few ? 16 : 224;
   a.snap = few ? 32 : 128;
-  a.min_share = few ? 32 : 192;
+  a.min_share = few ? 32 : 320;
   int box = 8;  // rows of one load: the largest power of two that divides a page, at most a tile
   while (box < tile && page_size % (2 * box) == 0) box *= 2;
   a.box_rows = box;
