@@ -1538,14 +1538,27 @@ int query_map(CUtensorMap* map, const void* q, int64_t tokens, int64_t heads, in
   return XB_OK;
 }
 
-// Addresses of the two status words on the current device.
+// Addresses of the two status words on the current device, looked up once per device.
 int status_words(int** bad, int** status, const char* what, char* err, size_t errlen) {
-  if (cudaGetSymbolAddress((void**)bad, g_bad_page) != cudaSuccess ||
-      cudaGetSymbolAddress((void**)status, g_paged_status) != cudaSuccess) {
-    set_err(err, errlen, "%s: status words unavailable: %s", what, cudaGetErrorString(cudaGetLastError()));
-    return XB_ERR_CUDA;
+  static std::atomic<int*> words[kMaxDevices][2];  // zero-initialised (static storage)
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= kMaxDevices)) e = cudaErrorInvalidDevice;
+  if (e == cudaSuccess) {
+    *bad = words[dev][0].load(std::memory_order_acquire);
+    *status = words[dev][1].load(std::memory_order_acquire);
+    if (*bad && *status) return XB_OK;
+    e = cudaGetSymbolAddress((void**)bad, g_bad_page);
+    if (e == cudaSuccess) e = cudaGetSymbolAddress((void**)status, g_paged_status);
+    if (e == cudaSuccess) {
+      words[dev][0].store(*bad, std::memory_order_release);
+      words[dev][1].store(*status, std::memory_order_release);
+      return XB_OK;
+    }
   }
-  return XB_OK;
+  set_err(err, errlen, "%s: status words unavailable: %s", what, cudaGetErrorString(e));
+  cudaGetLastError();
+  return XB_ERR_CUDA;
 }
 
 // What every page operand has to satisfy, device contents aside.

@@ -10,6 +10,7 @@ raises.  For the reference's host-tensor launch semantics see
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -1013,70 +1014,86 @@ def argmax(x, out=None):
 # lengths.  xb200.paged.PagedKVCache keeps them and the pool.
 
 
-class _on_device:
-    """Makes `device` the current one for a call (tensors of another device
-    than the current one are enqueued on their own device's current stream)."""
+def _device_of(*ts) -> int:
+    """Device index of CUDA tensors (None skipped), as _cuda checks them."""
+    dev = -1
+    for t in ts:
+        if t is not None:
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise ValueError("xb200.ops operates on CUDA tensors (use xb200.kernels for host tensors)")
+            i = t.get_device()
+            if dev != i:
+                if dev >= 0:
+                    raise ValueError(f"tensors on different devices: cuda:{dev} and cuda:{i}")
+                dev = i
+    return dev
 
-    def __init__(self, device):
-        self.prev, self.dev = torch.cuda.current_device(), device.index
 
-    def __enter__(self):
-        if self.dev != self.prev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.dev != self.prev:
-            torch.cuda.set_device(self.prev)
-        return False
+def _call_on(dev: int, name: str, *args) -> None:
+    """_lib.call on device `dev`'s current stream, whichever device is current
+    (a single-token step is bound by these calls, so the usual case is short)."""
+    if torch._C._cuda_getDevice() == dev:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def _page_args(k_pages, v_pages, page_table, q_start, kv_len):
-    """Checks what the host can see of a paged batch: (batch, max_pages, table pitch, the six page strides)."""
-    if k_pages.dtype != torch.bfloat16 or v_pages.dtype != torch.bfloat16:
+    """Checks what the host can see of a paged batch: (n_pages, n_kv_head,
+    page_size, head_dim, batch, max_pages, table pitch, the six page strides)."""
+    if k_pages.dtype is not torch.bfloat16 or v_pages.dtype is not torch.bfloat16:
         raise TypeError("k_pages and v_pages must be bf16")
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+    if page_table.dtype is not torch.int32 or q_start.dtype is not torch.int32 or kv_len.dtype is not torch.int32:
+        raise TypeError("page_table, q_start and kv_len must be int32")
+    shape = k_pages.shape
+    if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must share a shape [n_pages, n_kv_head, page_size, head_dim]")
-    for t, n in ((page_table, "page_table"), (q_start, "q_start"), (kv_len, "kv_len")):
-        if t.dtype != torch.int32:
-            raise TypeError(f"{n} must be int32")
-    B = kv_len.shape[0] if kv_len.dim() == 1 else -1
-    if B < 0 or tuple(q_start.shape) != (B + 1,) or page_table.dim() != 2 or page_table.shape[0] != B:
+    n, h, p, d = shape
+    ts, ls, qs = page_table.shape, kv_len.shape, q_start.shape
+    if len(ls) != 1 or len(ts) != 2 or len(qs) != 1 or ts[0] != ls[0] or qs[0] != ls[0] + 1:
         raise ValueError("a batch of B sequences has kv_len [B], q_start [B + 1] and page_table [B, max_pages]")
-    if not (q_start.is_contiguous() and kv_len.is_contiguous()) or (page_table.stride(1) != 1
-                                                                   and page_table.shape[1] > 1):
-        raise ValueError("q_start, kv_len and the rows of page_table must be contiguous")
-    if page_table.shape[1] == 0:
+    B, cols = ts
+    if cols == 0:
         raise ValueError("page_table needs at least one column")
-    n, h, p, d = k_pages.shape
-    lds = []
-    for t in (k_pages, v_pages):
-        if t.stride(3) != 1 and d > 1:
-            raise ValueError("page rows must be contiguous")
-        # the stride of a dimension of one is arbitrary: any multiple of 8 stands for it
-        lds += [t.stride(i) if size > 1 else h * p * d for i, size in ((0, n), (1, h), (2, p))]
-    return B, page_table.shape[1], page_table.stride(0) if B > 1 else page_table.shape[1], lds
+    ld, unit = page_table.stride()
+    if (unit != 1 and cols > 1) or not q_start.is_contiguous() or not kv_len.is_contiguous():
+        raise ValueError("q_start, kv_len and the rows of page_table must be contiguous")
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    if (k3 != 1 or v3 != 1) and d > 1:
+        raise ValueError("page rows must be contiguous")
+    if n == 1 or h == 1 or p == 1:  # the stride of a dimension of one is arbitrary: any multiple of 8 stands for it
+        any_ = h * p * d
+        k0, v0 = (any_, any_) if n == 1 else (k0, v0)
+        k1, v1 = (any_, any_) if h == 1 else (k1, v1)
+        k2, v2 = (any_, any_) if p == 1 else (k2, v2)
+    return n, h, p, d, B, cols, ld if B > 1 else cols, (k0, k1, k2, v0, v1, v2)
 
 
 def _token_rows(t, name, tokens, row) -> int:
-    """Row pitch of a [tokens, row] (or [tokens, heads, dim]) tensor whose rows are contiguous."""
-    if t.dtype != torch.bfloat16:
+    """Row pitch of a [tokens, row] (or [tokens, heads, dim]) bf16 tensor whose rows are contiguous."""
+    if t.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must be bf16")
-    inner = t.numel() // t.shape[0] if t.dim() > 1 and t.shape[0] else row
-    if t.dim() not in (2, 3) or t.shape[0] != tokens or inner != row:
+    shape = t.shape
+    dims = len(shape)
+    if dims not in (2, 3) or shape[0] != tokens or (shape[1] if dims == 2 else shape[1] * shape[2]) != row:
         raise ValueError(f"{name} must have {tokens} rows of {row} elements")
-    if tokens and (t.stride(-1) != 1 or (t.dim() == 3 and t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+    st = t.stride()
+    if tokens and (st[-1] != 1 or (dims == 3 and shape[1] > 1 and st[1] != shape[2])):
         raise ValueError(f"the rows of {name} must be contiguous")
-    return t.stride(0) if tokens > 1 else row
+    return st[0] if tokens > 1 else row
 
 
-def _overlap(a, b) -> bool:
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + (sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+def _apart(p, ld_p, row_p, q, ld_q, row_q, tokens, what) -> None:
+    """Two [tokens, row] bf16 tensors at p and q share no memory: one ends
+    before the other starts, or they are other columns of the same rows."""
+    if tokens == 0 or p + 2 * ((tokens - 1) * ld_p + row_p) <= q or q + 2 * ((tokens - 1) * ld_q + row_q) <= p:
+        return
+    off = (q - p) // 2 % ld_p if ld_p else 0
+    if ld_p == ld_q and off >= row_p and off + row_q <= ld_p:
+        return
+    raise ValueError(f"{what} must not share memory")
 
 
 def paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len):
@@ -1085,29 +1102,37 @@ def paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_star
     into the pages at their positions: rope_kv() for a paged cache, the same
     bits.  Tokens outside the sequences are left alone; page_status() tells of
     positions without a page or table row."""
-    _cuda(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len)
+    dev = _device_of(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len)
     if (cos_t is None) != (sin_t is None):
         raise ValueError("give both RoPE tables or neither")
-    B, max_pages, ld_table, lds = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
-    n, KVH, P, D = k_pages.shape
+    n, KVH, P, D, B, cols, ld_table, lds = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
     if q_out.dim() != 3 or q_out.shape[2] != D:
         raise ValueError(f"q_out must be [tokens, n_head, {D}]")
-    T, H = q_out.shape[0], q_out.shape[1]
-    rows = 0
+    T, H, _ = q_out.shape
+    rows, cos, sin = 0, None, None
     if cos_t is not None:
         for t in (cos_t, sin_t):
-            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != D or not t.is_contiguous():
+            if t.dtype is not torch.float32 or t.dim() != 2 or t.shape[1] != D or not t.is_contiguous():
                 raise ValueError(f"RoPE tables must be contiguous float32 [positions, {D}]")
-        rows = min(cos_t.shape[0], sin_t.shape[0])
-    ld_qkv, ld_q = _token_rows(qkv, "qkv", T, (H + 2 * KVH) * D), _token_rows(q_out, "q_out", T, H * D)
-    if _overlap(qkv, q_out):
-        raise ValueError("q_out must not share memory with qkv")
-    with _on_device(q_out.device):
-        _lib.call("xb_paged_rope_kv_bf16", qkv.data_ptr(), cos_t.data_ptr() if rows else None,
-                  sin_t.data_ptr() if rows else None, q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                  page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), T, B, H, KVH, D, n, P, max_pages,
-                  rows, ld_qkv, ld_q, ld_table, *lds, _stream())
+        rows, cos, sin = min(cos_t.shape[0], sin_t.shape[0]), cos_t.data_ptr(), sin_t.data_ptr()
+        if rows == 0:
+            raise ValueError("RoPE tables must have at least one row")
+    row = (H + 2 * KVH) * D
+    ld_qkv, ld_q = _token_rows(qkv, "qkv", T, row), _token_rows(q_out, "q_out", T, H * D)
+    px, pq = qkv.data_ptr(), q_out.data_ptr()
+    _apart(px, ld_qkv, row, pq, ld_q, H * D, T, "qkv and q_out")
+    _call_on(dev, "xb_paged_rope_kv_bf16", px, cos, sin, pq, k_pages.data_ptr(), v_pages.data_ptr(),
+             page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), T, B, H, KVH, D, n, P, cols, rows, ld_qkv,
+             ld_q, ld_table, *lds)
     return q_out
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_attention_bytes(dev, T, B, H, KVH) -> int:
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(dev):
+        _lib.call("xb_paged_attention_workspace_size", T, B, H, KVH, ctypes.byref(need))
+    return need.value
 
 
 def paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale):
@@ -1116,33 +1141,31 @@ def paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale
     sequence sees keys 0 .. p.  attention() for sequences of different lengths,
     from single tokens to whole prompts in one batch.  Rows outside the
     sequences are left as they are; a token that sees no key gets zeros."""
-    _cuda(q, k_pages, v_pages, out, page_table, q_start, kv_len)
-    B, max_pages, ld_table, lds = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
-    n, KVH, P, D = k_pages.shape
+    dev = _device_of(q, k_pages, v_pages, out, page_table, q_start, kv_len)
+    n, KVH, P, D, B, cols, ld_table, lds = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
     if q.dim() != 3 or q.shape[2] != D:
         raise ValueError(f"q must be [tokens, n_head, {D}]")
-    T, H = q.shape[0], q.shape[1]
-    ld_q, ld_out = _token_rows(q, "q", T, H * D), _token_rows(out, "out", T, H * D)
-    if _overlap(q, out):
-        raise ValueError("out must not share memory with q")
-    with _on_device(q.device):
-        need = ctypes.c_size_t(0)
-        _lib.call("xb_paged_attention_workspace_size", T, B, H, KVH, ctypes.byref(need))
-        # of this call alone: the caching allocator orders its reuse on the
-        # stream, and a captured graph keeps its own
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        _lib.call("xb_paged_attention_bf16", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
-                  page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), T, B, H, KVH, D, n, P, max_pages,
-                  ld_q, ld_out, ld_table, *lds, float(scale), ws.data_ptr(), ws.numel(), _stream())
+    T, H, _ = q.shape
+    row = H * D
+    ld_q, ld_out = _token_rows(q, "q", T, row), _token_rows(out, "out", T, row)
+    pq, po = q.data_ptr(), out.data_ptr()
+    _apart(pq, ld_q, row, po, ld_out, row, T, "q and out")
+    # of this call alone: the caching allocator orders its reuse on the stream,
+    # and a captured graph keeps its own
+    ws = torch.empty(_paged_attention_bytes(dev, T, B, H, KVH), dtype=torch.uint8, device=q.device)
+    _call_on(dev, "xb_paged_attention_bf16", pq, k_pages.data_ptr(), v_pages.data_ptr(), po, page_table.data_ptr(),
+             q_start.data_ptr(), kv_len.data_ptr(), T, B, H, KVH, D, n, P, cols, ld_q, ld_out, ld_table, *lds,
+             float(scale), ws.data_ptr(), ws.numel())
     return out
 
 
 def _page_list(ids, name) -> torch.Tensor:
-    t = torch.as_tensor(ids)
-    if t.device.type != "cpu" or t.dim() != 1 or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
-        if t.numel() or t.device.type != "cpu" or t.dim() != 1:
-            raise TypeError(f"{name} must be a sequence of page numbers on the host")
-    if t.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8) and t.numel():
+    t = ids if isinstance(ids, torch.Tensor) else torch.as_tensor(ids)
+    if t.dtype is torch.int32 and not t.is_cuda and t.dim() == 1:
+        return t.contiguous()
+    if t.is_cuda or t.dim() != 1 or (t.numel() and (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool)):
+        raise TypeError(f"{name} must be a sequence of page numbers on the host")
+    if t.numel():
         lo, hi = t.aminmax()
         if int(lo) < 0 or int(hi) > 0x7FFFFFFF:
             raise ValueError(f"{name} holds page numbers outside the pool")
@@ -1155,20 +1178,20 @@ def copy_pages(pages, src, dst, dim: int = 2):
     page_size, head_dim]): all layers' keys and values in one launch.  src and
     dst are page numbers on the host (lists or CPU integer tensors); no page
     may be a destination twice, or both a source and a destination."""
-    _cuda(pages)
-    if not -pages.dim() <= dim < pages.dim():
+    dev = _device_of(pages)
+    shape = pages.shape
+    if not -len(shape) <= dim < len(shape):
         raise ValueError(f"pages has no dimension {dim}")
-    dim %= pages.dim()
+    dim %= len(shape)
     if not pages.is_contiguous():
         raise ValueError("pages must be contiguous")
     src, dst = _page_list(src, "src"), _page_list(dst, "dst")
     if src.numel() != dst.numel():
         raise ValueError(f"{src.numel()} sources for {dst.numel()} destinations")
-    outer = math.prod(pages.shape[:dim])
-    page_bytes = math.prod(pages.shape[dim + 1:]) * pages.element_size()
-    with _on_device(pages.device):
-        _lib.call("xb_copy_pages", pages.data_ptr(), outer, pages.shape[dim] * page_bytes, pages.shape[dim],
-                  page_bytes, src.data_ptr(), dst.data_ptr(), src.numel(), _stream())
+    n = shape[dim]
+    page_bytes = math.prod(shape[dim + 1:]) * pages.element_size()
+    _call_on(dev, "xb_copy_pages", pages.data_ptr(), math.prod(shape[:dim]), n * page_bytes, n, page_bytes,
+             src.data_ptr(), dst.data_ptr(), src.numel())
     return pages
 
 
