@@ -122,3 +122,225 @@ def test_operators_refuse_host_tensors():
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA"):
         ops.paged_attention(x[0, 0, :, 0], x[0, 0], x[0, 1], x[0, 0, :, 0], i.view(1, 2), i, i[:1], 1.0)
+
+
+# ----------------------------------------------------------------------------- page bookkeeping
+
+
+class _Cfg:
+    n_layer, n_kv_head, head_dim = 2, 2, 16
+
+
+@pytest.fixture
+def copies(monkeypatch):
+    """ops.copy_pages on host tensors; the calls are recorded."""
+    calls = []
+
+    def copy(pages, src, dst, dim=2):
+        src, dst = list(src), list(dst)
+        assert len(set(dst)) == len(dst) and not set(src) & set(dst)
+        pages[:, :, dst] = pages[:, :, src]
+        calls.append((src, dst))
+        return pages
+
+    monkeypatch.setattr(ops, "copy_pages", copy)
+    return calls
+
+
+def _cache(n=12, page=8):
+    from xb200.paged import PagedKVCache
+
+    return PagedKVCache(_Cfg, n, page, device="cpu")
+
+
+def _check(cache):
+    """Reference counts are the sequences' uses, and the free pages are the unused ones."""
+    uses = [0] * cache.n_pages
+    for s in cache._seqs.values():
+        assert len(s.pages) == -(-s.length // cache.page_size)
+        for p in s.pages:
+            uses[p] += 1
+    assert uses == cache._refs
+    assert sorted(cache._free) == [p for p, n in enumerate(uses) if n == 0]
+
+
+def _write(cache, batch, seqs, counts, value):
+    """What a step's RoPE operator does: the position's value in every new position's page."""
+    start = batch.q_start.tolist()
+    for i, _ in enumerate(seqs):
+        for t in range(start[i], start[i + 1]):
+            p = int(batch.positions[t])
+            assert p == int(batch.kv_len[i]) - (start[i + 1] - t)
+            cache.pages[:, :, int(batch.page_table[i, p // cache.page_size]), :, p % cache.page_size] = value(i, p)
+
+
+def _read(cache, seq):
+    """The first element of every position of layer 0's keys."""
+    P = cache.page_size
+    return [float(cache.pages[0, 0, cache.page_ids(seq)[p // P], 0, p % P, 0]) for p in range(cache.length(seq))]
+
+
+def test_steps_tables_and_positions(copies):
+    c = _cache()
+    a, b = c.add(), c.add()
+    s = c.step([a, b], [10, 3])
+    assert s.page_table.tolist() == [[0, 1], [2, 0]] and s.kv_len.tolist() == [10, 3]
+    assert s.q_start.tolist() == [0, 10, 13] and s.last.tolist() == [9, 12]
+    assert s.positions.tolist() == list(range(10)) + [0, 1, 2]
+    s = c.step([b, a])
+    assert s.last is None and s.q_start.tolist() == [0, 1, 2] and s.positions.tolist() == [3, 10]
+    assert s.page_table.dtype == torch.int32 and s.positions.dtype == torch.int64
+    _check(c)
+    assert not copies
+
+
+def test_fork_copies_the_page_that_both_write(copies):
+    c = _cache()
+    a = c.add()
+    _write(c, c.step([a], [11]), [a], [11], lambda i, p: p)
+    b = c.fork(a)
+    d = c.fork(a)
+    assert c.free_pages == 10 and not copies
+    _write(c, c.step([a, b, d]), [a, b, d], [1] * 3, lambda i, p: 30 * (i + 1) + p)
+    assert copies == [([1, 1], [2, 3])]  # the last sharer writes in place
+    assert _read(c, a) == list(range(11)) + [41] and _read(c, b) == list(range(11)) + [71]
+    assert _read(c, d) == list(range(11)) + [101]
+    assert c.page_ids(a)[0] == c.page_ids(b)[0] == c.page_ids(d)[0]
+    _check(c)
+    c.free(a)
+    _check(c)
+    assert _read(c, b) == list(range(11)) + [71]
+
+
+def test_fork_at_a_page_end_copies_nothing(copies):
+    c = _cache()
+    a = c.add()
+    c.step([a], [8])
+    b = c.fork(a)
+    c.step([a, b])
+    assert not copies and c.page_ids(a)[1] != c.page_ids(b)[1]
+    empty = c.fork(c.add())
+    assert c.length(empty) == 0
+    _check(c)
+
+
+def test_a_step_that_does_not_fit_changes_nothing(copies):
+    c = _cache(n=4)
+    a = c.add()
+    c.step([a], [12])
+    b = c.fork(a)
+    before = (c.page_ids(a), c.page_ids(b), c.free_pages)
+    with pytest.raises(RuntimeError, match="full"):
+        c.step([a, b], [21, 2])  # a copy and three fresh pages
+    assert before == (c.page_ids(a), c.page_ids(b), c.free_pages) and c.length(a) == 12 and not copies
+    c.step([a, b], [1, 1])
+    _check(c)
+
+
+def test_truncate_gives_pages_back(copies):
+    c = _cache()
+    a = c.add()
+    c.step([a], [30])
+    b = c.fork(a)
+    c.truncate(a, 9)
+    assert c.length(a) == 9 and len(c.page_ids(a)) == 2 and c.length(b) == 30
+    _check(c)
+    c.truncate(b, 0)
+    assert c.page_ids(b) == []
+    with pytest.raises(ValueError):
+        c.truncate(a, 10)
+    _check(c)
+
+
+def test_compact_moves_high_pages_down(copies):
+    c = _cache(n=20)
+    seqs = [c.add() for _ in range(5)]
+    _write(c, c.step(seqs, [20, 9, 8, 25, 4]), seqs, None, lambda i, p: 50 * i + p)
+    fork = c.fork(seqs[3])
+    c.free(seqs[0])
+    c.free(seqs[2])
+    moved = c.compact()
+    assert moved > 0 and sorted(p for s in c._seqs.values() for p in set(s.pages))[-1] == 20 - c.free_pages - 1
+    assert _read(c, seqs[1]) == [50 + p for p in range(9)] and _read(c, seqs[4]) == [200 + p for p in range(4)]
+    assert _read(c, fork) == _read(c, seqs[3]) == [150 + p for p in range(25)]
+    _check(c)
+    assert c.compact() == 0
+    c.step([fork, seqs[3]])
+    _check(c)
+
+
+def test_random_histories_keep_the_books(copies):
+    import random
+
+    for seed in range(30):
+        rnd = random.Random(seed)
+        c = _cache(n=rnd.randint(3, 25))
+        want = {}
+        tick = 0
+        for _ in range(60):
+            op = rnd.choice(["add", "fork", "free", "step", "step", "step", "truncate", "compact"])
+            live = list(want)
+            if op == "add":
+                want[c.add()] = []
+            elif op == "compact":
+                c.compact()
+            elif live:
+                q = rnd.choice(live)
+                if op == "fork":
+                    want[c.fork(q)] = list(want[q])
+                elif op == "free":
+                    c.free(q)
+                    del want[q]
+                elif op == "truncate":
+                    n = rnd.randint(0, len(want[q]))
+                    c.truncate(q, n)
+                    del want[q][n:]
+                else:
+                    seqs = rnd.sample(live, rnd.randint(1, len(live)))
+                    counts = [rnd.randint(1, 12) for _ in seqs]
+                    try:
+                        b = c.step(seqs, counts)
+                    except RuntimeError:
+                        b = None
+                    if b is not None:
+                        tick = (tick + 1) % 100  # exact in bf16 with the sequence's place
+                        _write(c, b, seqs, counts, lambda i, p: tick + i / 64)
+                        for i, (s, n) in enumerate(zip(seqs, counts)):
+                            want[s] += [float(torch.tensor(tick + i / 64).to(torch.bfloat16))] * n
+            _check(c)
+            for s, w in want.items():
+                assert _read(c, s) == w
+
+
+def test_cache_refusals(copies):
+    from xb200.paged import PagedKVCache
+
+    c = _cache()
+    a = c.add()
+    for bad in ([], [a, a]):
+        with pytest.raises(ValueError):
+            c.step(bad)
+    with pytest.raises(ValueError):
+        c.step([a], [0])
+    with pytest.raises(ValueError):
+        c.step([a], [1, 1])
+    with pytest.raises(KeyError):
+        c.step([a, 99])
+    c.free(a)
+    with pytest.raises(KeyError):
+        c.free(a)
+    with pytest.raises(KeyError):
+        c.length(a)
+    for n, p in ((0, 8), (4, 12), (4, 0)):
+        with pytest.raises(ValueError):
+            PagedKVCache(_Cfg, n, p, device="cpu")
+
+
+def test_fresh_slots_and_taken_workspaces():
+    a, b = ops.fresh_slot(), ops.fresh_slot()
+    assert a != b
+    with ops.workspace_slot(a):
+        key = (torch.device("cuda:0"), a)
+        ops._workspaces[key] = "buffer"
+        assert ops.take_workspace("cuda:0") == "buffer" and key not in ops._workspaces
+        assert ops.take_workspace("cuda:0") is None

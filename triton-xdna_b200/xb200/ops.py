@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import itertools
 import math
 
 import torch
@@ -441,6 +442,23 @@ def _workspace(device, nbytes: int) -> torch.Tensor:
         ws = torch.empty(max(nbytes // 4, 1 << 20), dtype=torch.float32, device=device)
         _workspaces[key] = ws
     return ws
+
+
+_slots = itertools.count(1 << 16)  # above the numbers that callers give to workspace_slot
+
+
+def fresh_slot() -> int:
+    """A workspace slot number that nobody has used."""
+    return next(_slots)
+
+
+def take_workspace(device):
+    """The current slot's scratch buffer on `device` (None if it has none),
+    which no later operator gets: a captured graph keeps it alive."""
+    device = torch.device(device)
+    if device.index is None:
+        device = torch.device(device.type, torch.cuda.current_device())
+    return _workspaces.pop((device, _slot[0]), None)
 
 
 def linear(x, weight, bias=None, out=None, out_dtype=torch.bfloat16, residual=None, act=None):

@@ -31,6 +31,7 @@ from dataclasses import dataclass
 import torch
 
 from . import ops
+from .paged import PagedBatch, PagedKVCache, generate_paged
 
 
 @dataclass
@@ -266,6 +267,72 @@ class Qwen2Model:
             return None
         logits = ops.linear(x, self.embed, out_dtype=torch.float32)
         return logits if last_only else logits.reshape(B, S, c.vocab_size)
+
+    @property
+    def position_limit(self) -> int:
+        """Positions the RoPE table holds."""
+        return self.cos.shape[0]
+
+    @torch.no_grad()
+    def forward_packed(self, ids: torch.Tensor, cache: PagedKVCache, batch: PagedBatch,
+                       next_token: torch.Tensor | None = None) -> torch.Tensor | None:
+        """The layers over the packed new tokens `ids` [T] of a step of a paged
+        cache (`batch` from cache.step).  Returns fp32 logits [B, vocab] of each
+        sequence's last token, or writes its greedy token into `next_token`."""
+        c = self.cfg
+        T = ids.shape[0]
+        D, H, KVH, HD, eps = c.n_embd, c.n_head, c.n_kv_head, c.head_dim, c.rms_eps
+        x = ops.embedding(self.embed, ids)
+        q = torch.empty((T, H, HD), dtype=torch.bfloat16, device=self.device)
+        attn = torch.empty((T, H * HD), dtype=torch.bfloat16, device=self.device)
+        at = (batch.page_table, batch.q_start, batch.kv_len)
+        small = T <= ops.SMALL_M  # the one-launch linears of a decode step, whatever the tokens belong to
+        if small:
+            xin, xnorm = ops.rms_norm(x, self.layers[0]["input_ln"], eps), None
+        for i, L in enumerate(self.layers):
+            if small:
+                qkv = ops.decode_linear(xin, L["qkv_w"], L["qkv_b"], xnorm=xnorm)
+            else:
+                qkv = ops.linear(ops.rms_norm(x, L["input_ln"], eps), L["qkv_w"], L["qkv_b"])
+            ops.paged_rope_kv(qkv, self.cos, self.sin, q, cache.k[i], cache.v[i], *at)
+            ops.paged_attention(q, cache.k[i], cache.v[i], attn, *at, self.scale)
+            if small:
+                y, st = ops.decode_linear_residual(attn, L["o_w"], None, x, stats_kind="rms")
+                h = ops.decode_linear_swiglu(y, L["gate_up_w"], xnorm=(st, L["post_ln"], None, eps, "rms"))
+                last = i + 1 == len(self.layers)
+                x, st = ops.decode_linear_residual(h, L["down_w"], None, y, stats_kind=None if last else "rms")
+                if not last:
+                    xin, xnorm = x, (st, self.layers[i + 1]["input_ln"], None, eps, "rms")
+                continue
+            x = ops.linear(attn, L["o_w"], residual=x)
+            h = ops.linear_swiglu(ops.rms_norm(x, L["post_ln"], eps), L["gate_up_w"], interleaved=True)
+            x = ops.linear(h, L["down_w"], residual=x)
+        if batch.last is not None:
+            x = ops.embedding(x, batch.last)  # each sequence's last row
+        x = ops.rms_norm(x, self.norm_w, eps)
+        if next_token is not None:
+            ops.linear_argmax(x, self.embed, out=next_token)
+            return None
+        return ops.linear(x, self.embed, out_dtype=torch.float32)
+
+    def forward_paged(self, ids: torch.Tensor, cache: PagedKVCache, seqs, counts=None,
+                      next_token: torch.Tensor | None = None) -> torch.Tensor | None:
+        """A step of a paged cache: `ids` [sum(counts)] int64 packs counts[i]
+        new tokens of sequence seqs[i] (one each by default): prompts, chunks
+        of them and single tokens in any mixture.  Returns fp32 logits
+        [len(seqs), vocab] after each sequence's last token, or writes the
+        greedy tokens into `next_token` (int64) and returns None."""
+        counts = [1] * len(seqs) if counts is None else [int(n) for n in counts]
+        if ids.dim() != 1 or ids.shape[0] != sum(counts):
+            raise ValueError(f"ids must be 1-D with {sum(counts)} tokens")
+        for q, n in zip(seqs, counts):
+            if cache.length(q) + n > self.position_limit:
+                raise ValueError(f"sequence {q} would exceed the RoPE table ({self.position_limit})")
+        return self.forward_packed(ids, cache, cache.step(seqs, counts), next_token=next_token)
+
+    def generate_paged(self, prompts, max_new_tokens: int, **kw) -> torch.Tensor:
+        """Greedy continuation of prompts of different lengths (xb200.paged.generate_paged)."""
+        return generate_paged(self, prompts, max_new_tokens, **kw)
 
     @torch.no_grad()
     def generate(self, ids: torch.Tensor, max_new_tokens: int, cache: KVCache | None = None,
