@@ -667,16 +667,29 @@ XB_API int xb_attention_workspace_size(int64_t batch, int64_t seq,
  * replayed with other lengths and pages.  Rows before q_start[0] and from
  * q_start[batch] to `tokens` - 1 are left as they are.
  *
- * k_pages / v_pages: bf16 [n_pages, n_kv_head, page_size, head_dim] with
- * element strides (page, head, row), rows of contiguous elements; page_size a
- * multiple of 8; bases 16-byte aligned, strides and row pitches multiples of
- * 8 elements.
+ * The pages are bf16 [n_pages, n_kv_head, page_size, head_dim] with element
+ * strides (page, head, row), rows of contiguous elements; page_size a multiple
+ * of 8; bases 16-byte aligned, strides and row pitches multiples of 8
+ * elements.  xb_paged_kv (host memory, read during the call) describes them:
+ * a step makes several calls with the same one.
  *
  * No content of the device arrays makes a kernel leave its buffers.  A page
  * id outside [0, n_pages) that a sequence needs, a position with no table
  * column, or a RoPE position outside the tables sets the flag that
  * xb_page_status reports.
  * ------------------------------------------------------------------------- */
+
+typedef struct xb_paged_kv {
+  void* k_pages;
+  void* v_pages;
+  const int32_t* page_table;  /* device [batch, max_pages], pitch ld_table */
+  const int32_t* q_start;     /* device [batch + 1] */
+  const int32_t* kv_len;      /* device [batch] */
+  int64_t n_pages, n_kv_head, page_size, head_dim;
+  int64_t batch, max_pages, ld_table;
+  int64_t k_page, k_head, k_row;  /* element strides of k_pages */
+  int64_t v_page, v_head, v_row;
+} xb_paged_kv;
 
 /* RoPE of the packed fused QKV projection plus the write of its keys and
  * values into pages.  qkv [tokens, (n_head + 2 n_kv_head) * head_dim] (pitch
@@ -686,40 +699,35 @@ XB_API int xb_attention_workspace_size(int64_t batch, int64_t seq,
  * for bit.  A token whose page is missing still gets its q row (flagged, K / V
  * not written); one with a negative position or one past the tables is
  * skipped (flagged). */
-XB_API int xb_paged_rope_kv_bf16(
-    const void* qkv, const float* cos_t, const float* sin_t, void* q_out,
-    void* k_pages, void* v_pages, const int32_t* page_table,
-    const int32_t* q_start, const int32_t* kv_len, int64_t tokens,
-    int64_t batch, int64_t n_head, int64_t n_kv_head, int64_t head_dim,
-    int64_t n_pages, int64_t page_size, int64_t max_pages, int64_t rope_rows,
-    int64_t ld_qkv, int64_t ld_q, int64_t ld_table, int64_t k_page,
-    int64_t k_head, int64_t k_row, int64_t v_page, int64_t v_head,
-    int64_t v_row, void* stream, char* err, size_t errlen);
+XB_API int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t,
+                                 const float* sin_t, void* q_out,
+                                 const xb_paged_kv* kv, int64_t tokens,
+                                 int64_t n_head, int64_t rope_rows,
+                                 int64_t ld_qkv, int64_t ld_q, void* stream,
+                                 char* err, size_t errlen);
 
 /* Causal grouped-query attention of the packed new tokens over the pages: the
- * token at position p sees keys 0 .. p of its sequence.  q [tokens, n_head,
- * 64] (token pitch ld_q), out [tokens, n_head * 64] (pitch ld_out), head_dim
- * 64, scale > 0.  Online softmax in fp32, P rounded to bf16 before P V, as
- * xb_attention_bf16.  A token with a negative position (kv_len[b] < n) sees
- * nothing: its row is zero.  Lengths beyond the table count as max_pages *
- * page_size; a page id outside the pool reads as zeros (flagged).  Long
- * contexts are split over CTAs and joined in a fixed order: the same inputs
- * give the same bits, and the split depends on the whole batch's lengths.
- * `workspace` (16-byte aligned, size from the query below) holds the partial
- * results of one call; calls that may run at the same time need one each. */
+ * token at position p sees keys 0 .. p.  q [tokens, n_head, 64] (token pitch
+ * ld_q), out [tokens, n_head * 64] (pitch ld_out), head_dim 64, n_head /
+ * n_kv_head at most 128, scale > 0.  Online softmax in fp32, P rounded to bf16
+ * before P V, as xb_attention_bf16.  A token with a negative position
+ * (kv_len[b] < n) sees nothing: its row is zero.  Lengths beyond the table
+ * count as max_pages * page_size; a page id outside the pool reads as zeros
+ * (flagged).  Long contexts are split over CTAs and joined in a fixed order:
+ * the same inputs give the same bits, and the split depends on the whole
+ * batch's lengths.  `workspace` (16-byte aligned, size from the query below,
+ * any content) holds the partial results of one call; calls that may run at
+ * the same time need one each. */
 XB_API int xb_paged_attention_workspace_size(int64_t tokens, int64_t batch,
                                              int64_t n_head, int64_t n_kv_head,
                                              size_t* bytes, char* err,
                                              size_t errlen);
-XB_API int xb_paged_attention_bf16(
-    const void* q, const void* k_pages, const void* v_pages, void* out,
-    const int32_t* page_table, const int32_t* q_start, const int32_t* kv_len,
-    int64_t tokens, int64_t batch, int64_t n_head, int64_t n_kv_head,
-    int64_t head_dim, int64_t n_pages, int64_t page_size, int64_t max_pages,
-    int64_t ld_q, int64_t ld_out, int64_t ld_table, int64_t k_page,
-    int64_t k_head, int64_t k_row, int64_t v_page, int64_t v_head,
-    int64_t v_row, float scale, void* workspace, size_t workspace_bytes,
-    void* stream, char* err, size_t errlen);
+XB_API int xb_paged_attention_bf16(const void* q, void* out,
+                                   const xb_paged_kv* kv, int64_t tokens,
+                                   int64_t n_head, int64_t ld_q, int64_t ld_out,
+                                   float scale, void* workspace,
+                                   size_t workspace_bytes, void* stream,
+                                   char* err, size_t errlen);
 
 /* pages[o, dst[i]] = pages[o, src[i]] for i < n and every slab o < outer (a
  * layer's keys or values): page p of slab o is the page_bytes bytes at o *

@@ -48,13 +48,22 @@ def test_copy_pages_without_work_is_a_no_op():
     _copy([0], [1], outer=0)
 
 
+_KV = dict(k=1 << 13, v=1 << 14, table=1 << 16, q_start=1 << 17, kv_len=1 << 18, n_pages=10, n_kv_head=2, page_size=16,
+           head_dim=64, batch=2, max_pages=3, ld_table=3, k_page=2048, k_head=1024, k_row=64, v_page=2048, v_head=1024,
+           v_row=64)
+
+
+def _split(args, kw):
+    """The call's arguments and its packed xb_paged_kv, with `kw` over the defaults of either."""
+    kv = {k: kw.get(k, v) or 0 for k, v in _KV.items()}
+    assert set(kw) <= set(args) | set(_KV)
+    return {k: kw.get(k, v) for k, v in args.items()}, ops._PAGED_KV(*kv.values())
+
+
 def _attn(**kw):
-    a = dict(q=1 << 12, k=1 << 13, v=1 << 14, out=1 << 15, table=1 << 16, q_start=1 << 17, kv_len=1 << 18, tokens=4,
-             batch=2, n_head=14, n_kv_head=2, head_dim=64, n_pages=10, page_size=16, max_pages=3, ld_q=896, ld_out=896,
-             ld_table=3, k_page=2048, k_head=1024, k_row=64, v_page=2048, v_head=1024, v_row=64, scale=0.125, ws=None,
-             ws_bytes=0)
-    a.update(kw)
-    _lib.call("xb_paged_attention_bf16", *a.values(), None)
+    a, kv = _split(dict(q=1 << 12, out=1 << 15, tokens=4, n_head=14, ld_q=896, ld_out=896, scale=0.125, ws=None,
+                        ws_bytes=0), kw)
+    _lib.call("xb_paged_attention_bf16", a["q"], a["out"], kv, *list(a.values())[2:], None)
 
 
 @pytest.mark.parametrize("kw,code,text", [
@@ -91,12 +100,10 @@ def test_paged_attention_without_work_is_a_no_op():
 
 
 def _rope(**kw):
-    a = dict(qkv=1 << 12, cos=1 << 11, sin=1 << 10, q=1 << 15, k=1 << 13, v=1 << 14, table=1 << 16, q_start=1 << 17,
-             kv_len=1 << 18, tokens=4, batch=2, n_head=14, n_kv_head=2, head_dim=64, n_pages=10, page_size=16,
-             max_pages=3, rope_rows=64, ld_qkv=18 * 64, ld_q=896, ld_table=3, k_page=2048, k_head=1024, k_row=64,
-             v_page=2048, v_head=1024, v_row=64)
-    a.update(kw)
-    _lib.call("xb_paged_rope_kv_bf16", *a.values(), None)
+    a, kv = _split(dict(qkv=1 << 12, cos=1 << 11, sin=1 << 10, q=1 << 15, tokens=4, n_head=14, rope_rows=64,
+                        ld_qkv=18 * 64, ld_q=896), kw)
+    v = list(a.values())
+    _lib.call("xb_paged_rope_kv_bf16", *v[:4], kv, *v[4:], None)
 
 
 @pytest.mark.parametrize("kw,code,text", [

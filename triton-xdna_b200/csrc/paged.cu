@@ -1589,27 +1589,43 @@ int status_words(int** bad, int** status, const char* what, char* err, size_t er
   return XB_ERR_CUDA;
 }
 
-// What every page operand has to satisfy, device contents aside.
-int check_pages(int64_t n_pages, int64_t page_size, int64_t kv_heads, int64_t batch, int64_t max_pages,
-                int64_t table_ld, int64_t k_page, int64_t k_head, int64_t k_row, int64_t v_page, int64_t v_head,
-                int64_t v_row, const char* what, char* err, size_t errlen) {
-  if (n_pages <= 0 || page_size <= 0 || kv_heads <= 0 || batch < 0 || max_pages <= 0 || table_ld < max_pages) {
+// What a paged batch has to satisfy, device contents aside.
+int check_pages(const xb_paged_kv* kv, const char* what, char* err, size_t errlen) {
+  if (!kv) {
+    set_err(err, errlen, "%s: null pointer", what);
+    return XB_ERR_INVALID;
+  }
+  if (kv->n_pages <= 0 || kv->page_size <= 0 || kv->n_kv_head <= 0 || kv->head_dim <= 0 || kv->batch < 0 ||
+      kv->max_pages <= 0 || kv->ld_table < kv->max_pages) {
     set_err(err, errlen, "%s: bad shape", what);
     return XB_ERR_INVALID;
   }
-  if (page_size % 8) {
-    set_err(err, errlen, "%s: page_size %lld is not a multiple of 8", what, (long long)page_size);
+  if (kv->page_size % 8) {
+    set_err(err, errlen, "%s: page_size %lld is not a multiple of 8", what, (long long)kv->page_size);
     return XB_ERR_UNSUPPORTED;
   }
-  const int64_t lds[6] = {k_page, k_head, k_row, v_page, v_head, v_row};
+  const int64_t lds[6] = {kv->k_page, kv->k_head, kv->k_row, kv->v_page, kv->v_head, kv->v_row};
   for (int64_t ld : lds)
     if (ld <= 0 || ld % 8 || ld >= (1LL << 38)) {
       set_err(err, errlen, "%s: page strides must be positive multiples of 8 elements", what);
       return XB_ERR_UNSUPPORTED;
     }
-  if (n_pages > 0x7ffffffeLL || max_pages > 0x7fffffffLL || max_pages * page_size > 0x7fffffffLL ||
-      batch > 0x7ffffffeLL || kv_heads > 65535) {
+  if (kv->n_pages > 0x7ffffffeLL || kv->max_pages > 0x7fffffffLL || kv->page_size > 0x7fffffffLL ||
+      kv->max_pages * kv->page_size > 0x7fffffffLL || kv->batch > 0x7ffffffeLL || kv->n_kv_head > 65535) {
     set_err(err, errlen, "%s: more than 2^31 - 1 pages, positions or sequences", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  return XB_OK;
+}
+
+// Once there is work: the pointers.
+int check_page_pointers(const xb_paged_kv* kv, const char* what, char* err, size_t errlen) {
+  if (!kv->k_pages || !kv->v_pages || !kv->page_table || !kv->q_start || !kv->kv_len) {
+    set_err(err, errlen, "%s: null pointer", what);
+    return XB_ERR_INVALID;
+  }
+  if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages)) {
+    set_err(err, errlen, "%s: rows must be whole 16-byte vectors", what);
     return XB_ERR_UNSUPPORTED;
   }
   return XB_OK;
@@ -1740,34 +1756,32 @@ extern "C" int xb_copy_pages(void* pages, int64_t outer, int64_t outer_bytes, in
 }
 
 extern "C" int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t, const float* sin_t, void* q_out,
-                                     void* k_pages, void* v_pages, const int32_t* page_table, const int32_t* q_start,
-                                     const int32_t* kv_len, int64_t tokens, int64_t batch, int64_t n_head,
-                                     int64_t n_kv_head, int64_t head_dim, int64_t n_pages, int64_t page_size,
-                                     int64_t max_pages, int64_t rope_rows, int64_t ld_qkv, int64_t ld_q,
-                                     int64_t ld_table, int64_t k_page, int64_t k_head, int64_t k_row, int64_t v_page,
-                                     int64_t v_head, int64_t v_row, void* stream, char* err, size_t errlen) {
+                                     const xb_paged_kv* kv, int64_t tokens, int64_t n_head, int64_t rope_rows,
+                                     int64_t ld_qkv, int64_t ld_q, void* stream, char* err, size_t errlen) {
   const char* what = "xb_paged_rope_kv_bf16";
-  if (tokens < 0 || n_head <= 0 || head_dim <= 0 || n_head > 65535) {
+  int rc = check_pages(kv, what, err, errlen);
+  if (rc) return rc;
+  if (tokens < 0 || n_head <= 0 || n_head > 65535) {
     set_err(err, errlen, "%s: bad shape", what);
     return XB_ERR_INVALID;
   }
-  int rc = check_pages(n_pages, page_size, n_kv_head, batch, max_pages, ld_table, k_page, k_head, k_row, v_page,
-                       v_head, v_row, what, err, errlen);
-  if (rc) return rc;
-  if (head_dim % 16 || head_dim > 512 || 32 % (head_dim / 16)) {
-    set_err(err, errlen, "%s: head_dim %lld not supported (16, 32, 64, 128, 256, 512)", what, (long long)head_dim);
+  const int64_t D = kv->head_dim;
+  if (D % 16 || D > 512 || 32 % (D / 16)) {
+    set_err(err, errlen, "%s: head_dim %lld not supported (16, 32, 64, 128, 256, 512)", what, (long long)D);
     return XB_ERR_UNSUPPORTED;
   }
-  if (tokens == 0 || batch == 0) return XB_OK;
-  if (!qkv || !q_out || !k_pages || !v_pages || !page_table || !q_start || !kv_len || (!cos_t) != (!sin_t)) {
+  if (tokens == 0 || kv->batch == 0) return XB_OK;
+  rc = check_page_pointers(kv, what, err, errlen);
+  if (rc) return rc;
+  if (!qkv || !q_out || (!cos_t) != (!sin_t)) {
     set_err(err, errlen, "%s: null pointer", what);
     return XB_ERR_INVALID;
   }
-  if (ld_qkv < (n_head + 2 * n_kv_head) * head_dim || ld_q < n_head * head_dim) {
+  if (ld_qkv < (n_head + 2 * kv->n_kv_head) * D || ld_q < n_head * D) {
     set_err(err, errlen, "%s: row pitch shorter than the row", what);
     return XB_ERR_INVALID;
   }
-  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_pages) || !aligned16(v_pages) || ld_qkv % 8 || ld_q % 8 ||
+  if (!aligned16(qkv) || !aligned16(q_out) || ld_qkv % 8 || ld_q % 8 ||
       (cos_t && (!aligned16(cos_t) || !aligned16(sin_t)))) {
     set_err(err, errlen, "%s: rows must be whole 16-byte vectors", what);
     return XB_ERR_UNSUPPORTED;
@@ -1781,23 +1795,23 @@ extern "C" int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t, const 
   a.cos_t = cos_t;
   a.sin_t = sin_t;
   a.q = static_cast<bf16*>(q_out);
-  a.k = Pages{static_cast<bf16*>(k_pages), k_page, k_head, k_row};
-  a.v = Pages{static_cast<bf16*>(v_pages), v_page, v_head, v_row};
-  a.table = page_table;
-  a.q_start = q_start;
-  a.kv_len = kv_len;
+  a.k = Pages{static_cast<bf16*>(kv->k_pages), kv->k_page, kv->k_head, kv->k_row};
+  a.v = Pages{static_cast<bf16*>(kv->v_pages), kv->v_page, kv->v_head, kv->v_row};
+  a.table = kv->page_table;
+  a.q_start = kv->q_start;
+  a.kv_len = kv->kv_len;
   a.ld_qkv = ld_qkv;
   a.ld_q = ld_q;
-  a.ld_table = ld_table;
+  a.ld_table = kv->ld_table;
   a.rope_rows = rope_rows;
   a.T = (int)tokens;
-  a.B = (int)batch;
+  a.B = (int)kv->batch;
   a.H = (int)n_head;
-  a.KVH = (int)n_kv_head;
-  a.D = (int)head_dim;
-  a.page_size = (int)page_size;
-  a.max_pages = (int)max_pages;
-  a.n_pages = (int)n_pages;
+  a.KVH = (int)kv->n_kv_head;
+  a.D = (int)D;
+  a.page_size = (int)kv->page_size;
+  a.max_pages = (int)kv->max_pages;
+  a.n_pages = (int)kv->n_pages;
   int *bad = nullptr, *status = nullptr;
   rc = status_words(&bad, &status, what, err, errlen);
   if (rc) return rc;
@@ -1819,37 +1833,35 @@ extern "C" int xb_paged_attention_workspace_size(int64_t tokens, int64_t batch, 
   return XB_OK;
 }
 
-extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const void* v_pages, void* out,
-                                       const int32_t* page_table, const int32_t* q_start, const int32_t* kv_len,
-                                       int64_t tokens, int64_t batch, int64_t n_head, int64_t n_kv_head,
-                                       int64_t head_dim, int64_t n_pages, int64_t page_size, int64_t max_pages,
-                                       int64_t ld_q, int64_t ld_out, int64_t ld_table, int64_t k_page, int64_t k_head,
-                                       int64_t k_row, int64_t v_page, int64_t v_head, int64_t v_row, float scale,
-                                       void* workspace, size_t workspace_bytes, void* stream, char* err,
-                                       size_t errlen) {
+extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_kv* kv, int64_t tokens,
+                                       int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
+                                       size_t workspace_bytes, void* stream, char* err, size_t errlen) {
   const char* what = "xb_paged_attention_bf16";
-  if (tokens < 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head || n_head > 65535) {
+  int rc = check_pages(kv, what, err, errlen);
+  if (rc) return rc;
+  const int64_t n_kv_head = kv->n_kv_head, batch = kv->batch, n_pages = kv->n_pages, page_size = kv->page_size;
+  if (tokens < 0 || n_head <= 0 || n_head % n_kv_head || n_head > 65535) {
     set_err(err, errlen, "%s: bad shape", what);
     return XB_ERR_INVALID;
   }
-  int rc = check_pages(n_pages, page_size, n_kv_head, batch, max_pages, ld_table, k_page, k_head, k_row, v_page,
-                       v_head, v_row, what, err, errlen);
-  if (rc) return rc;
-  if (head_dim != kHD) {
-    set_err(err, errlen, "%s: head_dim %lld not supported (64)", what, (long long)head_dim);
+  if (kv->head_dim != kHD) {
+    set_err(err, errlen, "%s: head_dim %lld not supported (64)", what, (long long)kv->head_dim);
+    return XB_ERR_UNSUPPORTED;
+  }
+  if (n_head / n_kv_head > kTcRows) {
+    set_err(err, errlen, "%s: %lld query heads per KV head not supported (1..128)", what,
+            (long long)(n_head / n_kv_head));
     return XB_ERR_UNSUPPORTED;
   }
   const int n_rep = (int)(n_head / n_kv_head);
-  if (n_rep > kTcRows) {
-    set_err(err, errlen, "%s: %d query heads per KV head not supported (1..128)", what, n_rep);
-    return XB_ERR_UNSUPPORTED;
-  }
   if (!(scale > 0.0f)) {
     set_err(err, errlen, "%s: the scale must be positive", what);
     return XB_ERR_INVALID;
   }
   if (tokens == 0 || batch == 0) return XB_OK;
-  if (!q || !k_pages || !v_pages || !out || !page_table || !q_start || !kv_len) {
+  rc = check_page_pointers(kv, what, err, errlen);
+  if (rc) return rc;
+  if (!q || !out) {
     set_err(err, errlen, "%s: null pointer", what);
     return XB_ERR_INVALID;
   }
@@ -1857,12 +1869,12 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
     set_err(err, errlen, "%s: row pitch shorter than the row", what);
     return XB_ERR_INVALID;
   }
-  if (!aligned16(q) || !aligned16(out) || !aligned16(k_pages) || !aligned16(v_pages) || ld_q % 8 || ld_out % 8) {
+  if (!aligned16(q) || !aligned16(out) || ld_q % 8 || ld_out % 8) {
     set_err(err, errlen, "%s: rows must be whole 16-byte vectors", what);
     return XB_ERR_UNSUPPORTED;
   }
-  if (tokens > 0x7fffffffLL) {
-    set_err(err, errlen, "%s: too many tokens", what);
+  if (tokens > 0x7fffffffLL || ld_q >= (1LL << 38) || ld_out >= (1LL << 38)) {
+    set_err(err, errlen, "%s: too many tokens, or too long a row pitch", what);
     return XB_ERR_UNSUPPORTED;
   }
   size_t need = 0;
@@ -1876,19 +1888,19 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
   AttnArgs a;
   a.q = static_cast<const bf16*>(q);
   a.out = static_cast<bf16*>(out);
-  a.table = page_table;
-  a.q_start = q_start;
-  a.kv_len = kv_len;
+  a.table = kv->page_table;
+  a.q_start = kv->q_start;
+  a.kv_len = kv->kv_len;
   a.ws = static_cast<float*>(workspace);
   a.ld_q = ld_q;
   a.ld_out = ld_out;
-  a.ld_table = ld_table;
+  a.ld_table = kv->ld_table;
   a.T = (int)tokens;
   a.B = (int)batch;
   a.KVH = (int)n_kv_head;
   a.n_rep = n_rep;
   a.page_size = (int)page_size;
-  a.max_pages = (int)max_pages;
+  a.max_pages = (int)kv->max_pages;
   a.n_pages = (int)n_pages;
   a.scale_log2 = scale * 1.4426950408889634f;
   rc = status_words(&a.bad, &a.status, what, err, errlen);
@@ -1906,8 +1918,11 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
   a.box_rows = box;
   TcMaps maps;
   memset(&maps, 0, sizeof(maps));
-  rc = page_map(&maps.k, k_pages, n_pages, n_kv_head, page_size, k_page, k_head, k_row, box, what, err, errlen);
-  if (!rc) rc = page_map(&maps.v, v_pages, n_pages, n_kv_head, page_size, v_page, v_head, v_row, box, what, err, errlen);
+  rc = page_map(&maps.k, kv->k_pages, n_pages, n_kv_head, page_size, kv->k_page, kv->k_head, kv->k_row, box, what, err,
+                errlen);
+  if (!rc)
+    rc = page_map(&maps.v, kv->v_pages, n_pages, n_kv_head, page_size, kv->v_page, kv->v_head, kv->v_row, box, what,
+                  err, errlen);
   if (!rc && !few) rc = query_map(&maps.q, q, tokens, n_head, ld_q, n_rep, a.tpt, what, err, errlen);
   if (rc) return rc;
   int sms = 148;
@@ -1916,18 +1931,18 @@ extern "C" int xb_paged_attention_bf16(const void* q, const void* k_pages, const
   // The line's weight whatever the lengths are: at most tokens / tpt + batch
   // query tiles per KV head, each of at most the table's positions.  With the
   // pieces' rounding it stays an int below 2^30.
-  const double most = ((double)tokens / a.tpt + batch) * n_kv_head * ((double)max_pages * page_size + a.over + a.tpt);
+  const double most = ((double)tokens / a.tpt + batch) * n_kv_head * ((double)kv->max_pages * page_size + a.over + a.tpt);
   const bool wide = most + (double)a.min_share * ctas * 16 >= (double)(1 << 30);
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
   if (few) {
-    KvMaps kv;
-    kv.k = maps.k;
-    kv.v = maps.v;
-    e = eight ? (wide ? launch_few<8, int64_t>(ctas, s, kv, a)
-                      : launch_few<8, int>(ctas, s, kv, a))
-              : (wide ? launch_few<16, int64_t>(ctas, s, kv, a)
-                      : launch_few<16, int>(ctas, s, kv, a));
+    KvMaps pages;
+    pages.k = maps.k;
+    pages.v = maps.v;
+    e = eight ? (wide ? launch_few<8, int64_t>(ctas, s, pages, a)
+                      : launch_few<8, int>(ctas, s, pages, a))
+              : (wide ? launch_few<16, int64_t>(ctas, s, pages, a)
+                      : launch_few<16, int>(ctas, s, pages, a));
     if (e == cudaSuccess)
       e = launch_k(paged_attn_join_kernel<kFewRows, 4>, dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
   } else {

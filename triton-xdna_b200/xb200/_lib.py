@@ -65,6 +65,8 @@ _CTYPES = {
     "const char*": ctypes.c_char_p,
     "uint64_t": ctypes.c_uint64,
     "uint32_t": ctypes.c_uint32,
+    # a packed xb_paged_kv (ops.py): bytes are passed by address
+    "const xb_paged_kv*": ctypes.c_void_p,
     # an array of DecodePhase (ops.py), passed by address
     "const xb_decode_phase*": ctypes.c_void_p,
 }

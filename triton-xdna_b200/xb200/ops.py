@@ -13,6 +13,7 @@ import ctypes
 import functools
 import itertools
 import math
+import struct
 
 import torch
 
@@ -1057,9 +1058,12 @@ def _call_on(dev: int, name: str, *args) -> None:
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
+_PAGED_KV = struct.Struct("5P13q").pack  # xb_paged_kv of include/xb200.h
+
+
 def _page_args(k_pages, v_pages, page_table, q_start, kv_len):
-    """Checks what the host can see of a paged batch: (n_pages, n_kv_head,
-    page_size, head_dim, batch, max_pages, table pitch, the six page strides)."""
+    """Checks what the host can see of a paged batch: (n_kv_head, head_dim,
+    batch, the C struct xb_paged_kv as bytes)."""
     if k_pages.dtype is not torch.bfloat16 or v_pages.dtype is not torch.bfloat16:
         raise TypeError("k_pages and v_pages must be bf16")
     if page_table.dtype is not torch.int32 or q_start.dtype is not torch.int32 or kv_len.dtype is not torch.int32:
@@ -1086,7 +1090,8 @@ def _page_args(k_pages, v_pages, page_table, q_start, kv_len):
         k0, v0 = (any_, any_) if n == 1 else (k0, v0)
         k1, v1 = (any_, any_) if h == 1 else (k1, v1)
         k2, v2 = (any_, any_) if p == 1 else (k2, v2)
-    return n, h, p, d, B, cols, ld if B > 1 else cols, (k0, k1, k2, v0, v1, v2)
+    return h, d, B, _PAGED_KV(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), q_start.data_ptr(),
+                              kv_len.data_ptr(), n, h, p, d, B, cols, ld if B > 1 else cols, k0, k1, k2, v0, v1, v2)
 
 
 def _token_rows(t, name, tokens, row) -> int:
@@ -1123,7 +1128,7 @@ def paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_star
     dev = _device_of(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len)
     if (cos_t is None) != (sin_t is None):
         raise ValueError("give both RoPE tables or neither")
-    n, KVH, P, D, B, cols, ld_table, lds = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
+    KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
     if q_out.dim() != 3 or q_out.shape[2] != D:
         raise ValueError(f"q_out must be [tokens, n_head, {D}]")
     T, H, _ = q_out.shape
@@ -1139,9 +1144,7 @@ def paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_star
     ld_qkv, ld_q = _token_rows(qkv, "qkv", T, row), _token_rows(q_out, "q_out", T, H * D)
     px, pq = qkv.data_ptr(), q_out.data_ptr()
     _apart(px, ld_qkv, row, pq, ld_q, H * D, T, "qkv and q_out")
-    _call_on(dev, "xb_paged_rope_kv_bf16", px, cos, sin, pq, k_pages.data_ptr(), v_pages.data_ptr(),
-             page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), T, B, H, KVH, D, n, P, cols, rows, ld_qkv,
-             ld_q, ld_table, *lds)
+    _call_on(dev, "xb_paged_rope_kv_bf16", px, cos, sin, pq, kv, T, H, rows, ld_qkv, ld_q)
     return q_out
 
 
@@ -1160,7 +1163,7 @@ def paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale
     from single tokens to whole prompts in one batch.  Rows outside the
     sequences are left as they are; a token that sees no key gets zeros."""
     dev = _device_of(q, k_pages, v_pages, out, page_table, q_start, kv_len)
-    n, KVH, P, D, B, cols, ld_table, lds = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
+    KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
     if q.dim() != 3 or q.shape[2] != D:
         raise ValueError(f"q must be [tokens, n_head, {D}]")
     T, H, _ = q.shape
@@ -1171,9 +1174,7 @@ def paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale
     # of this call alone: the caching allocator orders its reuse on the stream,
     # and a captured graph keeps its own
     ws = torch.empty(_paged_attention_bytes(dev, T, B, H, KVH), dtype=torch.uint8, device=q.device)
-    _call_on(dev, "xb_paged_attention_bf16", pq, k_pages.data_ptr(), v_pages.data_ptr(), po, page_table.data_ptr(),
-             q_start.data_ptr(), kv_len.data_ptr(), T, B, H, KVH, D, n, P, cols, ld_q, ld_out, ld_table, *lds,
-             float(scale), ws.data_ptr(), ws.numel())
+    _call_on(dev, "xb_paged_attention_bf16", pq, po, kv, T, H, ld_q, ld_out, float(scale), ws.data_ptr(), ws.numel())
     return out
 
 
