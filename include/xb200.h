@@ -674,9 +674,10 @@ XB_API int xb_attention_workspace_size(int64_t batch, int64_t seq,
  * a step makes several calls with the same one.
  *
  * No content of the device arrays makes a kernel leave its buffers.  A page
- * id outside [0, n_pages) that a sequence needs, a position with no table
- * column, or a RoPE position outside the tables sets the flag that
- * xb_page_status reports.
+ * id outside [0, n_pages) that a sequence needs, and a new token whose position
+ * has no table column or RoPE row, set the flag that xb_page_status reports.
+ * The first call of each operator sets up its kernels: make it before a
+ * stream capture.
  * ------------------------------------------------------------------------- */
 
 typedef struct xb_paged_kv {

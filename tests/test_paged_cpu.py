@@ -81,6 +81,8 @@ def _attn(**kw):
     (dict(scale=0.0), _lib.XB_ERR_INVALID, "scale"),
     (dict(scale=-1.0), _lib.XB_ERR_INVALID, "scale"),
     (dict(scale=float("nan")), _lib.XB_ERR_INVALID, "scale"),
+    (dict(scale=float("inf")), _lib.XB_ERR_INVALID, "scale"),
+    (dict(n_head=258), _lib.XB_ERR_UNSUPPORTED, "heads per KV head"),
     (dict(q=None), _lib.XB_ERR_INVALID, "null"),
     (dict(table=None), _lib.XB_ERR_INVALID, "null"),
     (dict(ld_q=895), _lib.XB_ERR_INVALID, "pitch"),

@@ -231,6 +231,48 @@ def test_token_ranges_outside_the_rows_are_clamped():
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("new,cols", [([1] * 70, 300_000), ([200, 1, 57], 1_000_000)])
+def test_tables_so_wide_that_the_split_takes_64_bits(new, cols):
+    """The same bits as with a narrow table: only the host's bound on the work differs."""
+    b = Batch(new, [37 * i % 613 for i in range(len(new))], 14, 2, 16, seed=16)
+    want = b.attend()
+    wide = torch.full((len(new), cols), -1, dtype=torch.int32, device="cuda")
+    wide[:, :b.table.shape[1]] = b.table_dev
+    b.table_dev = wide
+    out = b.attend()
+    assert torch.equal(out, want)
+    b.check(out)
+
+
+def test_many_heads_share_a_kv_head():
+    """Up to 128 query heads per KV head: tiles of one token."""
+    for H, KVH in ((128, 1), (34, 2), (100, 2)):
+        b = Batch([1, 3, 40], [90, 5, 0], H, KVH, 16, seed=17)
+        b.check(b.attend())
+
+
+def test_calls_from_several_threads():
+    import threading
+
+    batches = [Batch([1] * 5, [300, 9, 77, 0, 1200], 14, 2, 16, seed=18), Batch([150, 2], [30, 500], 12, 12, 32, seed=19)]
+    qs, want = [b.q.cuda() for b in batches], [b.attend() for b in batches]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                if not torch.equal(batches[i % 2].attend(qs[i % 2]), want[i % 2]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and ops.device_status() == 0
+
+
 def test_attention_graph_replays_with_other_lengths_and_pages():
     a = Batch([1, 1, 1, 1], [40, 3, 700, 0], 14, 2, 16, seed=11, extra_cols=30)
     b = Batch([1, 2, 0, 1], [900, 64, 5, 17], 14, 2, 16, seed=12, extra_cols=17)
@@ -383,6 +425,23 @@ def test_rope_kv_skips_what_has_no_place():
     changed = (b.kp.view(torch.int16) != before_k.view(torch.int16)).any(-1).any(1).nonzero().tolist()
     where = sorted([[int(b.table[1, 0]), 0], [int(b.table[1, 0]), 1], [int(b.table[3, 1]), 4]])
     assert sorted(changed) == where
+
+
+def test_rope_kv_with_starts_that_do_not_ascend():
+    """Nothing outside the sequences' own pages is written, whatever the starts say."""
+    b = Batch([3, 3, 3], [10, 20, 30], 14, 2, 16, seed=26)
+    qkv = torch.randn((b.T, 18 * 64), generator=torch.Generator().manual_seed(27)).to(torch.bfloat16).cuda()
+    for starts in ([0, 9, 3, 9], [9, 6, 3, 0], [0, 3, -2 ** 31, 9], [2 ** 31 - 1] * 4, [-5, 2, 40, 1]):
+        b.q_start.copy_(torch.tensor(starts, dtype=torch.int64).to(torch.int32))
+        b.kv_len.fill_(2 ** 31 - 1 if starts[0] == 0 else 12)
+        kp, vp = b.kp.clone(), b.vp.clone()
+        q = torch.full((b.T, 14, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        ops.paged_rope_kv(qkv, None, None, q, kp, vp, b.table_dev, b.q_start, b.kv_len)
+        used = {int(p) for p in b.table.flatten() if p >= 0}
+        for pool, was in ((kp, b.kp), (vp, b.vp)):
+            changed = (pool.view(torch.int16) != was.view(torch.int16)).flatten(1).any(1).nonzero().flatten().tolist()
+            assert set(changed) <= used
+    ops.page_status()
 
 
 # ----------------------------------------------------------------------------- page copies
