@@ -1026,8 +1026,8 @@ template <typename I>
 __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __grid_constant__ TcMaps maps,
                                                                       const AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], drain_bar, o_full[2], o_empty;
-  __shared__ __align__(8) uint64_t s_full[2], p_full[2];
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], drain_bar, o_empty;
+  __shared__ __align__(8) uint64_t s_full[3], p_full[3], o_full[3];
   __shared__ __align__(8) uint64_t kv_full[kTcStages], kv_empty[kTcStages];
   __shared__ __align__(8) uint64_t seg_full[kTcSegs], seg_empty[kTcSegs];
   __shared__ Segment segs[kTcSegs];  // rows == 0: the end
@@ -1048,11 +1048,13 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
       mbar_init(&seg_empty[i], 5);  // the MMA warp and the four softmax warps
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&o_full[i], 1);  // P V of an even / odd tile accumulated into O
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 128);  // Q's buffer, which the output passes through, free
+    }
+    for (int i = 0; i < 3; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);  // P V of a tile accumulated into O
     }
     for (int i = 0; i < kTcStages; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -1071,7 +1073,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_base_sh;  // S / P buffers at columns 0 and 64, O at 128
+  const uint32_t tmem = tmem_base_sh;  // S / P buffers at columns 0, 64 and 128, O at 192
   pdl_wait();
   pdl_trigger();
 
@@ -1200,16 +1202,16 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     // base moved); a unit's first tile starts O afresh, after the softmax has
     // read the previous unit's
     auto pv = [&]() -> bool {
-      if (!mbar_wait(&p_full[pend & 1], (pend >> 1) & 1, kWaitLimit, &abort_flag)) return false;
+      if (!mbar_wait(&p_full[pend % 3], (pend / 3) & 1, kWaitLimit, &abort_flag)) return false;
       if (pend_first && pend_lu > 0 && !mbar_wait(&o_empty, (pend_lu - 1) & 1, kWaitLimit, &abort_flag)) return false;
       tc_fence_after();
       const uint32_t sv = sKV + (pend % kTcStages) * 2 * kTcTileBytes + kTcTileBytes;
-      const uint32_t p = tmem + (pend & 1) * 64;
+      const uint32_t p = tmem + (pend % 3) * 64;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)  // keys in steps of 16: 8 columns of P
-        mma_f16_ts(tmem + 128, p + ks * 8, umma_desc_sw128(sv + ks * 16 * 128, kTcTileBytes, 1024), kIdO,
+        mma_f16_ts(tmem + 192, p + ks * 8, umma_desc_sw128(sv + ks * 16 * 128, kTcTileBytes, 1024), kIdO,
                    (!pend_first || ks > 0) ? 1u : 0u);
-      tc_commit(&o_full[pend & 1]);
+      tc_commit(&o_full[pend % 3]);
       tc_commit(&kv_empty[pend % kTcStages]);
       return true;
     };
@@ -1220,10 +1222,11 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
         if (!mbar_wait(&q_full[lu & 1], (lu >> 1) & 1, kWaitLimit, &abort_flag)) ok = false;
         const uint32_t q = sQ + (lu & 1) * kTcQBytes;
         for (int j = s.t0; j < s.t1 && ok; ++j, ++g) {
-          // S_g over P_{g-2}, whose P V has completed
+          // S_g over P_{g-3}, whose P V has completed (two buffers would put the
+          // wait for P_{g-2} V, its own barrier trip included, before every S_g)
           const int st = g % kTcStages;
           if (!mbar_wait(&kv_full[st], (g / kTcStages) & 1, kWaitLimit, &abort_flag) ||
-              (g >= 2 && !mbar_wait(&o_full[g & 1], ((g - 2) >> 1) & 1, kWaitLimit, &abort_flag))) {
+              (g >= 3 && !mbar_wait(&o_full[g % 3], ((g - 3) / 3) & 1, kWaitLimit, &abort_flag))) {
             ok = false;
             break;
           }
@@ -1231,10 +1234,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
           const uint32_t sk = sKV + st * 2 * kTcTileBytes;
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)  // head dim in steps of 16
-            mma_f16(tmem + (g & 1) * 64, umma_desc_sw128(q + ks * 32, 16, 1024),
+            mma_f16(tmem + (g % 3) * 64, umma_desc_sw128(q + ks * 32, 16, 1024),
                     umma_desc_sw128(sk + ks * 32, 16, 1024), kIdS, ks > 0 ? 1u : 0u);
           any = true;
-          tc_commit(&s_full[g & 1]);
+          tc_commit(&s_full[g % 3]);
           if (pend >= 0 && !pv()) {
             ok = false;
             break;
@@ -1274,8 +1277,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
       const int seen = min(s.first_pos + tok, s.keys - 1);  // the last key this row sees
       float m = -INFINITY, l = 0.0f;                        // m: the base of P (log2 units)
       for (int j = s.t0; j < s.t1; ++j, ++g) {
-        const int sb = g & 1;
-        ok = wait_all(&s_full[sb], g >> 1);
+        const int sb = g % 3;
+        ok = wait_all(&s_full[sb], g / 3);
         if (!ok) break;
         tc_fence_after();
         const int k0 = j * kTcTK;
@@ -1316,17 +1319,17 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
             l *= alpha;
             m = mn;
             if (!first) {  // O, with P_{g-1} V in it, to the new bases before P_g V adds to it
-              ok = wait_all(&o_full[sb ^ 1], (g - 1) >> 1);
+              ok = wait_all(&o_full[(g + 2) % 3], (g - 1) / 3);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll
               for (int h = 0; h < 4; ++h) {
                 uint32_t ov[16];
-                tmem_ld_x16(tmem + 128 + h * 16 + lane_off, ov);
+                tmem_ld_x16(tmem + 192 + h * 16 + lane_off, ov);
                 tmem_ld_wait();
 #pragma unroll
                 for (int c = 0; c < 16; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
-                tmem_st_x16(tmem + 128 + h * 16 + lane_off, ov);
+                tmem_st_x16(tmem + 192 + h * 16 + lane_off, ov);
               }
             }
           }
@@ -1372,13 +1375,13 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
         continue;
       }
       // the unit's last P V, then O: read and released for the next unit
-      ok = wait_all(&o_full[(g - 1) & 1], (g - 1) >> 1);
+      ok = wait_all(&o_full[(g - 1) % 3], (g - 1) / 3);
       if (!ok) break;
       tc_fence_after();
       uint32_t ov[64];
       if (warp_valid) {
-        tmem_ld_32x32b_x32(tmem + 128 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[0]));
-        tmem_ld_32x32b_x32(tmem + 128 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[32]));
+        tmem_ld_32x32b_x32(tmem + 192 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[0]));
+        tmem_ld_32x32b_x32(tmem + 192 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[32]));
         tmem_ld_wait();
       }
       tc_fence_before();
