@@ -961,6 +961,15 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
 // rescaled.  Warps whose 32 rows are all past the unit's (a single token of a
 // decoding sequence in a mixed batch) skip the arithmetic.  Every wait is
 // bounded; a timeout sets the status word, drains what is in flight and ends.
+//
+// What bounds it: 4096 tokens at position 28672 (14 heads on 2) take 718 us,
+// 628 TFLOP/s; a tile takes 1900 clocks with two CTAs per SM, in which the
+// special-function unit works 1024 (53 %) and the eight N = 64 MMAs of each
+// CTA's tile are issued over as many.  With no exponentials it takes 677 us,
+// with hardly any softmax 585 us, with no K / V loads 714 us: the chain of
+// scores, softmax and P V through barriers and TMEM sets the pace.  Measured
+// slower: four CTAs per SM with one score buffer (757 us), three (862), each
+// tile's scores fetched during the one before (830 to 912).
 constexpr int kTcRows = 128;
 constexpr int kTcTK = 64;
 constexpr int kTcStages = 4;
@@ -1020,6 +1029,13 @@ __device__ __forceinline__ float2 add2(float2 x, float2 y) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
   return d;
+}
+
+// True in one lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
 }
 
 template <typename I>
@@ -1195,69 +1211,80 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     constexpr uint32_t kIdS = umma_idesc(1, 1, 1, 0, 0, kTcRows, kTcTK);  // Q (K-major) x K tile (K-major)
     constexpr uint32_t kIdO = umma_idesc(1, 1, 1, 0, 1, kTcRows, kHD);    // P (TMEM) x V tile (MN-major)
     bool any = false, ok = true;
-    int g = 0, lu = 0;
-    int pend = -1, pend_lu = 0;  // the tile whose P V is still to issue
-    bool pend_first = false;
-    // P_g V_g accumulated into O once P_g is written (and O rescaled where its
-    // base moved); a unit's first tile starts O afresh, after the softmax has
-    // read the previous unit's
+    int lu = 0;
+    // The whole warp runs the loop and one elected lane issues: descriptors
+    // differ by additions, ring positions by increments, all in uniform
+    // registers (1 to 2 % over one lane of a diverged warp doing all of it).
+    const bool leader = elect_one();
+    const uint64_t dq = umma_desc_sw128(sQ, 16, 1024), dk = umma_desc_sw128(sKV, 16, 1024),
+                   dv = umma_desc_sw128(sKV + kTcTileBytes, kTcTileBytes, 1024);
+    constexpr uint32_t kStep = 2 * kTcTileBytes >> 4, kQStep = kTcQBytes >> 4;  // descriptor units of 16 bytes
+    struct Slot {  // of a tile: ring position and S buffer with their phases
+      int st, sb;
+      uint32_t kph, sph;
+    };
+    Slot now = {0, 0, 0, 0}, pend = {-1, 0, 0, 0};  // pend: the tile whose P V is still to issue
+    int pend_first = 0;                             // unit + 1 when it is the unit's first tile
+    // P V of a tile accumulated into O once P is written (and O rescaled where
+    // its base moved); a unit's first tile starts O afresh, after the softmax
+    // has read the previous unit's
     auto pv = [&]() -> bool {
-      if (!mbar_wait(&p_full[pend % 3], (pend / 3) & 1, kWaitLimit, &abort_flag)) return false;
-      if (pend_first && pend_lu > 0 && !mbar_wait(&o_empty, (pend_lu - 1) & 1, kWaitLimit, &abort_flag)) return false;
+      if (!wait_all(&p_full[pend.sb], pend.sph)) return false;
+      if (pend_first > 1 && !wait_all(&o_empty, pend_first)) return false;
       tc_fence_after();
-      const uint32_t sv = sKV + (pend % kTcStages) * 2 * kTcTileBytes + kTcTileBytes;
-      const uint32_t p = tmem + (pend % 3) * 64;
+      const uint64_t d = dv + (uint64_t)(pend.st * kStep);
+      const uint32_t p = tmem + pend.sb * 64;
+      if (leader) {
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)  // keys in steps of 16: 8 columns of P
-        mma_f16_ts(tmem + 192, p + ks * 8, umma_desc_sw128(sv + ks * 16 * 128, kTcTileBytes, 1024), kIdO,
-                   (!pend_first || ks > 0) ? 1u : 0u);
-      tc_commit(&o_full[pend % 3]);
-      tc_commit(&kv_empty[pend % kTcStages]);
+        for (int ks = 0; ks < 4; ++ks)  // keys in steps of 16: 8 columns of P
+          mma_f16_ts(tmem + 192, p + ks * 8, d + ks * 128, kIdO, (ks > 0 || !pend_first) ? 1u : 0u);
+        tc_commit(&o_full[pend.sb]);
+        tc_commit(&kv_empty[pend.st]);
+      }
+      __syncwarp();
       return true;
     };
     Segment s;
     for (int n = 0; ok && take(n, s); ++n) {
-      if (s.t0 >= s.t1) continue;
-      if (lane == 0) {
-        if (!mbar_wait(&q_full[lu & 1], (lu >> 1) & 1, kWaitLimit, &abort_flag)) ok = false;
-        const uint32_t q = sQ + (lu & 1) * kTcQBytes;
-        for (int j = s.t0; j < s.t1 && ok; ++j, ++g) {
-          // S_g over P_{g-3}, whose P V has completed (two buffers would put the
-          // wait for P_{g-2} V, its own barrier trip included, before every S_g)
-          const int st = g % kTcStages;
-          if (!mbar_wait(&kv_full[st], (g / kTcStages) & 1, kWaitLimit, &abort_flag) ||
-              (g >= 3 && !mbar_wait(&o_full[g % 3], ((g - 3) / 3) & 1, kWaitLimit, &abort_flag))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sk = sKV + st * 2 * kTcTileBytes;
+      const int tiles = __shfl_sync(0xffffffffu, s.t1 - s.t0, 0);
+      if (tiles <= 0) continue;
+      ok = wait_all(&q_full[lu & 1], lu >> 1);
+      const uint64_t q = dq + (uint64_t)((lu & 1) * kQStep);
+      for (int j = 0; j < tiles && ok; ++j) {
+        // S over the P of three tiles before, whose P V has completed (two
+        // buffers would put the wait for the last but one P V before every S)
+        ok = wait_all(&kv_full[now.st], now.kph) && wait_all(&o_full[now.sb], now.sph ^ 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t k = dk + (uint64_t)(now.st * kStep);
+        const uint32_t d = tmem + now.sb * 64;
+        if (leader) {
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)  // head dim in steps of 16
-            mma_f16(tmem + (g % 3) * 64, umma_desc_sw128(q + ks * 32, 16, 1024),
-                    umma_desc_sw128(sk + ks * 32, 16, 1024), kIdS, ks > 0 ? 1u : 0u);
-          any = true;
-          tc_commit(&s_full[g % 3]);
-          if (pend >= 0 && !pv()) {
-            ok = false;
-            break;
-          }
-          pend = g;
-          pend_first = j == s.t0;
-          pend_lu = lu;
+            mma_f16(d, q + ks * 2, k + ks * 2, kIdS, ks > 0 ? 1u : 0u);
+          tc_commit(&s_full[now.sb]);
         }
-        if (!ok) fail();
+        __syncwarp();
+        any = true;
+        if (pend.st >= 0) ok = pv();
+        pend = now;
+        pend_first = j == 0 ? lu + 1 : 0;
+        if (++now.st == kTcStages) {
+          now.st = 0;
+          now.kph ^= 1;
+        }
+        if (++now.sb == 3) {
+          now.sb = 0;
+          now.sph ^= 1;
+        }
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
       ++lu;
     }
-    if (lane == 0) {
-      if (ok && pend >= 0 && !pv()) fail();
-      if (any) {  // every issued MMA completes before TMEM is released (also after an abort)
-        tc_commit(&drain_bar);
-        uint64_t deadline = 0;
-        if (!mbar_wait_deadline(&drain_bar, 0, &deadline, kWaitLimit)) fail();
-      }
+    if (ok && pend.st >= 0) pv();
+    if (any && leader) {  // every issued MMA completes before TMEM is released (also after an abort)
+      tc_commit(&drain_bar);
+      uint64_t deadline = 0;
+      if (!mbar_wait_deadline(&drain_bar, 0, &deadline, kWaitLimit)) fail();
     }
     __syncwarp();
   } else {
