@@ -541,6 +541,13 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                : "memory");
 }
 
+// True in one lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
+
 // transposes an 8 x 8 matrix of 16-bit elements held one row per four lanes
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
@@ -608,10 +615,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
     return;
   }
   if (found[warp].b >= 0) {
-    const int boxes = kTK / a.box_rows;
-    const bool is_v = lane >= boxes;
-    const int box = lane & (boxes - 1);  // boxes: a power of two
-    const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+    const bool leader = elect_one();
     // This thread's rows: 8 n + 2 t and the next one, and the tokens they belong to
     int tok[NT][2];
 #pragma unroll
@@ -634,45 +638,44 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
     // latency for many tiles
     uint32_t win = 0;
     int win_id = 0;
-    int pi = 0, row = 0;  // page index and row of this lane's box of the next tile
+    uint32_t pi = 0;  // page index and row where the next tile starts
+    int row = 0;
     auto window = [&](uint32_t first) {
       win = first;
       const uint32_t p = first + lane;
       win_id = p * (uint64_t)a.page_size < (uint32_t)si.keys ? __ldg(a.table + si.b * a.ld_table + p) : -1;
     };
     auto enter = [&]() {  // the first tile of a segment
-      const uint32_t key = (uint32_t)(ni * kTK);
-      const uint32_t p = key / (uint32_t)a.page_size;
-      window(p);
-      pi = (int)p;
-      row = (int)(key - p * (uint32_t)a.page_size) + box * a.box_rows;
-      while (row >= a.page_size) {
-        row -= a.page_size;
-        ++pi;
-      }
+      pi = (uint32_t)(ni * kTK) / (uint32_t)a.page_size;
+      row = ni * kTK - (int)pi * a.page_size;
+      window(pi);
     };
-    // lanes 0 .. boxes - 1 load K rows, the next `boxes` lanes V rows
+    // page piece by page piece (a piece never crosses a page), in uniform registers
     auto request = [&]() {
       const uint32_t buf = issued % kBufs;
-      const int k0 = ni * kTK, have = min(kTK, si.keys - k0);
+      const int have = min(kTK, si.keys - ni * kTK);
       const int nb = (have + a.box_rows - 1) / a.box_rows;
-      if (__any_sync(0xffffffffu, box < nb && pi - win >= 32u)) window(__shfl_sync(0xffffffffu, (uint32_t)pi, 0));
-      int id = __shfl_sync(0xffffffffu, win_id, (int)(pi - win));
-      if (lane == 0) mbar_arrive_expect_tx(&full[warp][buf], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
-      __syncwarp();
-      if (lane < 2 * boxes && box < nb) {
+      if (leader) mbar_arrive_expect_tx(&full[warp][buf], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
+      uint32_t dst = ring + buf * 2 * kTileBytes;
+      for (int i = 0; i < nb; ++i) {
+        if (pi - win >= 32u) window(pi);
+        int id = __shfl_sync(0xffffffffu, win_id, (int)(pi - win));
         if (id < 0 || id >= a.n_pages) {  // reads as zeros: a coordinate past the pool
-          atomicExch(a.bad, 1);
+          if (leader) atomicExch(a.bad, 1);
           id = a.n_pages;
         }
-        tma_load_4d(ring + buf * 2 * kTileBytes + (is_v ? kTileBytes : 0) + box * a.box_rows * kHD * 2, map,
-                    &full[warp][buf], 0, row, si.kvh, id);
+        if (leader) {
+          tma_load_4d(dst, &maps.k, &full[warp][buf], 0, row, si.kvh, id);
+          tma_load_4d(dst + kTileBytes, &maps.v, &full[warp][buf], 0, row, si.kvh, id);
+        }
+        dst += a.box_rows * kHD * 2;
+        row += a.box_rows;
+        if (row == a.page_size) {
+          row = 0;
+          ++pi;
+        }
       }
-      row += kTK;
-      while (row >= a.page_size) {
-        row -= a.page_size;
-        ++pi;
-      }
+      __syncwarp();
       ++issued;
       ++ni;
     };
@@ -1029,13 +1032,6 @@ __device__ __forceinline__ float2 add2(float2 x, float2 y) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
   return d;
-}
-
-// True in one lane of a converged warp, the same one every time.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
-  return r != 0;
 }
 
 template <typename I>
