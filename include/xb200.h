@@ -676,6 +676,8 @@ XB_API int xb_attention_workspace_size(int64_t batch, int64_t seq,
  * No content of the device arrays makes a kernel leave its buffers.  A page
  * id outside [0, n_pages) that a sequence needs, and a new token whose position
  * has no table column or RoPE row, set the flag that xb_page_status reports.
+ * New tokens' places (page, row) have to differ, within a call and between
+ * calls at the same time: which of two writes to one place stays is not said.
  * The first call of each operator sets up its kernels: make it before a
  * stream capture.
  * ------------------------------------------------------------------------- */
@@ -714,7 +716,10 @@ XB_API int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t,
  * before P V, as xb_attention_bf16.  A token with a negative position
  * (kv_len[b] < n) sees nothing: its row is zero.  Lengths beyond the table
  * count as max_pages * page_size; a page id outside the pool reads as zeros
- * (flagged).  Long contexts are split over CTAs and joined in a fixed order:
+ * (flagged).  What lies behind a sequence's last key may be anything; keys that a
+ * token does not see weigh zero, so as in xb_attention_bf16 a value of theirs
+ * that is infinite or NaN spoils the row of an earlier token of the same step.
+ * Long contexts are split over CTAs and joined in a fixed order:
  * the same inputs give the same bits, and the split depends on the whole
  * batch's lengths.  `workspace` (16-byte aligned, size from the query below,
  * any content) holds the partial results of one call; calls that may run at

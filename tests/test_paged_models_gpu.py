@@ -180,3 +180,37 @@ def test_forward_paged_refusals(qwen, gpt2):
     with pytest.raises(ValueError):
         model.generate_paged([torch.zeros(0, dtype=torch.int64)], 3)
 
+
+
+def test_refused_steps_leave_the_cache_as_it_was(qwen, gpt2):
+    """What the operators of a step would refuse is refused before the cache gives room for it."""
+    model, _ = qwen
+    cache = PagedKVCache(model.cfg, 4, 16)
+    a = cache.add()
+    ids = torch.zeros(3, dtype=torch.int64, device="cuda")
+    one = torch.zeros(1, dtype=torch.int64, device="cuda")
+    for kw in (dict(ids=ids.int()), dict(ids=ids.cpu()), dict(next_token=one.int()), dict(next_token=one.cpu()),
+               dict(next_token=ids), dict(next_token=torch.zeros((1, 1), dtype=torch.int64, device="cuda"))):
+        with pytest.raises(ValueError):
+            model.forward_paged(**{"ids": ids, "cache": cache, "seqs": [a], "counts": [3], **kw})
+    other = PagedKVCache(gpt2.cfg, 4, 16)
+    b = other.add()
+    with pytest.raises(ValueError, match="another model"):
+        model.forward_paged(ids, other, [b], [3])
+    with pytest.raises(ValueError, match="another model"):
+        PagedDecodeGraph(model, other, 1, 64)
+    graph = PagedDecodeGraph(model, cache, 1, 64)
+    with pytest.raises(ValueError, match="int64"):
+        graph.step([a], one.float())
+    assert cache.length(a) == other.length(b) == 0 and cache.free_pages == other.free_pages == 4
+
+
+def test_generation_up_to_the_last_position(qwen):
+    """A prompt and its continuation may fill the table: the last token is never fed back."""
+    model, _ = qwen
+    prompt = _ids(1024 - 4, model.cfg.vocab_size, 95)
+    cache = PagedKVCache(model.cfg, 64, 16)  # 1024 positions
+    out = model.generate_paged(iter([prompt]), 5, cache=cache)
+    assert torch.equal(out, model.generate_paged([prompt], 5, graph=False)) and cache.free_pages == 64
+    with pytest.raises(ValueError, match="positions"):
+        model.generate_paged([prompt], 6)

@@ -36,7 +36,7 @@ from dataclasses import dataclass
 import torch
 
 from . import ops
-from .paged import PagedBatch, PagedKVCache, generate_paged
+from .paged import PagedBatch, PagedKVCache, check_step, generate_paged
 from .qwen import DecodeGraphs
 
 # (n_layer, n_head, n_embd) of the four published sizes (model.py:90-108)
@@ -339,12 +339,7 @@ class GPT2Model:
         of them and single tokens in any mixture.  Returns fp32 logits
         [len(seqs), vocab] after each sequence's last token, or writes the
         greedy tokens into `next_token` (int64) and returns None."""
-        counts = [1] * len(seqs) if counts is None else [int(n) for n in counts]
-        if ids.dim() != 1 or ids.shape[0] != sum(counts):
-            raise ValueError(f"ids must be 1-D with {sum(counts)} tokens")
-        for q, n in zip(seqs, counts):
-            if cache.length(q) + n > self.position_limit:
-                raise ValueError(f"sequence {q} would exceed the position table ({self.position_limit})")
+        seqs, counts = check_step(self, ids, cache, seqs, counts, next_token, "position table")
         return self.forward_packed(ids, cache, cache.step(seqs, counts), next_token=next_token)
 
     def generate_paged(self, prompts, max_new_tokens: int, **kw) -> torch.Tensor:

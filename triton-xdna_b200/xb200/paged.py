@@ -236,6 +236,36 @@ class PagedKVCache:
         return len(high)
 
 
+def _check_cache(model, cache: PagedKVCache) -> None:
+    c = model.cfg
+    want, have = (c.n_layer, 2, c.n_kv_head, c.head_dim), tuple(cache.pages.shape)
+    if have[:2] + have[3:4] + have[5:] != want:
+        raise ValueError(f"the cache was made for another model: [n_layer, 2, n_kv_head, head_dim] is "
+                         f"{have[:2] + have[3:4] + have[5:]}, the model's {want}")
+    dev = model.layers[0]["qkv_w"].device
+    if cache.device != dev:
+        raise ValueError(f"the cache is on {cache.device}, the model on {dev}")
+
+
+def check_step(model, ids, cache: PagedKVCache, seqs, counts, next_token, table: str):
+    """Refuses what a step of `model` cannot take before the cache gives room
+    for it; (seqs, counts) as lists.  `table` names what limits positions."""
+    seqs = list(seqs)
+    counts = [1] * len(seqs) if counts is None else [int(n) for n in counts]
+    if ids.dim() != 1 or ids.shape[0] != sum(counts):
+        raise ValueError(f"ids must be 1-D with {sum(counts)} tokens")
+    for q, n in zip(seqs, counts):
+        if cache.length(q) + n > model.position_limit:
+            raise ValueError(f"sequence {q} would exceed the {table} ({model.position_limit})")
+    _check_cache(model, cache)
+    for name, t in (("ids", ids), ("next_token", next_token)):
+        if t is not None and (t.dtype is not torch.int64 or t.device != cache.device):
+            raise ValueError(f"{name} must be int64 on {cache.device}")
+    if next_token is not None and (next_token.shape != (len(seqs),) or not next_token.is_contiguous()):
+        raise ValueError(f"next_token must be contiguous [{len(seqs)}]")
+    return seqs, counts
+
+
 class PagedDecodeGraph:
     """One captured CUDA graph of a decode step for `batch` sequences of a
     paged cache.  The kernels read lengths and page tables from the device, so
@@ -246,6 +276,7 @@ class PagedDecodeGraph:
     def __init__(self, model, cache: PagedKVCache, batch: int, max_positions: int):
         if batch < 1 or not 0 < max_positions <= model.position_limit:
             raise ValueError(f"batch must be positive and max_positions 1 .. {model.position_limit}")
+        _check_cache(model, cache)
         self.cache, self.batch = cache, batch
         dev = cache.device
         self.columns = -(-max_positions // cache.page_size)
@@ -279,8 +310,8 @@ class PagedDecodeGraph:
         seqs = list(seqs)
         if len(seqs) != self.batch:
             raise ValueError(f"the graph was captured for {self.batch} sequences, got {len(seqs)}")
-        if ids.shape != self.ids.shape:
-            raise ValueError(f"ids must be [{self.batch}]")
+        if ids.shape != self.ids.shape or ids.dtype is not torch.int64:
+            raise ValueError(f"ids must be int64 [{self.batch}]")
         if any(self.cache.length(q) >= self._limit for q in seqs):
             raise ValueError(f"a sequence would outgrow the graph's {self._limit} positions")
         self.cache._grow(seqs, [1] * len(seqs))
@@ -299,13 +330,16 @@ def generate_paged(model, prompts, max_new_tokens: int, cache: PagedKVCache | No
     in one batch: the prompts are prefilled packed, then every sequence decodes
     a token per step.  Returns tokens [B, max_new_tokens] on the device; a
     `cache` that is passed in keeps nothing of the run."""
+    prompts = list(prompts)
     if not prompts or any(p.dim() != 1 or p.numel() == 0 for p in prompts) or max_new_tokens < 1:
         raise ValueError("prompts are non-empty 1-D tensors, and at least one token is generated")
     counts = [p.numel() for p in prompts]
-    longest = max(counts) + max_new_tokens
+    more = max_new_tokens - 1  # positions behind the prompts: the last token is never fed back
+    longest = max(counts) + more
+    if longest > model.position_limit:
+        raise ValueError(f"{longest} positions exceed the model's {model.position_limit}")
     if cache is None:
-        cache = PagedKVCache(model.cfg, sum(-(-(c + max_new_tokens) // page_size) for c in counts), page_size,
-                             model.device)
+        cache = PagedKVCache(model.cfg, sum(-(-(c + more) // page_size) for c in counts), page_size, model.device)
     B = len(prompts)
     ids = torch.cat([p.to(model.device) for p in prompts])
     toks = torch.empty((max_new_tokens, B), dtype=torch.int64, device=model.device)
