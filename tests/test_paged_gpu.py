@@ -165,6 +165,14 @@ def test_tokens_without_a_key_get_zeros(new, past):
     assert bool((out[:-past[0]] == 0).all())
 
 
+def test_many_sequences_without_a_key():
+    """Units without a key tile follow one with keys in the same share of work, more of them than a CTA looks ahead."""
+    b = Batch([70] + [1] * 4000 + [9] + [1] * 4000, [100] + [-1] * 4000 + [300] + [-1] * 4000, 32, 1, 16, seed=50)
+    out = b.attend()
+    b.check(out)
+    assert bool((out[70:4070] == 0).all()) and bool((out[4079:] == 0).all())
+
+
 def test_infinite_and_nan_inputs_stay_in_their_rows():
     """A NaN query spoils its own rows only; a NaN key those that see it; a -inf score weighs nothing."""
     b = Batch([40, 1], [0, 30], 14, 2, 16, seed=6)

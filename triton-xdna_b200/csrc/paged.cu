@@ -1243,7 +1243,13 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     Segment s;
     for (int n = 0; ok && take(n, s); ++n) {
       const int tiles = __shfl_sync(0xffffffffu, s.t1 - s.t0, 0);
-      if (tiles <= 0) continue;
+      if (tiles <= 0) {
+        // the softmax passes on (and the ring of segments with it) only once
+        // the unit before has its last P V
+        if (pend.st >= 0) ok = pv();
+        pend.st = -1;
+        continue;
+      }
       ok = wait_all(&q_full[lu & 1], lu >> 1);
       const uint64_t q = dq + (uint64_t)((lu & 1) * kQStep);
       for (int j = 0; j < tiles && ok; ++j) {
