@@ -950,29 +950,38 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
 //              ring, loads each unit's Q (two buffers) and streams K / V page
 //              rows into a ring of four tiles (one lane per page piece, TMA,
 //              128-byte swizzle);
-//   warp 1     issues S_g = Q K_g^T into one of two 64-column TMEM buffers and
-//              O += P_g V_g; P_g is the MMA's A operand straight from TMEM;
-//   warps 2-5  softmax, one query row per thread: scores from TMEM, bf16(P)
-//              back into the first half of the same TMEM buffer.
+//   warp 1     issues S_g = Q K_g^T into one of three 64-column TMEM buffers;
+//   warp 2     issues O += P_g V_g; P_g is the MMA's A operand straight from
+//              TMEM.  Values behind the last key are zeroed first;
+//   warps 4-7  softmax, one query row per thread: scores from TMEM, bf16(P)
+//              back into the first half of the same TMEM buffer (warp 3 only
+//              makes the warpgroups whole, which trade registers).
 // Keeping P in TMEM takes its write and its 16 KB operand read per tile off
 // shared memory, whose 128 bytes a clock would otherwise be the first limit
 // (Q, K, V and P reads, P writes and the TMA's writes: 640 of them a tile,
-// against 512 clocks of exponentials).  S_{g+1} is issued before P_g V_g, so
-// the softmax always has the next scores waiting.  O accumulates in TMEM
-// relative to a per-row base that moves only when a tile's maximum exceeds it
-// by more than 2^8 (bf16 keeps its 8 bits at any scale), and only then is O
-// rescaled.  Warps whose 32 rows are all past the unit's (a single token of a
-// decoding sequence in a mixed batch) skip the arithmetic.  Every wait is
-// bounded; a timeout sets the status word, drains what is in flight and ends.
+// against 512 clocks of exponentials).  S runs up to two tiles ahead, so the
+// softmax never waits for scores.  One warp issuing both products held it up:
+// each of a tile's eight dependent N = 64 MMAs takes some 66 clocks to issue and
+// each commit some 80 (4096 tokens at position 28672: 730 us, two warps 713).
+// O accumulates in TMEM relative to a per-row base that moves only when a
+// tile's maximum exceeds it by more than 2^8 (bf16 keeps its 8 bits at any
+// scale), and only then is O rescaled.  Warps whose 32 rows are all past the
+// unit's (a single token of a decoding sequence in a mixed batch) only pass the
+// tiles on.  Every wait is bounded; a timeout sets the status word, drains what
+// is in flight and ends.
 //
-// What bounds it: 4096 tokens at position 28672 (14 heads on 2) take 718 us,
-// 628 TFLOP/s; a tile takes 1900 clocks with two CTAs per SM, in which the
-// special-function unit works 1024 (53 %) and the eight N = 64 MMAs of each
-// CTA's tile are issued over as many.  With no exponentials it takes 677 us,
-// with hardly any softmax 585 us, with no K / V loads 714 us: the chain of
-// scores, softmax and P V through barriers and TMEM sets the pace.  Measured
-// slower: four CTAs per SM with one score buffer (757 us), three (862), each
-// tile's scores fetched during the one before (830 to 912).
+// What bounds it: the same 4096 tokens (14 heads on 2) take 666 us, 677
+// TFLOP/s, at 1.75 to 1.8 of 1.965 GHz (power).  Of the 1433 clocks a tile takes
+// the CTA that came first to its SM (the second: 1644) some 800 are the 64
+// exponentials of each row, which at 16 a clock and SM would be 512 alone;
+// waiting (110, the barrier's own latency: the scores are always there),
+// TMEM load (65), maximum (230) and store (45) come in between, and
+// the two CTAs fill each other's gaps only in part.  Measured no faster: maxima
+// only where a row's sum of P grows past 2^16 (677 us, prompts 59.8 against
+// 59.7), the next tile's scores loaded during the exponentials (713), key tiles
+// of 128 with one score buffer (760 where 64 took 730), four CTAs per SM with
+// one score buffer (757), three (862), longer pieces for an SM's first CTA
+// (prompts 56.2, but the chunk 676).
 constexpr int kTcRows = 128;
 constexpr int kTcTK = 64;
 constexpr int kTcStages = 4;
@@ -980,7 +989,8 @@ constexpr int kTcSegs = 4;  // segments published ahead
 constexpr int kTcQBytes = kTcRows * kHD * 2;
 constexpr int kTcTileBytes = kTcTK * kHD * 2;  // one K or V tile
 constexpr int kTcSmem = 2 * kTcQBytes + kTcStages * 2 * kTcTileBytes + 1024;
-constexpr int kTcThreads = 192;
+constexpr int kTcThreads = 256;
+constexpr int kTcFewRegs = 64, kTcSoftmaxRegs = 192;  // a thread, of the two warpgroups; 128 each at launch
 
 struct alignas(64) TcMaps {
   CUtensorMap q;  // [T][n_head][64], box {64, n_rep, tpt}
@@ -1038,9 +1048,9 @@ template <typename I>
 __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __grid_constant__ TcMaps maps,
                                                                       const AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], drain_bar, o_empty;
-  __shared__ __align__(8) uint64_t s_full[3], p_full[3], o_full[3];
-  __shared__ __align__(8) uint64_t kv_full[kTcStages], kv_empty[kTcStages];
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], drain_bar[2], o_empty;
+  __shared__ __align__(8) uint64_t s_full[3], p_full[3];
+  __shared__ __align__(8) uint64_t kv_full[kTcStages], pv_done[kTcStages];
   __shared__ __align__(8) uint64_t seg_full[kTcSegs], seg_empty[kTcSegs];
   __shared__ Segment segs[kTcSegs];  // rows == 0: the end
   __shared__ I sums[2][kTcThreads / 32];
@@ -1053,24 +1063,23 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
   const uint32_t sKV = sQ + 2 * kTcQBytes;
 
   if (threadIdx.x == 0) {
-    mbar_init(&drain_bar, 1);
     mbar_init(&o_empty, 128);  // a unit's O read by the softmax warps
     for (int i = 0; i < kTcSegs; ++i) {
       mbar_init(&seg_full[i], 1);
-      mbar_init(&seg_empty[i], 5);  // the MMA warp and the four softmax warps
+      mbar_init(&seg_empty[i], 6);  // the MMA warps and the four softmax warps
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&drain_bar[i], 1);
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 128);  // Q's buffer, which the output passes through, free
     }
     for (int i = 0; i < 3; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
-      mbar_init(&o_full[i], 1);  // P V of a tile accumulated into O
+      mbar_init(&p_full[i], 4);
     }
     for (int i = 0; i < kTcStages; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&pv_done[i], 1);  // P V accumulated into O: K, V and the tile's S buffer are free
     }
     abort_flag = 0;
     mbar_fence_init();
@@ -1111,185 +1120,187 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     return s.rows > 0;
   };
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ walk and TMA producer
-    uint32_t issued[kTcStages];
-#pragma unroll
-    for (int i = 0; i < kTcStages; ++i) issued[i] = 0;
-    const int boxes = kTcTK / a.box_rows;  // 1 .. 8 page pieces per tile; lane < boxes: K, the next ones: V
-    const bool is_v = lane >= boxes;
-    const int box = is_v ? lane - boxes : lane;
-    const CUtensorMap* map = is_v ? &maps.v : &maps.k;
-    const uint32_t q_bytes = (uint32_t)(a.tpt * a.n_rep * kHD * 2);
-    int g = 0, lu = 0, n = 0;  // tiles, units (with tiles) and segments so far
-    bool ok = true, open_unit = false;
-    Walk<I> w;
-    Segment s;
-    bool more = found[0].b >= 0;
-    if (more) {
-      place(a, w, (int)blockIdx.x, share, total, found[0]);
-      more = segment<kTcTK>(a, w, s);
-    }
-    auto publish = [&](int rows) -> bool {
-      if (!wait_all(&seg_empty[n % kTcSegs], n / kTcSegs + 1)) return false;
-      if (lane == 0) {
-        segs[n % kTcSegs] = s;
-        segs[n % kTcSegs].rows = rows;
-        mbar_arrive(&seg_full[n % kTcSegs]);
-      }
-      __syncwarp();
-      ++n;
-      return true;
-    };
-    for (; more && ok; more = next_unit(a, w) && segment<kTcTK>(a, w, s)) {
-      if (s.starts && !s.ends) {
-        open_unit = true;
-        if (lane == 0) meta[blockIdx.x] = Meta{s.last, s.token, s.rows, s.kvh};
-      }
-      ok = publish(s.rows);
-      if (!ok) break;
-      if (s.t0 >= s.t1) continue;
-      // this lane's page of the first tile, fetched while Q's buffer may still be in use
-      auto page_of = [&](int tile) -> int {
-        const int key = tile * kTcTK + box * a.box_rows;
-        return lane < 2 * boxes && key < s.keys ? __ldg(a.table + s.b * a.ld_table + (uint32_t)key / (uint32_t)a.page_size)
-                                                : 0;
-      };
-      int id = page_of(s.t0);
-      ok = wait_all(&q_empty[lu & 1], (lu >> 1) + 1);
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&q_full[lu & 1], q_bytes);
-        asm volatile(
-            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
-            "[%2];" ::"r"(sQ + (lu & 1) * kTcQBytes),
-            "l"(reinterpret_cast<uint64_t>(&maps.q)), "r"(smem_u32(&q_full[lu & 1])), "r"(0), "r"(s.kvh * a.n_rep),
-            "r"(s.token)
-            : "memory");
-      }
-      ++lu;
-      for (int j = s.t0; j < s.t1; ++j, ++g) {
-        const int st = g % kTcStages;
-        const int here = id;
-        if (j + 1 < s.t1) id = page_of(j + 1);
-        ok = wait_all(&kv_empty[st], g / kTcStages + 1);
-        if (!ok) break;
-        const int have = min(kTcTK, s.keys - j * kTcTK);
-        const int nb = (have + a.box_rows - 1) / a.box_rows;
-        if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
-        __syncwarp();
-        if (lane < 2 * boxes && box < nb) {
-          int page = here;
-          if (page < 0 || page >= a.n_pages) {  // reads as zeros: a coordinate past the pool
-            atomicExch(a.bad, 1);
-            page = a.n_pages;
-          }
-          const uint32_t row = (uint32_t)(j * kTcTK + box * a.box_rows) % (uint32_t)a.page_size;
-          tma_load_4d(sKV + st * 2 * kTcTileBytes + (is_v ? kTcTileBytes : 0) + box * a.box_rows * kHD * 2, map,
-                      &kv_full[st], 0, (int)row, s.kvh, page);
-        }
-        issued[st] = g / kTcStages + 1;
-      }
-    }
-    if (ok) publish(0);
-    if (!open_unit && lane == 0) meta[blockIdx.x].last = -1;
-    // every load issued must have landed before the CTA exits (also after an abort)
-    if (lane == 0) {
+  // Every MMA issued completes before TMEM is released (also after an abort)
+  auto drain = [&](int which, bool any) {
+    if (any && elect_one()) {
+      tc_commit(&drain_bar[which]);
       uint64_t deadline = 0;
-      for (int i = lu > 2 ? lu - 2 : 0; i < lu; ++i)
-        if (!mbar_wait_deadline(&q_full[i & 1], (i >> 1) & 1, &deadline, kWaitLimit)) fail();
-#pragma unroll
-      for (int st = 0; st < kTcStages; ++st)
-        if (issued[st] && !mbar_wait_deadline(&kv_full[st], (issued[st] - 1) & 1, &deadline, kWaitLimit)) fail();
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    constexpr uint32_t kIdS = umma_idesc(1, 1, 1, 0, 0, kTcRows, kTcTK);  // Q (K-major) x K tile (K-major)
-    constexpr uint32_t kIdO = umma_idesc(1, 1, 1, 0, 1, kTcRows, kHD);    // P (TMEM) x V tile (MN-major)
-    bool any = false, ok = true;
-    int lu = 0;
-    // The whole warp runs the loop and one elected lane issues: descriptors
-    // differ by additions, ring positions by increments, all in uniform
-    // registers (1 to 2 % over one lane of a diverged warp doing all of it).
-    const bool leader = elect_one();
-    const uint64_t dq = umma_desc_sw128(sQ, 16, 1024), dk = umma_desc_sw128(sKV, 16, 1024),
-                   dv = umma_desc_sw128(sKV + kTcTileBytes, kTcTileBytes, 1024);
-    constexpr uint32_t kStep = 2 * kTcTileBytes >> 4, kQStep = kTcQBytes >> 4;  // descriptor units of 16 bytes
-    struct Slot {  // of a tile: ring position and S buffer with their phases
-      int st, sb;
-      uint32_t kph, sph;
-    };
-    Slot now = {0, 0, 0, 0}, pend = {-1, 0, 0, 0};  // pend: the tile whose P V is still to issue
-    int pend_first = 0;                             // unit + 1 when it is the unit's first tile
-    // P V of a tile accumulated into O once P is written (and O rescaled where
-    // its base moved); a unit's first tile starts O afresh, after the softmax
-    // has read the previous unit's
-    auto pv = [&]() -> bool {
-      if (!wait_all(&p_full[pend.sb], pend.sph)) return false;
-      if (pend_first > 1 && !wait_all(&o_empty, pend_first)) return false;
-      tc_fence_after();
-      const uint64_t d = dv + (uint64_t)(pend.st * kStep);
-      const uint32_t p = tmem + pend.sb * 64;
-      if (leader) {
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)  // keys in steps of 16: 8 columns of P
-          mma_f16_ts(tmem + 192, p + ks * 8, d + ks * 128, kIdO, (ks > 0 || !pend_first) ? 1u : 0u);
-        tc_commit(&o_full[pend.sb]);
-        tc_commit(&kv_empty[pend.st]);
-      }
-      __syncwarp();
-      return true;
-    };
-    Segment s;
-    for (int n = 0; ok && take(n, s); ++n) {
-      const int tiles = __shfl_sync(0xffffffffu, s.t1 - s.t0, 0);
-      if (tiles <= 0) {
-        // the softmax passes on (and the ring of segments with it) only once
-        // the unit before has its last P V
-        if (pend.st >= 0) ok = pv();
-        pend.st = -1;
-        continue;
-      }
-      ok = wait_all(&q_full[lu & 1], lu >> 1);
-      const uint64_t q = dq + (uint64_t)((lu & 1) * kQStep);
-      for (int j = 0; j < tiles && ok; ++j) {
-        // S over the P of three tiles before, whose P V has completed (two
-        // buffers would put the wait for the last but one P V before every S)
-        ok = wait_all(&kv_full[now.st], now.kph) && wait_all(&o_full[now.sb], now.sph ^ 1);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t k = dk + (uint64_t)(now.st * kStep);
-        const uint32_t d = tmem + now.sb * 64;
-        if (leader) {
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)  // head dim in steps of 16
-            mma_f16(d, q + ks * 2, k + ks * 2, kIdS, ks > 0 ? 1u : 0u);
-          tc_commit(&s_full[now.sb]);
-        }
-        __syncwarp();
-        any = true;
-        if (pend.st >= 0) ok = pv();
-        pend = now;
-        pend_first = j == 0 ? lu + 1 : 0;
-        if (++now.st == kTcStages) {
-          now.st = 0;
-          now.kph ^= 1;
-        }
-        if (++now.sb == 3) {
-          now.sb = 0;
-          now.sph ^= 1;
-        }
-      }
-      ++lu;
-    }
-    if (ok && pend.st >= 0) pv();
-    if (any && leader) {  // every issued MMA completes before TMEM is released (also after an abort)
-      tc_commit(&drain_bar);
-      uint64_t deadline = 0;
-      if (!mbar_wait_deadline(&drain_bar, 0, &deadline, kWaitLimit)) fail();
+      if (!mbar_wait_deadline(&drain_bar[which], 0, &deadline, kWaitLimit)) fail();
     }
     __syncwarp();
+  };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcFewRegs));
+    if (warp == 0) {
+      // ------------------------------------------------------------ walk and TMA producer
+      uint32_t issued[kTcStages];
+#pragma unroll
+      for (int i = 0; i < kTcStages; ++i) issued[i] = 0;
+      const int boxes = kTcTK / a.box_rows;  // 1 .. 8 page pieces per tile; lane < boxes: K, the next ones: V
+      const bool is_v = lane >= boxes;
+      const int box = is_v ? lane - boxes : lane;
+      const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+      const uint32_t q_bytes = (uint32_t)(a.tpt * a.n_rep * kHD * 2);
+      int g = 0, lu = 0, n = 0;  // tiles, units (with tiles) and segments so far
+      bool ok = true, open_unit = false;
+      Walk<I> w;
+      Segment s;
+      bool more = found[0].b >= 0;
+      if (more) {
+        place(a, w, (int)blockIdx.x, share, total, found[0]);
+        more = segment<kTcTK>(a, w, s);
+      }
+      auto publish = [&](int rows) -> bool {
+        if (!wait_all(&seg_empty[n % kTcSegs], n / kTcSegs + 1)) return false;
+        if (lane == 0) {
+          segs[n % kTcSegs] = s;
+          segs[n % kTcSegs].rows = rows;
+          mbar_arrive(&seg_full[n % kTcSegs]);
+        }
+        __syncwarp();
+        ++n;
+        return true;
+      };
+      for (; more && ok; more = next_unit(a, w) && segment<kTcTK>(a, w, s)) {
+        if (s.starts && !s.ends) {
+          open_unit = true;
+          if (lane == 0) meta[blockIdx.x] = Meta{s.last, s.token, s.rows, s.kvh};
+        }
+        ok = publish(s.rows);
+        if (!ok) break;
+        if (s.t0 >= s.t1) continue;
+        // this lane's page of the first tile, fetched while Q's buffer may still be in use
+        auto page_of = [&](int tile) -> int {
+          const int key = tile * kTcTK + box * a.box_rows;
+          if (lane >= 2 * boxes || key >= s.keys) return 0;
+          return __ldg(a.table + s.b * a.ld_table + (uint32_t)key / (uint32_t)a.page_size);
+        };
+        int id = page_of(s.t0);
+        ok = wait_all(&q_empty[lu & 1], (lu >> 1) + 1);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&q_full[lu & 1], q_bytes);
+          asm volatile(
+              "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+              "[%2];" ::"r"(sQ + (lu & 1) * kTcQBytes),
+              "l"(reinterpret_cast<uint64_t>(&maps.q)), "r"(smem_u32(&q_full[lu & 1])), "r"(0), "r"(s.kvh * a.n_rep),
+              "r"(s.token)
+              : "memory");
+        }
+        ++lu;
+        for (int j = s.t0; j < s.t1; ++j, ++g) {
+          const int st = g % kTcStages;
+          const int here = id;
+          if (j + 1 < s.t1) id = page_of(j + 1);
+          ok = wait_all(&pv_done[st], g / kTcStages + 1);
+          if (!ok) break;
+          const int have = min(kTcTK, s.keys - j * kTcTK);
+          const int nb = (have + a.box_rows - 1) / a.box_rows;
+          if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
+          __syncwarp();
+          if (lane < 2 * boxes && box < nb) {
+            int page = here;
+            if (page < 0 || page >= a.n_pages) {  // reads as zeros: a coordinate past the pool
+              atomicExch(a.bad, 1);
+              page = a.n_pages;
+            }
+            const uint32_t row = (uint32_t)(j * kTcTK + box * a.box_rows) % (uint32_t)a.page_size;
+            tma_load_4d(sKV + st * 2 * kTcTileBytes + (is_v ? kTcTileBytes : 0) + box * a.box_rows * kHD * 2, map,
+                        &kv_full[st], 0, (int)row, s.kvh, page);
+          }
+          issued[st] = g / kTcStages + 1;
+        }
+      }
+      if (ok) publish(0);
+      if (!open_unit && lane == 0) meta[blockIdx.x].last = -1;
+      // every load issued must have landed before the CTA exits (also after an abort)
+      if (lane == 0) {
+        uint64_t deadline = 0;
+        for (int i = lu > 2 ? lu - 2 : 0; i < lu; ++i)
+          if (!mbar_wait_deadline(&q_full[i & 1], (i >> 1) & 1, &deadline, kWaitLimit)) fail();
+#pragma unroll
+        for (int st = 0; st < kTcStages; ++st)
+          if (issued[st] && !mbar_wait_deadline(&kv_full[st], (issued[st] - 1) & 1, &deadline, kWaitLimit)) fail();
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ S = Q K^T
+      // The whole warp runs the loop and one elected lane issues: descriptors
+      // differ by additions, ring positions by increments, all in uniform registers.
+      constexpr uint32_t kIdS = umma_idesc(1, 1, 1, 0, 0, kTcRows, kTcTK);  // Q (K-major) x K tile (K-major)
+      const bool leader = elect_one();
+      const uint64_t dq = umma_desc_sw128(sQ, 16, 1024), dk = umma_desc_sw128(sKV, 16, 1024);
+      bool ok = true;
+      int g = 0, lu = 0;
+      Segment s;
+      for (int n = 0; ok && take(n, s); ++n) {
+        const int tiles = __shfl_sync(0xffffffffu, s.t1 - s.t0, 0);
+        if (tiles <= 0) continue;
+        ok = wait_all(&q_full[lu & 1], lu >> 1);
+        const uint64_t q = dq + (uint64_t)((lu & 1) * (kTcQBytes >> 4));  // descriptors count 16 bytes
+        for (int j = 0; j < tiles && ok; ++j, ++g) {
+          const int st = g % kTcStages, sb = g % 3;
+          // S over the P of three tiles before, whose P V has completed
+          ok = wait_all(&kv_full[st], g / kTcStages);
+          if (ok && g >= 3) ok = wait_all(&pv_done[(g - 3) % kTcStages], (g - 3) / kTcStages);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t k = dk + (uint64_t)(st * (2 * kTcTileBytes >> 4));
+          if (leader) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)  // head dim in steps of 16
+              mma_f16(tmem + sb * 64, q + ks * 2, k + ks * 2, kIdS, ks > 0 ? 1u : 0u);
+            tc_commit(&s_full[sb]);
+          }
+          __syncwarp();
+        }
+        ++lu;
+      }
+      drain(0, g > 0);
+    } else if (warp == 2) {
+      // ------------------------------------------------------------ O += P V
+      constexpr uint32_t kIdO = umma_idesc(1, 1, 1, 0, 1, kTcRows, kHD);  // P (TMEM) x V tile (MN-major)
+      const bool leader = elect_one();
+      const uint64_t dv = umma_desc_sw128(sKV + kTcTileBytes, kTcTileBytes, 1024);
+      bool ok = true;
+      int g = 0, lu = 0;
+      Segment s;
+      for (int n = 0; ok && take(n, s); ++n) {
+        const int tiles = __shfl_sync(0xffffffffu, s.t1 - s.t0, 0);
+        if (tiles <= 0) continue;
+        const int last_keys = __shfl_sync(0xffffffffu, s.keys - (s.t1 - 1) * kTcTK, 0);  // may be more than a tile
+        for (int j = 0; j < tiles; ++j, ++g) {
+          const int st = g % kTcStages, sb = g % 3;
+          ok = wait_all(&kv_full[st], g / kTcStages);
+          if (ok && j + 1 == tiles && last_keys < kTcTK) {
+            // values behind the last key hold whatever the page or ring held: a
+            // NaN there would survive its zero weight
+            const uint32_t sv = sKV + st * 2 * kTcTileBytes + kTcTileBytes;
+            for (int i = last_keys * 8 + lane; i < kTcTK * 8; i += 32)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + i * 16), "r"(0) : "memory");
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          // P is written (and O rescaled where its base moved); a unit's first tile
+          // starts O afresh, after the softmax has read the previous unit's
+          ok = ok && wait_all(&p_full[sb], g / 3) && (j > 0 || lu == 0 || wait_all(&o_empty, lu - 1));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t d = dv + (uint64_t)(st * (2 * kTcTileBytes >> 4));
+          if (leader) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)  // keys in steps of 16: 8 columns of P
+              mma_f16_ts(tmem + 192, tmem + sb * 64 + ks * 8, d + ks * 128, kIdO, (ks > 0 || j > 0) ? 1u : 0u);
+            tc_commit(&pv_done[st]);
+          }
+          __syncwarp();
+        }
+        ++lu;
+      }
+      drain(1, g > 0);
+    }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcSoftmaxRegs));
     // ------------------------------------------------------------ softmax: one query row per thread
     const int q4 = warp & 3;  // TMEM lane quarter
     const int r = q4 * 32 + lane;
@@ -1297,92 +1308,87 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
     constexpr float kRebase = 8.0f;  // log2 of the largest P kept without rescaling
     const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
     bool ok = true;
-    int g = 0, lu = 0;
+    int g = 0, lu = 0;         // tiles, units with tiles
+    uint32_t sb = 0, sph = 0;  // S buffer of tile g and its phase
     Segment s;
     for (int n = 0; ok && take(n, s); ++n) {
       const bool valid = r < s.rows;
       const bool warp_valid = q4 * 32 < s.rows;  // uniform: some row of this warp is the unit's
-      const int tok = row_token(a, r);
-      const int seen = min(s.first_pos + tok, s.keys - 1);  // the last key this row sees
-      float m = -INFINITY, l = 0.0f;                        // m: the base of P (log2 units)
-      for (int j = s.t0; j < s.t1; ++j, ++g) {
-        const int sb = g % 3;
-        ok = wait_all(&s_full[sb], g / 3);
+      const int seen = min(s.first_pos + row_token(a, r), s.keys - 1);  // the last key this row sees
+      // key tiles that start up to here are seen whole by every row of the warp
+      const int clear = __reduce_min_sync(0xffffffffu, valid ? seen : 0x7fffffff) - (kTcTK - 1);
+      // m: the base of P (log2 units); rows past the unit's hold leftovers and have no say in moving bases
+      float m = valid ? -INFINITY : INFINITY, l = 0.0f;
+      const int g_end = g + max(s.t1 - s.t0, 0);
+      if (!warp_valid)
+        for (; ok && g < g_end; ++g) {
+          ok = wait_all(&s_full[sb], sph);
+          if (lane == 0) mbar_arrive(&p_full[sb]);
+          if (++sb == 3) sb = 0, sph ^= 1;
+        }
+      for (int k0 = s.t0 * kTcTK; ok && g < g_end; k0 += kTcTK, ++g) {
+        ok = wait_all(&s_full[sb], sph);
         if (!ok) break;
         tc_fence_after();
-        const int k0 = j * kTcTK;
-        if (s.keys - k0 < kTcTK) {
-          // values behind the last key hold whatever the page or ring held: a
-          // NaN there would survive its zero weight
-          const int st = g % kTcStages;
-          ok = wait_all(&kv_full[st], g / kTcStages);  // (landed: S_g has read K)
-          if (!ok) break;
-          const uint32_t sv = sKV + st * 2 * kTcTileBytes + kTcTileBytes;
-          for (int i = (s.keys - k0) * 8 + (int)threadIdx.x - 64; i < kTcTK * 8; i += 128)
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + i * 16), "r"(0) : "memory");
-          fence_proxy_async_smem();
+        float2 p[32];  // raw scores (the scale is positive: their maximum scales to the scaled ones')
+        tmem_ld_32x32b_x32(tmem + sb * 64 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
+        tmem_ld_32x32b_x32(tmem + sb * 64 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&p[16]));
+        tmem_ld_wait();
+        if (k0 > clear) {  // some row does not see the whole tile
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            if (k0 + 2 * c > seen) p[c].x = -INFINITY;
+            if (k0 + 2 * c + 1 > seen) p[c].y = -INFINITY;
+          }
         }
-        if (warp_valid) {
-          float2 p[32];  // raw scores (the scale is positive: their maximum scales to the scaled ones')
-          tmem_ld_32x32b_x32(tmem + sb * 64 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
-          tmem_ld_32x32b_x32(tmem + sb * 64 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&p[16]));
-          tmem_ld_wait();
-          if (!__all_sync(0xffffffffu, !valid || k0 + kTcTK - 1 <= seen)) {  // some row does not see the whole tile
+        float mx[4];
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              if (k0 + 2 * c > seen) p[c].x = -INFINITY;
-              if (k0 + 2 * c + 1 > seen) p[c].y = -INFINITY;
+        for (int i = 0; i < 4; ++i) mx[i] = fmaxf(p[i].x, p[i].y);
+#pragma unroll
+        for (int c = 4; c < 32; ++c) mx[c & 3] = fmaxf(fmaxf(mx[c & 3], p[c].x), p[c].y);
+        const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+        // a unit's first finite maximum moves the base from -inf
+        if (__any_sync(0xffffffffu, mn > m + kRebase)) {
+          const float to = fmaxf(m, mn), alpha = m == -INFINITY ? 0.0f : ex2_approx(m - to);
+          l *= alpha;
+          m = to;
+          if (k0 > s.t0 * kTcTK) {  // O, with P_{g-1} V in it, to the new bases before P_g V adds to it
+            ok = wait_all(&pv_done[(g - 1) % kTcStages], (g - 1) / kTcStages);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              uint32_t ov[16];
+              tmem_ld_x16(tmem + 192 + h * 16 + lane_off, ov);
+              tmem_ld_wait();
+#pragma unroll
+              for (int c = 0; c < 16; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+              tmem_st_x16(tmem + 192 + h * 16 + lane_off, ov);
             }
           }
-          float mx[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(p[i].x, p[i].y);
-#pragma unroll
-          for (int c = 4; c < 32; ++c) mx[c & 3] = fmaxf(fmaxf(mx[c & 3], p[c].x), p[c].y);
-          const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2);
-          const bool first = j == s.t0;
-          // rows past the unit's hold leftovers: they have no say
-          const bool rebase = first || __any_sync(0xffffffffu, valid && mn > m + kRebase);
-          if (rebase) {
-            const float alpha = m == -INFINITY ? 0.0f : ex2_approx(m - mn);
-            l *= alpha;
-            m = mn;
-            if (!first) {  // O, with P_{g-1} V in it, to the new bases before P_g V adds to it
-              ok = wait_all(&o_full[(g + 2) % 3], (g - 1) / 3);
-              if (!ok) break;
-              tc_fence_after();
-#pragma unroll
-              for (int h = 0; h < 4; ++h) {
-                uint32_t ov[16];
-                tmem_ld_x16(tmem + 192 + h * 16 + lane_off, ov);
-                tmem_ld_wait();
-#pragma unroll
-                for (int c = 0; c < 16; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
-                tmem_st_x16(tmem + 192 + h * 16 + lane_off, ov);
-              }
-            }
-          }
-          const float base = m == -INFINITY ? 0.0f : m;
-          const float2 base2 = make_float2(-base, -base);
-          float2 sum[2] = {make_float2(l, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {  // P = exp2(S * scale - base)
-              float2 e = fma2(p[16 * h + c], scale2, base2);
-              e.x = ex2_approx(e.x);
-              e.y = ex2_approx(e.y);
-              sum[c & 1] = add2(sum[c & 1], e);
-              pk[c] = pack2(e.x, e.y);
-            }
-            tmem_st_x16(tmem + sb * 64 + h * 16 + lane_off, pk);
-          }
-          l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          tmem_st_wait();
         }
+        const float base = m == -INFINITY ? 0.0f : m;
+        const float2 base2 = make_float2(-base, -base);
+        float2 sum[2] = {make_float2(l, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {  // P = exp2(S * scale - base)
+            float2 e = fma2(p[16 * h + c], scale2, base2);
+            e.x = ex2_approx(e.x);
+            e.y = ex2_approx(e.y);
+            sum[c & 1] = add2(sum[c & 1], e);
+            pk[c] = pack2(e.x, e.y);
+          }
+          tmem_st_x16(tmem + sb * 64 + h * 16 + lane_off, pk);
+        }
+        l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&p_full[sb]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[sb]);
+        if (++sb == 3) sb = 0, sph ^= 1;
       }
       if (!ok) break;
       const bool whole = s.starts && s.ends;
@@ -1404,7 +1410,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
         continue;
       }
       // the unit's last P V, then O: read and released for the next unit
-      ok = wait_all(&o_full[(g - 1) % 3], (g - 1) / 3);
+      ok = wait_all(&pv_done[(g - 1) % kTcStages], (g - 1) / kTcStages);
       if (!ok) break;
       tc_fence_after();
       uint32_t ov[64];
@@ -1947,9 +1953,9 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
   const int rows = few ? (eight ? 8 : kFewRows) : kTcRows, tile = few ? kTK : kTcTK;
   a.tpt = rows / n_rep;
   a.rep_magic = (65536u + (uint32_t)n_rep - 1u) / (uint32_t)n_rep;
-  a.over = few ? 16 : 224;
+  a.over = few ? 16 : 192;
   a.snap = few ? 32 : 128;
-  a.min_share = few ? 32 : 320;
+  a.min_share = few ? 32 : 288;
   int box = 8;  // rows of one load: the largest power of two that divides a page, at most a tile
   while (box < tile && page_size % (2 * box) == 0) box *= 2;
   a.box_rows = box;
