@@ -1044,6 +1044,15 @@ __device__ __forceinline__ float2 add2(float2 x, float2 y) {
   return d;
 }
 
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n"
+      " mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return d;
+}
+
 template <typename I>
 __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __grid_constant__ TcMaps maps,
                                                                       const AttnArgs a) {
@@ -1397,75 +1406,88 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
         part[kTcRows * kHD + r] = m;
         part[kTcRows * kHD + kTcRows + r] = l;
       }
-      auto out_row = [&](int row) -> bf16* {
-        const int tk = row_token(a, row);
-        return a.out + (int64_t)(s.token + tk) * a.ld_out + (s.kvh * a.n_rep + row - tk * a.n_rep) * kHD;
-      };
       if (s.t0 >= s.t1) {  // no key in this part: zeros
         if (valid)
           for (int c = 0; c < 16; ++c) {
-            if (!whole) *reinterpret_cast<float4*>(part + r * kHD + c * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
-            else *reinterpret_cast<uint2*>(out_row(r) + c * 4) = make_uint2(0u, 0u);
+            const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (!whole) *reinterpret_cast<float4*>(part + r * kHD + c * 4) = zero;
+            else store_out4(a, s.token, s.kvh, r, c * 4, zero);
           }
         continue;
       }
+      // Rows pass through the unit's own Q buffer (its scores are done), so
+      // that a store instruction writes whole 128-byte rows: a row per thread
+      // took 1.6 us a unit.  16-byte chunk c of row i at c ^ (i & 7).  What does
+      // not need O comes before the wait for it.
+      const uint32_t rows_base = sQ + (lu & 1) * kTcQBytes + q4 * 32 * 128;
+      const uint32_t put_at = rows_base + lane * 128 + ((lane & 7) << 4);
+      auto put = [&](int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(put_at ^ (c << 4)), "r"(x), "r"(y), "r"(z), "r"(w)
+                     : "memory");
+      };
+      // this lane stores chunk col of rows row0 + 4 k
+      const int col = lane & 7, row0 = q4 * 32 + (lane >> 3);
+      const uint32_t get_at = rows_base + (lane >> 3) * 128 + ((col ^ (lane >> 3)) << 4);
+      auto get = [&](int k) -> uint4 {
+        uint4 v;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"((get_at ^ ((k & 1) << 6)) + k * 512)
+                     : "memory");
+        return v;
+      };
+      bf16* to[8];
+      if (whole) {
+        bf16* first = a.out + (int64_t)s.token * a.ld_out + (s.kvh * a.n_rep + row0) * kHD + col * 8;
+        const int64_t skip = a.ld_out - a.n_rep * kHD;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) to[k] = first + 4 * k * kHD + row_token(a, row0 + 4 * k) * skip;
+      }
+      const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);  // no key: zeros
       // the unit's last P V, then O: read and released for the next unit
       ok = wait_all(&pv_done[(g - 1) % kTcStages], (g - 1) / kTcStages);
       if (!ok) break;
       tc_fence_after();
-      uint32_t ov[64];
+      float2 ov[32];
       if (warp_valid) {
         tmem_ld_32x32b_x32(tmem + 192 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[0]));
-        tmem_ld_32x32b_x32(tmem + 192 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[32]));
+        tmem_ld_32x32b_x32(tmem + 192 + 32 + lane_off, *reinterpret_cast<uint32_t(*)[32]>(&ov[16]));
         tmem_ld_wait();
       }
       tc_fence_before();
       mbar_arrive(&o_empty);
       if (warp_valid) {
-        // Rows pass through the unit's own Q buffer (its scores are done), so
-        // that a store instruction writes whole 128-byte rows: a row per
-        // thread took 1.6 us a unit.  16-byte chunk c of row i at c ^ (i & 7).
-        const uint32_t rows_base = sQ + (lu & 1) * kTcQBytes + q4 * 32 * 128;
-        const uint32_t mine = rows_base + lane * 128;
-        auto put = [&](int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((c ^ (lane & 7)) << 4)), "r"(x), "r"(y),
-                       "r"(z), "r"(w)
-                       : "memory");
-        };
-        auto get = [&](int row) -> uint4 {
-          uint4 v;
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                       : "r"(rows_base + row * 128 + (((lane & 7) ^ (row & 7)) << 4))
-                       : "memory");
-          return v;
-        };
         if (whole) {
-          const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+          const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) ov[c] = mul2(ov[c], inv2);
 #pragma unroll
           for (int c = 0; c < 8; ++c)
-            put(c, pack2(__uint_as_float(ov[8 * c + 0]) * inv, __uint_as_float(ov[8 * c + 1]) * inv),
-                pack2(__uint_as_float(ov[8 * c + 2]) * inv, __uint_as_float(ov[8 * c + 3]) * inv),
-                pack2(__uint_as_float(ov[8 * c + 4]) * inv, __uint_as_float(ov[8 * c + 5]) * inv),
-                pack2(__uint_as_float(ov[8 * c + 6]) * inv, __uint_as_float(ov[8 * c + 7]) * inv));
+            put(c, pack2(ov[4 * c].x, ov[4 * c].y), pack2(ov[4 * c + 1].x, ov[4 * c + 1].y),
+                pack2(ov[4 * c + 2].x, ov[4 * c + 2].y), pack2(ov[4 * c + 3].x, ov[4 * c + 3].y));
           __syncwarp();
+          uint4 v[8];
 #pragma unroll
-          for (int i0 = 0; i0 < 32; i0 += 4) {
-            const int i = i0 + (lane >> 3), row = q4 * 32 + i;
-            if (row < s.rows) *reinterpret_cast<uint4*>(out_row(row) + (lane & 7) * 8) = get(i);
-          }
+          for (int k = 0; k < 8; ++k) v[k] = get(k);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (row0 + 4 * k < s.rows) *reinterpret_cast<uint4*>(to[k]) = v[k];
         } else {
+          float* first = part + row0 * kHD + col * 4;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              put(c, ov[32 * h + 4 * c], ov[32 * h + 4 * c + 1], ov[32 * h + 4 * c + 2], ov[32 * h + 4 * c + 3]);
-            __syncwarp();
-#pragma unroll
-            for (int i0 = 0; i0 < 32; i0 += 4) {
-              const int i = i0 + (lane >> 3), row = q4 * 32 + i;
-              if (row < s.rows) *reinterpret_cast<uint4*>(part + row * kHD + h * 32 + (lane & 7) * 4) = get(i);
+            for (int c = 0; c < 8; ++c) {
+              const float2 x = ov[16 * h + 2 * c], y = ov[16 * h + 2 * c + 1];
+              put(c, __float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
             }
+            __syncwarp();
+            uint4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = get(k);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (row0 + 4 * k < s.rows) *reinterpret_cast<uint4*>(first + 4 * k * kHD + h * 32) = v[k];
             __syncwarp();
           }
         }
