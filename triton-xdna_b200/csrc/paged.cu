@@ -98,13 +98,16 @@ struct RopeArgs {
 // so up to three of a lane's slots are requested before the search for the
 // token's sequence, which all lanes do together (32 starts a step).  Products
 // and sums are rounded separately in fp32, as examples/qwen2_5/kernels/rope.py:
-// 63-66 and the contiguous kernel do: the same bits.  Three slots ahead in 80
-// registers measured best (36500 tokens of 14 + 2 x 2 heads: 39.5 us, 4.7 TB/s;
-// four in 94 registers 48.2, two in 64 41.0, loads after the search 47.1).
-__global__ void __launch_bounds__(256, 3) paged_rope_kv_kernel(const RopeArgs a, int* __restrict__ bad) {
+// 63-66 and the contiguous kernel do: the same bits.  36500 tokens of 14 + 2 x 2
+// heads take 33.8 us, 5.5 TB/s (0.85 of the measured copy).  Measured: four
+// slots ahead in 94 registers 48.2 us, two in 64 41.0, loads after the search
+// 47.1, three in 80 39.6; stores marked as streaming 35.8; then CTAs of two
+// warps instead of eight 33.8 (four 34.2, 24 46.0): a CTA's place is taken again
+// as soon as its own few tokens are done.
+__global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a, int* __restrict__ bad) {
   pdl_wait();
   pdl_trigger();
-  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int t = blockIdx.x * 2 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (t >= a.T) return;
   const int half = a.D / 2, groups = half / 8;  // groups of 8 dims of a half; divides 32
@@ -185,8 +188,8 @@ __global__ void __launch_bounds__(256, 3) paged_rope_kv_kernel(const RopeArgs a,
         const Pages& pg = is_k ? a.k : a.v;
         dst = pg.p + id * pg.page + (slot - a.H - (is_k ? 0 : a.KVH)) * pg.head + row * pg.row;
       }
-      st16(dst + c, u[i]);
-      st16(dst + half + c, w[i]);
+      st16_stream(dst + c, u[i]);
+      st16_stream(dst + half + c, w[i]);
     }
     first += kAhead * step;
     if (first >= slots) break;
@@ -1880,7 +1883,7 @@ extern "C" int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t, const 
   int *bad = nullptr, *status = nullptr;
   rc = status_words(&bad, &status, what, err, errlen);
   if (rc) return rc;
-  launch_k<false>(paged_rope_kv_kernel, (unsigned)((tokens + 7) / 8), 256, 0, (cudaStream_t)stream, a, bad);
+  launch_k<false>(paged_rope_kv_kernel, (unsigned)((tokens + 1) / 2), 64, 0, (cudaStream_t)stream, a, bad);
   return check_launch(what, err, errlen);
 }
 
