@@ -42,7 +42,8 @@ constexpr uint64_t kWaitLimit = 2000000000ull;  // 2 s per wait: far above any l
 // run in any order.  The pairs travel as kernel parameters: no upload, no
 // device buffer whose lifetime a captured graph would have to share.  A thread
 // moves four 16-byte vectors 256 apart (four loads in flight), a CTA 16 KB of
-// the outer slab's n * vpp vectors.
+// the outer slab's n * vpp vectors.  2500 pages of 4 KB in 48 slabs take 164 us,
+// 0.91 of the measured copy rate; 4 pages 2.2 us, the launch.
 constexpr int kCopyPairs = 500;  // 4000 bytes of parameters; larger lists take several launches
 template <int N>
 struct CopyPairs {
@@ -484,7 +485,7 @@ __device__ __forceinline__ bool segment(const AttnArgs& a, Walk<I>& w, Segment& 
 // place they took 32, and those were the longest part of a short call (0.7 of
 // the 1.4 us of two tiles).  A unit inside one warp's piece goes straight to
 // the output; parts of one that spans warps of the CTA meet in shared memory
-// after the CTA's only barrier, and what spans CTAs goes on to the joining
+// after the last barrier, and what spans CTAs goes on to the joining
 // kernel.  Calls of few keys are bound by latency and by fetching instructions
 // (each line is cold in a new launch): every long piece of code is there once.
 constexpr int kHD = 64;
@@ -493,9 +494,9 @@ constexpr int kTileBytes = kTK * kHD * 2;  // one K or V tile
 constexpr int kFewRows = 16;               // rows of a partial in the workspace
 constexpr int kQueue = 4;                  // segments a warp's requests may be ahead of its computation
 constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared memory: conflict-free stores
-// 12 warps x 2 buffers and 8 x 3 of the 8-row kernel measured no faster
-// (64 sequences of 576 keys: 12.1 and 11.0 us, 8 x 2 11.0; 160 long ones 87.4
-// and 90.2, 8 x 2 86.1).
+// Warps x buffers of the 8-row kernel, 64 sequences of 576 keys / 160 long ones:
+// 8 x 2 11.0 / 86.1 us, 8 x 3 11.0 / 90.2, 12 x 2 12.1 / 87.4, 16 x 1 13.1 / 86.5,
+// 12 x 1 12.3 / 85.8, 8 x 1 11.1 / 93.8, 6 x 3 11.3 / 91.7, 4 x 4 12.6 / 116.
 template <int ROWS>
 struct FewCfg {
   static constexpr int kWarps = 8, kBufs = 2;
