@@ -985,7 +985,8 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
 // 59.7), the next tile's scores loaded during the exponentials (713), key tiles
 // of 128 with one score buffer (760 where 64 took 730), four CTAs per SM with
 // one score buffer (757), three (862), longer pieces for an SM's first CTA
-// (prompts 56.2, but the chunk 676).
+// (prompts 56.2 against 58.4, but the chunk 676), one in eight exponentials as a
+// polynomial on the FMA pipe (652, but prompts 57.4 against 56.3).
 constexpr int kTcRows = 128;
 constexpr int kTcTK = 64;
 constexpr int kTcStages = 4;
