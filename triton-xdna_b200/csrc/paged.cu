@@ -22,6 +22,7 @@
 // page id outside the pool reads as zeros (attention) or is skipped (writes)
 // and sets the flag that xb_page_status reports.
 #include "common.cuh"
+#include "paged_walk.cuh"
 #include "tc.cuh"
 
 namespace xb {
@@ -219,14 +220,13 @@ __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a,
 // are a closed form, so a CTA finds its piece with one scan over the sequences
 // and a binary search inside one, from lengths that only the device knows.
 
-struct AttnArgs {
+struct AttnArgs : Line {
   const bf16* q;
   bf16* out;
-  const int32_t *table, *q_start, *kv_len;
+  const int32_t* table;
   float* ws;  // [2 G] partials, then G Meta
   int64_t ld_q, ld_out, ld_table;
-  int T, B, KVH, n_rep, tpt, page_size, max_pages, n_pages, box_rows;
-  int min_share, over, snap;
+  int n_pages, box_rows;
   uint32_t rep_magic;  // ceil(2^16 / n_rep)
   float scale_log2;
   int *bad, *status;
@@ -239,90 +239,6 @@ struct Meta {
 
 // r / n_rep for a row r < 128: the product is above the quotient by less than r / 2^16 < 1 / n_rep.
 __device__ __forceinline__ int row_token(const AttnArgs& a, int r) { return (int)(((uint32_t)r * a.rep_magic) >> 16); }
-
-// I: int where the host has seen that the line's weight stays below 2^30
-// whatever the device arrays hold, else int64_t (the walks are a good part of a short
-// call's instructions).
-template <typename I>
-struct Seq {
-  int s0, n;      // first packed token, number of new tokens
-  int len, base;  // keys held, keys before the new tokens (negative: the first tokens see none)
-  int nt;         // query tiles
-  I perh;         // weight of one KV head
-};
-
-template <typename I>
-__device__ __forceinline__ I cum_keys(const AttnArgs& a, const Seq<I>& q, int j) {  // weight of tiles 0 .. j - 1
-  const I b = max(q.base, 0) + a.over;
-  if (sizeof(I) == 4)  // the product of two tile numbers may pass 2^31 before it is halved
-    return j * b + (j < q.nt ? (I)((int64_t)a.tpt * j * (j + 1) / 2) : (I)((int64_t)a.tpt * q.nt * (q.nt - 1) / 2) + q.n);
-  return j * b + (j < q.nt ? (I)a.tpt * j * (j + 1) / 2 : (I)a.tpt * q.nt * (q.nt - 1) / 2 + q.n);
-}
-
-template <typename I>
-__device__ __forceinline__ Seq<I> make_seq(const AttnArgs& a, int s0, int n, int len) {
-  Seq<I> q;
-  q.s0 = s0;
-  q.n = n;
-  q.len = len;
-  q.base = len - n;
-  q.nt = n <= a.tpt ? (n > 0) : (n + a.tpt - 1) / a.tpt;
-  q.perh = q.nt == 0 ? (I)0 : q.nt == 1 ? (I)(max(q.base, 0) + a.over + n) : cum_keys(a, q, q.nt);
-  return q;
-}
-
-template <typename I>
-__device__ __forceinline__ Seq<I> load_seq(const AttnArgs& a, int b) {
-  const int s0 = min(max(__ldg(a.q_start + b), 0), a.T);
-  const int s1 = min(max(__ldg(a.q_start + b + 1), s0), a.T);
-  return make_seq<I>(a, s0, s1 - s0, min(max(__ldg(a.kv_len + b), 0), a.max_pages * a.page_size));
-}
-
-// Where a piece starts: a sequence, its first point on the line and its numbers.
-template <typename I>
-struct Found {
-  I start;
-  int b, s0, n, len;  // b < 0: the piece is empty
-};
-
-// A walk over one piece [lo, hi) of the line.
-template <typename I>
-struct Walk {
-  I lo, hi, share;
-  int snap;  // cuts this close to a unit's end or first key move there
-  I u0;    // where the current unit starts
-  I ulen;  // its weight
-  int b, kvh, j;
-  Seq<I> q;
-};
-
-// The part of one unit that belongs to a piece.
-struct Segment {
-  int b, kvh;
-  int token, rows;   // first packed token and rows of the query tile
-  int first_pos;     // position of the tile's first token (may be negative)
-  int keys;          // keys the unit's last token sees; 0 when none of its tokens sees any
-  int t0, t1;        // key tiles of this part
-  int starts, ends;  // the unit starts / ends in this piece
-  int last;          // where it starts and goes on: the piece in which it ends
-};
-
-// Share of `pieces` equal pieces of the line: at least total / pieces (the
-// product is rounded up by more than the float error; every thread of the grid
-// computes the same value).
-template <typename I>
-__device__ __forceinline__ I share_of(const AttnArgs& a, I total, int pieces) {
-  const I share = (I)((float)total * __frcp_rn((float)pieces) * 1.000001f) + 1;
-  return share < a.min_share ? a.min_share : share;
-}
-
-// How far a cut moves to a unit's boundary: a part of one costs a warp or CTA
-// as much as `snap` keys (starting the second unit, merging the parts), but no
-// piece may grow by more than two thirds, nor lie between two moved cuts.
-template <typename I>
-__device__ __forceinline__ int cut_snap(const AttnArgs& a, I share) {
-  return (int)min((I)a.snap, (share - a.over) / 3);
-}
 
 // Weight of the whole line and, for the piece that starts at `first` + i times
 // the share (i < N), the sequence that holds its start.  Every thread of the
@@ -380,95 +296,6 @@ __device__ __forceinline__ I find_pieces(const AttnArgs& a, int pieces, int firs
   return share;
 }
 
-template <typename I>
-__device__ __forceinline__ I unit_weight(const AttnArgs& a, const Walk<I>& w) {
-  return a.over + max(w.q.base, 0) + min(a.tpt * (w.j + 1), w.q.n);
-}
-
-// Places a walk at piece `piece`'s start.
-template <typename I>
-__device__ __forceinline__ void place(const AttnArgs& a, Walk<I>& w, int piece, I share, I total, const Found<I>& f) {
-  w.share = share;
-  w.snap = cut_snap(a, share);
-  w.lo = piece * share;
-  w.hi = total - w.lo < share ? total : w.lo + share;
-  w.b = f.b;
-  w.q = make_seq<I>(a, f.s0, f.n, f.len);
-  I in = w.lo - f.start;
-  w.kvh = 0;
-  if (in >= w.q.perh) {
-    w.kvh = (int)(in / w.q.perh);
-    in -= w.kvh * w.q.perh;
-  }
-  w.j = 0;
-  w.u0 = f.start + w.kvh * w.q.perh;
-  if (w.q.nt > 1) {
-    int lo = 0, hi = w.q.nt - 1;  // the last tile j with cum(j) <= in
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (cum_keys(a, w.q, mid) <= in) lo = mid;
-      else hi = mid - 1;
-    }
-    w.j = lo;
-    w.u0 += cum_keys(a, w.q, lo);
-  }
-  w.ulen = unit_weight(a, w);
-}
-
-// Steps to the next unit; false behind the piece's last one.
-template <typename I>
-__device__ __forceinline__ bool next_unit(const AttnArgs& a, Walk<I>& w) {
-  w.u0 += w.ulen;
-  if (w.u0 >= w.hi) return false;
-  if (++w.j >= w.q.nt) {
-    w.j = 0;
-    if (++w.kvh >= a.KVH) {
-      w.kvh = 0;
-      do {
-        if (++w.b >= a.B) return false;
-        w.q = load_seq<I>(a, w.b);
-      } while (w.q.n == 0);
-    }
-  }
-  w.ulen = unit_weight(a, w);
-  return true;
-}
-
-// The part of the current unit that belongs to this piece, stepping over a
-// unit whose cut was moved away; false when nothing is left.
-template <int TK, typename I>
-__device__ __forceinline__ bool segment(const AttnArgs& a, Walk<I>& w, Segment& g) {
-  for (;;) {
-    const I cut0 = w.lo - w.u0, cut1 = w.hi - w.u0;  // the piece's ends inside the unit
-    g.starts = cut0 < a.over + w.snap;
-    if (!g.starts && w.ulen - cut0 < w.snap) {  // only at the piece's start: the unit ended in the piece before
-      if (!next_unit(a, w)) return false;
-      continue;
-    }
-    if (cut1 < a.over + w.snap && cut1 < w.ulen) return false;  // the unit starts in the next piece
-    g.ends = w.ulen - cut1 < w.snap;
-    const int done = w.j * a.tpt;
-    const int tokens = min(a.tpt, w.q.n - done);
-    g.b = w.b;
-    g.kvh = w.kvh;
-    g.token = w.q.s0 + done;
-    g.rows = tokens * a.n_rep;
-    g.first_pos = w.q.base + done;
-    g.keys = max(g.first_pos + tokens, 0);
-    const int nk = (int)(((unsigned)g.keys + TK - 1) / TK);
-    g.t0 = g.starts ? 0 : min((int)((unsigned)(cut0 - a.over) / TK), nk);  // cuts fall on tile boundaries
-    g.t1 = g.ends ? nk : min((int)((unsigned)(cut1 - a.over) / TK), nk);
-    if (g.starts && !g.ends) {
-      // the piece that holds the unit's last key, or the one before it if that cut was moved to the unit's end
-      const I end = w.u0 + w.ulen;
-      I last = (end - 1) / w.share;
-      if (last * w.share > w.u0 && end - last * w.share < w.snap) --last;
-      g.last = (int)last;
-    }
-    return true;
-  }
-}
-
 // ----------------------------------------------------------------------------- attention: few rows (mma.sync)
 //
 // For batches whose sequences bring few tokens each (decoding, verification of
@@ -489,9 +316,8 @@ __device__ __forceinline__ bool segment(const AttnArgs& a, Walk<I>& w, Segment& 
 // kernel.  Calls of few keys are bound by latency and by fetching instructions
 // (each line is cold in a new launch): every long piece of code is there once.
 constexpr int kHD = 64;
-constexpr int kTK = 32;
+constexpr int kTK = kFewTK;
 constexpr int kTileBytes = kTK * kHD * 2;  // one K or V tile
-constexpr int kFewRows = 16;               // rows of a partial in the workspace
 constexpr int kQueue = 4;                  // segments a warp's requests may be ahead of its computation
 constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared memory: conflict-free stores
 // Warps x buffers of the 8-row kernel, 64 sequences of 576 keys / 160 long ones:
@@ -499,7 +325,7 @@ constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared m
 // 12 x 1 12.3 / 85.8, 8 x 1 11.1 / 93.8, 6 x 3 11.3 / 91.7, 4 x 4 12.6 / 116.
 template <int ROWS>
 struct FewCfg {
-  static constexpr int kWarps = 8, kBufs = 2;
+  static constexpr int kWarps = kFewWarps, kBufs = 2;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kRing = kBufs * 2 * kTileBytes;  // of one warp
   static constexpr int kHead = ROWS * kPartLd * 4;      // a warp's kind 0 partial; kind 1 goes into its own ring
@@ -988,7 +814,6 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
 // (prompts 56.2 against 58.4, but the chunk 676), one in eight exponentials as a
 // polynomial on the FMA pipe (652, but prompts 57.4 against 56.3).
 constexpr int kTcRows = 128;
-constexpr int kTcTK = 64;
 constexpr int kTcStages = 4;
 constexpr int kTcSegs = 4;  // segments published ahead
 constexpr int kTcQBytes = kTcRows * kHD * 2;
@@ -1977,12 +1802,9 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
   if (rc) return rc;
   const bool few = few_rows(tokens, batch, n_rep);
   const bool eight = few && n_rep <= 8 && tokens * n_rep <= 8 * batch;  // the same rule for half a tile
-  const int rows = few ? (eight ? 8 : kFewRows) : kTcRows, tile = few ? kTK : kTcTK;
-  a.tpt = rows / n_rep;
+  const int tile = few ? kTK : kTcTK;
+  line_kernel(a, few ? (eight ? 8 : kFewRows) : kTcRows);
   a.rep_magic = (65536u + (uint32_t)n_rep - 1u) / (uint32_t)n_rep;
-  a.over = few ? 16 : 192;
-  a.snap = few ? 32 : 128;
-  a.min_share = few ? 32 : 288;
   int box = 8;  // rows of one load: the largest power of two that divides a page, at most a tile
   while (box < tile && page_size % (2 * box) == 0) box *= 2;
   a.box_rows = box;
@@ -1998,18 +1820,12 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
   int sms = 148;
   xb::sm_count(&sms);
   const int ctas = few ? sms : 2 * sms;
-  // The line's weight whatever the device arrays hold: every sequence at most
-  // all tokens' query tiles per KV head, each of at most the table's positions
-  // (starts that ascend give far less).  Below 2^30 an int holds it, the
-  // pieces' rounding included.
-  const double most =
-      (double)batch * n_kv_head * ((double)tokens / a.tpt + 1) * ((double)kv->max_pages * page_size + a.over + a.tpt);
-  if (most >= 4e18) {
+  if (line_bound(a) >= 4e18) {
     set_err(err, errlen, "%s: %lld tokens of %lld sequences over %lld pages each are too many", what,
             (long long)tokens, (long long)batch, (long long)kv->max_pages);
     return XB_ERR_UNSUPPORTED;
   }
-  const bool wide = most + (double)a.min_share * ctas * 16 >= (double)(1 << 30);
+  const bool wide = line_is_wide(a, ctas);
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
   if (few) {
