@@ -1,0 +1,43 @@
+"""Paged attention where the sizes are unlike a usual step's.  Tolerance as in test_paged_gpu.py."""
+
+import pytest
+import torch
+
+from xb200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _pool(positions, KVH, page, seed):
+    """K and V of one sequence on the device: pages in reverse order, and the page table [1, columns]."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = positions // page
+    k, v = (torch.randn((n, KVH, page, 64), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    return k, v, torch.arange(n - 1, -1, -1, dtype=torch.int32, device="cuda").view(1, n)
+
+
+@pytest.mark.parametrize("n,H,KVH,kv_len", [(200_000, 14, 2, 1024), (200_000, 28, 4, 1024), (95_000, 128, 1, 8192),
+                                            (200_000, 14, 2, 0)])
+def test_many_more_new_tokens_than_keys(n, H, KVH, kv_len):
+    """Rows without a key are zeros and the last kv_len rows right; so is a short sequence beside it."""
+    page, few = 16, 3
+    k, v, table = _pool(max(kv_len, 1024) // page * page, KVH, page, n + H)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn((n + few, H, 64), generator=g, device="cuda").to(torch.bfloat16)
+    out = torch.full((n + few, H * 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    starts = torch.tensor([0, n, n + few], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([kv_len, 40], dtype=torch.int32, device="cuda")
+    ops.paged_attention(q, k, v, out, table.repeat(2, 1), starts, lens, 0.125)
+    out = out.view(-1, H, 64)
+    assert bool((out[:n - kv_len] == 0).all())
+    keys, values = (x[table[0].long()].transpose(1, 2).reshape(-1, KVH, 64).double() for x in (k, v))
+    for lo, hi, length in ((n - kv_len, n, kv_len), (n, n + few, 40)):
+        pos = length - (hi - lo) + torch.arange(hi - lo, device="cuda")
+        for h in range(0, H, 5):
+            s = q[lo:hi, h].double() @ keys[:length, h // (H // KVH)].T * 0.125
+            p = torch.softmax(s.masked_fill(torch.arange(length, device="cuda") > pos[:, None], -torch.inf), -1)
+            x = values[:length, h // (H // KVH)]
+            want = p @ x
+            bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * (p @ x.abs())
+            assert bool(((out[lo:hi, h].double() - want).abs() <= bound).all())
+    assert ops.device_status() == 0 and ops.page_status() == 0

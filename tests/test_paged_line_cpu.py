@@ -85,3 +85,31 @@ def test_the_host_takes_64_bits_for_a_long_line(line):
         assert wrong == "" and wide and 2 ** 31 < weight <= bound
     wrong, *_, wide = line(8, [1] * 64, [600] * 64, 14, 2, 16, 40)
     assert wrong == "" and not wide
+
+
+@pytest.mark.parametrize("rows,T,H,KVH,kv_len", [
+    (128, 200_000, 14, 2, 0), (128, 200_000, 14, 2, 1024), (128, 200_000, 28, 4, 1024), (128, 330_000, 12, 12, 1024),
+    (128, 70_000, 128, 1, 1024), (128, 95_000, 128, 1, 8192), (16, 330_000, 12, 12, 500)])
+def test_more_new_tokens_than_keys(line, rows, T, H, KVH, kv_len):
+    """The first tokens of a sequence see nothing; the line is no longer than the host's bound, which goes by the table."""
+    wrong, units, weight, bound, wide = line(rows, [T], [kv_len], H, KVH, 16, max(1, kv_len // 16))
+    assert wrong == "" and weight <= bound
+    assert units == KVH * -(-T // (rows // (H // KVH)))
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_short_sequences_weigh_the_keys_they_see(line, seed):
+    rnd = random.Random(1000 + seed)
+    H, KVH = LAYOUTS[seed % len(LAYOUTS)]
+    new, lens = _batch(rnd, True)
+    cols = -(-max(lens + [1]) // 8)
+    over = {8: 16, 16: 16, 128: 192}
+    for rows in (8, 16, 128):
+        tpt = rows // (H // KVH)
+        if tpt == 0:
+            continue
+        want = KVH * sum(over[rows] + max(0, n_kv - n + min(n, t + tpt))
+                         for n, n_kv in zip(new, lens) for t in range(0, n, tpt))
+        for bits in (0, 32, 64):
+            wrong, _, weight, bound, _ = line(rows, new, lens, H, KVH, 8, cols, bits)
+            assert wrong == "" and weight == want and weight <= bound

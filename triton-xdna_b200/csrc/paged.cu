@@ -1348,7 +1348,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
   const int ln = threadIdx.x % LANES, col = (threadIdx.x / LANES) % 16;
   const int r = blockIdx.y * kRows + threadIdx.x / (16 * LANES), d = col * 4;
   if (m.last < 0 || (int)blockIdx.y * kRows >= m.rows) return;
-  const int c0 = blockIdx.x, n = m.last - c0 + 1;
+  const int c0 = blockIdx.x, n = min(m.last, ctas - 1) - c0 + 1;
   float M = -INFINITY, l = 0.0f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = ln; i0 < n; i0 += 4 * LANES) {  // four partials in flight

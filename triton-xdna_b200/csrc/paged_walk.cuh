@@ -69,12 +69,17 @@ struct Seq {
   I perh;         // weight of one KV head
 };
 
+// Weight of tiles 0 .. j - 1: each the fixed cost and the keys its last token
+// sees, base + tpt (i + 1) for tile i, up to n for the last.  Where the sequence
+// holds fewer keys than it brings tokens (base < 0) the first tiles see none;
+// tokens without a key weigh nothing, however many they are.
 template <typename I>
-XB_LINE_FN I cum_keys(const Line& a, const Seq<I>& q, int j) {  // weight of tiles 0 .. j - 1
-  const I b = max(q.base, 0) + a.over;
-  if (sizeof(I) == 4)  // the product of two tile numbers may pass 2^31 before it is halved
-    return j * b + (j < q.nt ? (I)((int64_t)a.tpt * j * (j + 1) / 2) : (I)((int64_t)a.tpt * q.nt * (q.nt - 1) / 2) + q.n);
-  return j * b + (j < q.nt ? (I)a.tpt * j * (j + 1) / 2 : (I)a.tpt * q.nt * (q.nt - 1) / 2 + q.n);
+XB_LINE_FN I cum_keys(const Line& a, const Seq<I>& q, int j) {
+  const int z = q.base < 0 ? (int)((unsigned)-q.base / (unsigned)a.tpt) : 0;  // tiles without a key
+  if (j <= z) return (I)j * a.over;
+  const int m = j - z;  // the product of two tile numbers may pass 2^31 before it is halved
+  const I keys = (I)((int64_t)m * q.base + (int64_t)a.tpt * ((int64_t)m * (z + 1 + j) / 2));
+  return (I)j * a.over + keys - (j < q.nt ? 0 : a.tpt * q.nt - q.n);
 }
 
 template <typename I>
@@ -85,7 +90,7 @@ XB_LINE_FN Seq<I> make_seq(const Line& a, int s0, int n, int len) {
   q.len = len;
   q.base = len - n;
   q.nt = n <= a.tpt ? (n > 0) : (n + a.tpt - 1) / a.tpt;
-  q.perh = q.nt == 0 ? (I)0 : q.nt == 1 ? (I)(max(q.base, 0) + a.over + n) : cum_keys(a, q, q.nt);
+  q.perh = q.nt == 0 ? (I)0 : q.nt == 1 ? (I)(a.over + len) : cum_keys(a, q, q.nt);
   return q;
 }
 
@@ -144,7 +149,7 @@ XB_LINE_FN int cut_snap(const Line& a, I share) {
 
 template <typename I>
 XB_LINE_FN I unit_weight(const Line& a, const Walk<I>& w) {
-  return a.over + max(w.q.base, 0) + min(a.tpt * (w.j + 1), w.q.n);
+  return a.over + max(w.q.base + min(a.tpt * (w.j + 1), w.q.n), 0);
 }
 
 // Places a walk at piece `piece`'s start.
