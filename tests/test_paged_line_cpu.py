@@ -113,3 +113,13 @@ def test_short_sequences_weigh_the_keys_they_see(line, seed):
         for bits in (0, 32, 64):
             wrong, _, weight, bound, _ = line(rows, new, lens, H, KVH, 8, cols, bits)
             assert wrong == "" and weight == want and weight <= bound
+
+
+@pytest.mark.parametrize("rows", [8, 128])
+@pytest.mark.parametrize("new", [1, 20, 300])
+def test_positions_up_to_the_last_that_is_accepted(line, rows, new):
+    """Tables of just below 2^31 positions: a unit's weight passes 2^31."""
+    top = 2 ** 31 - 8
+    for lens in ([top], [top - 200, 5, top]):
+        wrong, units, weight, bound, wide = line(rows, [new] * len(lens), lens, 8, 4, 8, top // 8)
+        assert wrong == "" and wide and weight <= bound and units == 4 * len(lens) * -(-new // (rows // 2))

@@ -90,7 +90,7 @@ XB_LINE_FN Seq<I> make_seq(const Line& a, int s0, int n, int len) {
   q.len = len;
   q.base = len - n;
   q.nt = n <= a.tpt ? (n > 0) : (n + a.tpt - 1) / a.tpt;
-  q.perh = q.nt == 0 ? (I)0 : q.nt == 1 ? (I)(a.over + len) : cum_keys(a, q, q.nt);
+  q.perh = q.nt == 0 ? (I)0 : q.nt == 1 ? (I)a.over + len : cum_keys(a, q, q.nt);
   return q;
 }
 
@@ -149,7 +149,7 @@ XB_LINE_FN int cut_snap(const Line& a, I share) {
 
 template <typename I>
 XB_LINE_FN I unit_weight(const Line& a, const Walk<I>& w) {
-  return a.over + max(w.q.base + min(a.tpt * (w.j + 1), w.q.n), 0);
+  return (I)a.over + max(w.q.base + min(a.tpt * (w.j + 1), w.q.n), 0);
 }
 
 // Places a walk at piece `piece`'s start.
