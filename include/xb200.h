@@ -672,6 +672,7 @@ XB_API int xb_attention_workspace_size(int64_t batch, int64_t seq,
  * of 8; bases 16-byte aligned, strides and row pitches multiples of 8
  * elements.  xb_paged_kv (host memory, read during the call) describes them:
  * a step makes several calls with the same one.
+ * Limits: 2^20 sequences, 2^31 - 1 pages, 2^31 - 1 positions a sequence.
  *
  * No content of the device arrays makes a kernel leave its buffers.  A page
  * id outside [0, n_pages) that a sequence needs, and a new token whose position

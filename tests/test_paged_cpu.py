@@ -353,3 +353,12 @@ def test_fresh_slots_and_taken_workspaces():
         ops._workspaces[key] = "buffer"
         assert ops.take_workspace("cuda:0") == "buffer" and key not in ops._workspaces
         assert ops.take_workspace("cuda:0") is None
+
+
+def test_more_sequences_than_a_kernel_scans_are_refused():
+    """Every CTA scans all sequences with 32-bit counters, and a run of empty ones is passed while others wait."""
+    for call in (_attn, _rope):
+        for batch in ((1 << 20) + 1, 2 ** 31 - 2):
+            with pytest.raises(XbError) as e:
+                call(batch=batch)
+            assert e.value.code == _lib.XB_ERR_UNSUPPORTED and "2^20 sequences" in e.value.message, e.value.message

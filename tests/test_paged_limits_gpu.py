@@ -41,3 +41,25 @@ def test_many_more_new_tokens_than_keys(n, H, KVH, kv_len):
             bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * (p @ x.abs())
             assert bool(((out[lo:hi, h].double() - want).abs() <= bound).all())
     assert ops.device_status() == 0 and ops.page_status() == 0
+
+
+@pytest.mark.parametrize("H,new", [(8, 3), (32, 70)])
+def test_a_million_sequences_most_of_them_empty(H, new):
+    """The largest batch: tokens of the first, a middle and the last sequence (few rows, many rows)."""
+    B, page, kv_len = 1 << 20, 16, 1000
+    k, v, table = _pool(1024, 1, page, H)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q = torch.randn((3 * new, H, 64), generator=g, device="cuda").to(torch.bfloat16)
+    counts = torch.zeros(B + 1, dtype=torch.int64, device="cuda")
+    counts[[1, B // 2 + 1, B]] = new
+    starts = counts.cumsum(0).to(torch.int32)
+    lens = torch.full((B,), kv_len, dtype=torch.int32, device="cuda")
+    out = torch.full((3 * new, H * 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.paged_attention(q, k, v, out, table.repeat(B, 1), starts, lens, 0.125)
+    keys, values = (x[table[0].long()].transpose(1, 2).reshape(-1, 64).double()[:kv_len] for x in (k, v))
+    pos = kv_len - new + torch.arange(new, device="cuda")
+    s = q.double().view(3, new, H, 64).transpose(1, 2) @ keys.T * 0.125
+    p = torch.softmax(s.masked_fill(torch.arange(kv_len, device="cuda") > pos[:, None], -torch.inf), -1)
+    want, a = ((p @ x).transpose(1, 2).reshape(3 * new, -1) for x in (values, values.abs()))
+    assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * a).all())
+    assert ops.device_status() == 0 and ops.page_status() == 0

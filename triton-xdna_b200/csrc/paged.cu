@@ -1506,8 +1506,13 @@ int check_pages(const xb_paged_kv* kv, const char* what, char* err, size_t errle
       return XB_ERR_UNSUPPORTED;
     }
   if (kv->n_pages > 0x7ffffffeLL || kv->max_pages > 0x7fffffffLL || kv->page_size > 0x7fffffffLL ||
-      kv->max_pages * kv->page_size > 0x7fffffffLL || kv->batch > 0x7ffffffeLL || kv->n_kv_head > 65535) {
-    set_err(err, errlen, "%s: more than 2^31 - 1 pages, positions or sequences", what);
+      kv->max_pages * kv->page_size > 0x7fffffffLL || kv->n_kv_head > 65535) {
+    set_err(err, errlen, "%s: more than 2^31 - 1 pages or positions", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  // every CTA scans the sequences, and its other warps wait (at most kWaitLimit) while it passes empty ones
+  if (kv->batch > (1LL << 20)) {
+    set_err(err, errlen, "%s: more than 2^20 sequences", what);
     return XB_ERR_UNSUPPORTED;
   }
   return XB_OK;
