@@ -32,6 +32,7 @@ using namespace tc;
 typedef __nv_bfloat16 bf16;
 
 __device__ int g_bad_page = 0;      // a page id outside the pool, or a position without a page
+__device__ int g_taken = 0;         // a flag on its way to the host (take_flag)
 __device__ int g_paged_status = 0;  // XB_ERR_TIMEOUT once a bounded wait ran out (xb_device_status)
 constexpr uint64_t kWaitLimit = 2000000000ull;  // 2 s per wait: far above any legitimate wait
 
@@ -1484,6 +1485,22 @@ int status_words(int** bad, int** status, const char* what, char* err, size_t er
   return XB_ERR_CUDA;
 }
 
+// A flag's value, the flag cleared in the same step: a kernel on another stream
+// that sets it between a copy and a clearing would not be heard.
+__global__ void take_flag_kernel(int* flag) {
+  pdl_wait();
+  pdl_trigger();
+  g_taken = atomicExch(flag, 0);
+}
+
+cudaError_t take_flag(int* flag, int* value, cudaStream_t s) {
+  static std::mutex mu;  // g_taken is one word a device
+  std::lock_guard<std::mutex> lock(mu);
+  cudaError_t e = launch_k<false>(take_flag_kernel, 1, 1, 0, s, flag);
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(value, g_taken, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
+  return e == cudaSuccess ? cudaStreamSynchronize(s) : e;
+}
+
 // What a paged batch has to satisfy, device contents aside.
 int check_pages(const xb_paged_kv* kv, const char* what, char* err, size_t errlen) {
   if (!kv) {
@@ -1570,13 +1587,9 @@ cudaError_t launch_copy(const int32_t* src, const int32_t* dst, int n, uint8_t* 
 
 // The timeout flag of this file's kernels, read and cleared by xb_device_status.
 cudaError_t paged_status_take(int* status, cudaStream_t s) {
-  int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(status, paged::g_paged_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  if (e == cudaSuccess)
-    e = cudaMemcpyToSymbolAsync(paged::g_paged_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  return e;
+  int *bad = nullptr, *flag = nullptr;
+  if (paged::status_words(&bad, &flag, "", nullptr, 0)) return cudaErrorUnknown;
+  return paged::take_flag(flag, status, s);
 }
 
 }  // namespace xb
@@ -1861,12 +1874,10 @@ extern "C" int xb_page_status(void* stream, int* status, char* err, size_t errle
     set_err(err, errlen, "xb_page_status: null output");
     return XB_ERR_INVALID;
   }
-  cudaStream_t s = (cudaStream_t)stream;
-  int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(status, g_bad_page, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_bad_page, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  int *bad = nullptr, *timeout = nullptr;
+  int rc = status_words(&bad, &timeout, "xb_page_status", err, errlen);
+  if (rc) return rc;
+  cudaError_t e = take_flag(bad, status, (cudaStream_t)stream);
   if (e != cudaSuccess) {
     set_err(err, errlen, "xb_page_status: %s", cudaGetErrorString(e));
     return XB_ERR_CUDA;
