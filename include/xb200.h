@@ -679,8 +679,9 @@ XB_API int xb_attention_workspace_size(int64_t batch, int64_t seq,
  * has no table column or RoPE row, set the flag that xb_page_status reports.
  * New tokens' places (page, row) have to differ, within a call and between
  * calls at the same time: which of two writes to one place stays is not said.
- * The first call of each operator sets up its kernels: make it before a
- * stream capture.
+ * The first call that takes a kernel sets it up, and an operator picks one by
+ * its sizes (tokens, batch, heads, the table's width): make a call of the same
+ * sizes before a stream capture.
  * ------------------------------------------------------------------------- */
 
 typedef struct xb_paged_kv {

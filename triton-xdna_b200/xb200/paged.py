@@ -292,11 +292,13 @@ class PagedDecodeGraph:
         self._limit = max_positions
         # scratch buffers of this graph's own: no other call reuses or regrows them
         with ops.workspace_slot(ops.fresh_slot()):
-            # one eager step on a small pool sets up the kernels (attributes,
+            # one eager step of the captured sizes, a position in a page of a
+            # small pool for each sequence, sets up the kernels (attributes,
             # scratch) before the capture
             small = PagedKVCache(model.cfg, batch, cache.page_size, dev)
-            first = [small.add() for _ in range(batch)]
-            model.forward_packed(self.ids, small, small.step(first), next_token=self.next_token)
+            self._step.page_table[:, 0] = torch.arange(batch, device=dev)
+            self._step.kv_len.fill_(1)
+            model.forward_packed(self.ids, small, self._step, next_token=self.next_token)
             torch.cuda.synchronize(dev)
             del small
             self.graph = torch.cuda.CUDAGraph()
