@@ -1,7 +1,9 @@
 """PagedDecodeGraph: what it prepares before its capture, and what it keeps."""
 
+import gc
 import subprocess
 import sys
+import weakref
 
 import pytest
 import torch
@@ -67,3 +69,18 @@ def test_a_graph_whose_table_takes_64_bit_walks_is_the_first_call_of_a_process()
     got = subprocess.run([sys.executable, "-c", WIDE.format(pkg=PKG_ROOT, cfg=CFG)], capture_output=True, text=True,
                          timeout=300)
     assert got.returncode == 0, got.stderr[-2000:]
+
+
+def test_a_graph_keeps_its_model():
+    """The captured kernels read the model's weights and tables: they live as long as the graph."""
+    model = _model()
+    cache, eager = (PagedKVCache(model.cfg, 8, 16) for _ in range(2))
+    graph = PagedDecodeGraph(model, cache, 2, 64)
+    toks = torch.tensor([3, 4], device="cuda")
+    want = torch.empty_like(toks)
+    model.forward_paged(toks, eager, [eager.add(), eager.add()], next_token=want)
+    alive = weakref.ref(model)
+    del model
+    gc.collect()
+    assert alive() is not None
+    assert torch.equal(graph.step([cache.add(), cache.add()], toks), want)

@@ -277,7 +277,7 @@ class PagedDecodeGraph:
         if batch < 1 or not 0 < max_positions <= model.position_limit:
             raise ValueError(f"batch must be positive and max_positions 1 .. {model.position_limit}")
         _check_cache(model, cache)
-        self.cache, self.batch = cache, batch
+        self.model, self.cache, self.batch = model, cache, batch  # the graph reads the model's weights
         dev = cache.device
         self.columns = -(-max_positions // cache.page_size)
         n = batch * self.columns
