@@ -362,3 +362,25 @@ def test_more_sequences_than_a_kernel_scans_are_refused():
             with pytest.raises(XbError) as e:
                 call(batch=batch)
             assert e.value.code == _lib.XB_ERR_UNSUPPORTED and "2^20 sequences" in e.value.message, e.value.message
+
+
+def test_a_copy_that_fails_leaves_the_books(copies, monkeypatch):
+    c = _cache()
+    a = c.add()
+    _write(c, c.step([a], [11]), [a], [11], lambda i, p: p)
+    b = c.fork(a)
+    before = (c.page_ids(a), c.page_ids(b), list(c._refs), sorted(c._free))
+
+    def fails(*args, **kw):
+        raise RuntimeError("no copy")
+
+    with monkeypatch.context() as m:
+        m.setattr(ops, "copy_pages", fails)
+        with pytest.raises(RuntimeError, match="no copy"):
+            c.step([b, a], [9, 3])
+    assert before == (c.page_ids(a), c.page_ids(b), c._refs, sorted(c._free)) and c.length(a) == c.length(b) == 11
+    _check(c)
+    _write(c, c.step([b, a], [9, 3]), [b, a], [9, 3], lambda i, p: 50 * (i + 1) + p)
+    assert _read(c, b) == list(range(11)) + [50 + p for p in range(11, 20)]
+    assert _read(c, a) == list(range(11)) + [100 + p for p in range(11, 14)]
+    _check(c)

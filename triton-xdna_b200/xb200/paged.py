@@ -167,22 +167,30 @@ class PagedKVCache:
             plan.append((s, c, fresh, own))
         if need > len(self._free):
             raise RuntimeError(f"KV cache full: the step needs {need} pages, {len(self._free)} are free")
-        src, dst = [], []
+        taken = [heapq.heappop(self._free) for _ in range(need)]
+        src, dst, at = [], [], 0
         for s, c, fresh, own in plan:
             if own:
-                p = heapq.heappop(self._free)
                 src.append(s.pages[-1])
-                dst.append(p)
-                self._refs[p] = 1
+                dst.append(taken[at])
+            at += own + fresh
+        try:  # before the books change: a copy that fails leaves them as they were
+            if src:
+                ops.copy_pages(self.pages, src, dst)
+        except BaseException:
+            for p in taken:
+                heapq.heappush(self._free, p)
+            raise
+        for p in taken:
+            self._refs[p] = 1
+        at = 0
+        for s, c, fresh, own in plan:
+            if own:
                 self._refs[s.pages[-1]] -= 1
-                s.pages[-1] = p
-            for _ in range(fresh):
-                p = heapq.heappop(self._free)
-                self._refs[p] = 1
-                s.pages.append(p)
+                s.pages[-1] = taken[at]
+            s.pages += taken[at + own:at + own + fresh]
+            at += own + fresh
             s.length += c
-        if src:
-            ops.copy_pages(self.pages, src, dst)
 
     def _table(self, seqs, columns: int) -> np.ndarray:
         table = np.zeros((len(seqs), columns), dtype=np.int32)
