@@ -384,3 +384,9 @@ def test_a_copy_that_fails_leaves_the_books(copies, monkeypatch):
     assert _read(c, b) == list(range(11)) + [50 + p for p in range(11, 20)]
     assert _read(c, a) == list(range(11)) + [100 + p for p in range(11, 14)]
     _check(c)
+
+
+def test_copy_pages_refuses_pages_of_2_36_bytes():
+    with pytest.raises(XbError) as e:
+        _copy([0], [1], n_pages=2, page_bytes=1 << 36)
+    assert e.value.code == _lib.XB_ERR_UNSUPPORTED

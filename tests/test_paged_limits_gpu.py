@@ -63,3 +63,14 @@ def test_a_million_sequences_most_of_them_empty(H, new):
     want, a = ((p @ x).transpose(1, 2).reshape(3 * new, -1) for x in (values, values.abs()))
     assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * a).all())
     assert ops.device_status() == 0 and ops.page_status() == 0
+
+
+def test_copies_of_pages_of_half_a_gigabyte():
+    """As a cache with pages of 2^20 positions of four heads has them: 500 would pass a launch's 2^32 vectors."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pool = torch.randint(0, 1 << 30, (2, 5, 1 << 27), dtype=torch.int32, generator=g, device="cuda")
+    want = pool[:, :2].clone()
+    last = pool[:, 4].clone()
+    assert ops.copy_pages(pool, [0, 1], [3, 2], dim=1) is pool
+    for at, page in ((0, want[:, 0]), (1, want[:, 1]), (3, want[:, 0]), (2, want[:, 1]), (4, last)):
+        assert torch.equal(pool[:, at], page)

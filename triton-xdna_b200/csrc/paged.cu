@@ -46,7 +46,7 @@ constexpr uint64_t kWaitLimit = 2000000000ull;  // 2 s per wait: far above any l
 // moves four 16-byte vectors 256 apart (four loads in flight), a CTA 16 KB of
 // the outer slab's n * vpp vectors.  2500 pages of 4 KB in 48 slabs take 164 us,
 // 0.91 of the measured copy rate; 4 pages 2.2 us, the launch.
-constexpr int kCopyPairs = 500;  // 4000 bytes of parameters; larger lists take several launches
+constexpr int kCopyPairs = 500;  // 4000 bytes of parameters; larger lists, and very large pages, take several launches
 template <int N>
 struct CopyPairs {
   int32_t src[N], dst[N];
@@ -1647,15 +1647,17 @@ extern "C" int xb_copy_pages(void* pages, int64_t outer, int64_t outer_bytes, in
     set_err(err, errlen, "%s: pages must be whole 16-byte vectors in slabs that do not overlap", what);
     return XB_ERR_UNSUPPORTED;
   }
-  if (outer > 65535 || page_bytes / 16 * kCopyPairs > 0xffff0000LL) {
+  const int64_t vectors = 0xffff0000LL;  // of a launch, counted in 32 bits
+  if (outer > 65535 || page_bytes / 16 > vectors) {
     set_err(err, errlen, "%s: %lld slabs of %lld-byte pages not supported", what, (long long)outer,
             (long long)page_bytes);
     return XB_ERR_UNSUPPORTED;
   }
   const uint32_t vpp = (uint32_t)(page_bytes / 16);
+  const int64_t most = vectors / vpp < kCopyPairs ? vectors / vpp : kCopyPairs;
   uint8_t* base = static_cast<uint8_t*>(pages);
-  for (int64_t i = 0; i < n; i += kCopyPairs) {
-    const int c = (int)(n - i < kCopyPairs ? n - i : kCopyPairs);
+  for (int64_t i = 0; i < n; i += most) {
+    const int c = (int)(n - i < most ? n - i : most);
     cudaError_t e = c <= 28 ? launch_copy<28>(src + i, dst + i, c, base, outer, outer_bytes, page_bytes, vpp,
                                               (cudaStream_t)stream)
                             : launch_copy<kCopyPairs>(src + i, dst + i, c, base, outer, outer_bytes, page_bytes, vpp,
