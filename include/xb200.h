@@ -714,13 +714,14 @@ XB_API int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t,
 /* Causal grouped-query attention of the packed new tokens over the pages: the
  * token at position p sees keys 0 .. p.  q [tokens, n_head, 64] (token pitch
  * ld_q), out [tokens, n_head * 64] (pitch ld_out), head_dim 64, n_head /
- * n_kv_head at most 128, scale > 0.  Online softmax in fp32, P rounded to bf16
- * before P V, as xb_attention_bf16.  A token with a negative position
- * (kv_len[b] < n) sees nothing: its row is zero.  Lengths beyond the table
- * count as max_pages * page_size; a page id outside the pool reads as zeros
- * (flagged).  What lies behind a sequence's last key may be anything; keys that a
- * token does not see weigh zero, so as in xb_attention_bf16 a value of theirs
- * that is infinite or NaN spoils the row of an earlier token of the same step.
+ * n_kv_head at most 128, scale > 0 and scale * log2(e) finite.  Online softmax
+ * in fp32, P rounded to bf16 before P V, as xb_attention_bf16.  A token with a
+ * negative position (kv_len[b] < n) sees nothing: its row is zero.  Lengths
+ * beyond the table count as max_pages * page_size; a page id outside the pool
+ * reads as zeros (flagged).  What lies behind a sequence's last key may be
+ * anything; keys that a token does not see weigh zero, so as in
+ * xb_attention_bf16 a value of theirs that is infinite or NaN spoils the row of
+ * an earlier token of the same step.
  * Long contexts are split over CTAs and joined in a fixed order:
  * the same inputs give the same bits, and the split depends on the whole
  * batch's lengths.  `workspace` (16-byte aligned, size from the query below,

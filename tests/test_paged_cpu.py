@@ -390,3 +390,11 @@ def test_copy_pages_refuses_pages_of_2_36_bytes():
     with pytest.raises(XbError) as e:
         _copy([0], [1], n_pages=2, page_bytes=1 << 36)
     assert e.value.code == _lib.XB_ERR_UNSUPPORTED
+
+
+def test_a_scale_whose_base_2_form_overflows_is_refused():
+    """scores are scaled by scale * log2(e) in fp32: infinite from 2.4e38 on, and then every score of zero is NaN."""
+    for scale, refused in ((2.35e38, False), (2.37e38, True), (3e38, True)):
+        with pytest.raises(XbError) as e:  # without a workspace: nothing is launched
+            _attn(scale=scale)
+        assert ("scale" in e.value.message) == refused, e.value.message

@@ -1769,8 +1769,9 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
     return XB_ERR_UNSUPPORTED;
   }
   const int n_rep = (int)(n_head / n_kv_head);
-  if (!(scale > 0.0f && scale < INFINITY)) {
-    set_err(err, errlen, "%s: the scale must be positive and finite", what);
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale_log2 > 0.0f && scale_log2 < INFINITY)) {
+    set_err(err, errlen, "%s: the scale must be positive and, times log2(e), finite", what);
     return XB_ERR_INVALID;
   }
   if (tokens == 0 || batch == 0) return XB_OK;
@@ -1817,7 +1818,7 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
   a.page_size = (int)page_size;
   a.max_pages = (int)kv->max_pages;
   a.n_pages = (int)n_pages;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   rc = status_words(&a.bad, &a.status, what, err, errlen);
   if (rc) return rc;
   const bool few = few_rows(tokens, batch, n_rep);
