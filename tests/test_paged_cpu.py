@@ -398,3 +398,14 @@ def test_a_scale_whose_base_2_form_overflows_is_refused():
         with pytest.raises(XbError) as e:  # without a workspace: nothing is launched
             _attn(scale=scale)
         assert ("scale" in e.value.message) == refused, e.value.message
+
+
+@pytest.mark.parametrize("page_size", [0, -16, 12])
+def test_generation_refuses_a_page_size_as_the_cache_does(page_size):
+    from xb200.paged import generate_paged
+
+    class Model:
+        cfg, position_limit, device = _Cfg, 64, torch.device("cpu")
+
+    with pytest.raises(ValueError, match="multiple of 8"):
+        generate_paged(Model, [torch.ones(3, dtype=torch.int64)], 4, page_size=page_size)

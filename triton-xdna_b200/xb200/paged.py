@@ -349,7 +349,8 @@ def generate_paged(model, prompts, max_new_tokens: int, cache: PagedKVCache | No
     if longest > model.position_limit:
         raise ValueError(f"{longest} positions exceed the model's {model.position_limit}")
     if cache is None:
-        cache = PagedKVCache(model.cfg, sum(-(-(c + more) // page_size) for c in counts), page_size, model.device)
+        unit = max(page_size, 1)  # what no page may have is for the cache to refuse
+        cache = PagedKVCache(model.cfg, sum(-(-(c + more) // unit) for c in counts), page_size, model.device)
     B = len(prompts)
     ids = torch.cat([p.to(model.device) for p in prompts])
     toks = torch.empty((max_new_tokens, B), dtype=torch.int64, device=model.device)
