@@ -206,8 +206,9 @@ __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a,
 // new tokens of a sequence times the n_rep query heads that share the KV head,
 // which are the rows of one matrix tile, so every key and value is read once
 // for all of them.  Query tile j of a sequence with `base` earlier positions
-// sees base + min(tpt (j + 1), n) keys; its weight is those keys plus `over`,
-// what starting and finishing a unit costs in keys.  All units laid end to end
+// sees base + min(tpt (j + 1), n) keys (none where that is negative); its weight
+// is those keys plus `over`, what starting and finishing a unit costs in keys
+// (csrc/paged_walk.cuh has the arithmetic).  All units laid end to end
 // are one line of weight `total`; CTA c takes the piece [c share, (c + 1) share)
 // of it, whatever unit boundaries lie inside, so the CTAs finish together
 // however uneven the batch is (in the few-row kernel every warp has a piece).
@@ -1549,8 +1550,15 @@ int check_page_pointers(const xb_paged_kv* kv, const char* what, char* err, size
 }
 
 // Which attention kernel: the mma.sync one while the batch's rows per (sequence,
-// KV head) fill at most one of its 16-row tiles on average, so K and V are
-// read about once; the host knows this much without the lengths.
+// KV head) fill at most one of its 16-row tiles on average; the host knows
+// this much without the lengths.  Few-row / tcgen05 kernel, us in a graph, 14
+// heads on 2, rows a sequence: 33 sequences of 300-4000 keys 7 13.8 / 19.1, 14
+// 16.4 / 19.8, 21 23.4 / 19.7, 35 25.4 / 18.7; 160 of 500-1500 14 23.4 / 28.9, 21
+// 36.5 / 30.4, 56 56.8 / 31.1.  12 heads of their own, 160 sequences: 16 89.3 /
+// 110.4, 24 160.6 / 109.8.  It is an average: where one sequence brings most of
+// the tokens, its 16-row units read its keys once each.  With 12 / 12 heads, 49
+// single tokens and a chunk of 512 (11.2 rows on average) take 31.3 / 33.1, 99
+// and 1024 with 25 / 25 113.9 / 110.5, but 199 and 3000 (16.0) 205 / 126.
 bool few_rows(int64_t tokens, int64_t batch, int64_t n_rep) {
   return n_rep <= kFewRows && tokens * n_rep <= kFewRows * batch;
 }

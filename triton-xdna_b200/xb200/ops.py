@@ -1194,10 +1194,10 @@ def _page_list(ids, name) -> torch.Tensor:
 def copy_pages(pages, src, dst, dim: int = 2):
     """pages[.., dst[i], ..] = pages[.., src[i], ..] along dimension `dim` of a
     contiguous pool (PagedKVCache.pages: [n_layer, 2, n_pages, n_kv_head,
-    page_size, head_dim]): all layers' keys and values in one launch.  src and
-    dst are page numbers on the host (lists or CPU integer tensors), read
-    during the call (a captured copy repeats the same pairs); no page may be a
-    destination twice, or both a source and a destination."""
+    page_size, head_dim]): all layers' keys and values, 500 pairs to a launch.
+    src and dst are page numbers on the host (lists or CPU integer tensors),
+    read during the call (a captured copy repeats the same pairs); no page may
+    be a destination twice, or both a source and a destination."""
     dev = _device_of(pages)
     shape = pages.shape
     if not -len(shape) <= dim < len(shape):
