@@ -45,6 +45,7 @@ extern "C" {
 #define XB_DT_I8 2
 #define XB_DT_I16 3
 #define XB_DT_I32 4
+#define XB_DT_F8E4M3 5 /* pages of a paged KV cache */
 
 /* Library ABI version (bumped when a signature changes). */
 XB_API int xb_abi_version(void);
@@ -748,6 +749,55 @@ XB_API int xb_copy_pages(void* pages, int64_t outer, int64_t outer_bytes,
                          const int32_t* src, const int32_t* dst, int64_t n,
                          void* stream, char* err, size_t errlen);
 
+/* 8-bit pages: keys and values as int8 or float8 e4m3 codes, half the bytes of
+ * bf16 pages.  `kv` describes the codes (strides multiples of 16 elements); each row
+ * of a page and KV head has an exponent byte beside it: a code c stands for c *
+ * 2^(byte - 127).  The byte is 127 + the smallest e with max |x| <= M 2^e over
+ * the row's bf16 numbers x (M = 127 for int8, 448 for e4m3), kept within 47 .. 248
+ * (int8) or 246 (e4m3), the codes are x 2^-e rounded to nearest even and
+ * saturated; so what a code stands for is a bf16 number.  Byte 255 with codes of
+ * zero: the row holds an infinity or NaN, and reads as NaN throughout.  Other
+ * bytes and e4m3's NaN codes are not written and have no defined meaning.
+ * k_scale / v_scale [n_pages, n_kv_head, page_size] uint8, 8-byte aligned, byte
+ * strides of page and head multiples of 8, unit row stride. */
+typedef struct xb_paged_kv8 {
+  xb_paged_kv kv;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int64_t ks_page, ks_head, vs_page, vs_head;
+  int64_t dtype; /* XB_DT_I8, XB_DT_F8E4M3; xb_paged_read_kv: also XB_DT_BF16 */
+} xb_paged_kv8;
+
+/* xb_paged_rope_kv_bf16 with the bf16 keys and values it would write quantised. */
+XB_API int xb_paged_rope_kv_q8(const void* qkv, const float* cos_t,
+                               const float* sin_t, void* q_out,
+                               const xb_paged_kv8* kv, int64_t tokens,
+                               int64_t n_head, int64_t rope_rows,
+                               int64_t ld_qkv, int64_t ld_q, void* stream,
+                               char* err, size_t errlen);
+
+/* The inverse of the write: k_out / v_out [tokens, n_kv_head * head_dim] bf16
+ * (pitches ld_k, ld_v) are what the pages hold at the positions of the packed
+ * tokens (q_start and kv_len as for the write; with n = kv_len whole
+ * sequences).  dtype XB_DT_BF16 reads bf16 pages (exponents unused).  A token
+ * without a page reads as zeros (flagged).  head_dim a multiple of 8. */
+XB_API int xb_paged_read_kv(void* k_out, void* v_out, const xb_paged_kv8* kv,
+                            int64_t tokens, int64_t ld_k, int64_t ld_v,
+                            void* stream, char* err, size_t errlen);
+
+/* xb_paged_attention_bf16 over 8-bit pages: the attention over what the codes
+ * stand for. */
+XB_API int xb_paged_attention_q8_workspace_size(
+    int64_t tokens, int64_t batch, int64_t n_head, int64_t n_kv_head,
+    int64_t n_pages, int64_t page_size, int64_t max_pages, size_t* bytes,
+    char* err, size_t errlen);
+XB_API int xb_paged_attention_q8(const void* q, void* out,
+                                 const xb_paged_kv8* kv, int64_t tokens,
+                                 int64_t n_head, int64_t ld_q, int64_t ld_out,
+                                 float scale, void* workspace,
+                                 size_t workspace_bytes, void* stream,
+                                 char* err, size_t errlen);
+
 /* *status = 1 if a paged operator met a page id outside its pool or a
  * position without a page or RoPE row since the previous call (then clears
  * the flag), else 0.  Synchronises `stream`. */
@@ -760,6 +810,31 @@ XB_API int xb_page_status(void* stream, int* status, char* err,
 XB_API int xb_argmax_f32(const float* x, int64_t rows, int64_t cols,
                          int64_t ld, int64_t* idx, void* stream, char* err,
                          size_t errlen);
+
+/* The selection of a beam search step.  logits [groups * beams, vocab] (bf16 or
+ * f32, row pitch ld, rows of contiguous elements) of each group's beams, scores
+ * [groups, beams] f32 (pitch ld_scores): of all beams k and tokens v of a
+ * group the `count` largest of
+ *   scores[k] + logits[k, v] - log(sum_u exp(logits[k, u])),
+ * largest first, equal ones by the lowest (k, v): their sums (values f32),
+ * beams (parents) and tokens, [groups, count] contiguous.  Sums are compared in 64
+ * bits.  A beam with a score that is not finite (-inf: one that is out), with a
+ * NaN or +inf among its logits or with none above -inf has no continuation,
+ * nor has a token whose logit is -inf; where fewer than `count` are left the rest
+ * is -inf, -1, -1.  At most 64 beams, 64 continuations, 2^20 groups.  `workspace`
+ * (16-byte aligned, size from the query) belongs to the call.  Extends the greedy
+ * choice of model.py:1155, 1171. */
+XB_API int xb_beam_select_workspace_size(int64_t groups, int64_t beams,
+                                         int64_t vocab, int64_t count,
+                                         size_t* bytes, char* err,
+                                         size_t errlen);
+XB_API int xb_beam_select(const void* logits, const float* scores,
+                          int64_t groups, int64_t beams, int64_t vocab,
+                          int64_t ld, int64_t ld_scores, int64_t count,
+                          int dtype, float* values, int64_t* parents,
+                          int64_t* tokens, void* workspace,
+                          size_t workspace_bytes, void* stream, char* err,
+                          size_t errlen);
 
 /* Read (synchronising `stream`) and clear the device status word that the
  * tensor-core kernels set when a bounded wait runs out: 0 = fine,

@@ -1,0 +1,97 @@
+// 8-bit codes of a KV cache's head vectors.  A vector of bf16 numbers whose
+// largest magnitude is a has the exponent e, the smallest whole number with a <=
+// M 2^e (M = 127 for int8, 448 for e4m3), and the codes rne(x 2^-e); a code c
+// stands for c 2^e.  e is kept as the byte e + 127.  The scale is a power of two, so
+// what a code stands for is a bf16 number: reading back rounds nothing, and a
+// matrix product sees exactly what is stored.  It costs int8 up to one of its
+// seven bits (a scale of a / 127 would use them all) and e4m3 nothing.
+// Bytes: 47 (so that sums of weights 2^-e stay far inside fp32; smaller vectors
+// round to zeros) to 248 / 246 (what the largest codes stand for is finite;
+// vectors beyond saturate), and 255: an infinity or NaN in the vector, which
+// reads as NaN throughout.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace xb {
+namespace codes {
+
+constexpr int kLeastByte = 47, kNanByte = 255;
+
+// Format of a cache's pages (template argument of the kernels that serve all three)
+enum Format : int { kBf16 = 0, kInt8 = 1, kE4m3 = 2 };
+
+// The exponent byte of a vector whose largest magnitude has the bf16 bits `top`.
+// a = (1 + f / 128) 2^(top / 128 - 127) with f = top % 128: 127 = (1 + 126 / 128) 2^6,
+// 448 = (1 + 96 / 128) 2^8.
+template <Format F>
+__device__ __forceinline__ int exponent_byte(uint32_t top) {
+  constexpr int bits = F == kInt8 ? 6 : 8, fraction = F == kInt8 ? 126 : 96, last = F == kInt8 ? 248 : 246;
+  if (top >= 0x7f80u) return kNanByte;
+  const int b = (int)(top >> 7) - bits + ((int)(top & 127u) > fraction);
+  return min(max(b, kLeastByte), last);
+}
+
+// 2^e of a byte (NaN for 255), and 2^-e (0 for 255)
+__device__ __forceinline__ float byte_scale(int b) {
+  return b == kNanByte ? __int_as_float(0x7fc00000) : __int_as_float(b << 23);
+}
+__device__ __forceinline__ float byte_inverse(int b) {
+  return b == kNanByte ? 0.0f : __int_as_float((254 - b) << 23);
+}
+
+// Four codes of x 2^-e
+template <Format F>
+__device__ __forceinline__ uint32_t encode4(float x0, float x1, float x2, float x3, float inverse) {
+  x0 *= inverse;
+  x1 *= inverse;
+  x2 *= inverse;
+  x3 *= inverse;
+  if constexpr (F == kInt8) {
+    auto whole = [](float x) -> uint32_t { return (uint32_t)__float2int_rn(fminf(fmaxf(x, -127.0f), 127.0f)) & 255u; };
+    return whole(x0) | whole(x1) << 8 | whole(x2) << 16 | whole(x3) << 24;
+  } else {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x1), "f"(x0));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x3), "f"(x2));
+    return (uint32_t)lo | (uint32_t)hi << 16;
+  }
+}
+
+// Two e4m3 codes as fp16 (exact)
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return r;
+}
+
+// Two int8 codes as fp16 (exact): byte c + 128 in the low bits of 1024 is 1024 + 128 + c.
+// `x` has the sign bits flipped, `pick` places the two bytes below 0x64's.
+__device__ __forceinline__ uint32_t int8x2_to_half2(uint32_t x, uint32_t pick) {
+  const uint32_t m = __byte_perm(x, 0x64646464u, pick);
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// What four codes stand for, as bf16 (exact)
+template <Format F>
+__device__ __forceinline__ uint2 decode4(uint32_t v, float scale) {
+  float x[4];
+  if constexpr (F == kInt8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(v >> (8 * i));
+  } else {
+    const uint32_t lo = e4m3x2_to_half2((uint16_t)v), hi = e4m3x2_to_half2((uint16_t)(v >> 16));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+  }
+  const __nv_bfloat162 p = __floats2bfloat162_rn(x[0] * scale, x[1] * scale);
+  const __nv_bfloat162 q = __floats2bfloat162_rn(x[2] * scale, x[3] * scale);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
+}
+
+}  // namespace codes
+}  // namespace xb

@@ -21,6 +21,7 @@
 // are clamped to the rows given, lengths to what the table can hold, and a
 // page id outside the pool reads as zeros (attention) or is skipped (writes)
 // and sets the flag that xb_page_status reports.
+#include "codes.cuh"
 #include "common.cuh"
 #include "paged_walk.cuh"
 #include "tc.cuh"
@@ -29,8 +30,10 @@ namespace xb {
 namespace paged {
 
 using namespace tc;
+using namespace codes;
 typedef __nv_bfloat16 bf16;
 
+constexpr int kRowDims = 64;        // head dim of every attention
 __device__ int g_bad_page = 0;      // a page id outside the pool, or a position without a page
 __device__ int g_taken = 0;         // a flag on its way to the host (take_flag)
 __device__ int g_paged_status = 0;  // XB_ERR_TIMEOUT once a bounded wait ran out (xb_device_status)
@@ -80,8 +83,13 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__
 // ----------------------------------------------------------------------------- RoPE + page write
 
 struct Pages {  // K or V pages: element strides of page, head and row; rows of D contiguous elements
-  bf16* p;
+  bf16* p;      // (8-bit pages: codes, strides in bytes)
   int64_t page, head, row;
+};
+
+struct Exponents {  // of 8-bit K or V pages: a byte for each row, byte strides of page and head
+  uint8_t* p;
+  int64_t page, head;
 };
 
 struct RopeArgs {
@@ -92,7 +100,23 @@ struct RopeArgs {
   const int32_t *table, *q_start, *kv_len;
   int64_t ld_qkv, ld_q, ld_table, rope_rows;
   int T, B, H, KVH, D, page_size, max_pages, n_pages;
+  Exponents ke, ve;  // 8-bit pages only
 };
+
+// The last b with q_start[b] <= t, all lanes together (32 starts a step); empty
+// sequences share their start with the next one.  -1: a row before the first.
+__device__ __forceinline__ int sequence_of(const int32_t* q_start, int B, int t, int lane) {
+  int b = 0;
+  for (int len = B + 1;;) {
+    const int stride = (len + 31) / 32;
+    const bool le = lane * stride < len && __ldg(q_start + b + lane * stride) <= t;
+    const int n = __popc(__ballot_sync(0xffffffffu, le));
+    if (n == 0) return -1;
+    b += (n - 1) * stride;
+    if (stride == 1) return b;
+    len = min(stride, len - (n - 1) * stride);
+  }
+}
 
 // One warp per packed token.  A lane keeps one group of 8 dims (and the 8 of
 // the other half they rotate with) and walks the head slots, so it reads its
@@ -107,6 +131,11 @@ struct RopeArgs {
 // 47.1, three in 80 39.6; stores marked as streaming 35.8; then CTAs of two
 // warps instead of eight 33.8 (four 34.2, 24 46.0): a CTA's place is taken again
 // as soon as its own few tokens are done.
+//
+// 8-bit pages: the lanes of a slot (a divisor of 32 of them, side by side) find its largest
+// magnitude by shuffles and store 8 codes each per half.  What is quantised is
+// the bf16 number that a bf16 page would hold.
+template <Format F>
 __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a, int* __restrict__ bad) {
   pdl_wait();
   pdl_trigger();
@@ -130,17 +159,8 @@ __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a,
     }
   };
   load(slot0);
-  // the last b with q_start[b] <= t; empty sequences share their start with the next one
-  int b = 0;
-  for (int len = a.B + 1;;) {
-    const int stride = (len + 31) / 32;
-    const bool le = lane * stride < len && __ldg(a.q_start + b + lane * stride) <= t;
-    const int n = __popc(__ballot_sync(0xffffffffu, le));
-    if (n == 0) return;  // a row before the first sequence
-    b += (n - 1) * stride;
-    if (stride == 1) break;
-    len = min(stride, len - (n - 1) * stride);
-  }
+  const int b = sequence_of(a.q_start, a.B, t, lane);
+  if (b < 0) return;
   if (b >= a.B) return;  // behind the last sequence
   const int end = __ldg(a.q_start + b + 1);
   if (end <= t) return;  // (starts that do not ascend)
@@ -189,6 +209,31 @@ __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a,
         if (!page_ok) continue;
         const bool is_k = slot < a.H + a.KVH;
         const Pages& pg = is_k ? a.k : a.v;
+        if constexpr (F != kBf16) {
+          const int head = slot - a.H - (is_k ? 0 : a.KVH);
+          uint32_t top = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            top = max(top, max(__bfloat16_as_ushort(u[i].v[e]) & 0x7fffu, __bfloat16_as_ushort(w[i].v[e]) & 0x7fffu));
+          const uint32_t team = (0xffffffffu >> (32 - groups)) << (lane & ~(groups - 1));
+          for (int o = 1; o < groups; o <<= 1) top = max(top, __shfl_xor_sync(team, top, o));
+          const int byte = exponent_byte<F>(top);
+          const float inverse = byte_inverse(byte);
+          float x0[8], x1[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x0[e] = byte == kNanByte ? 0.0f : __bfloat162float(u[i].v[e]);
+            x1[e] = byte == kNanByte ? 0.0f : __bfloat162float(w[i].v[e]);
+          }
+          uint8_t* at = reinterpret_cast<uint8_t*>(pg.p) + id * pg.page + head * pg.head + row * pg.row + c;
+          *reinterpret_cast<uint2*>(at) = make_uint2(encode4<F>(x0[0], x0[1], x0[2], x0[3], inverse),
+                                                     encode4<F>(x0[4], x0[5], x0[6], x0[7], inverse));
+          *reinterpret_cast<uint2*>(at + half) = make_uint2(encode4<F>(x1[0], x1[1], x1[2], x1[3], inverse),
+                                                            encode4<F>(x1[4], x1[5], x1[6], x1[7], inverse));
+          const Exponents& ex = is_k ? a.ke : a.ve;
+          if (c == 0) ex.p[id * ex.page + head * ex.head + row] = (uint8_t)byte;
+          continue;
+        }
         dst = pg.p + id * pg.page + (slot - a.H - (is_k ? 0 : a.KVH)) * pg.head + row * pg.row;
       }
       st16_stream(dst + c, u[i]);
@@ -197,6 +242,113 @@ __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a,
     first += kAhead * step;
     if (first >= slots) break;
     load(first);
+  }
+}
+
+// ----------------------------------------------------------------------------- reading back
+
+struct ReadArgs {
+  bf16 *k_out, *v_out;
+  Pages k, v;
+  Exponents ke, ve;
+  const int32_t *table, *q_start, *kv_len;
+  int64_t ld_k, ld_v, ld_table;
+  int T, B, KVH, D, page_size, max_pages, n_pages;
+};
+
+// k_out[t] and v_out[t]: what the pages hold at the position of packed token t
+// (the inverse of the write).  One warp per token, 8 elements a lane.
+template <Format F>
+__global__ void __launch_bounds__(256) paged_read_kv_kernel(const ReadArgs a, int* __restrict__ bad) {
+  pdl_wait();
+  pdl_trigger();
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (t >= a.T) return;
+  const int b = sequence_of(a.q_start, a.B, t, lane);
+  if (b < 0 || b >= a.B) return;
+  const int end = __ldg(a.q_start + b + 1);
+  if (end <= t || __ldg(a.q_start + b) > t) return;  // (starts that do not ascend)
+  const int64_t pos = (int64_t)__ldg(a.kv_len + b) - ((int64_t)end - t);
+  const int64_t slot_page = pos >= 0 ? (int64_t)((uint32_t)pos / (uint32_t)a.page_size) : -1;  // pos < 2^31
+  int id = -1;
+  if (pos >= 0 && slot_page < a.max_pages) id = __ldg(a.table + (int64_t)b * a.ld_table + slot_page);
+  const bool page_ok = id >= 0 && id < a.n_pages;  // otherwise zeros
+  if (!page_ok && lane == 0) atomicExch(bad, 1);
+  const int row = (int)(pos - slot_page * a.page_size);
+  const int per = a.D / 8, items = a.KVH * per;
+  for (int i = lane; i < 2 * items; i += 32) {
+    const bool is_v = i >= items;
+    const int j = is_v ? i - items : i, head = j / per, d = (j - head * per) * 8;
+    const Pages& pg = is_v ? a.v : a.k;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (page_ok) {
+      const int64_t at = id * pg.page + head * pg.head + row * pg.row + d;
+      if constexpr (F == kBf16) {
+        x = __ldcs(reinterpret_cast<const uint4*>(pg.p + at));
+      } else {
+        const Exponents& ex = is_v ? a.ve : a.ke;
+        const float scale = byte_scale(ex.p[id * ex.page + head * ex.head + row]);
+        const uint2 c = __ldcs(reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(pg.p) + at));
+        const uint2 lo = decode4<F>(c.x, scale), hi = decode4<F>(c.y, scale);
+        x = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      }
+    }
+    bf16* out = is_v ? a.v_out + (int64_t)t * a.ld_v : a.k_out + (int64_t)t * a.ld_k;
+    __stcs(reinterpret_cast<uint4*>(out + head * a.D + d), x);
+  }
+}
+
+struct ExpandArgs {
+  Pages k, v;          // codes
+  Exponents ke, ve;
+  bf16 *k_out, *v_out;  // [slots][KVH][page][64]
+  int32_t* slots;       // [B][max_pages]: where a page went; a bad page id stays
+  const int32_t *table, *q_start, *kv_len;
+  int64_t ld_table;
+  int T, B, KVH, page_size, max_pages, n_pages;
+  int compact;  // slot b max_pages + column; otherwise the page's own number
+};
+
+// The pages that a batch names as bf16, for the tcgen05 attention kernel, whose
+// operands are bf16 tiles in shared memory.  A warp takes 8 rows of a page and
+// head at a time: 16 codes a lane of K and of V.  Where pages go by their own
+// number and sequences share one, each writes the same values.
+template <Format F>
+__global__ void __launch_bounds__(256) paged_expand_kernel(const ExpandArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, first = blockIdx.x * 8 + (threadIdx.x >> 5), step = gridDim.x * 8;
+  const int r = lane >> 2, d = (lane & 3) * 16;
+  for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
+    const int s0 = min(max(__ldg(a.q_start + b), 0), a.T), s1 = min(max(__ldg(a.q_start + b + 1), s0), a.T);
+    if (s0 == s1) continue;
+    const int len = min(max(__ldg(a.kv_len + b), 0), a.max_pages * a.page_size);
+    const int64_t parts = (int64_t)((len + 7) / 8) * a.KVH;
+    for (int64_t i = first; i < parts; i += step) {
+      const int head = (int)(i % a.KVH), p0 = (int)(i / a.KVH) * 8;
+      const int col = p0 / a.page_size, row = p0 - col * a.page_size + r;
+      const int id = __ldg(a.table + b * a.ld_table + col);
+      const bool ok = id >= 0 && id < a.n_pages;
+      const int64_t entry = (int64_t)b * a.max_pages + col;
+      const int64_t slot = a.compact ? entry : id;
+      if (head == 0 && row == 0 && lane == 0) a.slots[entry] = ok ? (int)slot : -1;
+      if (!ok) continue;
+      const int64_t to = ((slot * a.KVH + head) * a.page_size + row) * kRowDims + d;
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind) {
+        const Pages& pg = kind ? a.v : a.k;
+        const Exponents& ex = kind ? a.ve : a.ke;
+        const uint4 c = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pg.p) + id * pg.page +
+                                                             head * pg.head + row * pg.row + d));
+        const float scale = byte_scale(__ldg(ex.p + id * ex.page + head * ex.head + row));
+        const uint2 x0 = decode4<F>(c.x, scale), x1 = decode4<F>(c.y, scale);
+        const uint2 x2 = decode4<F>(c.z, scale), x3 = decode4<F>(c.w, scale);
+        uint4* out = reinterpret_cast<uint4*>((kind ? a.v_out : a.k_out) + to);
+        out[0] = make_uint4(x0.x, x0.y, x1.x, x1.y);
+        out[1] = make_uint4(x2.x, x2.y, x3.x, x3.y);
+      }
+    }
   }
 }
 
@@ -1549,6 +1701,40 @@ int check_page_pointers(const xb_paged_kv* kv, const char* what, char* err, size
   return XB_OK;
 }
 
+// What 8-bit pages have to satisfy beside that (bf16: pages of xb_paged_kv, no exponents).
+int check_codes(const xb_paged_kv8* kv, bool bf16_too, const char* what, char* err, size_t errlen) {
+  if (kv->dtype == XB_DT_BF16 && bf16_too) return XB_OK;
+  if (kv->dtype != XB_DT_I8 && kv->dtype != XB_DT_F8E4M3) {
+    set_err(err, errlen, "%s: unsupported dtype code %lld of the pages", what, (long long)kv->dtype);
+    return XB_ERR_UNSUPPORTED;
+  }
+  const int64_t lds[6] = {kv->kv.k_page, kv->kv.k_head, kv->kv.k_row, kv->kv.v_page, kv->kv.v_head, kv->kv.v_row};
+  for (int64_t ld : lds)
+    if (ld % 16) {
+      set_err(err, errlen, "%s: 8-bit page strides must be multiples of 16 elements", what);
+      return XB_ERR_UNSUPPORTED;
+    }
+  const int64_t es[4] = {kv->ks_page, kv->ks_head, kv->vs_page, kv->vs_head};
+  for (int64_t ld : es)
+    if (ld <= 0 || ld % 8 || ld >= (1LL << 38)) {
+      set_err(err, errlen, "%s: exponent strides must be positive multiples of 8", what);
+      return XB_ERR_UNSUPPORTED;
+    }
+  return XB_OK;
+}
+
+int check_exponent_pointers(const xb_paged_kv8* kv, const char* what, char* err, size_t errlen) {
+  if (!kv->k_scale || !kv->v_scale) {
+    set_err(err, errlen, "%s: null pointer", what);
+    return XB_ERR_INVALID;
+  }
+  if ((reinterpret_cast<uintptr_t>(kv->k_scale) | reinterpret_cast<uintptr_t>(kv->v_scale)) & 7) {
+    set_err(err, errlen, "%s: exponents must be 8-byte aligned", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  return XB_OK;
+}
+
 // Which attention kernel: the mma.sync one while the batch's rows per (sequence,
 // KV head) fill at most one of its 16-row tiles on average; the host knows
 // this much without the lengths.  Few-row / tcgen05 kernel, us in a graph, 14
@@ -1678,11 +1864,12 @@ extern "C" int xb_copy_pages(void* pages, int64_t outer, int64_t outer_bytes, in
   return check_launch(what, err, errlen);
 }
 
-extern "C" int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t, const float* sin_t, void* q_out,
-                                     const xb_paged_kv* kv, int64_t tokens, int64_t n_head, int64_t rope_rows,
-                                     int64_t ld_qkv, int64_t ld_q, void* stream, char* err, size_t errlen) {
-  const char* what = "xb_paged_rope_kv_bf16";
+// xb_paged_rope_kv_bf16 and, with `q8`, xb_paged_rope_kv_q8.
+static int rope_kv(const char* what, const void* qkv, const float* cos_t, const float* sin_t, void* q_out,
+                   const xb_paged_kv* kv, const xb_paged_kv8* q8, int64_t tokens, int64_t n_head, int64_t rope_rows,
+                   int64_t ld_qkv, int64_t ld_q, void* stream, char* err, size_t errlen) {
   int rc = check_pages(kv, what, err, errlen);
+  if (!rc && q8) rc = check_codes(q8, false, what, err, errlen);
   if (rc) return rc;
   if (tokens < 0 || n_head <= 0 || n_head > 65535) {
     set_err(err, errlen, "%s: bad shape", what);
@@ -1695,6 +1882,7 @@ extern "C" int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t, const 
   }
   if (tokens == 0 || kv->batch == 0) return XB_OK;
   rc = check_page_pointers(kv, what, err, errlen);
+  if (!rc && q8) rc = check_exponent_pointers(q8, what, err, errlen);
   if (rc) return rc;
   if (!qkv || !q_out || (!cos_t) != (!sin_t)) {
     set_err(err, errlen, "%s: null pointer", what);
@@ -1735,10 +1923,93 @@ extern "C" int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t, const 
   a.page_size = (int)kv->page_size;
   a.max_pages = (int)kv->max_pages;
   a.n_pages = (int)kv->n_pages;
+  a.ke = q8 ? Exponents{q8->k_scale, q8->ks_page, q8->ks_head} : Exponents{};
+  a.ve = q8 ? Exponents{q8->v_scale, q8->vs_page, q8->vs_head} : Exponents{};
   int *bad = nullptr, *status = nullptr;
   rc = status_words(&bad, &status, what, err, errlen);
   if (rc) return rc;
-  launch_k<false>(paged_rope_kv_kernel, (unsigned)((tokens + 1) / 2), 64, 0, (cudaStream_t)stream, a, bad);
+  auto kernel = !q8 ? paged_rope_kv_kernel<kBf16>
+                    : q8->dtype == XB_DT_I8 ? paged_rope_kv_kernel<kInt8> : paged_rope_kv_kernel<kE4m3>;
+  launch_k<false>(kernel, (unsigned)((tokens + 1) / 2), 64, 0, (cudaStream_t)stream, a, bad);
+  return check_launch(what, err, errlen);
+}
+
+extern "C" int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t, const float* sin_t, void* q_out,
+                                     const xb_paged_kv* kv, int64_t tokens, int64_t n_head, int64_t rope_rows,
+                                     int64_t ld_qkv, int64_t ld_q, void* stream, char* err, size_t errlen) {
+  return rope_kv("xb_paged_rope_kv_bf16", qkv, cos_t, sin_t, q_out, kv, nullptr, tokens, n_head, rope_rows, ld_qkv,
+                 ld_q, stream, err, errlen);
+}
+
+extern "C" int xb_paged_rope_kv_q8(const void* qkv, const float* cos_t, const float* sin_t, void* q_out,
+                                   const xb_paged_kv8* kv, int64_t tokens, int64_t n_head, int64_t rope_rows,
+                                   int64_t ld_qkv, int64_t ld_q, void* stream, char* err, size_t errlen) {
+  return rope_kv("xb_paged_rope_kv_q8", qkv, cos_t, sin_t, q_out, kv ? &kv->kv : nullptr, kv, tokens, n_head,
+                 rope_rows, ld_qkv, ld_q, stream, err, errlen);
+}
+
+extern "C" int xb_paged_read_kv(void* k_out, void* v_out, const xb_paged_kv8* kv8, int64_t tokens, int64_t ld_k,
+                                int64_t ld_v, void* stream, char* err, size_t errlen) {
+  const char* what = "xb_paged_read_kv";
+  const xb_paged_kv* kv = kv8 ? &kv8->kv : nullptr;
+  int rc = check_pages(kv, what, err, errlen);
+  if (!rc) rc = check_codes(kv8, true, what, err, errlen);
+  if (rc) return rc;
+  const int64_t row = kv->n_kv_head * kv->head_dim;
+  if (tokens < 0) {
+    set_err(err, errlen, "%s: bad shape", what);
+    return XB_ERR_INVALID;
+  }
+  if (kv->head_dim % 8 || kv->head_dim > 65536) {
+    set_err(err, errlen, "%s: head_dim %lld is not a multiple of 8 up to 65536", what, (long long)kv->head_dim);
+    return XB_ERR_UNSUPPORTED;
+  }
+  if (tokens == 0 || kv->batch == 0) return XB_OK;
+  rc = check_page_pointers(kv, what, err, errlen);
+  if (!rc && kv8->dtype != XB_DT_BF16) rc = check_exponent_pointers(kv8, what, err, errlen);
+  if (rc) return rc;
+  if (!k_out || !v_out) {
+    set_err(err, errlen, "%s: null pointer", what);
+    return XB_ERR_INVALID;
+  }
+  if (ld_k < row || ld_v < row) {
+    set_err(err, errlen, "%s: row pitch shorter than the row", what);
+    return XB_ERR_INVALID;
+  }
+  if (!aligned16(k_out) || !aligned16(v_out) || ld_k % 8 || ld_v % 8) {
+    set_err(err, errlen, "%s: rows must be whole 16-byte vectors", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  if (tokens > 0x7ffffff0LL || 2 * row / 8 > 0x7fffffe0LL) {
+    set_err(err, errlen, "%s: too many tokens or heads", what);
+    return XB_ERR_UNSUPPORTED;
+  }
+  ReadArgs a;
+  a.k_out = static_cast<bf16*>(k_out);
+  a.v_out = static_cast<bf16*>(v_out);
+  a.k = Pages{static_cast<bf16*>(kv->k_pages), kv->k_page, kv->k_head, kv->k_row};
+  a.v = Pages{static_cast<bf16*>(kv->v_pages), kv->v_page, kv->v_head, kv->v_row};
+  a.ke = Exponents{kv8->k_scale, kv8->ks_page, kv8->ks_head};
+  a.ve = Exponents{kv8->v_scale, kv8->vs_page, kv8->vs_head};
+  a.table = kv->page_table;
+  a.q_start = kv->q_start;
+  a.kv_len = kv->kv_len;
+  a.ld_k = ld_k;
+  a.ld_v = ld_v;
+  a.ld_table = kv->ld_table;
+  a.T = (int)tokens;
+  a.B = (int)kv->batch;
+  a.KVH = (int)kv->n_kv_head;
+  a.D = (int)kv->head_dim;
+  a.page_size = (int)kv->page_size;
+  a.max_pages = (int)kv->max_pages;
+  a.n_pages = (int)kv->n_pages;
+  int *bad = nullptr, *status = nullptr;
+  rc = status_words(&bad, &status, what, err, errlen);
+  if (rc) return rc;
+  auto kernel = kv8->dtype == XB_DT_BF16 ? paged_read_kv_kernel<kBf16>
+                : kv8->dtype == XB_DT_I8 ? paged_read_kv_kernel<kInt8> : paged_read_kv_kernel<kE4m3>;
+  launch_k<false>(kernel, (unsigned)((tokens + 7) / 8), 256, 0, (cudaStream_t)stream, a, bad);
   return check_launch(what, err, errlen);
 }
 
@@ -1756,14 +2027,10 @@ extern "C" int xb_paged_attention_workspace_size(int64_t tokens, int64_t batch, 
   return XB_OK;
 }
 
-extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_kv* kv, int64_t tokens,
-                                       int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
-                                       size_t workspace_bytes, void* stream, char* err, size_t errlen) {
-  const char* what = "xb_paged_attention_bf16";
-  int rc = check_pages(kv, what, err, errlen);
-  if (rc) return rc;
-  const int64_t n_kv_head = kv->n_kv_head, batch = kv->batch, n_pages = kv->n_pages, page_size = kv->page_size;
-  if (tokens < 0 || n_head <= 0 || n_head % n_kv_head || n_head > 65535) {
+// Arguments of an attention call: sizes, then, once there is work, rows and workspace.
+static int check_attention(const xb_paged_kv* kv, int64_t tokens, int64_t n_head, float scale, const char* what,
+                           char* err, size_t errlen) {
+  if (tokens < 0 || n_head <= 0 || n_head % kv->n_kv_head || n_head > 65535) {
     set_err(err, errlen, "%s: bad shape", what);
     return XB_ERR_INVALID;
   }
@@ -1771,20 +2038,21 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
     set_err(err, errlen, "%s: head_dim %lld not supported (64)", what, (long long)kv->head_dim);
     return XB_ERR_UNSUPPORTED;
   }
-  if (n_head / n_kv_head > kTcRows) {
+  if (n_head / kv->n_kv_head > kTcRows) {
     set_err(err, errlen, "%s: %lld query heads per KV head not supported (1..128)", what,
-            (long long)(n_head / n_kv_head));
+            (long long)(n_head / kv->n_kv_head));
     return XB_ERR_UNSUPPORTED;
   }
-  const int n_rep = (int)(n_head / n_kv_head);
   const float scale_log2 = scale * 1.4426950408889634f;
   if (!(scale_log2 > 0.0f && scale_log2 < INFINITY)) {
     set_err(err, errlen, "%s: the scale must be positive and, times log2(e), finite", what);
     return XB_ERR_INVALID;
   }
-  if (tokens == 0 || batch == 0) return XB_OK;
-  rc = check_page_pointers(kv, what, err, errlen);
-  if (rc) return rc;
+  return XB_OK;
+}
+
+static int check_attention_rows(const void* q, const void* out, int64_t tokens, int64_t n_head, int64_t ld_q,
+                                int64_t ld_out, const char* what, char* err, size_t errlen) {
   if (!q || !out) {
     set_err(err, errlen, "%s: null pointer", what);
     return XB_ERR_INVALID;
@@ -1801,14 +2069,33 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
     set_err(err, errlen, "%s: too many tokens, or too long a row pitch", what);
     return XB_ERR_UNSUPPORTED;
   }
-  size_t need = 0;
-  rc = xb_paged_attention_workspace_size(tokens, batch, n_head, n_kv_head, &need, err, errlen);
+  return XB_OK;
+}
+
+static int check_workspace(const void* workspace, size_t bytes, size_t need, const char* what, char* err,
+                           size_t errlen) {
+  if (workspace && bytes >= need && aligned16(workspace)) return XB_OK;
+  set_err(err, errlen, "%s: needs a 16-byte aligned workspace of %zu bytes (%zu given)", what, need, bytes);
+  return XB_ERR_INVALID;
+}
+
+extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_kv* kv, int64_t tokens,
+                                       int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
+                                       size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  const char* what = "xb_paged_attention_bf16";
+  int rc = check_pages(kv, what, err, errlen);
+  if (!rc) rc = check_attention(kv, tokens, n_head, scale, what, err, errlen);
   if (rc) return rc;
-  if (!workspace || workspace_bytes < need || !aligned16(workspace)) {
-    set_err(err, errlen, "%s: needs a 16-byte aligned workspace of %zu bytes (%zu given)", what, need,
-            workspace_bytes);
-    return XB_ERR_INVALID;
-  }
+  const int64_t n_kv_head = kv->n_kv_head, batch = kv->batch, n_pages = kv->n_pages, page_size = kv->page_size;
+  const int n_rep = (int)(n_head / n_kv_head);
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (tokens == 0 || batch == 0) return XB_OK;
+  rc = check_page_pointers(kv, what, err, errlen);
+  if (!rc) rc = check_attention_rows(q, out, tokens, n_head, ld_q, ld_out, what, err, errlen);
+  size_t need = 0;
+  if (!rc) rc = xb_paged_attention_workspace_size(tokens, batch, n_head, n_kv_head, &need, err, errlen);
+  if (!rc) rc = check_workspace(workspace, workspace_bytes, need, what, err, errlen);
+  if (rc) return rc;
   AttnArgs a;
   a.q = static_cast<const bf16*>(q);
   a.out = static_cast<bf16*>(out);
@@ -1878,6 +2165,105 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
     return XB_ERR_CUDA;
   }
   return check_launch(what, err, errlen);
+}
+
+// Where an 8-bit call's pages go as bf16: a slot for each table entry, or for
+// each page of the pool where that is less.
+static int64_t expand_slots(int64_t batch, int64_t max_pages, int64_t n_pages, bool* compact) {
+  *compact = batch <= n_pages / max_pages;
+  return *compact ? batch * max_pages : n_pages;
+}
+
+static int64_t up(int64_t bytes) { return (bytes + 255) & ~255LL; }
+
+extern "C" int xb_paged_attention_q8_workspace_size(int64_t tokens, int64_t batch, int64_t n_head, int64_t n_kv_head,
+                                                    int64_t n_pages, int64_t page_size, int64_t max_pages,
+                                                    size_t* bytes, char* err, size_t errlen) {
+  const char* what = "xb_paged_attention_q8_workspace_size";
+  size_t own = 0;
+  int rc = xb_paged_attention_workspace_size(tokens, batch, n_head, n_kv_head, &own, err, errlen);
+  if (rc) return rc;
+  if (!bytes || n_pages <= 0 || page_size <= 0 || max_pages <= 0 || n_pages > 0x7fffffffLL ||
+      page_size > 0x7fffffffLL || max_pages > 0x7fffffffLL || batch > (1LL << 20) || n_kv_head > 65535) {
+    set_err(err, errlen, "%s: bad arguments", what);
+    return XB_ERR_INVALID;
+  }
+  bool compact;
+  const int64_t slots = expand_slots(batch, max_pages, n_pages, &compact);
+  const double all = (double)slots * n_kv_head * page_size * kHD * 4;
+  if (all > 1e15) {
+    set_err(err, errlen, "%s: %.3g bytes of pages are too many", what, all);
+    return XB_ERR_UNSUPPORTED;
+  }
+  *bytes = (size_t)(up((int64_t)own) + up(batch * max_pages * 4) + slots * n_kv_head * page_size * kHD * 4);
+  return XB_OK;
+}
+
+extern "C" int xb_paged_attention_q8(const void* q, void* out, const xb_paged_kv8* kv8, int64_t tokens, int64_t n_head,
+                                     int64_t ld_q, int64_t ld_out, float scale, void* workspace,
+                                     size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  const char* what = "xb_paged_attention_q8";
+  const xb_paged_kv* kv = kv8 ? &kv8->kv : nullptr;
+  int rc = check_pages(kv, what, err, errlen);
+  if (!rc) rc = check_codes(kv8, false, what, err, errlen);
+  if (!rc) rc = check_attention(kv, tokens, n_head, scale, what, err, errlen);
+  if (rc) return rc;
+  if (tokens == 0 || kv->batch == 0) return XB_OK;
+  rc = check_page_pointers(kv, what, err, errlen);
+  if (!rc) rc = check_exponent_pointers(kv8, what, err, errlen);
+  if (!rc) rc = check_attention_rows(q, out, tokens, n_head, ld_q, ld_out, what, err, errlen);
+  size_t need = 0, own = 0;
+  if (!rc)
+    rc = xb_paged_attention_q8_workspace_size(tokens, kv->batch, n_head, kv->n_kv_head, kv->n_pages, kv->page_size,
+                                              kv->max_pages, &need, err, errlen);
+  if (!rc) rc = xb_paged_attention_workspace_size(tokens, kv->batch, n_head, kv->n_kv_head, &own, err, errlen);
+  if (!rc) rc = check_workspace(workspace, workspace_bytes, need, what, err, errlen);
+  if (rc) return rc;
+  ExpandArgs e;
+  bool compact;
+  const int64_t slots = expand_slots(kv->batch, kv->max_pages, kv->n_pages, &compact);
+  const int64_t half = slots * kv->n_kv_head * kv->page_size * kHD;  // elements of K, and of V
+  uint8_t* at = static_cast<uint8_t*>(workspace) + up((int64_t)own);
+  e.slots = reinterpret_cast<int32_t*>(at);
+  e.k_out = reinterpret_cast<bf16*>(at + up(kv->batch * kv->max_pages * 4));
+  e.v_out = e.k_out + half;
+  e.k = Pages{static_cast<bf16*>(kv->k_pages), kv->k_page, kv->k_head, kv->k_row};
+  e.v = Pages{static_cast<bf16*>(kv->v_pages), kv->v_page, kv->v_head, kv->v_row};
+  e.ke = Exponents{kv8->k_scale, kv8->ks_page, kv8->ks_head};
+  e.ve = Exponents{kv8->v_scale, kv8->vs_page, kv8->vs_head};
+  e.table = kv->page_table;
+  e.q_start = kv->q_start;
+  e.kv_len = kv->kv_len;
+  e.ld_table = kv->ld_table;
+  e.T = (int)tokens;
+  e.B = (int)kv->batch;
+  e.KVH = (int)kv->n_kv_head;
+  e.page_size = (int)kv->page_size;
+  e.max_pages = (int)kv->max_pages;
+  e.n_pages = (int)kv->n_pages;
+  e.compact = compact;
+  int sms = 148;
+  xb::sm_count(&sms);
+  // CTAs of 8 warps for each sequence: as many as its longest could use, 8 per SM over all of them
+  const int64_t most = (kv->max_pages * kv->page_size / 8 * kv->n_kv_head + 7) / 8;
+  const int64_t rows = kv->batch < 65535 ? kv->batch : 65535;
+  int64_t x = (8 * sms + rows - 1) / rows;
+  x = x < most ? x : most;
+  launch_k<false>(kv8->dtype == XB_DT_I8 ? paged_expand_kernel<kInt8> : paged_expand_kernel<kE4m3>,
+                  dim3((unsigned)x, (unsigned)rows), 256, 0, (cudaStream_t)stream, e);
+  rc = check_launch(what, err, errlen);
+  if (rc) return rc;
+  xb_paged_kv wide = *kv;
+  wide.k_pages = e.k_out;
+  wide.v_pages = e.v_out;
+  wide.page_table = e.slots;
+  wide.n_pages = slots;
+  wide.ld_table = kv->max_pages;
+  wide.k_row = wide.v_row = kHD;
+  wide.k_head = wide.v_head = kv->page_size * kHD;
+  wide.k_page = wide.v_page = kv->n_kv_head * kv->page_size * kHD;
+  return xb_paged_attention_bf16(q, out, &wide, tokens, n_head, ld_q, ld_out, scale, workspace, own, stream, err,
+                                 errlen);
 }
 
 extern "C" int xb_page_status(void* stream, int* status, char* err, size_t errlen) {

@@ -32,7 +32,7 @@ XB_ERR_CUDA = -2
 XB_ERR_UNSUPPORTED = -3
 XB_ERR_TIMEOUT = -4
 
-XB_DT_BF16, XB_DT_F32, XB_DT_I8, XB_DT_I16, XB_DT_I32 = 0, 1, 2, 3, 4
+XB_DT_BF16, XB_DT_F32, XB_DT_I8, XB_DT_I16, XB_DT_I32, XB_DT_F8E4M3 = 0, 1, 2, 3, 4, 5
 
 _ERR_NAMES = {
     XB_ERR_INVALID: "XB_ERR_INVALID",
@@ -67,6 +67,7 @@ _CTYPES = {
     "uint32_t": ctypes.c_uint32,
     # a packed xb_paged_kv (ops.py): bytes are passed by address
     "const xb_paged_kv*": ctypes.c_void_p,
+    "const xb_paged_kv8*": ctypes.c_void_p,  # the same with exponents
     # an array of DecodePhase (ops.py), passed by address
     "const xb_decode_phase*": ctypes.c_void_p,
 }

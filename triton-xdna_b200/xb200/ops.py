@@ -1024,6 +1024,43 @@ def argmax(x, out=None):
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _beam_select_bytes(dev, G, K, V, N) -> int:
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(dev):
+        _lib.call("xb_beam_select_workspace_size", G, K, V, N, ctypes.byref(need))
+    return need.value
+
+
+def beam_select(logits, scores, count):
+    """A beam search step's choice: logits [G * K, V] (fp32 or bf16) of G groups
+    of K beams and their scores [G, K] (fp32); of each group's beams k and
+    tokens v the `count` largest scores[k] + log_softmax(logits[k])[v], largest
+    first, equal ones by the lowest (k, v).  Returns (values [G, count] fp32,
+    parents int64, tokens int64); a beam whose score is -inf is out, and places
+    for which no continuation is left hold -inf, -1, -1."""
+    dev = _device_of(logits, scores)
+    dt = DT.get(logits.dtype)
+    if logits.dtype not in FLOAT_DTYPES or scores.dtype is not torch.float32:
+        raise TypeError("beam_select takes bf16 or fp32 logits and fp32 scores")
+    if logits.dim() != 2 or scores.dim() != 2 or logits.shape[0] != scores.numel():
+        raise ValueError("G groups of K beams have logits [G * K, V] and scores [G, K]")
+    G, K = scores.shape
+    V = logits.shape[1]
+    count = int(count)
+    if (logits.stride(1) != 1 and V > 1) or (scores.stride(1) != 1 and K > 1):
+        raise ValueError("the rows of logits and scores must be contiguous")
+    values = torch.empty((G, count) if count > 0 else (0,), dtype=torch.float32, device=logits.device)
+    parents = torch.empty(values.shape, dtype=torch.int64, device=logits.device)
+    tokens = torch.empty_like(parents)
+    # the call's own, as in paged_attention
+    ws = torch.empty(_beam_select_bytes(dev, G, K, V, count), dtype=torch.uint8, device=logits.device)
+    _call_on(dev, "xb_beam_select", logits.data_ptr(), scores.data_ptr(), G, K, V,
+             logits.stride(0) if G * K > 1 else V, scores.stride(0) if G > 1 else K, count, dt, values.data_ptr(),
+             parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel())
+    return values, parents, tokens
+
+
 # --------------------------------------------------------------------------- paged KV cache
 #
 # A step packs the new tokens of many sequences: tokens q_start[b] ..
@@ -1059,13 +1096,20 @@ def _call_on(dev: int, name: str, *args) -> None:
 
 
 _PAGED_KV = struct.Struct("5P13q").pack  # xb_paged_kv of include/xb200.h
+_EXPONENTS = struct.Struct("2P5q").pack  # what xb_paged_kv8 has behind it
+_CODES = {torch.int8: 2, torch.float8_e4m3fn: 5}
 
 
-def _page_args(k_pages, v_pages, page_table, q_start, kv_len):
+def _page_args(k_pages, v_pages, page_table, q_start, kv_len, k_scale=None, v_scale=None):
     """Checks what the host can see of a paged batch: (n_kv_head, head_dim,
-    batch, the C struct xb_paged_kv as bytes)."""
-    if k_pages.dtype is not torch.bfloat16 or v_pages.dtype is not torch.bfloat16:
-        raise TypeError("k_pages and v_pages must be bf16")
+    batch, the C struct as bytes: xb_paged_kv for bf16 pages, xb_paged_kv8 for
+    8-bit ones)."""
+    dtype = k_pages.dtype
+    coded = dtype is not torch.bfloat16
+    if dtype is not v_pages.dtype or (coded and dtype not in _CODES):
+        raise TypeError("k_pages and v_pages must both be bf16, int8 or float8_e4m3fn")
+    if coded != (k_scale is not None) or coded != (v_scale is not None):
+        raise ValueError("8-bit pages come with k_scale and v_scale, bf16 pages without")
     if page_table.dtype is not torch.int32 or q_start.dtype is not torch.int32 or kv_len.dtype is not torch.int32:
         raise TypeError("page_table, q_start and kv_len must be int32")
     shape = k_pages.shape
@@ -1090,8 +1134,19 @@ def _page_args(k_pages, v_pages, page_table, q_start, kv_len):
         k0, v0 = (any_, any_) if n == 1 else (k0, v0)
         k1, v1 = (any_, any_) if h == 1 else (k1, v1)
         k2, v2 = (any_, any_) if p == 1 else (k2, v2)
+    tail = b""
+    if coded:
+        strides = []
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t.dtype is not torch.uint8 or t.shape != (n, h, p):
+                raise ValueError(f"{name} must be uint8 [n_pages, n_kv_head, page_size] = {[n, h, p]}")
+            e0, e1, e2 = t.stride()
+            if e2 != 1 and p > 1:
+                raise ValueError(f"the rows of {name} must be contiguous")
+            strides += [h * p if n == 1 else e0, p if h == 1 else e1]
+        tail = _EXPONENTS(k_scale.data_ptr(), v_scale.data_ptr(), *strides, _CODES[dtype])
     return h, d, B, _PAGED_KV(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), q_start.data_ptr(),
-                              kv_len.data_ptr(), n, h, p, d, B, cols, ld if B > 1 else cols, k0, k1, k2, v0, v1, v2)
+                              kv_len.data_ptr(), n, h, p, d, B, cols, ld if B > 1 else cols, k0, k1, k2, v0, v1, v2) + tail
 
 
 def _token_rows(t, name, tokens, row) -> int:
@@ -1119,16 +1174,21 @@ def _apart(p, ld_p, row_p, q, ld_q, row_q, tokens, what) -> None:
     raise ValueError(f"{what} must not share memory")
 
 
-def paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len):
+def paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale=None,
+                  v_scale=None):
     """RoPE of the packed QKV projection [T, (H + 2 KVH) * D] (none when the
     tables are None) into q_out [T, H, D], and the write of its keys and values
     into the pages at their positions: rope_kv() for a paged cache, the same
     bits.  Tokens outside the sequences are left alone; page_status() tells of
-    positions without a page or table row."""
-    dev = _device_of(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len)
+    positions without a page or table row.
+
+    8-bit pages (int8 or float8_e4m3fn, with k_scale and v_scale): the same bf16
+    numbers are written as codes, with one exponent byte a position and KV head
+    (include/xb200.h has the arithmetic)."""
+    dev = _device_of(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
     if (cos_t is None) != (sin_t is None):
         raise ValueError("give both RoPE tables or neither")
-    KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
+    KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
     if q_out.dim() != 3 or q_out.shape[2] != D:
         raise ValueError(f"q_out must be [tokens, n_head, {D}]")
     T, H, _ = q_out.shape
@@ -1144,8 +1204,28 @@ def paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_star
     ld_qkv, ld_q = _token_rows(qkv, "qkv", T, row), _token_rows(q_out, "q_out", T, H * D)
     px, pq = qkv.data_ptr(), q_out.data_ptr()
     _apart(px, ld_qkv, row, pq, ld_q, H * D, T, "qkv and q_out")
-    _call_on(dev, "xb_paged_rope_kv_bf16", px, cos, sin, pq, kv, T, H, rows, ld_qkv, ld_q)
+    _call_on(dev, "xb_paged_rope_kv_bf16" if k_scale is None else "xb_paged_rope_kv_q8", px, cos, sin, pq, kv, T, H,
+             rows, ld_qkv, ld_q)
     return q_out
+
+
+def paged_read_kv(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale=None, v_scale=None):
+    """k_out, v_out [T, KVH, D] (or [T, KVH * D]) bf16: what the pages hold at the
+    positions of the packed tokens, the inverse of paged_rope_kv's write (with
+    q_start counting every position of the sequences, all they hold).  bf16 and
+    8-bit pages; what a code stands for is a bf16 number, so nothing is
+    rounded.  Tokens outside the sequences are left alone; one without a page
+    reads as zeros (page_status())."""
+    dev = _device_of(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
+    KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
+    if k_scale is None:
+        kv += _EXPONENTS(0, 0, 0, 0, 0, 0, 0)
+    T, row = k_out.shape[0] if k_out.dim() else 0, KVH * D
+    ld_k, ld_v = _token_rows(k_out, "k_out", T, row), _token_rows(v_out, "v_out", T, row)
+    pk, pv = k_out.data_ptr(), v_out.data_ptr()
+    _apart(pk, ld_k, row, pv, ld_v, row, T, "k_out and v_out")
+    _call_on(dev, "xb_paged_read_kv", pk, pv, kv, T, ld_k, ld_v)
+    return k_out, v_out
 
 
 @functools.lru_cache(maxsize=256)
@@ -1156,14 +1236,25 @@ def _paged_attention_bytes(dev, T, B, H, KVH) -> int:
     return need.value
 
 
-def paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale):
+@functools.lru_cache(maxsize=256)
+def _paged_attention_q8_bytes(dev, T, B, H, KVH, n_pages, page_size, max_pages) -> int:
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(dev):
+        _lib.call("xb_paged_attention_q8_workspace_size", T, B, H, KVH, n_pages, page_size, max_pages,
+                  ctypes.byref(need))
+    return need.value
+
+
+def paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale, k_scale=None, v_scale=None):
     """Causal GQA attention of packed new tokens over a paged cache: q [T, H,
     64], out [T, H * 64] (or [T, H, 64]); the token at position p of its
     sequence sees keys 0 .. p.  attention() for sequences of different lengths,
     from single tokens to whole prompts in one batch.  Rows outside the
-    sequences are left as they are; a token that sees no key gets zeros."""
-    dev = _device_of(q, k_pages, v_pages, out, page_table, q_start, kv_len)
-    KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len)
+    sequences are left as they are; a token that sees no key gets zeros.
+    8-bit pages (int8 or float8_e4m3fn, with k_scale and v_scale): the attention
+    over what the codes stand for."""
+    dev = _device_of(q, k_pages, v_pages, out, page_table, q_start, kv_len, k_scale, v_scale)
+    KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
     if q.dim() != 3 or q.shape[2] != D:
         raise ValueError(f"q must be [tokens, n_head, {D}]")
     T, H, _ = q.shape
@@ -1173,8 +1264,13 @@ def paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale
     _apart(pq, ld_q, row, po, ld_out, row, T, "q and out")
     # of this call alone: the caching allocator orders its reuse on the stream,
     # and a captured graph keeps its own
-    ws = torch.empty(_paged_attention_bytes(dev, T, B, H, KVH), dtype=torch.uint8, device=q.device)
-    _call_on(dev, "xb_paged_attention_bf16", pq, po, kv, T, H, ld_q, ld_out, float(scale), ws.data_ptr(), ws.numel())
+    if k_scale is None:
+        name, need = "xb_paged_attention_bf16", _paged_attention_bytes(dev, T, B, H, KVH)
+    else:
+        name = "xb_paged_attention_q8"
+        need = _paged_attention_q8_bytes(dev, T, B, H, KVH, k_pages.shape[0], k_pages.shape[2], page_table.shape[1])
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _call_on(dev, name, pq, po, kv, T, H, ld_q, ld_out, float(scale), ws.data_ptr(), ws.numel())
     return out
 
 
