@@ -384,6 +384,7 @@ struct AttnArgs : Line {
   uint32_t rep_magic;  // ceil(2^16 / n_rep)
   float scale_log2;
   int *bad, *status;
+  Exponents ke, ve;  // 8-bit pages only
 };
 
 // What the joining kernel needs of CTA c: the unit that starts in c and goes on, and the CTA it ends in.
@@ -477,13 +478,16 @@ constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared m
 // Warps x buffers of the 8-row kernel, 64 sequences of 576 keys / 160 long ones:
 // 8 x 2 11.0 / 86.1 us, 8 x 3 11.0 / 90.2, 12 x 2 12.1 / 87.4, 16 x 1 13.1 / 86.5,
 // 12 x 1 12.3 / 85.8, 8 x 1 11.1 / 93.8, 6 x 3 11.3 / 91.7, 4 x 4 12.6 / 116.
-template <int ROWS>
+template <int ROWS, Format F>
 struct FewCfg {
   static constexpr int kWarps = kFewWarps, kBufs = 2;
   static constexpr int kThreads = kWarps * 32;
+  static constexpr int kTile = F == kBf16 ? kTK : kFewTK8;       // keys
+  static constexpr int kRowBytes = F == kBf16 ? kHD * 2 : kHD;
   static constexpr int kRing = kBufs * 2 * kTileBytes;  // of one warp
   static constexpr int kHead = ROWS * kPartLd * 4;      // a warp's kind 0 partial; kind 1 goes into its own ring
   static constexpr int kSmem = kWarps * (kRing + kHead) + 1024;
+  static_assert(kTile * kRowBytes == kTileBytes, "a tile");
   static_assert(kHead <= kRing && kSmem <= 224 * 1024, "shared memory");
 };
 
@@ -512,6 +516,58 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_16816_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 8 bytes (zeros where !ok) into shared memory, without a wait
+__device__ __forceinline__ void copy8_async(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
+}
+// An arrival on `bar` once this thread's copies so far have landed (counted at the barrier's set-up)
+__device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Codes in a 32-bit register as fp16 pairs: bytes (0, 1) and (2, 3) ...
+template <Format F>
+__device__ __forceinline__ void halves_side_by_side(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  if constexpr (F == kInt8) {
+    v ^= 0x80808080u;
+    lo = int8x2_to_half2(v, 0x4140);
+    hi = int8x2_to_half2(v, 0x4342);
+  } else {
+    lo = e4m3x2_to_half2((uint16_t)v);
+    hi = e4m3x2_to_half2((uint16_t)(v >> 16));
+  }
+}
+// ... or (0, 2) and (1, 3)
+template <Format F>
+__device__ __forceinline__ void halves_across(uint32_t v, uint32_t& even, uint32_t& odd) {
+  if constexpr (F == kInt8) {
+    v ^= 0x80808080u;
+    even = int8x2_to_half2(v, 0x4240);
+    odd = int8x2_to_half2(v, 0x4341);
+  } else {
+    v = __byte_perm(v, 0, 0x3120);
+    even = e4m3x2_to_half2((uint16_t)v);
+    odd = e4m3x2_to_half2((uint16_t)(v >> 16));
+  }
+}
+
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -551,11 +607,12 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int token, int kvh
   *reinterpret_cast<uint2*>(op) = pk;
 }
 
-template <int ROWS, typename I>
-__global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kernel(const __grid_constant__ KvMaps maps,
+template <int ROWS, typename I, Format F>
+__global__ void __launch_bounds__(FewCfg<ROWS, F>::kThreads, 1) paged_attn_few_kernel(const __grid_constant__ KvMaps maps,
                                                                         const AttnArgs a) {
-  using C = FewCfg<ROWS>;
-  constexpr int kWarps = C::kWarps, kBufs = C::kBufs;
+  using C = FewCfg<ROWS, F>;
+  constexpr bool kCoded = F != kBf16;
+  constexpr int kWarps = C::kWarps, kBufs = C::kBufs, TK = C::kTile, MT = TK / 16;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kWarps][kBufs];
   __shared__ I sums[2][kWarps];
@@ -566,6 +623,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
   __shared__ float part_m[2][kWarps][ROWS], part_l[2][kWarps][ROWS];
   __shared__ uint32_t comes, ends0, opens;  // one bit per warp: has a kind 0, its unit ends there, has a kind 1
   __shared__ Segment queue[kWarps][kQueue];
+  __shared__ __align__(16) uint8_t exps[kCoded ? kWarps : 1][kBufs][2][TK];  // exponent bytes of the tiles, K then V
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -579,7 +637,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
     return reinterpret_cast<float*>(kind == 0 ? smem + kWarps * C::kRing + w_ * C::kHead : smem + w_ * C::kRing);
   };
   if (lane == 0) {
-    for (int i = 0; i < kBufs; ++i) mbar_init(&full[warp][i], 1);
+    for (int i = 0; i < kBufs; ++i) mbar_init(&full[warp][i], kCoded ? 33 : 1);  // every lane's copies of exponents
     mbar_fence_init();
   }
   if (threadIdx.x == 0) {
@@ -630,16 +688,16 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
       win_id = p * (uint64_t)a.page_size < (uint32_t)si.keys ? __ldg(a.table + si.b * a.ld_table + p) : -1;
     };
     auto enter = [&]() {  // the first tile of a segment
-      pi = (uint32_t)(ni * kTK) / (uint32_t)a.page_size;
-      row = ni * kTK - (int)pi * a.page_size;
+      pi = (uint32_t)(ni * TK) / (uint32_t)a.page_size;
+      row = ni * TK - (int)pi * a.page_size;
       window(pi);
     };
     // page piece by page piece (a piece never crosses a page), in uniform registers
     auto request = [&]() {
       const uint32_t buf = issued % kBufs;
-      const int have = min(kTK, si.keys - ni * kTK);
+      const int have = min(TK, si.keys - ni * TK);
       const int nb = (have + a.box_rows - 1) / a.box_rows;
-      if (leader) mbar_arrive_expect_tx(&full[warp][buf], (uint32_t)(nb * a.box_rows * kHD * 2 * 2));
+      if (leader) mbar_arrive_expect_tx(&full[warp][buf], (uint32_t)(nb * a.box_rows * C::kRowBytes * 2));
       uint32_t dst = ring + buf * 2 * kTileBytes;
       for (int i = 0; i < nb; ++i) {
         if (pi - win >= 32u) window(pi);
@@ -652,19 +710,59 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
           tma_load_4d(dst, &maps.k, &full[warp][buf], 0, row, si.kvh, id);
           tma_load_4d(dst + kTileBytes, &maps.v, &full[warp][buf], 0, row, si.kvh, id);
         }
-        dst += a.box_rows * kHD * 2;
+        if constexpr (kCoded) {  // 8 positions a lane, K and V by turns
+          if (lane < a.box_rows / 4) {
+            const Exponents& ex = lane & 1 ? a.ve : a.ke;
+            const bool ok = id < a.n_pages;
+            const int at = (lane >> 1) * 8;
+            copy8_async(smem_u32(&exps[warp][buf][lane & 1][i * a.box_rows + at]),
+                        ex.p + (ok ? id * ex.page + si.kvh * ex.head + row + at : 0), ok);
+          }
+        }
+        dst += a.box_rows * C::kRowBytes;
         row += a.box_rows;
         if (row == a.page_size) {
           row = 0;
           ++pi;
         }
       }
+      if constexpr (kCoded) arrive_after_copies(&full[warp][buf]);
       __syncwarp();
       ++issued;
       ++ni;
     };
     uint32_t qb[NT][4][2];
+    float cq[NT][2];  // 8-bit pages: what turns a row's products into scores, in log2 units
     auto load_q = [&]() {
+      if constexpr (kCoded) {
+        // A dim's place in the product is K's: four in a row a lane.  As fp16, scaled by a power of two to magnitudes
+        // below 2^14: exact, but what is 2^-28 of a row's largest element.
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int r = 8 * n + g, tk = row_token(a, r);
+          const bf16* p = a.q + (int64_t)(sc.token + tk) * a.ld_q + (sc.kvh * a.n_rep + r - tk * a.n_rep) * kHD + 4 * t;
+          uint2 x[4];
+          uint32_t top = 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            x[c] = r < sc.rows ? *reinterpret_cast<const uint2*>(p + c * 16) : make_uint2(0, 0);
+            top = max(max(top, max(x[c].x & 0x7fffu, x[c].x >> 16 & 0x7fffu)),
+                      max(x[c].y & 0x7fffu, x[c].y >> 16 & 0x7fffu));
+          }
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int E = max((int)(top >> 7), 14);
+          const float mul = __int_as_float((267 - E) << 23), back = __int_as_float((E - 13) << 23);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            qb[n][c][0] = pack2_half(__uint_as_float(x[c].x << 16) * mul, __uint_as_float(x[c].x & 0xffff0000u) * mul);
+            qb[n][c][1] = pack2_half(__uint_as_float(x[c].y << 16) * mul, __uint_as_float(x[c].y & 0xffff0000u) * mul);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) cq[n][e] = a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
+        }
+        return;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int r = 8 * n + g, tk = row_token(a, r);
@@ -687,7 +785,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
           request();
         } else {
           if (pushed - popped == kQueue) break;
-          more_i = (fresh || next_unit(a, wi)) && segment<kTK>(a, wi, si);
+          more_i = (fresh || next_unit(a, wi)) && segment<TK>(a, wi, si);
           fresh = false;
           if (!more_i) break;
           if (lane == 0) queue[warp][pushed % kQueue] = si;
@@ -707,23 +805,41 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
           dead = true;
           break;
         }
-        const int k0 = tile * kTK;
+        const int k0 = tile * TK;
         const uint32_t sk = ring + buf * 2 * kTileBytes, sv = sk + kTileBytes;
-        const int have = min(kTK, sc.keys - k0);
-        if (have < kTK) {
+        const int have = min(TK, sc.keys - k0);
+        if (F != kInt8 && have < TK) {
           // values behind the last key hold whatever the page or buffer held: a
-          // NaN there would survive its zero weight
-          for (int i = have * 8 + lane; i < kTK * 8; i += 32)
+          // NaN there would survive its zero weight (int8 codes have none)
+          for (int i = have * (C::kRowBytes / 16) + lane; i < TK * (C::kRowBytes / 16); i += 32)
             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + i * 16), "r"(0) : "memory");
           fence_proxy_async_smem();  // before a later TMA write to the buffer
           __syncwarp();
         }
         // S^T = K Q^T: keys are the MMA's 16 rows, query rows its 8 columns
-        float s[NT][2][4];
+        float s[NT][MT][4];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
           for (int n = 0; n < NT; ++n) s[n][mt][0] = s[n][mt][1] = s[n][mt][2] = s[n][mt][3] = 0.0f;
+          if constexpr (kCoded) {
+            // 16-byte chunk c of row r at c ^ (r / 2 & 3).  A lane's 32 bits of a row are four dims in a row, two for
+            // either half of the 16 of a step.
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+              const int mi = lane >> 3, r = mt * 16 + (mi & 1) * 8 + (lane & 7), c = 2 * cc + (mi >> 1);
+              uint32_t x[4], ka[2][4];
+              ldsm4(x, sk + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) halves_side_by_side<F>(x[i], ka[i >> 1][i & 1], ka[i >> 1][2 + (i & 1)]);
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                  mma_16816_half(s[n][mt], ka[i], qb[n][2 * cc + i][0], qb[n][2 * cc + i][1]);
+            }
+            continue;
+          }
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
             const int mi = lane >> 3, r = mt * 16 + (mi & 1) * 8 + (lane & 7), c = 2 * kk + (mi >> 1);
@@ -733,9 +849,29 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
             for (int n = 0; n < NT; ++n) mma_16816(s[n][mt], ka, qb[n][kk][0], qb[n][kk][1]);
           }
         }
-        if (k0 + kTK - 1 > first_pos) {  // some row does not see the whole tile
+        // 8-bit pages: with K's exponent e_k and V's e_v a score is S c 2^e_k (c = cq), and e_v joins it: the weight
+        // 2^(score + e_v - m) of a code of V is at most one and fits fp16 whatever the values' sizes; times 2^-e_v
+        // it is the key's share of the denominator.
+        float fv[kCoded ? MT : 1][2];  // 2^-e_v
+        if constexpr (kCoded) {
+          const uint32_t at = smem_u32(&exps[warp][buf][0][g]);
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int bk = (int)lds_u8(at + mt * 16 + h * 8), bv = (int)lds_u8(at + TK + mt * 16 + h * 8);
+              const float kf = byte_scale(bk), ev = (float)(bv - 127);
+              fv[mt][h] = bv == kNanByte ? __int_as_float(0x7fc00000) : __int_as_float((254 - bv) << 23);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) s[n][mt][2 * h + e] = fmaf(s[n][mt][2 * h + e], kf * cq[n][e], ev);
+            }
+        }
+        const bool edge = k0 + TK - 1 > first_pos;
+        if (edge) {  // some row does not see the whole tile
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int key = k0 + mt * 16 + g + (e >> 1) * 8;
@@ -744,7 +880,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
                 if (key > pos[n][e & 1]) s[n][mt][e] = -INFINITY;
             }
         }
-        uint32_t pb[NT][4];  // P as the B operand of O^T = V^T P^T, 8 keys each
+        uint32_t pb[NT][2 * MT];  // P as the B operand of O^T = V^T P^T, 8 keys each
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float base[2], al[2];
@@ -754,8 +890,10 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
             // raw scores: the scale is positive, so their maximum scales to the scaled ones'
             float mx = fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2]));
 #pragma unroll
+            for (int mt = 2; mt < MT; ++mt) mx = fmaxf(mx, fmaxf(s[n][mt][e], s[n][mt][e + 2]));
+#pragma unroll
             for (int o_ = 4; o_ <= 16; o_ <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o_));
-            const float mn = fmaxf(m[n][e], mx * a.scale_log2);
+            const float mn = fmaxf(m[n][e], kCoded ? mx : mx * a.scale_log2);
             base[e] = mn == -INFINITY ? 0.0f : mn;
             al[e] = ex2_approx(m[n][e] - base[e]);
             moved |= mn > m[n][e];
@@ -772,8 +910,25 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
               o[n][mt][3] *= al[1];
             }
           }
+          if constexpr (kCoded) {
+            // up to 2^14, so that fp16 holds weights from 2^-38 of the largest on; numerator and denominator alike
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float w = ex2_approx(s[n][mt][e] - (base[e & 1] - 14.0f));
+                // an unseen key's exponent may be anything
+                const float f = edge && s[n][mt][e] == -INFINITY ? 0.0f : fv[mt][e >> 1];
+                l[n][e & 1] = fmaf(w, f, l[n][e & 1]);
+                s[n][mt][e] = w;
+              }
+              pb[n][2 * mt] = transpose8(pack2_half(s[n][mt][0], s[n][mt][1]));
+              pb[n][2 * mt + 1] = transpose8(pack2_half(s[n][mt][2], s[n][mt][3]));
+            }
+            continue;
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               s[n][mt][e] = ex2_approx(fmaf(s[n][mt][e], a.scale_log2, -base[e & 1]));
@@ -783,8 +938,28 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
             pb[n][2 * mt + 1] = transpose8(pack2(s[n][mt][2], s[n][mt][3]));
           }
         }
+        if constexpr (kCoded) {
+          // A lane's 32 bits are dims 2 g and 2 g + 1 of a chunk, keys 2 t and 2 t + 1: row g of the product is the even dim,
+          // row g + 8 the odd one.
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+          for (int ks = 0; ks < MT; ++ks)
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+              const int mi = lane >> 3, r = ks * 16 + (mi & 1) * 8 + (lane & 7), c = 2 * cc + (mi >> 1);
+              uint32_t x[4], va[2][4];
+              ldsm4_t(x, sv + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                halves_across<F>(x[i], va[i >> 1][2 * (i & 1)], va[i >> 1][2 * (i & 1) + 1]);
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                  mma_16816_half(o[n][2 * cc + i], va[i], pb[n][2 * ks], pb[n][2 * ks + 1]);
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < (kCoded ? 0 : 2); ++ks)
 #pragma unroll
           for (int mt = 0; mt < 4; ++mt) {  // dims 16 mt .. 16 mt + 15
             const int mi = lane >> 3, r = ks * 16 + (mi >> 1) * 8 + (lane & 7), c = 2 * mt + (mi & 1);
@@ -825,7 +1000,22 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int o_ = 4; o_ <= 16; o_ <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o_);
-      if (sc.starts && sc.ends) {
+      if (kCoded && sc.starts && sc.ends) {
+        // a thread has both dims of a pair
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float inv = l[n][e] == 0.0f ? 0.0f : 1.0f / l[n][e];  // no key: zeros
+            const int r = 8 * n + 2 * t + e, tk = tok[n][e];
+            bf16* p = a.out + (int64_t)(sc.token + tk) * a.ld_out + (sc.kvh * a.n_rep + r - tk * a.n_rep) * kHD + 2 * g;
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+              const uint32_t pk = pack2(o[n][mt][e] * inv, o[n][mt][e + 2] * inv);
+              if (r < sc.rows) *reinterpret_cast<uint32_t*>(p + mt * 16) = pk;
+            }
+          }
+      } else if (sc.starts && sc.ends) {
         // neighbours in g swap a row each, so that a thread stores two dims of one row
         const int odd = g & 1;
 #pragma unroll
@@ -854,8 +1044,8 @@ __global__ void __launch_bounds__(FewCfg<ROWS>::kThreads, 1) paged_attn_few_kern
             const int r = 8 * n + 2 * t + e;
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
-              po[r * kPartLd + mt * 16 + g] = o[n][mt][e];
-              po[r * kPartLd + mt * 16 + g + 8] = o[n][mt][e + 2];
+              po[r * kPartLd + mt * 16 + (kCoded ? 2 * g : g)] = o[n][mt][e];
+              po[r * kPartLd + mt * 16 + (kCoded ? 2 * g + 1 : g + 8)] = o[n][mt][e + 2];
             }
             if (g == 0) {
               part_m[kind][warp][r] = m[n][e];
@@ -1571,18 +1761,21 @@ EncodeTiledFn encoder() {
 }
 
 int page_map(CUtensorMap* map, const void* p, int64_t n_pages, int64_t heads, int64_t page_size, int64_t page_ld,
-             int64_t head_ld, int64_t row_ld, int box_rows, const char* what, char* err, size_t errlen) {
+             int64_t head_ld, int64_t row_ld, int box_rows, bool coded, const char* what, char* err,
+             size_t errlen) {
   EncodeTiledFn enc = encoder();
   if (!enc) {
     set_err(err, errlen, "%s: cuTensorMapEncodeTiled unavailable", what);
     return XB_ERR_CUDA;
   }
   cuuint64_t dims[4] = {(cuuint64_t)kHD, (cuuint64_t)page_size, (cuuint64_t)heads, (cuuint64_t)n_pages};
-  cuuint64_t strides[3] = {(cuuint64_t)row_ld * 2, (cuuint64_t)head_ld * 2, (cuuint64_t)page_ld * 2};
+  const cuuint64_t size = coded ? 1 : 2;
+  cuuint64_t strides[3] = {row_ld * size, head_ld * size, page_ld * size};
   cuuint32_t box[4] = {(cuuint32_t)kHD, (cuuint32_t)box_rows, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  CUresult r = enc(map, coded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                   const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   coded ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_err(err, errlen, "%s: cuTensorMapEncodeTiled failed (%d) for pages [%lld][%lld][%lld][64]", what, (int)r,
@@ -1759,10 +1952,15 @@ cudaError_t launch_main(void (*kernel)(M, AttnArgs), int ctas, int threads, int 
   return e != cudaSuccess ? e : launch_k(kernel, (unsigned)ctas, threads, smem, s, maps, a);
 }
 
-template <int ROWS, typename I>
+template <int ROWS, typename I, Format F>
 cudaError_t launch_few(int ctas, cudaStream_t s, const KvMaps& maps, const AttnArgs& a) {
-  using C = FewCfg<ROWS>;
-  return launch_main(paged_attn_few_kernel<ROWS, I>, ctas, C::kThreads, C::kSmem, s, maps, a);
+  using C = FewCfg<ROWS, F>;
+  return launch_main(paged_attn_few_kernel<ROWS, I, F>, ctas, C::kThreads, C::kSmem, s, maps, a);
+}
+template <Format F>
+cudaError_t launch_few(bool eight, bool wide, int ctas, cudaStream_t s, const KvMaps& maps, const AttnArgs& a) {
+  return eight ? (wide ? launch_few<8, int64_t, F>(ctas, s, maps, a) : launch_few<8, int, F>(ctas, s, maps, a))
+               : (wide ? launch_few<16, int64_t, F>(ctas, s, maps, a) : launch_few<16, int, F>(ctas, s, maps, a));
 }
 
 template <int N>
@@ -2079,10 +2277,10 @@ static int check_workspace(const void* workspace, size_t bytes, size_t need, con
   return XB_ERR_INVALID;
 }
 
-extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_kv* kv, int64_t tokens,
-                                       int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
-                                       size_t workspace_bytes, void* stream, char* err, size_t errlen) {
-  const char* what = "xb_paged_attention_bf16";
+// xb_paged_attention_bf16 and, with `q8` (few rows), the attention over 8-bit pages.
+static int attend(const char* what, const void* q, void* out, const xb_paged_kv* kv, const xb_paged_kv8* q8,
+                  int64_t tokens, int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
+                  size_t workspace_bytes, void* stream, char* err, size_t errlen) {
   int rc = check_pages(kv, what, err, errlen);
   if (!rc) rc = check_attention(kv, tokens, n_head, scale, what, err, errlen);
   if (rc) return rc;
@@ -2118,19 +2316,21 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
   if (rc) return rc;
   const bool few = few_rows(tokens, batch, n_rep);
   const bool eight = few && n_rep <= 8 && tokens * n_rep <= 8 * batch;  // the same rule for half a tile
-  const int tile = few ? kTK : kTcTK;
-  line_kernel(a, few ? (eight ? 8 : kFewRows) : kTcRows);
+  const int tile = !few ? kTcTK : q8 ? kFewTK8 : kFewTK;
+  line_kernel(a, few ? (eight ? 8 : kFewRows) : kTcRows, q8 ? kFewTK8 : kFewTK);
+  a.ke = q8 ? Exponents{q8->k_scale, q8->ks_page, q8->ks_head} : Exponents{};
+  a.ve = q8 ? Exponents{q8->v_scale, q8->vs_page, q8->vs_head} : Exponents{};
   a.rep_magic = (65536u + (uint32_t)n_rep - 1u) / (uint32_t)n_rep;
   int box = 8;  // rows of one load: the largest power of two that divides a page, at most a tile
   while (box < tile && page_size % (2 * box) == 0) box *= 2;
   a.box_rows = box;
   TcMaps maps;
   memset(&maps, 0, sizeof(maps));
-  rc = page_map(&maps.k, kv->k_pages, n_pages, n_kv_head, page_size, kv->k_page, kv->k_head, kv->k_row, box, what, err,
-                errlen);
+  rc = page_map(&maps.k, kv->k_pages, n_pages, n_kv_head, page_size, kv->k_page, kv->k_head, kv->k_row, box, q8,
+                what, err, errlen);
   if (!rc)
-    rc = page_map(&maps.v, kv->v_pages, n_pages, n_kv_head, page_size, kv->v_page, kv->v_head, kv->v_row, box, what,
-                  err, errlen);
+    rc = page_map(&maps.v, kv->v_pages, n_pages, n_kv_head, page_size, kv->v_page, kv->v_head, kv->v_row, box, q8,
+                  what, err, errlen);
   if (!rc && !few) rc = query_map(&maps.q, q, tokens, n_head, ld_q, n_rep, a.tpt, what, err, errlen);
   if (rc) return rc;
   int sms = 148;
@@ -2148,10 +2348,9 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
     KvMaps pages;
     pages.k = maps.k;
     pages.v = maps.v;
-    e = eight ? (wide ? launch_few<8, int64_t>(ctas, s, pages, a)
-                      : launch_few<8, int>(ctas, s, pages, a))
-              : (wide ? launch_few<16, int64_t>(ctas, s, pages, a)
-                      : launch_few<16, int>(ctas, s, pages, a));
+    e = !q8 ? launch_few<kBf16>(eight, wide, ctas, s, pages, a)
+            : q8->dtype == XB_DT_I8 ? launch_few<kInt8>(eight, wide, ctas, s, pages, a)
+                                    : launch_few<kE4m3>(eight, wide, ctas, s, pages, a);
     if (e == cudaSuccess)
       e = launch_k(paged_attn_join_kernel<kFewRows, 4>, dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
   } else {
@@ -2165,6 +2364,13 @@ extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_
     return XB_ERR_CUDA;
   }
   return check_launch(what, err, errlen);
+}
+
+extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_kv* kv, int64_t tokens,
+                                       int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
+                                       size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  return attend("xb_paged_attention_bf16", q, out, kv, nullptr, tokens, n_head, ld_q, ld_out, scale, workspace,
+                workspace_bytes, stream, err, errlen);
 }
 
 // Where an 8-bit call's pages go as bf16: a slot for each table entry, or for
@@ -2187,6 +2393,10 @@ extern "C" int xb_paged_attention_q8_workspace_size(int64_t tokens, int64_t batc
       page_size > 0x7fffffffLL || max_pages > 0x7fffffffLL || batch > (1LL << 20) || n_kv_head > 65535) {
     set_err(err, errlen, "%s: bad arguments", what);
     return XB_ERR_INVALID;
+  }
+  if (few_rows(tokens, batch, n_head / n_kv_head)) {
+    *bytes = own;
+    return XB_OK;
   }
   bool compact;
   const int64_t slots = expand_slots(batch, max_pages, n_pages, &compact);
@@ -2219,6 +2429,9 @@ extern "C" int xb_paged_attention_q8(const void* q, void* out, const xb_paged_kv
   if (!rc) rc = xb_paged_attention_workspace_size(tokens, kv->batch, n_head, kv->n_kv_head, &own, err, errlen);
   if (!rc) rc = check_workspace(workspace, workspace_bytes, need, what, err, errlen);
   if (rc) return rc;
+  if (few_rows(tokens, kv->batch, n_head / kv->n_kv_head))
+    return attend(what, q, out, kv, kv8, tokens, n_head, ld_q, ld_out, scale, workspace, workspace_bytes, stream, err,
+                  errlen);
   ExpandArgs e;
   bool compact;
   const int64_t slots = expand_slots(kv->batch, kv->max_pages, kv->n_pages, &compact);
@@ -2262,8 +2475,7 @@ extern "C" int xb_paged_attention_q8(const void* q, void* out, const xb_paged_kv
   wide.k_row = wide.v_row = kHD;
   wide.k_head = wide.v_head = kv->page_size * kHD;
   wide.k_page = wide.v_page = kv->n_kv_head * kv->page_size * kHD;
-  return xb_paged_attention_bf16(q, out, &wide, tokens, n_head, ld_q, ld_out, scale, workspace, own, stream, err,
-                                 errlen);
+  return attend(what, q, out, &wide, nullptr, tokens, n_head, ld_q, ld_out, scale, workspace, own, stream, err, errlen);
 }
 
 extern "C" int xb_page_status(void* stream, int* status, char* err, size_t errlen) {

@@ -32,18 +32,19 @@ struct Line {
 };
 
 constexpr int kFewTK = 32, kTcTK = 64;  // keys of a tile of the two kernels
+constexpr int kFewTK8 = 64;             // of the few-row kernel over 8-bit pages: the same bytes
 constexpr int kFewRows = 16;            // rows of a tile of the few-row kernel (at most)
 constexpr int kFewWarps = 8;            // its warps in a CTA, each with a piece of the line
 
 // What belongs to the kernel with tiles of `rows` rows (8 or kFewRows: few
 // rows; 128: tcgen05).  A unit's fixed cost and the smallest cut and piece were
 // found by measurement, in keys.
-inline void line_kernel(Line& a, int rows) {
+inline void line_kernel(Line& a, int rows, int few_tile = kFewTK) {
   const bool few = rows <= kFewRows;
   a.tpt = rows / a.n_rep;
-  a.over = few ? 16 : 192;
-  a.snap = few ? 32 : 128;
-  a.min_share = few ? 32 : 288;
+  a.over = few ? few_tile / 2 : 192;
+  a.snap = few ? few_tile : 128;
+  a.min_share = few ? few_tile : 288;
 }
 
 // The line's weight is at most this whatever the device arrays hold: every
