@@ -1,11 +1,15 @@
-"""Argument checks of the beam selection's C entry points (no GPU)."""
+"""Beam search without a GPU: argument checks of the selection's C entry points, and the search over a paged cache."""
 
 import ctypes
+import math
 
 import pytest
+import torch
 
-from xb200 import _lib
+from xb200 import _lib, ops
 from xb200._lib import XbError
+from xb200.beam import generate_beams
+from xb200.paged import PagedKVCache
 
 
 def _select(**kw):
@@ -56,3 +60,160 @@ def test_workspace_size():
         sizes.append(need.value)
         assert need.value >= groups * 4 * (8 * 8 + 8)
     assert sizes == sorted(sizes)
+
+
+# ----------------------------------------------------------------------------- the search, on a model of tables
+
+
+class _Cfg:
+    n_layer, n_kv_head, head_dim = 1, 1, 16
+
+
+class _Table:
+    """A model whose logits depend on the tokens so far, which it finds in the cache's pages: what the cache shares,
+    forks and frees has to be right for the search to be."""
+
+    position_limit, device, cfg = 64, torch.device("cpu"), _Cfg
+
+    def __init__(self, vocab, seed, end_bias=0.0):
+        self.vocab, self.seed, self.end_bias = vocab, seed, end_bias
+        self.steps = 0
+
+    def logits(self, tokens):
+        g = torch.Generator().manual_seed(hash((self.seed, *tokens)) & 0x7FFFFFFF)
+        x = torch.randn(self.vocab, generator=g) * 2
+        x[0] += self.end_bias
+        return x
+
+    def forward_paged(self, ids, cache, seqs, counts=None, next_token=None):
+        self.steps += 1
+        batch = cache.step(seqs, counts)
+        start, P = batch.q_start.tolist(), cache.page_size
+        out = []
+        for i, q in enumerate(seqs):
+            for t in range(start[i], start[i + 1]):
+                p = int(batch.positions[t])
+                cache.pages[0, 0, int(batch.page_table[i, p // P]), 0, p % P, 0] = int(ids[t])
+            out.append(self.logits([int(cache.pages[0, 0, cache.page_ids(q)[p // P], 0, p % P, 0])
+                                    for p in range(cache.length(q))]))
+        return torch.stack(out)
+
+
+def _plain_select(logits, scores, count):
+    G, K = scores.shape
+    total = scores.view(-1, 1) + torch.log_softmax(logits, 1)
+    total = torch.where(total.isfinite(), total, -math.inf).view(G, -1)
+    best, at = total.sort(dim=1, descending=True, stable=True)
+    V = logits.shape[1]
+    pad = max(0, count - best.shape[1])
+    best = torch.nn.functional.pad(best[:, :count], (0, pad), value=-math.inf)
+    at = torch.nn.functional.pad(at[:, :count], (0, pad))
+    none = best == -math.inf
+    return best, (at // V).masked_fill(none, -1), (at % V).masked_fill(none, -1)
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    def copy(pages, src, dst, dim=2):
+        pages[:, :, dst] = pages[:, :, src]
+
+    monkeypatch.setattr(ops, "copy_pages", copy)
+    monkeypatch.setattr(ops, "beam_select", _plain_select)
+
+
+def _search(model, prompt, K, steps, end, penalty):
+    """The same search on lists."""
+    live, done = [([], 0.0)], []
+    for _ in range(steps):
+        c = []
+        for b, (toks, s) in enumerate(live):
+            lp = torch.log_softmax(model.logits(prompt + toks), 0)
+            c += [(torch.tensor(s, dtype=torch.float32) + lp[v], -(b * model.vocab + v), toks + [v])
+                  for v in range(model.vocab)]
+        c.sort(key=lambda x: (-float(x[0]), -x[1]))
+        live, more = [], c[:2 * K]
+        for rank, (s, _, toks) in enumerate(more):
+            if len(live) == K:
+                break
+            if toks[-1] == end:
+                if rank < K:
+                    done.append((float(s) / len(toks) ** penalty, toks))
+            else:
+                live.append((toks, float(s)))
+        done.sort(key=lambda x: -x[0])
+        done = done[:K]
+        if not live or (len(done) == K and done[-1][0] >= live[0][1] / len(live[0][0]) ** penalty):
+            live = []
+            break
+    done += [(s / len(t) ** penalty, t) for t, s in live]
+    return sorted(done, key=lambda x: -x[0])[:K]
+
+
+@pytest.mark.parametrize("page", [8, 16])
+@pytest.mark.parametrize("K,steps,end,penalty,bias", [(1, 7, None, 1.0, 0), (3, 9, None, 1.0, 0), (4, 12, 0, 1.0, 0),
+                                                      (4, 12, 0, 0.0, 3), (2, 20, 0, 2.0, 1), (5, 1, 0, 1.0, 2),
+                                                      (32, 4, 0, 1.0, 0)])
+def test_search_matches_a_search_on_lists(plain, K, steps, end, penalty, bias, page):
+    model = _Table(11, seed=K, end_bias=bias)
+    prompts = [[3, 1, 4, 1, 5], [2], list(range(1, 11)) * 2, [7] * 8]
+    need = sum(len(p) // page + K * -(-(len(p) % page + steps - 1) // page) for p in prompts)
+    cache = PagedKVCache(_Cfg, need, page, device="cpu")
+    got = generate_beams(model, [torch.tensor(p) for p in prompts], K, steps, end, penalty, cache=cache, graph=False)
+    assert cache.free_pages == need and len(cache) == 0
+    for p, h in zip(prompts, got):
+        want = _search(model, p, K, steps, end, penalty)
+        assert [x.tokens for x in h] == [t for _, t in want]
+        for x, (score, t) in zip(h, want):
+            assert abs(x.score - score) < 1e-4 and abs(x.logprob - score * len(t) ** penalty) < 1e-3
+
+
+def test_one_beam_is_greedy(plain):
+    model = _Table(50, seed=9)
+    (h,), = generate_beams(model, [torch.tensor([5, 6])], 1, 6, graph=False)
+    tokens = []
+    for _ in range(6):
+        tokens.append(int(model.logits([5, 6] + tokens).argmax()))
+    assert h.tokens == tokens
+
+
+def test_fewer_continuations_than_beams(plain):
+    """Two tokens and five beams: places are left over in the first steps."""
+    model = _Table(2, seed=4)
+    got, = generate_beams(model, [torch.tensor([1])], 5, 4, graph=False)
+    want = _search(model, [1], 5, 4, None, 1.0)
+    assert [h.tokens for h in got] == [t for _, t in want]
+    only_end = _Table(1, seed=4)
+    got, = generate_beams(only_end, [torch.tensor([0])], 3, 4, end_token=0, graph=False)
+    assert [h.tokens for h in got] == [[0]] and only_end.steps == 1
+
+
+def test_search_refuses(plain):
+    model = _Table(5, seed=1)
+    one = torch.tensor([1])
+    for args in (([one], 0, 3), ([one], 33, 3), ([], 2, 3), ([one], 2, 0), ([torch.tensor([[1]])], 2, 3),
+                 ([torch.ones(60, dtype=torch.int64)], 2, 6)):
+        with pytest.raises(ValueError):
+            generate_beams(model, *args, graph=False)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        generate_beams(model, [one], 2, 3, page_size=12, graph=False)
+    cache = PagedKVCache(_Cfg, 3, 8, device="cpu")
+    with pytest.raises(RuntimeError, match="full"):
+        generate_beams(model, [one], 4, 9, cache=cache, graph=False)
+    assert cache.free_pages == 3 and len(cache) == 0
+
+
+def test_reorder_keeps_the_books(plain):
+    c = PagedKVCache(_Cfg, 20, 8, device="cpu")
+    a, b, d = c.add(), c.add(), c.add()
+    c.step([a, b, d], [9, 9, 9])
+    new = c.reorder([a, b, d], [2, 2, 0, 2])
+    assert new[0] == d and new[2] == a and len(set(new)) == 4 and len(c) == 4
+    assert c.page_ids(new[1]) == c.page_ids(d) == c.page_ids(new[3]) and c.free_pages == 16
+    with pytest.raises(KeyError):
+        c.length(b)
+    for seqs, parents in (([a, a], [0, 1]), ([a, d], [2]), ([a, d], [-1])):
+        with pytest.raises(ValueError):
+            c.reorder(seqs, parents)
+    with pytest.raises(KeyError):
+        c.reorder([a, 99], [0])
+    assert len(c) == 4 and c.reorder(new, []) == [] and c.free_pages == 20 and len(c) == 0

@@ -3,6 +3,7 @@
 import ctypes
 
 import pytest
+import torch
 from test_paged_cpu import _KV
 
 from xb200 import _lib, ops
@@ -130,3 +131,39 @@ def test_workspace_size():
     _lib.call("xb_paged_attention_workspace_size", 400, 2, 14, 2, ctypes.byref(need))
     small, pool, wide = (_bytes(400, 2, 14, 2, n, 16, c) - need.value for n, c in ((1000, 3), (1000, 600), (1000, 700)))
     assert 6 * page <= small < 7 * page and 1000 * page <= pool <= wide < 1003 * page
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+def test_cache_copies_codes_with_their_exponents(dtype, monkeypatch):
+    from test_paged_cpu import _Cfg
+    from xb200.paged import PagedKVCache
+
+    calls = []
+
+    def copy(pages, src, dst, dim=2):
+        assert pages.is_contiguous() and pages.stride(dim) * pages.element_size() % 16 == 0
+        view = pages.view(torch.uint8)
+        view.index_copy_(dim, torch.tensor(dst), view.index_select(dim, torch.tensor(src)))
+        calls.append((pages.data_ptr(), list(src), list(dst), dim))
+
+    monkeypatch.setattr(ops, "copy_pages", copy)
+    c = PagedKVCache(_Cfg, 6, 8, device="cpu", dtype=dtype)
+    assert c.pages.dtype is dtype and c.k_scale[1].shape == (6, 2, 8) and c.v_scale[0].dtype is torch.uint8
+    a = c.add()
+    c.step([a], [11])
+    c.pages.view(torch.uint8)[:, :, 1] = 7
+    c.k_scale[1][1] = 90
+    c.v_scale[0][1] = 91
+    b = c.fork(a)
+    c.step([b], [1])
+    page = c.page_ids(b)[1]
+    assert page != 1 and [x[1:] for x in calls] == [([1], [page], 2), ([1], [page], 1)]
+    assert bool((c.pages.view(torch.uint8)[:, :, page] == 7).all())
+    assert bool((c.k_scale[1][page] == 90).all()) and bool((c.v_scale[0][page] == 91).all())
+    c.free(a)
+    assert c.compact() == 1 and bool((c.k_scale[1][c.page_ids(b)[1]] == 90).all())
+    bf16 = PagedKVCache(_Cfg, 6, 8, device="cpu")
+    assert bf16.scales is None and bf16.k_scale == bf16.v_scale == [None, None]
+    for bad in (torch.float32, torch.float16, torch.uint8, torch.float8_e5m2):
+        with pytest.raises(ValueError, match="bf16, int8"):
+            PagedKVCache(_Cfg, 6, 8, device="cpu", dtype=bad)

@@ -15,6 +15,11 @@ any time, and a step takes any of them with any number of new tokens each::
 
 The bookkeeping (who owns which page) lives on the host; the pool and the
 tables that the kernels read are on the device.
+
+With ``dtype=torch.int8`` or ``torch.float8_e4m3fn`` the pool holds codes and an
+exponent byte for each position and KV head: half the bytes, so twice the
+positions in the same memory and half the reading of a decode step over long
+contexts.  Nothing else changes for the caller.
 """
 
 from __future__ import annotations
@@ -57,22 +62,33 @@ class _Sequence:
 
 
 class PagedKVCache:
-    """Pool [n_layer, 2, n_pages, n_kv_head, page_size, head_dim] (bf16) and
-    the pages of every sequence in it.
+    """Pool [n_layer, 2, n_pages, n_kv_head, page_size, head_dim] (bf16, or
+    int8 / float8_e4m3fn codes) and the pages of every sequence in it.
 
-    ``k[i]`` / ``v[i]`` are layer i's pages as the operators take them.  A page
+    ``k[i]`` / ``v[i]`` are layer i's pages as the operators take them, ``k_scale[i]``
+    / ``v_scale[i]`` the exponents of 8-bit ones (None in bf16).  A page
     is handed out lowest number first.  Methods that move or copy pages enqueue
     the copies on the current stream, where the steps that use the cache run.
     """
 
-    def __init__(self, cfg, n_pages: int, page_size: int = 16, device="cuda"):
+    def __init__(self, cfg, n_pages: int, page_size: int = 16, device="cuda", dtype=torch.bfloat16):
         if n_pages < 1 or page_size < 8 or page_size % 8:
             raise ValueError("a pool has at least one page of a multiple of 8 positions")
-        self.n_pages, self.page_size = n_pages, page_size
-        self.pages = torch.zeros((cfg.n_layer, 2, n_pages, cfg.n_kv_head, page_size, cfg.head_dim),
-                                 dtype=torch.bfloat16, device=device)
+        if dtype not in (torch.bfloat16, torch.int8, torch.float8_e4m3fn):
+            raise ValueError("a pool holds bf16, int8 or float8_e4m3fn")
+        self.n_pages, self.page_size, self.dtype = n_pages, page_size, dtype
+        self.pages = torch.zeros((cfg.n_layer, 2, n_pages, cfg.n_kv_head, page_size, cfg.head_dim), dtype=dtype,
+                                 device=device)
         self.k = [layer[0] for layer in self.pages]
         self.v = [layer[1] for layer in self.pages]
+        self.scales = None
+        self.k_scale = self.v_scale = [None] * cfg.n_layer
+        if dtype is not torch.bfloat16:
+            # K's and V's beside each other: a page's exponents are whole 16-byte vectors for the page copies
+            self.scales = torch.zeros((cfg.n_layer, n_pages, 2, cfg.n_kv_head, page_size), dtype=torch.uint8,
+                                      device=device)
+            self.k_scale = [layer[:, 0] for layer in self.scales]
+            self.v_scale = [layer[:, 1] for layer in self.scales]
         self.device = self.pages.device
         self._refs = [0] * n_pages
         self._free = list(range(n_pages))  # a heap
@@ -139,7 +155,34 @@ class PagedKVCache:
         del s.pages[keep:]
         s.length = length
 
+    def reorder(self, seqs, parents) -> list[int]:
+        """The sequences of a beam search's next step: place i goes on from
+        seqs[parents[i]], which may be named several times or not at all.
+        Returns the handles of the new ones; those of `seqs` that none of them
+        takes over are gone."""
+        seqs, parents = list(seqs), [int(p) for p in parents]
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence may appear once in a step")
+        if any(not 0 <= p < len(seqs) for p in parents):
+            raise ValueError(f"parents are places 0 .. {len(seqs) - 1}")
+        for q in seqs:
+            self._get(q)
+        kept, out = set(), []
+        for p in parents:  # the first to name a sequence takes it over, the others share its pages
+            out.append(self.fork(seqs[p]) if p in kept else seqs[p])
+            kept.add(p)
+        for p, q in enumerate(seqs):
+            if p not in kept:
+                self.free(q)
+        return out
+
     # ------------------------------------------------------------- steps
+
+    def _copy(self, src, dst) -> None:
+        """Pages of every layer, keys and values and their exponents."""
+        ops.copy_pages(self.pages, src, dst)
+        if self.scales is not None:
+            ops.copy_pages(self.scales, src, dst, dim=1)
 
     def _grow(self, seqs, counts) -> None:
         """Room for counts[i] more positions of seqs[i], all or none: pages
@@ -176,7 +219,7 @@ class PagedKVCache:
             at += own + fresh
         try:  # before the books change: a copy that fails leaves them as they were
             if src:
-                ops.copy_pages(self.pages, src, dst)
+                self._copy(src, dst)
         except BaseException:
             for p in taken:
                 heapq.heappush(self._free, p)
@@ -222,6 +265,24 @@ class PagedKVCache:
         return PagedBatch(ints[:n].view(B, columns), ints[n:n + B + 1], ints[n + B + 1:], longs[:T],
                           longs[T:] if T > B else None)
 
+    def read(self, seqs, layer: int):
+        """Keys and values of whole sequences in one layer, packed one after the
+        other: two bf16 tensors [sum of lengths, n_kv_head, head_dim] (what
+        8-bit codes stand for is a bf16 number), to hand a sequence on to
+        another cache or program."""
+        seqs = list(seqs)
+        lens = [self._get(q).length for q in seqs]
+        T, B = sum(lens), len(seqs)
+        k, v = (torch.empty((T, self.pages.shape[3], self.pages.shape[5]), dtype=torch.bfloat16, device=self.device)
+                for _ in range(2))
+        if T:
+            columns = max(len(self._seqs[q].pages) for q in seqs)
+            ints = np.concatenate([self._table(seqs, columns).reshape(-1), [0], np.cumsum(lens), lens]).astype(np.int32)
+            ints, n = _upload(ints, self.device), B * columns
+            ops.paged_read_kv(k, v, self.k[layer], self.v[layer], ints[:n].view(B, columns), ints[n:n + B + 1],
+                              ints[n + B + 1:], self.k_scale[layer], self.v_scale[layer])
+        return k, v
+
     # ------------------------------------------------------------- the pool
 
     def compact(self) -> int:
@@ -234,7 +295,7 @@ class PagedKVCache:
         assert len(holes) == len(high)
         if not high:
             return 0
-        ops.copy_pages(self.pages, high, holes)
+        self._copy(high, holes)
         to = dict(zip(high, holes))
         for p, q in to.items():
             self._refs[q], self._refs[p] = self._refs[p], 0
@@ -279,9 +340,10 @@ class PagedDecodeGraph:
     paged cache.  The kernels read lengths and page tables from the device, so
     the same graph serves every step, whichever sequences take part and however
     long they are (up to `max_positions`).  Steps of the cache and replays run
-    on one stream, or ordered by events, like any two users of the same pages."""
+    on one stream, or ordered by events, like any two users of the same pages.
+    A step gives the greedy next tokens, or with `logits` the logits."""
 
-    def __init__(self, model, cache: PagedKVCache, batch: int, max_positions: int):
+    def __init__(self, model, cache: PagedKVCache, batch: int, max_positions: int, logits: bool = False):
         if batch < 1 or not 0 < max_positions <= model.position_limit:
             raise ValueError(f"batch must be positive and max_positions 1 .. {model.position_limit}")
         _check_cache(model, cache)
@@ -303,20 +365,22 @@ class PagedDecodeGraph:
             # one eager step of the captured sizes, a position in a page of a
             # small pool for each sequence, sets up the kernels (attributes,
             # scratch) before the capture
-            small = PagedKVCache(model.cfg, batch, cache.page_size, dev)
+            small = PagedKVCache(model.cfg, batch, cache.page_size, dev, cache.dtype)
             self._step.page_table[:, 0] = torch.arange(batch, device=dev)
             self._step.kv_len.fill_(1)
-            model.forward_packed(self.ids, small, self._step, next_token=self.next_token)
+            token = None if logits else self.next_token
+            model.forward_packed(self.ids, small, self._step, next_token=token)
             torch.cuda.synchronize(dev)
             del small
             self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph):
-                model.forward_packed(self.ids, cache, self._step, next_token=self.next_token)
+                self.logits = model.forward_packed(self.ids, cache, self._step, next_token=token)
             self._scratch = ops.take_workspace(dev)
 
     def step(self, seqs, ids: torch.Tensor) -> torch.Tensor:
-        """The greedy next token (int64 [batch], overwritten by the next step)
-        of every sequence after its token in `ids`."""
+        """The greedy next token (int64 [batch]) of every sequence after its
+        token in `ids`, or the logits (fp32 [batch, vocab]); overwritten by the
+        next step."""
         seqs = list(seqs)
         if len(seqs) != self.batch:
             raise ValueError(f"the graph was captured for {self.batch} sequences, got {len(seqs)}")
@@ -331,26 +395,33 @@ class PagedDecodeGraph:
         _upload(lens - 1, self.cache.device, self._positions)
         self.ids.copy_(ids)
         self.graph.replay()
-        return self.next_token
+        return self.next_token if self.logits is None else self.logits
 
 
-def generate_paged(model, prompts, max_new_tokens: int, cache: PagedKVCache | None = None, page_size: int = 16,
-                   graph: bool = True) -> torch.Tensor:
-    """Greedy continuation of prompts of different lengths (1-D int64 tensors)
-    in one batch: the prompts are prefilled packed, then every sequence decodes
-    a token per step.  Returns tokens [B, max_new_tokens] on the device; a
-    `cache` that is passed in keeps nothing of the run."""
+def check_prompts(model, prompts, max_new_tokens: int):
+    """(prompts, their lengths, positions behind them: the last token is never fed back)"""
     prompts = list(prompts)
     if not prompts or any(p.dim() != 1 or p.numel() == 0 for p in prompts) or max_new_tokens < 1:
         raise ValueError("prompts are non-empty 1-D tensors, and at least one token is generated")
     counts = [p.numel() for p in prompts]
-    more = max_new_tokens - 1  # positions behind the prompts: the last token is never fed back
+    more = max_new_tokens - 1
+    if max(counts) + more > model.position_limit:
+        raise ValueError(f"{max(counts) + more} positions exceed the model's {model.position_limit}")
+    return prompts, counts, more
+
+
+def generate_paged(model, prompts, max_new_tokens: int, cache: PagedKVCache | None = None, page_size: int = 16,
+                   graph: bool = True, dtype=torch.bfloat16) -> torch.Tensor:
+    """Greedy continuation of prompts of different lengths (1-D int64 tensors)
+    in one batch: the prompts are prefilled packed, then every sequence decodes
+    a token per step.  Returns tokens [B, max_new_tokens] on the device; a
+    `cache` that is passed in keeps nothing of the run, otherwise one of `dtype`
+    is made for it."""
+    prompts, counts, more = check_prompts(model, prompts, max_new_tokens)
     longest = max(counts) + more
-    if longest > model.position_limit:
-        raise ValueError(f"{longest} positions exceed the model's {model.position_limit}")
     if cache is None:
         unit = max(page_size, 1)  # what no page may have is for the cache to refuse
-        cache = PagedKVCache(model.cfg, sum(-(-(c + more) // unit) for c in counts), page_size, model.device)
+        cache = PagedKVCache(model.cfg, sum(-(-(c + more) // unit) for c in counts), page_size, model.device, dtype)
     B = len(prompts)
     ids = torch.cat([p.to(model.device) for p in prompts])
     toks = torch.empty((max_new_tokens, B), dtype=torch.int64, device=model.device)

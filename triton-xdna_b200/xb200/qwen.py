@@ -31,6 +31,7 @@ from dataclasses import dataclass
 import torch
 
 from . import ops
+from .beam import generate_beams
 from .paged import PagedBatch, PagedKVCache, check_step, generate_paged
 
 
@@ -294,8 +295,9 @@ class Qwen2Model:
                 qkv = ops.decode_linear(xin, L["qkv_w"], L["qkv_b"], xnorm=xnorm)
             else:
                 qkv = ops.linear(ops.rms_norm(x, L["input_ln"], eps), L["qkv_w"], L["qkv_b"])
-            ops.paged_rope_kv(qkv, self.cos, self.sin, q, cache.k[i], cache.v[i], *at)
-            ops.paged_attention(q, cache.k[i], cache.v[i], attn, *at, self.scale)
+            ex = (cache.k_scale[i], cache.v_scale[i])  # of 8-bit pages
+            ops.paged_rope_kv(qkv, self.cos, self.sin, q, cache.k[i], cache.v[i], *at, *ex)
+            ops.paged_attention(q, cache.k[i], cache.v[i], attn, *at, self.scale, *ex)
             if small:
                 y, st = ops.decode_linear_residual(attn, L["o_w"], None, x, stats_kind="rms")
                 h = ops.decode_linear_swiglu(y, L["gate_up_w"], xnorm=(st, L["post_ln"], None, eps, "rms"))
@@ -328,6 +330,10 @@ class Qwen2Model:
     def generate_paged(self, prompts, max_new_tokens: int, **kw) -> torch.Tensor:
         """Greedy continuation of prompts of different lengths (xb200.paged.generate_paged)."""
         return generate_paged(self, prompts, max_new_tokens, **kw)
+
+    def generate_beams(self, prompts, beams: int, max_new_tokens: int, **kw):
+        """Beam search from prompts of different lengths (xb200.beam.generate_beams)."""
+        return generate_beams(self, prompts, beams, max_new_tokens, **kw)
 
     @torch.no_grad()
     def generate(self, ids: torch.Tensor, max_new_tokens: int, cache: KVCache | None = None,
