@@ -17,9 +17,16 @@
 namespace xb {
 namespace beam {
 
-constexpr int kThreads = 256;
-constexpr int kMaxCount = 64, kMaxBeams = 64, kMaxParts = 64;
-constexpr int kBuffer = 1024;  // candidates of a part held at a time
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMaxCount = 64, kMaxBeams = 64;
+constexpr int kLane = 16, kGroup = 32 * kLane;  // tokens that a lane and its warp take at a time
+constexpr int kBlocks = 8;      // runs of groups of which a lane keeps the maximum
+constexpr int kHeld = 128;      // candidates of a warp held at a time
+constexpr int kPicked = 1024;   // candidates of a group's choice held at a time
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kLog2e = 1.4426950408889634f;
+// exp2(x kLog2e) = exp(x (1 + kLog2eOff)): what rounding log2(e) to fp32 does
+constexpr double kLog2eOff = (double)kLog2e * 0.69314718055994530942 - 1.0;
 
 // Orders floats as unsigned numbers (NaN aside).
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -35,185 +42,243 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t token) {
   return (uint64_t)ordered(x + 0.0f) << 32 | (0xffffffffu - token);
 }
 
-__device__ __forceinline__ void unpack(const uint4& v, float (&x)[4]) {
-  x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
-}
-__device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-
-// Tokens W v .. W v + W - 1 of a row, W = 16 bytes of them; behind the row's end
-// -inf.  Which thread adds up which tokens in which order thus does not depend on
-// the row's address: rows that are alike have the same sum, to the bit.  A row
-// that does not start on a 16-byte boundary: the 16 bytes out of the two aligned
-// vectors that hold them (the second is the neighbour's first, in the L1); at its ends, where those reach
-// out of the row, element by element.
-template <bool ALIGNED, typename T, int W>
-__device__ __forceinline__ void load_tokens(const T* row, int64_t vocab, int64_t v, float (&x)[W]) {
-  const T* p = row + v * W;
-  if ((ALIGNED || (v > 0 && (v + 2) * W <= vocab)) && (v + 1) * W <= vocab) {
-    if constexpr (ALIGNED) {
-      unpack(__ldcs(reinterpret_cast<const uint4*>(p)), x);
-    } else {
-      const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;  // the same all along a row
-      const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) - off);
-      const uint4 lo = __ldg(q), hi = __ldg(q + (off != 0));
-      uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-      if (off & 8) {
-#pragma unroll
-        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-      }
-      if (off & 4) {
-#pragma unroll
-        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-      }
-      if (off & 2) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
-      }
-      unpack(make_uint4(w[0], w[1], w[2], w[3]), x);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < W; ++j) x[j] = v * W + j < vocab ? Cvt<T>::to_f(p[j]) : -INFINITY;
-  }
-}
-
-struct Stats {  // of a part: its maximum (-inf: none), the sum of exp(x - maximum)
+// Of a part: its maximum (-inf: none) and sum 2^shift, the sum of exp2(x kLog2e).
+// The shift is a whole number, so sums of different shifts are brought to one
+// without rounding, and x kLog2e - shift is one fused multiply-add, rounded in the size of
+// its result.
+struct Stats {
   float top, sum;
+  int shift, unused;
+};
+__device__ __forceinline__ int shift_of(float top) {
+  return top > -INFINITY && top < INFINITY ? (int)fminf(fmaxf(rintf(top * kLog2e), -1e9f), 1e9f) : 0;
+}
+// 2^n, n <= 0
+__device__ __forceinline__ float power(int n) { return n < -126 ? 0.0f : __int_as_float((n + 127) << 23); }
+
+// A number that at least `count` of the block's threads' `mine` reach, close to the
+// largest such one (-inf where none is known): the count-th of the count / 4 largest of
+// each warp.  `few` is shared and this call's own.  Every thread calls this.
+constexpr int kFew = 2 * kMaxCount;
+__device__ __forceinline__ float reached_by(float mine, int count, float* few) {
+  const int part = (2 * count + kWarps - 1) / kWarps, lane = threadIdx.x & 31;
+  float* to = few + (threadIdx.x >> 5) * part;
+  for (int n = 0; n < part;) {
+    const float best = unordered(__reduce_max_sync(0xffffffffu, ordered(mine)));
+    const bool at = mine == best;
+    const uint32_t who = __ballot_sync(0xffffffffu, at);
+    if (at) {
+      mine = -INFINITY;
+      const int i = n + __popc(who & ((1u << lane) - 1u));
+      if (i < part) to[i] = best;
+    }
+    n += __popc(who);  // every lane, once all are -inf
+  }
+  __syncthreads();
+  // the least of those that fewer than count are above
+  const int all = part * kWarps;
+  float bound = INFINITY;
+  for (int i = lane; i < all; i += 32) {
+    int above = 0;
+    for (int j = 0; j < all; ++j) above += few[j] > few[i];
+    if (above < count) bound = fminf(bound, few[i]);
+  }
+  return unordered(__reduce_min_sync(0xffffffffu, ordered(bound)));
+}
+
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <typename T>
+struct Ring {  // a warp's groups of tokens on their way from memory
+  static constexpr int kBytes = kGroup * (int)sizeof(T);
+  static constexpr int kStages = 8 / (int)sizeof(T);
+  static constexpr int kStage = kBytes + 16;  // a row may start anywhere in a vector
+  static constexpr int kSmem = kWarps * kStages * kStage;
 };
 
-// Keeps the `count` best of the n <= kBuffer candidates in `buf`, best first, and
-// returns how many that are.  All threads; keys differ from each other, so a
-// key's place is the number of larger ones.
-__device__ __forceinline__ int keep_best(uint64_t* buf, uint64_t* sorted, int n, int count) {
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t mine = buf[i];
-    int place = 0;
-    for (int j = 0; j < n; ++j) place += buf[j] > mine;
-    if (place < count) sorted[place] = mine;
-  }
-  __syncthreads();
-  const int kept = min(n, count);
-  for (int i = threadIdx.x; i < kept; i += kThreads) buf[i] = sorted[i];
-  __syncthreads();
-  return kept;
-}
-
-// One part of a row: `vps` vectors of 16 bytes.
-template <bool ALIGNED, typename T>
-__global__ void __launch_bounds__(kThreads) beam_scan_kernel(const T* __restrict__ logits, int64_t ld, int64_t vocab,
-                                                             int count, int parts, int64_t vps,
-                                                             uint64_t* __restrict__ lists, Stats* __restrict__ stats) {
-  constexpr int W = 16 / sizeof(T), NV = 32 / W;  // 32 logits a thread at a time
-  __shared__ uint64_t buf[kBuffer], sorted[kMaxCount];
-  __shared__ float warp_low[kThreads / 32], warp_top[kThreads / 32], warp_sum[kThreads / 32];
-  __shared__ int held;
+// One part of a row: groups of tokens, by turns to the CTA's warps, which run
+// on their own, each with a ring of asynchronous 16-byte copies (cp.async, 4 KB a
+// warp in flight).  Which lane adds up which tokens in which order does not
+// depend on the row's address, so rows that are alike have the same sum, to the
+// bit.
+//
+// While the tokens stream by, a lane keeps its running maximum and sum and the
+// maximum of each of 8 runs of its tokens, nothing else.  Then a bound that at
+// least `count` lanes' maxima reach is one that the `count` best tokens reach, and
+// only the few runs whose maximum reaches it are looked through again, in the ring
+// or in the L2: some 20 of 2048 for count = 16.  Keeping the candidates during the
+// stream took 44 instructions a token, mostly to find that there is none.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const T* __restrict__ logits, int64_t ld, int64_t vocab,
+                                                                int count, int parts, uint64_t* __restrict__ lists,
+                                                                Stats* __restrict__ stats) {
+  using R = Ring<T>;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ uint64_t cand[kWarps][kHeld];
+  __shared__ float run_top[kBlocks][kThreads];
+  __shared__ uint16_t runs[kBlocks * kThreads];
+  __shared__ float few[kFew], warp_top[kWarps], warp_sum[kWarps];
+  __shared__ int listed, total;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x / (uint32_t)parts;
   const int part = blockIdx.x - (int)row * parts;
-  if (threadIdx.x == 0) held = 0;
+  if (threadIdx.x == 0) listed = total = 0;
   pdl_wait();
   pdl_trigger();
   const T* x = logits + row * ld;
-  const int64_t v0 = part * vps, v1 = min((vocab + W - 1) / W, v0 + vps);
+  const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15);
+  const uint8_t* from = reinterpret_cast<const uint8_t*>(x) - off;
+  const int64_t end = off + vocab * (int64_t)sizeof(T);
+  const int64_t groups = (vocab + kGroup - 1) / kGroup;
+  const int64_t p0 = part * groups / parts, g1 = (part + 1) * groups / parts, g0 = p0 + warp;
+  const int n = g0 < g1 ? (int)((g1 - g0 + kWarps - 1) / kWarps) : 0;
+  const int run = (int)((g1 - p0 + kWarps * kBlocks - 1) / (kWarps * kBlocks));  // groups of a run
+  uint8_t* mine = ring + warp * R::kStages * R::kStage;
+  const uint32_t mine_u32 = (uint32_t)__cvta_generic_to_shared(mine);
 
-  float top = -INFINITY, sum = 0.0f;
-  uint64_t bar = 0;  // candidates lie above it
-  float low = -3.402823466e38f;  // and so their logits at or above this
-  __syncthreads();
-  for (int64_t v = v0;; v += kThreads * NV) {
-    const bool first = v == v0;
-    float e[NV][W];
+  auto fill = [&](int it) {
+    if (it < n) {
+      const int64_t at = (g0 + (int64_t)it * kWarps) * R::kBytes;
+      const uint32_t to = mine_u32 + it % R::kStages * R::kStage + lane * 16;
+      const uint8_t* src = from + at + lane * 16;
+      if (at >= off && at + R::kStage <= end) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int64_t at = v + i * kThreads + threadIdx.x;
-      if (at < v1) load_tokens<ALIGNED>(x, vocab, at, e[i]);
-      else
-#pragma unroll
-        for (int j = 0; j < W; ++j) e[i][j] = -INFINITY;
+        for (int k = 0; k < R::kBytes / 512; ++k) copy16_async(to + k * 512, src + k * 512);
+        if (lane == 0 && off != 0) copy16_async(to + R::kBytes, src + R::kBytes);
+      } else {
+        for (int k = lane * 16; k < R::kStage; k += 512, src += 512) {
+          const int64_t pos = at + k;
+          if (pos >= off && pos + 16 <= end) {
+            copy16_async(mine_u32 + it % R::kStages * R::kStage + k, src);
+          } else {  // vectors that reach out of the row: what of them lies in it
+            for (int e = 0; e < 16; e += (int)sizeof(T))
+              if (pos + e >= off && pos + e < end)
+                *reinterpret_cast<T*>(mine + it % R::kStages * R::kStage + k + e) = *reinterpret_cast<const T*>(src + e);
+          }
+        }
+      }
     }
-    // running maximum and sum
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < R::kStages; ++i) fill(i);
+
+  float top = -INFINITY, sum = 0.0f, here = -INFINITY;  // here: of the present run
+  int shift = 0;
+  int left = run, block = 0;
+#pragma unroll
+  for (int i = 0; i < kBlocks; ++i) run_top[i][threadIdx.x] = -INFINITY;
+  for (int it = 0; it < n; ++it) {
+    float v[kLane];
+    asm volatile("cp.async.wait_group %0;" ::"n"(R::kStages - 1) : "memory");
+    __syncwarp();
+    const uint8_t* p = mine + it % R::kStages * R::kStage + off + lane * (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) v[i] = Cvt<T>::to_f(*reinterpret_cast<const T*>(p + i * 32 * (int)sizeof(T)));
+    const int64_t behind = vocab - (g0 + (int64_t)it * kWarps) * kGroup - lane;  // tokens from this lane's first on
+    if (behind <= kGroup - 32) {
+#pragma unroll
+      for (int i = 0; i < kLane; ++i)
+        if (i * 32 >= behind) v[i] = -INFINITY;
+    }
+    __syncwarp();
+    if (it + R::kStages < n) fill(it + R::kStages);  // the last groups stay in the ring
+    else asm volatile("cp.async.commit_group;" ::: "memory");
     float m = -INFINITY;  // never NaN: fmaxf passes over NaN, which the sum keeps
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < kLane; ++i) m = fmaxf(m, v[i]);
+    here = fmaxf(here, m);
+    if (m > top) {
+      top = m;
+      const int to = shift_of(m);
+      sum *= power(min(shift - to, 0));  // a sum of nothing may have had any
+      shift = to;
+    }
+    const float base = -(float)shift;
+    float s[2] = {sum, 0.0f};
 #pragma unroll
-      for (int j = 0; j < W; ++j) m = fmaxf(m, e[i][j]);
-    const float to = fmaxf(top, m), base = to == -INFINITY ? 0.0f : to;
-    constexpr float kLog2e = 1.4426950408889634f;
-    float s[2] = {sum * ex2_approx((top - base) * kLog2e), 0.0f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < W; ++j) s[j & 1] += ex2_approx((e[i][j] - base) * kLog2e);
+    for (int i = 0; i < kLane; ++i) s[i & 1] += ex2_approx(fmaf(v[i], kLog2e, base));
     sum = s[0] + s[1];
-    top = to;
-    if (first) {
-      // a bound below the count best: in every warp at least count / 8 threads have a maximum at or above the least of
-      // the warps' own bounds
-      float mine = m, bound = -3.402823466e38f;
-      for (int need = (count + kThreads / 32 - 1) / (kThreads / 32); need > 0;) {
-        bound = unordered(__reduce_max_sync(0xffffffffu, ordered(mine)));
-        if (bound == -INFINITY) break;
-        need -= __popc(__ballot_sync(0xffffffffu, mine == bound));
-        if (mine == bound) mine = -INFINITY;
-      }
-      if (lane == 0) warp_low[warp] = bound;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) bound = fminf(bound, warp_low[i]);
-      low = fmaxf(low, bound);
-      bar = (uint64_t)ordered(low + 0.0f) << 32;
+    if (--left == 0 || it + 1 == n) {
+      run_top[block++][threadIdx.x] = here;
+      here = -INFINITY;
+      left = run;
     }
-    // candidates into the buffer; where it is full its best stay, and the bar rises
-    uint32_t want = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < W; ++j) want |= e[i][j] >= low ? 1u << (i * W + j) : 0u;
-    int n;
-    for (;;) {
-      if (want) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int j = 0; j < W; ++j)
-            if (want >> (i * W + j) & 1) {
-              const uint64_t key =
-                  key_of(e[i][j], (uint32_t)((v + i * kThreads + threadIdx.x) * W + j));
-              if (key > bar) {
-                const int at = atomicAdd(&held, 1);
-                if (at >= kBuffer) continue;  // stays wanted
-                buf[at] = key;
-              }
-              want &= ~(1u << (i * W + j));
-            }
-      }
-      __syncthreads();
-      n = held;
-      __syncthreads();
-      if (n <= kBuffer && n < 3 * count + 64 && !first) break;
-      const bool over = n > kBuffer;
-      n = keep_best(buf, sorted, min(n, kBuffer), count);
-      if (n == count) {
-        bar = buf[count - 1];
-        low = unordered((uint32_t)(bar >> 32));
-      }
-      if (threadIdx.x == 0) held = n;
-      __syncthreads();
-      if (!over) break;
-    }
-    if (v + kThreads * NV >= v1) break;
   }
-  const int n = keep_best(buf, sorted, held, count);
-  uint64_t* list = lists + (int64_t)blockIdx.x * count;
-  for (int i = threadIdx.x; i < count; i += kThreads) list[i] = i < n ? buf[i] : 0;
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  uint64_t* own = cand[warp];
+  int held = 0;
+  uint64_t bar = 0;
+  // the best `count` of this warp's candidates, best first; later ones have to lie above the last
+  auto keep_best = [&]() {
+    __syncwarp();
+    uint64_t e[kHeld / 32];
+    int place[kHeld / 32];
+#pragma unroll
+    for (int i = 0; i < kHeld / 32; ++i) {
+      e[i] = i * 32 + lane < held ? own[i * 32 + lane] : 0;
+      place[i] = 0;
+    }
+    for (int j = 0; j < held; ++j) {
+      const uint64_t other = own[j];
+#pragma unroll
+      for (int i = 0; i < kHeld / 32; ++i) place[i] += other > e[i];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kHeld / 32; ++i)
+      if (e[i] != 0 && place[i] < count) own[place[i]] = e[i];
+    __syncwarp();
+    if (held >= count) {
+      bar = own[count - 1];
+      held = count;
+    }
+  };
+  const float low = fmaxf(kLowest, reached_by(top, count, few));  // -inf is no candidate
+  // the runs to look through
+  if (top >= low)
+    for (int b = 0; b < block; ++b)
+      if (run_top[b][threadIdx.x] >= low) runs[atomicAdd(&listed, 1)] = (uint16_t)(b * kThreads + threadIdx.x);
+  __syncthreads();
+  // a half-warp takes a run, a lane a token of each of its groups
+  const int half = warp * 2 + (lane >> 4), inside = (lane & 15) * 32;
+  for (int q0 = 0; q0 < listed; q0 += 2 * kWarps) {
+    const int q = q0 + half, r = q < listed ? runs[q] : 0;
+    const int w = (r % kThreads) >> 5, within = (r & 31) + inside, it0 = r / kThreads * run;
+    const int64_t gw = p0 + w;
+    const int nw = gw < g1 ? (int)((g1 - gw + kWarps - 1) / kWarps) : 0;  // that warp's groups
+    const uint8_t* slots = ring + w * R::kStages * R::kStage + off + within * (int)sizeof(T);
+    for (int u0 = 0; u0 < run; u0 += 4) {  // four loads in flight
+      float v[4];
+      uint32_t token[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int it = it0 + u0 + u;
+        const int64_t t = (gw + (int64_t)it * kWarps) * kGroup + within;
+        v[u] = -INFINITY;
+        token[u] = (uint32_t)t;
+        if (q < listed && u0 + u < run && it < nw && t < vocab)
+          v[u] = Cvt<T>::to_f(it + R::kStages >= nw
+                                  ? *reinterpret_cast<const T*>(slots + it % R::kStages * R::kStage)
+                                  : x[t]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t who = __ballot_sync(0xffffffffu, v[u] >= low);
+        if (!who) continue;
+        const uint64_t key = key_of(v[u], token[u]);
+        if (held > kHeld - 32) keep_best();
+        who = __ballot_sync(0xffffffffu, v[u] >= low && key > bar);
+        if (who >> lane & 1) own[held + __popc(who & ((1u << lane) - 1u))] = key;
+        held += __popc(who);
+      }
+    }
+  }
+  __syncthreads();  // the ring is read
+  uint64_t* all = reinterpret_cast<uint64_t*>(ring);  // [kWarps * kHeld] at most
+  for (int i = lane; i < held; i += 32) all[atomicAdd(&total, 1)] = own[i];
   // the part's maximum and sum
   float m = top;
 #pragma unroll
@@ -222,15 +287,26 @@ __global__ void __launch_bounds__(kThreads) beam_scan_kernel(const T* __restrict
   __syncthreads();
   m = warp_top[0];
 #pragma unroll
-  for (int i = 1; i < kThreads / 32; ++i) m = fmaxf(m, warp_top[i]);
-  float s = sum * ex2_approx((top - (m == -INFINITY ? 0.0f : m)) * 1.4426950408889634f);
+  for (int i = 1; i < kWarps; ++i) m = fmaxf(m, warp_top[i]);
+  const int to = shift_of(m);
+  float s = sum * power(min(shift - to, 0));
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) warp_sum[warp] = s;
+  // a key's place is the number of larger ones
+  uint64_t* list = lists + (int64_t)blockIdx.x * count;
+  const int found = total;
+  for (int i = threadIdx.x; i < found; i += kThreads) {
+    const uint64_t key = all[i];
+    int place = 0;
+    for (int j = 0; j < found; ++j) place += all[j] > key;
+    if (place < count) list[place] = key;
+  }
+  for (int i = found + threadIdx.x; i < count; i += kThreads) list[i] = 0;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < kThreads / 32; ++i) s += warp_sum[i];
-    stats[blockIdx.x] = Stats{m, s};
+    for (int i = 1; i < kWarps; ++i) s += warp_sum[i];
+    stats[blockIdx.x] = Stats{m, s, to, 0};
   }
 }
 
@@ -242,18 +318,19 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
   return a.total > b.total || (a.total == b.total && a.place < b.place);
 }
 
-// One group: its beams' lists joined.  At most count lists have a first entry among
-// the count best first entries, and only they can hold one of the count best
-// candidates; of those, entries below the count-th first entry fall away.
+// One group: its beams' lists joined.  At least `count` entries reach a bound; what
+// lies below it (compared in fp32, which no rounding turns round) falls away.
+// Should more be left than fit, as where very many sums are equal, the choice
+// goes step by step, the best of all entries behind the last choice each time.
 __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const float* __restrict__ scores, int64_t ld_scores,
                                                              const uint64_t* __restrict__ lists,
                                                              const Stats* __restrict__ stats, int beams, int parts,
                                                              int count, float* __restrict__ values,
                                                              int64_t* __restrict__ parents,
                                                              int64_t* __restrict__ tokens) {
-  extern __shared__ Candidate found[];  // [beams * parts] first entries, then [count * count]
-  __shared__ double shift[kMaxBeams];   // score - log sum; NaN: the beam is out
-  __shared__ Candidate least;
+  __shared__ Candidate found[kPicked];
+  __shared__ double shifts[kMaxBeams];  // score - log sum; NaN: the beam is out
+  __shared__ float few[kFew];
   __shared__ int n;
   pdl_wait();
   pdl_trigger();
@@ -262,85 +339,117 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const float* __rest
   const int total_lists = beams * parts;
   lists += g * total_lists * count;
   stats += g * total_lists;
-  Candidate* firsts = found;
-  Candidate* all = found + total_lists;
-  for (int k = warp; k < beams; k += kThreads / 32) {
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, stats[k * parts + i].top);
+  // every entry of every list, a thread has every 256th: the first ones ahead of what they wait for
+  const int entries = total_lists * count;
+  constexpr int kAhead = 8;
+  uint64_t ahead[kAhead];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    double sum = 0.0;
-    for (int i = lane; i < parts; i += 32) {
-      const Stats s = stats[k * parts + i];
-      if (s.top != -INFINITY || s.sum != 0.0f) sum += (double)s.sum * exp((double)s.top - (double)top);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-      const double score = scores[g * ld_scores + k], lse = (double)top + log(sum);
-      shift[k] = isfinite(score) && isfinite(lse) ? score - lse : __longlong_as_double(0x7ff8000000000000ll);
-    }
+  for (int j = 0; j < kAhead; ++j) {
+    const int f = j * kThreads + threadIdx.x;
+    ahead[j] = f < entries ? lists[f] : 0;
   }
-  if (threadIdx.x == 0) {
-    n = 0;
-    least = Candidate{-INFINITY, ~0ull};
+  if (threadIdx.x == 0) n = 0;
+  for (int k = warp; k < beams; k += kWarps) {
+    const float score = scores[g * ld_scores + k];
+    float top = -INFINITY;
+    int shift = -0x40000000;
+    double sum = 0.0;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      const Stats s = i0 + lane < parts ? stats[k * parts + i0 + lane] : Stats{-INFINITY, 0.0f, 0, 0};
+      const bool any = s.top != -INFINITY || s.sum != 0.0f;
+      top = fmaxf(top, s.top);
+      const int to = max(shift, __reduce_max_sync(0xffffffffu, any ? s.shift : -0x40000000));
+      sum = scalbn(sum, max(shift - to, -2000)) + (any ? scalbn((double)s.sum, max(s.shift - to, -2000)) : 0.0);
+      shift = to;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    if (lane == 0) {
+      // sum 2^shift = sum exp(x (1 + off)), which exp(top off) times the sum of exp(x) is but for off (x - top)
+      const double lse = log(sum) + 0.69314718055994530942 * shift - kLog2eOff * top;
+      shifts[k] = isfinite(score) && isfinite(lse) ? score - lse : __longlong_as_double(0x7ff8000000000000ll);
+    }
   }
   __syncthreads();
-  // candidate i of list l; total -inf: none
-  auto entry = [&](int l, int i) -> Candidate {
-    const uint64_t key = lists[(int64_t)l * count + i];
-    const int k = l / parts;
-    const double t = shift[k] + (double)unordered((uint32_t)(key >> 32));
+  // entry f of the lists; total -inf: none
+  auto candidate = [&](int f, uint64_t key) -> Candidate {
+    const int k = f / (parts * count);
+    const double t = shifts[k] + (double)unordered((uint32_t)(key >> 32));
     Candidate c;
     c.total = key != 0 && isfinite(t) ? t : -INFINITY;
     c.place = (uint64_t)k << 32 | (0xffffffffu - (uint32_t)key);
     return c;
   };
-  for (int l = threadIdx.x; l < total_lists; l += kThreads) firsts[l] = entry(l, 0);
+  auto each = [&](auto&& take) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (j * kThreads < entries) take(candidate(min(j * kThreads + (int)threadIdx.x, entries - 1), ahead[j]));
+    for (int f = kAhead * kThreads + threadIdx.x; f < entries; f += kThreads) take(candidate(f, lists[f]));
+  };
+  float best = -INFINITY;
+  each([&](const Candidate& c) { best = fmaxf(best, (float)c.total); });
+  const float bound = reached_by(best, count, few);
+  each([&](const Candidate& c) {
+    if (c.total == -INFINITY || (float)c.total < bound) return;
+    const int at = atomicAdd(&n, 1);
+    if (at < kPicked) found[at] = c;
+  });
   __syncthreads();
-  for (int l = threadIdx.x; l < total_lists; l += kThreads) {
-    const Candidate mine = firsts[l];
-    int place = 0;
-    for (int j = 0; j < total_lists; ++j) place += before(firsts[j], mine);
-    if (place == count - 1 && mine.total != -INFINITY) least = mine;  // places of candidates differ
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < total_lists * count; i += kThreads) {
-    const int l = i / count;
-    if (firsts[l].total == -INFINITY || before(least, firsts[l])) continue;
-    const Candidate c = entry(l, i - l * count);
-    if (c.total != -INFINITY && !before(least, c)) all[atomicAdd(&n, 1)] = c;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const Candidate mine = all[i];
-    int place = 0;
-    for (int j = 0; j < n; ++j) place += before(all[j], mine);
-    if (place < count) {
-      values[g * count + place] = (float)mine.total;
-      parents[g * count + place] = (int64_t)(mine.place >> 32);
-      tokens[g * count + place] = (int64_t)(mine.place & 0xffffffffu);
+  float* value = values + g * count;
+  int64_t *parent = parents + g * count, *token = tokens + g * count;
+  auto put = [&](int at, const Candidate& c) {
+    value[at] = (float)c.total;
+    parent[at] = (int64_t)(c.place >> 32);
+    token[at] = (int64_t)(c.place & 0xffffffffu);
+  };
+  const int left = n;
+  if (left <= kPicked) {
+    for (int i0 = 0; i0 < left; i0 += kThreads / 4) {  // four lanes count those before a candidate
+      const int i = i0 + threadIdx.x / 4;
+      const Candidate mine = found[min(i, left - 1)];
+      int place = 0;
+#pragma unroll 4
+      for (int j = threadIdx.x & 3; j < left; j += 4) place += before(found[j], mine);
+      place += __shfl_xor_sync(0xffffffffu, place, 1);
+      place += __shfl_xor_sync(0xffffffffu, place, 2);
+      if (i < left && place < count && (threadIdx.x & 3) == 0) put(place, mine);
     }
+    for (int i = left + threadIdx.x; i < count; i += kThreads) {  // fewer candidates than asked for
+      value[i] = -INFINITY;
+      parent[i] = token[i] = -1;
+    }
+    return;
   }
-  for (int i = n + threadIdx.x; i < count; i += kThreads) {  // fewer candidates than asked for
-    values[g * count + i] = -INFINITY;
-    parents[g * count + i] = tokens[g * count + i] = -1;
+  Candidate last{INFINITY, 0};  // the candidate before
+  for (int at = 0; at < count; ++at) {
+    Candidate mine{-INFINITY, ~0ull};
+    each([&](const Candidate& c) {
+      if ((at == 0 || before(last, c)) && before(c, mine)) mine = c;
+    });
+    __syncthreads();
+    found[threadIdx.x] = mine;
+    __syncthreads();
+    for (int o = kThreads / 2; o > 0; o >>= 1) {
+      if (threadIdx.x < o && before(found[threadIdx.x + o], found[threadIdx.x])) found[threadIdx.x] = found[threadIdx.x + o];
+      __syncthreads();
+    }
+    last = found[0];
+    if (threadIdx.x == 0) put(at, last);
   }
 }
 
-// Parts of a row: enough CTAs to fill the GPU a few times over, each with at least
-// 2048 logits.
+// Parts of a row, the same for all rows, so that rows that are alike have the same
+// sum to the bit.
 int parts_of(int64_t rows, int64_t vocab) {
   int sms = 148;
   sm_count(&sms);
-  int64_t parts = (4 * sms + rows - 1) / rows;
-  if (parts > vocab / 2048) parts = vocab / 2048;
-  return (int)(parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : parts);
-}
-
-// all first entries, and count entries of each of the count best lists
-size_t pick_smem(int64_t beams, int parts, int64_t count) {
-  return (size_t)(beams * parts + count * count) * sizeof(Candidate);
+  const int64_t groups = (vocab + kGroup - 1) / kGroup;
+  int64_t n = 4 * sms / rows;
+  if (n > groups / kWarps) n = groups / kWarps;  // a warp has a group at least
+  return (int)(n < 1 ? 1 : n);
 }
 
 int check_sizes(int64_t groups, int64_t beams, int64_t vocab, int64_t count, const char* what, char* err,
@@ -374,7 +483,7 @@ extern "C" int xb_beam_select_workspace_size(int64_t groups, int64_t beams, int6
     set_err(err, errlen, "%s: null output", what);
     return XB_ERR_INVALID;
   }
-  const int64_t lists = groups * beams * (groups ? parts_of(groups * beams, vocab) : 0);
+  const int64_t lists = groups ? groups * beams * parts_of(groups * beams, vocab) : 0;
   *bytes = (size_t)(lists * (count * 8 + (int64_t)sizeof(Stats)));
   return XB_OK;
 }
@@ -416,29 +525,20 @@ extern "C" int xb_beam_select(const void* logits, const float* scores, int64_t g
   uint64_t* lists = static_cast<uint64_t*>(workspace);
   Stats* stats = reinterpret_cast<Stats*>(lists + rows * parts * count);
   cudaStream_t s = (cudaStream_t)stream;
-  const unsigned ctas = (unsigned)(rows * parts);
-  const int64_t W = dtype == XB_DT_F32 ? 4 : 8, vps = ((vocab + W - 1) / W + parts - 1) / parts;
-  const bool aligned = xb::aligned16(logits) && (rows == 1 || ld % W == 0);
-  auto scan = [&](auto kernel, auto* x) {
-    return launch_k(kernel, ctas, kThreads, 0, s, x, ld, vocab, (int)count, parts, vps, lists, stats);
-  };
-  cudaError_t e;
-  if (dtype == XB_DT_F32) {
-    const float* x = static_cast<const float*>(logits);
-    e = aligned ? scan(beam_scan_kernel<true, float>, x) : scan(beam_scan_kernel<false, float>, x);
-  } else {
-    const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(logits);
-    e = aligned ? scan(beam_scan_kernel<true, __nv_bfloat16>, x) : scan(beam_scan_kernel<false, __nv_bfloat16>, x);
-  }
-  const size_t smem = pick_smem(beams, parts, count);
-  if (e == cudaSuccess)
-    e = xb::once_per_device(reinterpret_cast<const void*>(beam_pick_kernel), xb::kOnceSmem, [&](int*) {
-      return cudaFuncSetAttribute(beam_pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  (int)pick_smem(kMaxBeams, kMaxParts, kMaxCount));
+  auto scan = [&](auto kernel, auto* x, int smem) {
+    cudaError_t e = xb::once_per_device(reinterpret_cast<const void*>(kernel), xb::kOnceSmem, [&](int*) {
+      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     });
+    return e != cudaSuccess ? e : launch_k(kernel, (unsigned)(rows * parts), kThreads, smem, s, x, ld, vocab,
+                                           (int)count, parts, lists, stats);
+  };
+  cudaError_t e = dtype == XB_DT_F32
+                      ? scan(beam_scan_kernel<float>, static_cast<const float*>(logits), Ring<float>::kSmem)
+                      : scan(beam_scan_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(logits),
+                             Ring<__nv_bfloat16>::kSmem);
   if (e == cudaSuccess)
-    e = launch_k(beam_pick_kernel, (unsigned)groups, kThreads, smem, s, scores, ld_scores, lists, stats, (int)beams,
-                 parts, (int)count, values, parents, tokens);
+    e = launch_k(beam_pick_kernel, (unsigned)groups, kThreads, 0, s, scores, ld_scores, lists, stats, (int)beams, parts,
+                 (int)count, values, parents, tokens);
   if (e != cudaSuccess) {
     set_err(err, errlen, "%s: %s", what, cudaGetErrorString(e));
     return XB_ERR_CUDA;
