@@ -264,8 +264,10 @@ def _write(b, qkv, cos, sin, H, D):
 @pytest.mark.parametrize("rope", [True, False])
 @pytest.mark.parametrize("new,past,H,KVH,page", [([1], [0], 14, 2, 16), ([1] * 40, [i * 13 for i in range(40)], 14, 2, 16),
                                                  ([70, 0, 1, 129], [5, 9, 200, 0], 12, 12, 8),
-                                                 ([3, 30], [47, 33], 9, 3, 48)])
+                                                 ([3, 30], [47, 33], 9, 3, 48),
+                                                 ([2001, 0, 1, 1, 0, 1700], [3, 2, 40, 0, 9, 16], 3, 1, 16)])
 def test_write_quantises_what_a_bf16_page_would_hold(D, rope, new, past, H, KVH, page, dtype):
+    """Few tokens have a warp each, more than a GPU's 3552 warps half of one (up to D = 256)."""
     b = Coded(dtype, new, past, H, KVH, page, seed=20, pad=3, D=D)
     plain = Batch(new, past, H, KVH, page, seed=20, pad=3, D=D)
     g = torch.Generator().manual_seed(21)
@@ -279,10 +281,10 @@ def test_write_quantises_what_a_bf16_page_would_hold(D, rope, new, past, H, KVH,
     ops.paged_rope_kv(qkv, cos, sin, want_q, plain.kp, plain.vp, plain.table_dev, plain.q_start, plain.kv_len)
     assert torch.equal(q, want_q)
     for pool, codes, byte in ((plain.kp.cpu(), want[0], want[2]), (plain.vp.cpu(), want[1], want[3])):
-        for i, n in enumerate(new):
-            for p in range(past[i], past[i] + n):
-                at = b.table[i, p // page], slice(None), p % page
-                codes[at], byte[at] = quantise(pool[at], dtype)
+        seq = torch.tensor([i for i, n in enumerate(new) for _ in range(n)])
+        p = torch.tensor([past[i] + j for i, n in enumerate(new) for j in range(n)])
+        at = b.table[seq, p // page].long(), slice(None), p % page
+        codes.view(torch.uint8)[at], byte[at] = (x.view(torch.uint8) for x in quantise(pool[at], dtype))
     for got, expect in zip((b.kp, b.vp, b.ks, b.vs), want):  # bits: what was there before too
         assert torch.equal(got.cpu().view(torch.uint8), expect.view(torch.uint8))
     assert ops.page_status() == 0

@@ -42,22 +42,33 @@ __device__ __forceinline__ float byte_inverse(int b) {
   return b == kNanByte ? 0.0f : __int_as_float((254 - b) << 23);
 }
 
-// Four codes of x 2^-e
+// Eight codes of x 2^-e (x: eight bf16 numbers in 32-bit words), |x 2^-e| < 128.5 or 512.
 template <Format F>
-__device__ __forceinline__ uint32_t encode4(float x0, float x1, float x2, float x3, float inverse) {
-  x0 *= inverse;
-  x1 *= inverse;
-  x2 *= inverse;
-  x3 *= inverse;
-  if constexpr (F == kInt8) {
-    auto whole = [](float x) -> uint32_t { return (uint32_t)__float2int_rn(fminf(fmaxf(x, -127.0f), 127.0f)) & 255u; };
-    return whole(x0) | whole(x1) << 8 | whole(x2) << 16 | whole(x3) << 24;
-  } else {
-    uint16_t lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x1), "f"(x0));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x3), "f"(x2));
-    return (uint32_t)lo | (uint32_t)hi << 16;
+__device__ __forceinline__ uint2 encode8(const uint4& x, float inverse) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t r[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      v[2 * i] = __uint_as_float(w[2 * h + i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[2 * h + i] & 0xffff0000u);
+    }
+    if constexpr (F == kInt8) {
+      // 1.5 2^23 more, a number's last byte is the nearest whole number's, to even in the middle
+      uint32_t b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(fmaf(v[i], inverse, 12582912.0f));
+      r[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    } else {
+      uint16_t lo, hi;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v[1] * inverse), "f"(v[0] * inverse));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(v[3] * inverse), "f"(v[2] * inverse));
+      r[h] = (uint32_t)lo | (uint32_t)hi << 16;
+    }
   }
+  return make_uint2(r[0], r[1]);
 }
 
 // Two e4m3 codes as fp16 (exact)
@@ -67,12 +78,23 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint16_t v) {
   return r;
 }
 
-// Two int8 codes as fp16 (exact): byte c + 128 in the low bits of 1024 is 1024 + 128 + c.
-// `x` has the sign bits flipped, `pick` places the two bytes below 0x64's.
-__device__ __forceinline__ uint32_t int8x2_to_half2(uint32_t x, uint32_t pick) {
-  const uint32_t m = __byte_perm(x, 0x64646464u, pick);
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&v);
+// Four codes in a register as fp16 pairs (exact): bytes 0 and 2, bytes 1 and 3.
+// int8: the byte c + 128 (the sign bit flipped) in the low bits of 1024 is 1152 + c.
+template <Format F>
+__device__ __forceinline__ void to_half2(uint32_t v, uint32_t& even, uint32_t& odd) {
+  if constexpr (F == kInt8) {
+    v ^= 0x80808080u;
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+    const uint32_t m0 = __byte_perm(v, 0x64646464u, 0x4240), m1 = __byte_perm(v, 0x64646464u, 0x4341);
+    const __half2 h0 = __hsub2(*reinterpret_cast<const __half2*>(&m0), bias);
+    const __half2 h1 = __hsub2(*reinterpret_cast<const __half2*>(&m1), bias);
+    even = *reinterpret_cast<const uint32_t*>(&h0);
+    odd = *reinterpret_cast<const uint32_t*>(&h1);
+  } else {
+    v = __byte_perm(v, 0, 0x3120);
+    even = e4m3x2_to_half2((uint16_t)v);
+    odd = e4m3x2_to_half2((uint16_t)(v >> 16));
+  }
 }
 
 // What four codes stand for, as bf16 (exact)

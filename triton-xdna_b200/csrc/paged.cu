@@ -101,6 +101,7 @@ struct RopeArgs {
   int64_t ld_qkv, ld_q, ld_table, rope_rows;
   int T, B, H, KVH, D, page_size, max_pages, n_pages;
   Exponents ke, ve;  // 8-bit pages only
+  int span;          // 32 or 16 lanes of a token, which groups of 8 dims of a half divide
 };
 
 // The last b with q_start[b] <= t, all lanes together (32 starts a step); empty
@@ -118,6 +119,30 @@ __device__ __forceinline__ int sequence_of(const int32_t* q_start, int B, int t,
   }
 }
 
+// The same for a lane's token t among the N from t0 on.  The next 32 starts are held
+// one a lane; where more sequences than that start among the tokens, one by one.
+template <int N>
+__device__ __forceinline__ int sequences_of(const int32_t* q_start, int B, int t0, int t, int lane) {
+  int b = sequence_of(q_start, B, t0, lane);
+  bool far = b < 0;
+  if (!far) {
+    const int start = b + 1 + lane <= B ? __ldg(q_start + b + 1 + lane) : 0x7fffffff;
+    int n = 0;
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1)
+      if (__shfl_sync(0xffffffffu, start, n + step - 1) <= t) n += step;
+    if (__shfl_sync(0xffffffffu, start, n) <= t) ++n;
+    far = n == 32;
+    b += n;
+  }
+  if (__any_sync(0xffffffffu, far))
+    for (int i = 0; i < N; ++i) {
+      const int found = sequence_of(q_start, B, t0 + i, lane);
+      if (t == t0 + i) b = found;
+    }
+  return b;
+}
+
 // One warp per packed token.  A lane keeps one group of 8 dims (and the 8 of
 // the other half they rotate with) and walks the head slots, so it reads its
 // 32 table values once; 16-byte loads and stores.  HBM-bound: every element is
@@ -132,35 +157,44 @@ __device__ __forceinline__ int sequence_of(const int32_t* q_start, int B, int t,
 // warps instead of eight 33.8 (four 34.2, 24 46.0): a CTA's place is taken again
 // as soon as its own few tokens are done.
 //
-// 8-bit pages: the lanes of a slot (a divisor of 32 of them, side by side) find its largest
-// magnitude by shuffles and store 8 codes each per half.  What is quantised is
-// the bf16 number that a bf16 page would hold.
+// 8-bit pages: the lanes of a slot (a power of two of them, side by side) find its
+// largest magnitude by shuffles and store 8 codes each per half.  What is
+// quantised is the bf16 number that a bf16 page would hold.  Instructions bound it
+// (920 a token, 0.72 issued a clock), so that many tokens go to half a warp each,
+// which shares those of the search, the page and the tables: 36500 tokens 42.3 ->
+// 37.6 us (e4m3), 42.9 -> 38.1 (int8).  Few ones have a warp each (64 tokens 7.8
+// against 9.0 with reading back).  Before that, rounding by an addition instead of
+// conversions 47.9 -> 42.9 (int8); 10 or 14 CTAs an SM instead of 12 39.0 / 39.5.
 template <Format F>
 __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a, int* __restrict__ bad) {
   pdl_wait();
   pdl_trigger();
-  const int t = blockIdx.x * 2 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (t >= a.T) return;
   const int half = a.D / 2, groups = half / 8;  // groups of 8 dims of a half; divides 32
-  const int c = (lane % groups) * 8, slot0 = lane / groups, step = 32 / groups;
-  const int slots = a.H + 2 * a.KVH;
+  const int span = F == kBf16 ? 32 : a.span, per = 32 / span;  // lanes of a token, tokens of a warp
+  const int lane = threadIdx.x & 31, in = lane & (span - 1);
+  const int t0 = (blockIdx.x * 2 + (threadIdx.x >> 5)) * per, t = t0 + lane / span;
+  if (t0 >= a.T) return;
+  const int c = (in % groups) * 8, slot0 = in / groups, step = span / groups;
+  // 8-bit pages: the key slots start a step of their own, so that no step takes both ways
+  const int pad = F == kBf16 ? 0 : (step - a.H % step) % step, slots = a.H + 2 * a.KVH;
+  auto slot_at = [&](int v) -> int { return v < a.H ? v : v < a.H + pad ? slots : v - pad; };  // `slots`: none
   const bf16* x = a.qkv + (int64_t)t * a.ld_qkv + c;
   constexpr int kAhead = 3;
   Vec16<bf16> u[kAhead], w[kAhead];
   auto load = [&](int first) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int slot = first + i * step;
-      if (slot < slots) {
+      const int slot = slot_at(first + i * step);
+      if (slot < slots && (F == kBf16 || t < a.T)) {
         u[i] = ld16_stream(x + slot * a.D);
         w[i] = ld16_stream(x + slot * a.D + half);
       }
     }
   };
   load(slot0);
-  const int b = sequence_of(a.q_start, a.B, t, lane);
-  if (b < 0) return;
+  const int b = F == kBf16 || per == 1 ? sequence_of(a.q_start, a.B, t, lane)
+                                       : sequences_of<2>(a.q_start, a.B, t0, min(t, a.T - 1), lane);
+  if (b < 0 || t >= a.T) return;
   if (b >= a.B) return;  // behind the last sequence
   const int end = __ldg(a.q_start + b + 1);
   if (end <= t) return;  // (starts that do not ascend)
@@ -169,11 +203,11 @@ __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a,
   int id = -1;
   if (pos >= 0 && slot_page < a.max_pages) id = __ldg(a.table + (int64_t)b * a.ld_table + slot_page);
   const bool page_ok = id >= 0 && id < a.n_pages;
-  if (!page_ok && lane == 0) atomicExch(bad, 1);
+  if (!page_ok && in == 0) atomicExch(bad, 1);
   if (pos < 0) return;
   const bool rotate = a.cos_t != nullptr;
   if (rotate && pos >= a.rope_rows) {
-    if (lane == 0) atomicExch(bad, 1);
+    if (in == 0) atomicExch(bad, 1);
     return;
   }
   const int row = (int)(pos - slot_page * a.page_size);
@@ -192,8 +226,8 @@ __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a,
   for (int first = slot0;;) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int slot = first + i * step;
-      if (slot >= slots) break;
+      const int slot = slot_at(first + i * step);
+      if (slot >= slots) continue;
       if (rotate && slot < a.H + a.KVH) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -211,25 +245,32 @@ __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a,
         const Pages& pg = is_k ? a.k : a.v;
         if constexpr (F != kBf16) {
           const int head = slot - a.H - (is_k ? 0 : a.KVH);
-          uint32_t top = 0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            top = max(top, max(__bfloat16_as_ushort(u[i].v[e]) & 0x7fffu, __bfloat16_as_ushort(w[i].v[e]) & 0x7fffu));
+          uint4 lo, hi;
+          memcpy(&lo, &u[i], 16);
+          memcpy(&hi, &w[i], 16);
+          // the bits of numbers without their signs are ordered as the numbers
+          uint32_t top2 = __vmaxu2(__vmaxu2(lo.x & 0x7fff7fffu, lo.y & 0x7fff7fffu),
+                                   __vmaxu2(lo.z & 0x7fff7fffu, lo.w & 0x7fff7fffu));
+          top2 = __vmaxu2(top2, __vmaxu2(__vmaxu2(hi.x & 0x7fff7fffu, hi.y & 0x7fff7fffu),
+                                         __vmaxu2(hi.z & 0x7fff7fffu, hi.w & 0x7fff7fffu)));
+          uint32_t top = max(top2 & 0xffffu, top2 >> 16);
           const uint32_t team = (0xffffffffu >> (32 - groups)) << (lane & ~(groups - 1));
           for (int o = 1; o < groups; o <<= 1) top = max(top, __shfl_xor_sync(team, top, o));
           const int byte = exponent_byte<F>(top);
           const float inverse = byte_inverse(byte);
-          float x0[8], x1[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x0[e] = byte == kNanByte ? 0.0f : __bfloat162float(u[i].v[e]);
-            x1[e] = byte == kNanByte ? 0.0f : __bfloat162float(w[i].v[e]);
+          if (F == kInt8 && byte == 248) {  // bf16's largest number, 127.5 2^121, counts as the one below it
+            auto within = [](uint32_t x) { return __vminu2(x & 0x7fff7fffu, 0x7f7e7f7eu) | (x & 0x80008000u); };
+            lo = make_uint4(within(lo.x), within(lo.y), within(lo.z), within(lo.w));
+            hi = make_uint4(within(hi.x), within(hi.y), within(hi.z), within(hi.w));
+          }
+          uint2 c0 = make_uint2(0, 0), c1 = c0;  // byte 255: zeros
+          if (byte != kNanByte) {
+            c0 = encode8<F>(lo, inverse);
+            c1 = encode8<F>(hi, inverse);
           }
           uint8_t* at = reinterpret_cast<uint8_t*>(pg.p) + id * pg.page + head * pg.head + row * pg.row + c;
-          *reinterpret_cast<uint2*>(at) = make_uint2(encode4<F>(x0[0], x0[1], x0[2], x0[3], inverse),
-                                                     encode4<F>(x0[4], x0[5], x0[6], x0[7], inverse));
-          *reinterpret_cast<uint2*>(at + half) = make_uint2(encode4<F>(x1[0], x1[1], x1[2], x1[3], inverse),
-                                                            encode4<F>(x1[4], x1[5], x1[6], x1[7], inverse));
+          *reinterpret_cast<uint2*>(at) = c0;
+          *reinterpret_cast<uint2*>(at + half) = c1;
           const Exponents& ex = is_k ? a.ke : a.ve;
           if (c == 0) ex.p[id * ex.page + head * ex.head + row] = (uint8_t)byte;
           continue;
@@ -240,7 +281,7 @@ __global__ void __launch_bounds__(64, 12) paged_rope_kv_kernel(const RopeArgs a,
       st16_stream(dst + half + c, w[i]);
     }
     first += kAhead * step;
-    if (first >= slots) break;
+    if (first >= slots + pad) break;
     load(first);
   }
 }
@@ -257,45 +298,73 @@ struct ReadArgs {
 };
 
 // k_out[t] and v_out[t]: what the pages hold at the position of packed token t
-// (the inverse of the write).  One warp per token, 8 elements a lane.
+// (the inverse of the write).  A warp takes 8 tokens: its lanes find their sequences and pages
+// together, then fetch all tokens' elements, 8 a lane, before the first is
+// stored.  HBM-bound; with a warp a token the chain start -> length -> table ->
+// codes was most of the time (100000 tokens 31.9 us).
+constexpr int kReadTokens = 8;
 template <Format F>
 __global__ void __launch_bounds__(256) paged_read_kv_kernel(const ReadArgs a, int* __restrict__ bad) {
   pdl_wait();
   pdl_trigger();
-  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (t >= a.T) return;
-  const int b = sequence_of(a.q_start, a.B, t, lane);
-  if (b < 0 || b >= a.B) return;
-  const int end = __ldg(a.q_start + b + 1);
-  if (end <= t || __ldg(a.q_start + b) > t) return;  // (starts that do not ascend)
-  const int64_t pos = (int64_t)__ldg(a.kv_len + b) - ((int64_t)end - t);
-  const int64_t slot_page = pos >= 0 ? (int64_t)((uint32_t)pos / (uint32_t)a.page_size) : -1;  // pos < 2^31
-  int id = -1;
-  if (pos >= 0 && slot_page < a.max_pages) id = __ldg(a.table + (int64_t)b * a.ld_table + slot_page);
-  const bool page_ok = id >= 0 && id < a.n_pages;  // otherwise zeros
-  if (!page_ok && lane == 0) atomicExch(bad, 1);
-  const int row = (int)(pos - slot_page * a.page_size);
-  const int per = a.D / 8, items = a.KVH * per;
-  for (int i = lane; i < 2 * items; i += 32) {
+  const int64_t first = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * kReadTokens;
+  if (first >= a.T) return;
+  const int t0 = (int)first, t = (int)min(first + (lane & (kReadTokens - 1)), (int64_t)a.T - 1);  // lanes past 8 repeat
+  const int b = sequences_of<kReadTokens>(a.q_start, a.B, t0, t, lane);
+  int id = -2, row = 0;  // -2: of no sequence, left alone; -1: no page, zeros
+  if (b >= 0 && b < a.B) {
+    const int end = __ldg(a.q_start + b + 1);
+    if (end > t && __ldg(a.q_start + b) <= t) {  // (starts that do not ascend)
+      const int64_t pos = (int64_t)__ldg(a.kv_len + b) - ((int64_t)end - t);
+      const int64_t page = pos >= 0 ? (int64_t)((uint32_t)pos / (uint32_t)a.page_size) : -1;  // pos < 2^31
+      id = -1;
+      if (pos >= 0 && page < a.max_pages) id = __ldg(a.table + (int64_t)b * a.ld_table + page);
+      if (id < 0 || id >= a.n_pages) id = -1;
+      row = (int)(pos - page * a.page_size);
+      if (id < 0 && lane < kReadTokens) atomicExch(bad, 1);
+    }
+  }
+  const int per = a.D / 8, items = a.KVH * per, count = (int)min(a.T - first, (int64_t)kReadTokens);
+  for (int i0 = 0; i0 < 2 * items; i0 += 32) {
+    const int i = i0 + lane;
     const bool is_v = i >= items;
     const int j = is_v ? i - items : i, head = j / per, d = (j - head * per) * 8;
     const Pages& pg = is_v ? a.v : a.k;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (page_ok) {
-      const int64_t at = id * pg.page + head * pg.head + row * pg.row + d;
-      if constexpr (F == kBf16) {
-        x = __ldcs(reinterpret_cast<const uint4*>(pg.p + at));
-      } else {
-        const Exponents& ex = is_v ? a.ve : a.ke;
-        const float scale = byte_scale(ex.p[id * ex.page + head * ex.head + row]);
-        const uint2 c = __ldcs(reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(pg.p) + at));
-        const uint2 lo = decode4<F>(c.x, scale), hi = decode4<F>(c.y, scale);
-        x = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    const Exponents& ex = is_v ? a.ve : a.ke;
+    const int64_t at = head * pg.head + d, e_at = head * ex.head;
+    uint4 x[kReadTokens];
+    uint32_t e[kReadTokens];
+#pragma unroll
+    for (int u = 0; u < kReadTokens; ++u) {
+      const int uid = __shfl_sync(0xffffffffu, id, u), urow = __shfl_sync(0xffffffffu, row, u);
+      x[u] = make_uint4(0, 0, 0, 0);
+      e[u] = 0;
+      if (i < 2 * items && uid >= 0) {
+        const int64_t from = uid * pg.page + urow * pg.row + at;
+        if constexpr (F == kBf16) {
+          x[u] = __ldcs(reinterpret_cast<const uint4*>(pg.p + from));
+        } else {
+          const uint2 c = __ldcs(reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(pg.p) + from));
+          x[u].x = c.x, x[u].y = c.y;
+          e[u] = __ldg(ex.p + uid * ex.page + urow + e_at);
+        }
       }
     }
-    bf16* out = is_v ? a.v_out + (int64_t)t * a.ld_v : a.k_out + (int64_t)t * a.ld_k;
-    __stcs(reinterpret_cast<uint4*>(out + head * a.D + d), x);
+    bf16* out = (is_v ? a.v_out + first * a.ld_v : a.k_out + first * a.ld_k) + head * a.D + d;
+    const int64_t ld = is_v ? a.ld_v : a.ld_k;
+#pragma unroll
+    for (int u = 0; u < kReadTokens; ++u) {
+      const int uid = __shfl_sync(0xffffffffu, id, u);
+      if (u < count && i < 2 * items && uid != -2) {
+        if constexpr (F != kBf16) {
+          const float scale = byte_scale((int)e[u]);
+          const uint2 lo = decode4<F>(x[u].x, scale), hi = decode4<F>(x[u].y, scale);
+          x[u] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+        __stcs(reinterpret_cast<uint4*>(out + u * ld), x[u]);
+      }
+    }
   }
 }
 
@@ -478,16 +547,24 @@ constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared m
 // Warps x buffers of the 8-row kernel, 64 sequences of 576 keys / 160 long ones:
 // 8 x 2 11.0 / 86.1 us, 8 x 3 11.0 / 90.2, 12 x 2 12.1 / 87.4, 16 x 1 13.1 / 86.5,
 // 12 x 1 12.3 / 85.8, 8 x 1 11.1 / 93.8, 6 x 3 11.3 / 91.7, 4 x 4 12.6 / 116.
-template <int ROWS, Format F>
+// 8-bit pages: tiles of 64 keys and, in the 8-row kernel, 12 warps; with at most 96
+// keys a warp (SHORT) tiles of 32 and 8 warps.  GPU us of e4m3 / int8, 8 x 32 / 8 x 64 /
+// 12 x 64 / 16 x 64 with one buffer: one sequence of 512 keys 8.1 / 9.3 / 10.0 /
+// 11.1, 64 of 513-640 12.3 / 12.4 / 13.9 / 14.9, 128 of them 16.2 / 15.8 / 15.8 /
+// 16.1, 160 of 200-30000 84.4 / 64.4 / 56.3 / 55.6 (e4m3), 85.4 / 67.1 / 57.4 / 57.6
+// (int8).  Either way 32 keys are computed at a time: code for 64 is fetched in more
+// time than it saves.
+template <int ROWS, Format F, bool SHORT>
 struct FewCfg {
-  static constexpr int kWarps = kFewWarps, kBufs = 2;
+  static constexpr bool kLong = F != kBf16 && !SHORT;
+  static constexpr int kWarps = kLong && ROWS == 8 ? 12 : kFewWarps, kBufs = 2;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kTile = F == kBf16 ? kTK : kFewTK8;       // keys
+  static constexpr int kTile = kLong ? kFewTK8 : kTK;  // keys
   static constexpr int kRowBytes = F == kBf16 ? kHD * 2 : kHD;
+  static constexpr int kTileBytes = kTile * kRowBytes;  // of K, and of V
   static constexpr int kRing = kBufs * 2 * kTileBytes;  // of one warp
   static constexpr int kHead = ROWS * kPartLd * 4;      // a warp's kind 0 partial; kind 1 goes into its own ring
   static constexpr int kSmem = kWarps * (kRing + kHead) + 1024;
-  static_assert(kTile * kRowBytes == kTileBytes, "a tile");
   static_assert(kHead <= kRing && kSmem <= 224 * 1024, "shared memory");
 };
 
@@ -528,44 +605,22 @@ __device__ __forceinline__ uint32_t pack2_half(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// 8 bytes (zeros where !ok) into shared memory, without a wait
-__device__ __forceinline__ void copy8_async(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
+// 8 bytes into shared memory, without a wait
+__device__ __forceinline__ void copy8_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 // An arrival on `bar` once this thread's copies so far have landed (counted at the barrier's set-up)
 __device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
+__device__ __forceinline__ uint32_t lds_u32(uint32_t addr) {
   uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-
-// Codes in a 32-bit register as fp16 pairs: bytes (0, 1) and (2, 3) ...
-template <Format F>
-__device__ __forceinline__ void halves_side_by_side(uint32_t v, uint32_t& lo, uint32_t& hi) {
-  if constexpr (F == kInt8) {
-    v ^= 0x80808080u;
-    lo = int8x2_to_half2(v, 0x4140);
-    hi = int8x2_to_half2(v, 0x4342);
-  } else {
-    lo = e4m3x2_to_half2((uint16_t)v);
-    hi = e4m3x2_to_half2((uint16_t)(v >> 16));
-  }
-}
-// ... or (0, 2) and (1, 3)
-template <Format F>
-__device__ __forceinline__ void halves_across(uint32_t v, uint32_t& even, uint32_t& odd) {
-  if constexpr (F == kInt8) {
-    v ^= 0x80808080u;
-    even = int8x2_to_half2(v, 0x4240);
-    odd = int8x2_to_half2(v, 0x4341);
-  } else {
-    v = __byte_perm(v, 0, 0x3120);
-    even = e4m3x2_to_half2((uint16_t)v);
-    odd = e4m3x2_to_half2((uint16_t)(v >> 16));
-  }
+// What a sum of weights divides by: nothing seen gives zeros; a negative sum comes of a NaN among 8-bit values
+__device__ __forceinline__ float inverse_of(float l) {
+  return l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : __int_as_float(0x7fc00000);
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -607,12 +662,12 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int token, int kvh
   *reinterpret_cast<uint2*>(op) = pk;
 }
 
-template <int ROWS, typename I, Format F>
-__global__ void __launch_bounds__(FewCfg<ROWS, F>::kThreads, 1) paged_attn_few_kernel(const __grid_constant__ KvMaps maps,
+template <int ROWS, typename I, Format F, bool SHORT>
+__global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT>::kThreads, 1) paged_attn_few_kernel(const __grid_constant__ KvMaps maps,
                                                                         const AttnArgs a) {
-  using C = FewCfg<ROWS, F>;
+  using C = FewCfg<ROWS, F, SHORT>;
   constexpr bool kCoded = F != kBf16;
-  constexpr int kWarps = C::kWarps, kBufs = C::kBufs, TK = C::kTile, MT = TK / 16;
+  constexpr int kWarps = C::kWarps, kBufs = C::kBufs, TK = C::kTile, MT = kTK / 16;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kWarps][kBufs];
   __shared__ I sums[2][kWarps];
@@ -698,7 +753,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F>::kThreads, 1) paged_attn_few_k
       const int have = min(TK, si.keys - ni * TK);
       const int nb = (have + a.box_rows - 1) / a.box_rows;
       if (leader) mbar_arrive_expect_tx(&full[warp][buf], (uint32_t)(nb * a.box_rows * C::kRowBytes * 2));
-      uint32_t dst = ring + buf * 2 * kTileBytes;
+      uint32_t dst = ring + buf * 2 * C::kTileBytes;
       for (int i = 0; i < nb; ++i) {
         if (pi - win >= 32u) window(pi);
         int id = __shfl_sync(0xffffffffu, win_id, (int)(pi - win));
@@ -708,15 +763,15 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F>::kThreads, 1) paged_attn_few_k
         }
         if (leader) {
           tma_load_4d(dst, &maps.k, &full[warp][buf], 0, row, si.kvh, id);
-          tma_load_4d(dst + kTileBytes, &maps.v, &full[warp][buf], 0, row, si.kvh, id);
+          tma_load_4d(dst + C::kTileBytes, &maps.v, &full[warp][buf], 0, row, si.kvh, id);
         }
-        if constexpr (kCoded) {  // 8 positions a lane, K and V by turns
+        if constexpr (kCoded) {  // exponents: 8 positions a lane, K and V by turns
           if (lane < a.box_rows / 4) {
             const Exponents& ex = lane & 1 ? a.ve : a.ke;
-            const bool ok = id < a.n_pages;
             const int at = (lane >> 1) * 8;
-            copy8_async(smem_u32(&exps[warp][buf][lane & 1][i * a.box_rows + at]),
-                        ex.p + (ok ? id * ex.page + si.kvh * ex.head + row + at : 0), ok);
+            const uint32_t to = smem_u32(&exps[warp][buf][lane & 1][i * a.box_rows + at]);
+            if (id < a.n_pages) copy8_async(to, ex.p + id * ex.page + si.kvh * ex.head + row + at);
+            else asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(to), "r"(0x7f7f7f7f) : "memory");  // 2^0
           }
         }
         dst += a.box_rows * C::kRowBytes;
@@ -735,8 +790,8 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F>::kThreads, 1) paged_attn_few_k
     float cq[NT][2];  // 8-bit pages: what turns a row's products into scores, in log2 units
     auto load_q = [&]() {
       if constexpr (kCoded) {
-        // A dim's place in the product is K's: four in a row a lane.  As fp16, scaled by a power of two to magnitudes
-        // below 2^14: exact, but what is 2^-28 of a row's largest element.
+        // A dim's place in the product is K's: four in a row a lane, even and odd ones apart.  As fp16, scaled by a power
+        // of two to magnitudes below 2^14: exact, but what is 2^-28 of a row's largest element.
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const int r = 8 * n + g, tk = row_token(a, r);
@@ -755,26 +810,30 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F>::kThreads, 1) paged_attn_few_k
           const float mul = __int_as_float((267 - E) << 23), back = __int_as_float((E - 13) << 23);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            qb[n][c][0] = pack2_half(__uint_as_float(x[c].x << 16) * mul, __uint_as_float(x[c].x & 0xffff0000u) * mul);
-            qb[n][c][1] = pack2_half(__uint_as_float(x[c].y << 16) * mul, __uint_as_float(x[c].y & 0xffff0000u) * mul);
+            qb[n][c][0] = pack2_half(__uint_as_float(x[c].x << 16) * mul, __uint_as_float(x[c].y << 16) * mul);
+            qb[n][c][1] = pack2_half(__uint_as_float(x[c].x & 0xffff0000u) * mul,
+                                     __uint_as_float(x[c].y & 0xffff0000u) * mul);
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) cq[n][e] = a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
         }
-        return;
-      }
+      } else {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int r = 8 * n + g, tk = row_token(a, r);
-        const bf16* p = a.q + (int64_t)(sc.token + tk) * a.ld_q + (sc.kvh * a.n_rep + r - tk * a.n_rep) * kHD + 2 * t;
-        const bool in = r < sc.rows;
+        for (int n = 0; n < NT; ++n) {
+          const int r = 8 * n + g, tk = row_token(a, r);
+          const bf16* p = a.q + (int64_t)(sc.token + tk) * a.ld_q + (sc.kvh * a.n_rep + r - tk * a.n_rep) * kHD + 2 * t;
+          const bool in = r < sc.rows;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          qb[n][kk][0] = in ? *reinterpret_cast<const uint32_t*>(p + kk * 16) : 0u;
-          qb[n][kk][1] = in ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 8) : 0u;
+          for (int kk = 0; kk < 4; ++kk) {
+            qb[n][kk][0] = in ? *reinterpret_cast<const uint32_t*>(p + kk * 16) : 0u;
+            qb[n][kk][1] = in ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 8) : 0u;
+          }
         }
       }
     };
+    // 8-bit pages: which of 32 rows is row i of the products' j-th group of 8 keys.  A thread's keys, i = g for all j, are
+    // then four in a row, and the rows of a group differ in their last three bits, by which the swizzle spreads them.
+    auto row_of = [](int j, int i) -> int { return 4 * i + (j ^ (i >> 1)); };
     int pos[NT][2], first_pos = 0;  // the last keys that this thread's rows see, and that every row sees
     int tile = 0;
     float o[NT][4][4], m[NT][2], l[NT][2];
@@ -805,169 +864,206 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F>::kThreads, 1) paged_attn_few_k
           dead = true;
           break;
         }
-        const int k0 = tile * TK;
-        const uint32_t sk = ring + buf * 2 * kTileBytes, sv = sk + kTileBytes;
-        const int have = min(TK, sc.keys - k0);
+        const uint32_t tile_k = ring + buf * 2 * C::kTileBytes, tile_v = tile_k + C::kTileBytes;
+        const int have = min(TK, sc.keys - tile * TK);
         if (F != kInt8 && have < TK) {
           // values behind the last key hold whatever the page or buffer held: a
           // NaN there would survive its zero weight (int8 codes have none)
           for (int i = have * (C::kRowBytes / 16) + lane; i < TK * (C::kRowBytes / 16); i += 32)
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sv + i * 16), "r"(0) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile_v + i * 16), "r"(0) : "memory");
           fence_proxy_async_smem();  // before a later TMA write to the buffer
           __syncwarp();
         }
-        // S^T = K Q^T: keys are the MMA's 16 rows, query rows its 8 columns
-        float s[NT][MT][4];
+        // 32 keys at a time: code for 64 is longer than what a short call saves by it
+#pragma unroll 1
+        for (int part0 = 0; part0 < have; part0 += kTK) {
+          const int k0 = tile * TK + part0;
+          const uint32_t sk = tile_k + part0 * C::kRowBytes, sv = tile_v + part0 * C::kRowBytes;
+          // S^T = K Q^T: keys are the MMA's 16 rows, query rows its 8 columns
+          float s[NT][MT][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) s[n][mt][0] = s[n][mt][1] = s[n][mt][2] = s[n][mt][3] = 0.0f;
+            for (int mt = 0; mt < MT; ++mt) s[n][mt][0] = s[n][mt][1] = s[n][mt][2] = s[n][mt][3] = 0.0f;
           if constexpr (kCoded) {
-            // 16-byte chunk c of row r at c ^ (r / 2 & 3).  A lane's 32 bits of a row are four dims in a row, two for
-            // either half of the 16 of a step.
+            // 16-byte chunk c of row r at c ^ (r / 2 & 3).  A lane's 32 bits of a row are four dims in a row, the even two
+            // for one half of the 16 of a step, the odd two for the other.
+            uint32_t x[2][MT][4];
 #pragma unroll
-            for (int cc = 0; cc < 2; ++cc) {
-              const int mi = lane >> 3, r = mt * 16 + (mi & 1) * 8 + (lane & 7), c = 2 * cc + (mi >> 1);
-              uint32_t x[4], ka[2][4];
-              ldsm4(x, sk + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
+            for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) halves_side_by_side<F>(x[i], ka[i >> 1][i & 1], ka[i >> 1][2 + (i & 1)]);
+              for (int mt = 0; mt < MT; ++mt) {
+                const int mi = lane >> 3, c = 2 * cc + (mi >> 1), r = row_of(2 * mt + (mi & 1), lane & 7);
+                ldsm4(x[cc][mt], sk + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
+              }
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
               for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-                  mma_16816_half(s[n][mt], ka[i], qb[n][2 * cc + i][0], qb[n][2 * cc + i][1]);
-            }
-            continue;
+                for (int mt = 0; mt < MT; ++mt) {
+                  uint32_t ka[4];
+                  to_half2<F>(x[cc][mt][2 * i], ka[0], ka[2]);
+                  to_half2<F>(x[cc][mt][2 * i + 1], ka[1], ka[3]);
+#pragma unroll
+                  for (int n = 0; n < NT; ++n)
+                    mma_16816_half(s[n][mt], ka, qb[n][2 * cc + i][0], qb[n][2 * cc + i][1]);
+                }
+          } else {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) {
+                const int mi = lane >> 3, r = mt * 16 + (mi & 1) * 8 + (lane & 7), c = 2 * kk + (mi >> 1);
+                uint32_t ka[4];
+                ldsm4(ka, sk + r * 128 + ((c ^ (r & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_16816(s[n][mt], ka, qb[n][kk][0], qb[n][kk][1]);
+              }
           }
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const int mi = lane >> 3, r = mt * 16 + (mi & 1) * 8 + (lane & 7), c = 2 * kk + (mi >> 1);
-            uint32_t ka[4];
-            ldsm4(ka, sk + r * 128 + ((c ^ (r & 7)) << 4));
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16816(s[n][mt], ka, qb[n][kk][0], qb[n][kk][1]);
-          }
-        }
-        // 8-bit pages: with K's exponent e_k and V's e_v a score is S c 2^e_k (c = cq), and e_v joins it: the weight
-        // 2^(score + e_v - m) of a code of V is at most one and fits fp16 whatever the values' sizes; times 2^-e_v
-        // it is the key's share of the denominator.
-        float fv[kCoded ? MT : 1][2];  // 2^-e_v
-        if constexpr (kCoded) {
-          const uint32_t at = smem_u32(&exps[warp][buf][0][g]);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int bk = (int)lds_u8(at + mt * 16 + h * 8), bv = (int)lds_u8(at + TK + mt * 16 + h * 8);
-              const float kf = byte_scale(bk), ev = (float)(bv - 127);
-              fv[mt][h] = bv == kNanByte ? __int_as_float(0x7fc00000) : __int_as_float((254 - bv) << 23);
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) s[n][mt][2 * h + e] = fmaf(s[n][mt][2 * h + e], kf * cq[n][e], ev);
-            }
-        }
-        const bool edge = k0 + TK - 1 > first_pos;
-        if (edge) {  // some row does not see the whole tile
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = k0 + mt * 16 + g + (e >> 1) * 8;
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-                if (key > pos[n][e & 1]) s[n][mt][e] = -INFINITY;
-            }
-        }
-        uint32_t pb[NT][2 * MT];  // P as the B operand of O^T = V^T P^T, 8 keys each
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float base[2], al[2];
-          bool moved = false;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            // raw scores: the scale is positive, so their maximum scales to the scaled ones'
-            float mx = fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2]));
-#pragma unroll
-            for (int mt = 2; mt < MT; ++mt) mx = fmaxf(mx, fmaxf(s[n][mt][e], s[n][mt][e + 2]));
-#pragma unroll
-            for (int o_ = 4; o_ <= 16; o_ <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o_));
-            const float mn = fmaxf(m[n][e], kCoded ? mx : mx * a.scale_log2);
-            base[e] = mn == -INFINITY ? 0.0f : mn;
-            al[e] = ex2_approx(m[n][e] - base[e]);
-            moved |= mn > m[n][e];
-            m[n][e] = mn;
-          }
-          if (__any_sync(0xffffffffu, moved)) {
-            l[n][0] *= al[0];
-            l[n][1] *= al[1];
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-              o[n][mt][0] *= al[0];
-              o[n][mt][1] *= al[1];
-              o[n][mt][2] *= al[0];
-              o[n][mt][3] *= al[1];
-            }
-          }
+          // 8-bit pages: with K's exponent e_k and V's e_v a score is S c 2^e_k (c = cq), and e_v joins it: the weight
+          // 2^(score + e_v - m) of a code of V is at most one and fits fp16 whatever the values' sizes; times 2^-e_v
+          // it is the key's share of the denominator.
+          float fv[kCoded ? MT : 1][2];  // 2^-e_v
           if constexpr (kCoded) {
-            // up to 2^14, so that fp16 holds weights from 2^-38 of the largest on; numerator and denominator alike
+            // the bytes of this thread's keys, one of each group: the XOR of their order undone by a byte move
+            const uint32_t at = smem_u32(&exps[warp][buf][0][part0 + 4 * g]), pick = 0x3210u ^ (uint32_t)(g >> 1) * 0x1111u;
+            const uint32_t wk = __byte_perm(lds_u32(at), 0, pick), wv = __byte_perm(lds_u32(at + TK), 0, pick);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int j = 2 * mt + h, by = 8 * j;
+                auto exponent = [&](uint32_t w) { return (by == 24 ? w >> 1 : w << (23 - by)) & 0x7f800000u; };
+                // byte 255: an infinite factor, and the codes are zeros: NaN
+                const float kf = __uint_as_float(exponent(wk));
+                // the byte as a float: below 2^23's bits
+                const float ev = __uint_as_float(__byte_perm(wv, 0x4b000000u, 0x7650u | j)) - (8388608.0f + 127.0f);
+                // byte 255: -infinity, which turns the sum negative or NaN
+                fv[mt][h] = __uint_as_float(0x7f000000u - exponent(wv));
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) s[n][mt][2 * h + e] = fmaf(s[n][mt][2 * h + e], kf * cq[n][e], ev);
+              }
+          }
+          const bool edge = k0 + kTK - 1 > first_pos;
+          if (edge) {  // some row does not see the whole tile
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float w = ex2_approx(s[n][mt][e] - (base[e & 1] - 14.0f));
-                // an unseen key's exponent may be anything
-                const float f = edge && s[n][mt][e] == -INFINITY ? 0.0f : fv[mt][e >> 1];
-                l[n][e & 1] = fmaf(w, f, l[n][e & 1]);
-                s[n][mt][e] = w;
-              }
-              pb[n][2 * mt] = transpose8(pack2_half(s[n][mt][0], s[n][mt][1]));
-              pb[n][2 * mt + 1] = transpose8(pack2_half(s[n][mt][2], s[n][mt][3]));
-            }
-            continue;
-          }
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s[n][mt][e] = ex2_approx(fmaf(s[n][mt][e], a.scale_log2, -base[e & 1]));
-              l[n][e & 1] += s[n][mt][e];
-            }
-            pb[n][2 * mt] = transpose8(pack2(s[n][mt][0], s[n][mt][1]));
-            pb[n][2 * mt + 1] = transpose8(pack2(s[n][mt][2], s[n][mt][3]));
-          }
-        }
-        if constexpr (kCoded) {
-          // A lane's 32 bits are dims 2 g and 2 g + 1 of a chunk, keys 2 t and 2 t + 1: row g of the product is the even dim,
-          // row g + 8 the odd one.
-#pragma unroll
-          for (int ks = 0; ks < MT; ++ks)
-#pragma unroll
-            for (int cc = 0; cc < 2; ++cc) {
-              const int mi = lane >> 3, r = ks * 16 + (mi & 1) * 8 + (lane & 7), c = 2 * cc + (mi >> 1);
-              uint32_t x[4], va[2][4];
-              ldsm4_t(x, sv + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                halves_across<F>(x[i], va[i >> 1][2 * (i & 1)], va[i >> 1][2 * (i & 1) + 1]);
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
+                const int key = k0 + (kCoded ? row_of(2 * mt + (e >> 1), g) : mt * 16 + g + (e >> 1) * 8);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                  mma_16816_half(o[n][2 * cc + i], va[i], pb[n][2 * ks], pb[n][2 * ks + 1]);
-            }
-        }
-#pragma unroll
-        for (int ks = 0; ks < (kCoded ? 0 : 2); ++ks)
-#pragma unroll
-          for (int mt = 0; mt < 4; ++mt) {  // dims 16 mt .. 16 mt + 15
-            const int mi = lane >> 3, r = ks * 16 + (mi >> 1) * 8 + (lane & 7), c = 2 * mt + (mi & 1);
-            uint32_t va[4];
-            ldsm4_t(va, sv + r * 128 + ((c ^ (r & 7)) << 4));
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16816(o[n][mt], va, pb[n][2 * ks], pb[n][2 * ks + 1]);
+                  if (key > pos[n][e & 1]) s[n][mt][e] = -INFINITY;
+                // what no row sees may have any exponent, also one that is NaN times a weight of zero
+                if (kCoded && key >= sc.keys) fv[mt][e >> 1] = 0.0f;
+              }
           }
+          uint32_t pb[NT][2 * MT];  // P as the B operand of O^T = V^T P^T, 8 keys each
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float mx[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              mx[e] = fmaxf(fmaxf(s[n][0][e], s[n][0][e + 2]), fmaxf(s[n][1][e], s[n][1][e + 2]));
+#pragma unroll
+              for (int mt = 2; mt < MT; ++mt) mx[e] = fmaxf(mx[e], fmaxf(s[n][mt][e], s[n][mt][e + 2]));
+            }
+            // Over 8-bit pages a row's base moves only where a score is above it by more than one: fp16 has the room, and
+            // most tiles need no exchange between lanes.
+            float base[2], al[2] = {1.0f, 1.0f};
+            bool moved = !kCoded || __any_sync(0xffffffffu, mx[0] > m[n][0] + 1.0f || mx[1] > m[n][1] + 1.0f);
+            if (moved) {
+              moved = false;
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                // raw scores: the scale is positive, so their maximum scales to the scaled ones'
+#pragma unroll
+                for (int o_ = 4; o_ <= 16; o_ <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o_));
+                const float mn = fmaxf(m[n][e], kCoded ? mx[e] : mx[e] * a.scale_log2);
+                base[e] = mn == -INFINITY ? 0.0f : mn;
+                al[e] = ex2_approx(m[n][e] - base[e]);
+                moved |= mn > m[n][e];
+                m[n][e] = mn;
+              }
+              if (__any_sync(0xffffffffu, moved)) {
+                l[n][0] *= al[0];
+                l[n][1] *= al[1];
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt) {
+                  o[n][mt][0] *= al[0];
+                  o[n][mt][1] *= al[1];
+                  o[n][mt][2] *= al[0];
+                  o[n][mt][3] *= al[1];
+                }
+              }
+            }
+            if constexpr (kCoded) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) base[e] = m[n][e] == -INFINITY ? 0.0f : m[n][e];
+            }
+            if constexpr (kCoded) {
+              // up to 2^15, the largest at least 2^14, so that fp16 holds weights from 2^-38 of it on; numerator and
+              // denominator alike
+              const float up[2] = {base[0] - 14.0f, base[1] - 14.0f};
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  s[n][mt][e] = ex2_approx(s[n][mt][e] - up[e & 1]);
+                  l[n][e & 1] = fmaf(s[n][mt][e], fv[mt][e >> 1], l[n][e & 1]);
+                }
+                pb[n][2 * mt] = transpose8(pack2_half(s[n][mt][0], s[n][mt][1]));
+                pb[n][2 * mt + 1] = transpose8(pack2_half(s[n][mt][2], s[n][mt][3]));
+              }
+            } else {
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  s[n][mt][e] = ex2_approx(fmaf(s[n][mt][e], a.scale_log2, -base[e & 1]));
+                  l[n][e & 1] += s[n][mt][e];
+                }
+                pb[n][2 * mt] = transpose8(pack2(s[n][mt][0], s[n][mt][1]));
+                pb[n][2 * mt + 1] = transpose8(pack2(s[n][mt][2], s[n][mt][3]));
+              }
+            }
+          }
+          if constexpr (kCoded) {
+            // A lane's 32 bits are dims 2 g and 2 g + 1 of a chunk, keys 2 t and 2 t + 1: row g of the product is the even dim,
+            // row g + 8 the odd one.
+#pragma unroll
+            for (int ks = 0; ks < MT; ++ks)
+#pragma unroll
+              for (int cc = 0; cc < 2; ++cc) {
+                const int mi = lane >> 3, c = 2 * cc + (mi >> 1), r = row_of(2 * ks + (mi & 1), lane & 7);
+                uint32_t va[2][4];
+                uint32_t x[4];
+                ldsm4_t(x, sv + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  to_half2<F>(x[i], va[i >> 1][2 * (i & 1)], va[i >> 1][2 * (i & 1) + 1]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                  for (int n = 0; n < NT; ++n)
+                    mma_16816_half(o[n][2 * cc + i], va[i], pb[n][2 * ks], pb[n][2 * ks + 1]);
+              }
+          } else {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+              for (int mt = 0; mt < 4; ++mt) {  // dims 16 mt .. 16 mt + 15
+                const int mi = lane >> 3, r = ks * 16 + (mi >> 1) * 8 + (lane & 7), c = 2 * mt + (mi & 1);
+                uint32_t va[4];
+                ldsm4_t(va, sv + r * 128 + ((c ^ (r & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_16816(o[n][mt], va, pb[n][2 * ks], pb[n][2 * ks + 1]);
+              }
+          }
+        }
         ++use;
         ++tile;
         __syncwarp();  // the buffer is read: it takes a tile further on
@@ -1006,7 +1102,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F>::kThreads, 1) paged_attn_few_k
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float inv = l[n][e] == 0.0f ? 0.0f : 1.0f / l[n][e];  // no key: zeros
+            const float inv = inverse_of(l[n][e]);
             const int r = 8 * n + 2 * t + e, tk = tok[n][e];
             bf16* p = a.out + (int64_t)(sc.token + tk) * a.ld_out + (sc.kvh * a.n_rep + r - tk * a.n_rep) * kHD + 2 * g;
 #pragma unroll
@@ -1099,7 +1195,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F>::kThreads, 1) paged_attn_few_k
         M = mn;
       }
       if (whole) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = inverse_of(l);
         store_out4(a, p.token, p.kvh, r, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
       } else {
         float* out_part = a.ws + (2 * (int64_t)blockIdx.x + (c >= 0)) * part_floats(kFewRows);
@@ -1736,7 +1832,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
     M = mn;
   }
   if (ln == 0 && r < m.rows) {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = inverse_of(l);
     store_out4(a, m.token, m.kvh, r, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   }
 }
@@ -1952,15 +2048,23 @@ cudaError_t launch_main(void (*kernel)(M, AttnArgs), int ctas, int threads, int 
   return e != cudaSuccess ? e : launch_k(kernel, (unsigned)ctas, threads, smem, s, maps, a);
 }
 
-template <int ROWS, typename I, Format F>
+template <int ROWS, typename I, Format F, bool SHORT>
 cudaError_t launch_few(int ctas, cudaStream_t s, const KvMaps& maps, const AttnArgs& a) {
-  using C = FewCfg<ROWS, F>;
-  return launch_main(paged_attn_few_kernel<ROWS, I, F>, ctas, C::kThreads, C::kSmem, s, maps, a);
+  using C = FewCfg<ROWS, F, SHORT>;
+  return launch_main(paged_attn_few_kernel<ROWS, I, F, SHORT>, ctas, C::kThreads, C::kSmem, s, maps, a);
 }
 template <Format F>
 cudaError_t launch_few(bool eight, bool wide, int ctas, cudaStream_t s, const KvMaps& maps, const AttnArgs& a) {
-  return eight ? (wide ? launch_few<8, int64_t, F>(ctas, s, maps, a) : launch_few<8, int, F>(ctas, s, maps, a))
-               : (wide ? launch_few<16, int64_t, F>(ctas, s, maps, a) : launch_few<16, int, F>(ctas, s, maps, a));
+  return eight ? (wide ? launch_few<8, int64_t, F, false>(ctas, s, maps, a) : launch_few<8, int, F, false>(ctas, s, maps, a))
+               : (wide ? launch_few<16, int64_t, F, false>(ctas, s, maps, a)
+                       : launch_few<16, int, F, false>(ctas, s, maps, a));
+}
+template <Format F>
+cudaError_t launch_few8(bool eight, bool wide, bool brief, int ctas, cudaStream_t s, const KvMaps& maps,
+                        const AttnArgs& a) {
+  if (brief)
+    return eight ? launch_few<8, int, F, true>(ctas, s, maps, a) : launch_few<16, int, F, true>(ctas, s, maps, a);
+  return launch_few<F>(eight, wide, ctas, s, maps, a);
 }
 
 template <int N>
@@ -2123,12 +2227,16 @@ static int rope_kv(const char* what, const void* qkv, const float* cos_t, const 
   a.n_pages = (int)kv->n_pages;
   a.ke = q8 ? Exponents{q8->k_scale, q8->ks_page, q8->ks_head} : Exponents{};
   a.ve = q8 ? Exponents{q8->v_scale, q8->vs_page, q8->vs_head} : Exponents{};
+  int sms = 148;
+  xb::sm_count(&sms);
+  a.span = q8 && D <= 256 && tokens > 24 * sms ? 16 : 32;  // more than the warps that are there at once
+  const int per = 64 / a.span;                              // tokens of a CTA
   int *bad = nullptr, *status = nullptr;
   rc = status_words(&bad, &status, what, err, errlen);
   if (rc) return rc;
   auto kernel = !q8 ? paged_rope_kv_kernel<kBf16>
                     : q8->dtype == XB_DT_I8 ? paged_rope_kv_kernel<kInt8> : paged_rope_kv_kernel<kE4m3>;
-  launch_k<false>(kernel, (unsigned)((tokens + 1) / 2), 64, 0, (cudaStream_t)stream, a, bad);
+  launch_k<false>(kernel, (unsigned)((tokens + per - 1) / per), 64, 0, (cudaStream_t)stream, a, bad);
   return check_launch(what, err, errlen);
 }
 
@@ -2207,7 +2315,8 @@ extern "C" int xb_paged_read_kv(void* k_out, void* v_out, const xb_paged_kv8* kv
   if (rc) return rc;
   auto kernel = kv8->dtype == XB_DT_BF16 ? paged_read_kv_kernel<kBf16>
                 : kv8->dtype == XB_DT_I8 ? paged_read_kv_kernel<kInt8> : paged_read_kv_kernel<kE4m3>;
-  launch_k<false>(kernel, (unsigned)((tokens + 7) / 8), 256, 0, (cudaStream_t)stream, a, bad);
+  launch_k<false>(kernel, (unsigned)((tokens + 8 * kReadTokens - 1) / (8 * kReadTokens)), 256, 0, (cudaStream_t)stream, a,
+                  bad);
   return check_launch(what, err, errlen);
 }
 
@@ -2316,8 +2425,17 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
   if (rc) return rc;
   const bool few = few_rows(tokens, batch, n_rep);
   const bool eight = few && n_rep <= 8 && tokens * n_rep <= 8 * batch;  // the same rule for half a tile
-  const int tile = !few ? kTcTK : q8 ? kFewTK8 : kFewTK;
-  line_kernel(a, few ? (eight ? 8 : kFewRows) : kTcRows, q8 ? kFewTK8 : kFewTK);
+  int sms = 148;
+  xb::sm_count(&sms);
+  const int ctas = few ? sms : 2 * sms;
+  // at most 96 keys to each of 8 warps an SM, by what the table can hold (and a short line)
+  const int rows = few ? (eight ? 8 : kFewRows) : kTcRows;
+  line_kernel(a, rows);
+  const bool brief = q8 && (double)batch * n_kv_head * kv->max_pages * page_size <= 96.0 * kFewWarps * sms &&
+                     !line_is_wide(a, ctas);
+  const int tile = !few ? kTcTK : q8 && !brief ? kFewTK8 : kFewTK;
+  if (few) line_kernel(a, rows, tile);
+  const bool wide = line_is_wide(a, ctas);
   a.ke = q8 ? Exponents{q8->k_scale, q8->ks_page, q8->ks_head} : Exponents{};
   a.ve = q8 ? Exponents{q8->v_scale, q8->vs_page, q8->vs_head} : Exponents{};
   a.rep_magic = (65536u + (uint32_t)n_rep - 1u) / (uint32_t)n_rep;
@@ -2326,22 +2444,18 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
   a.box_rows = box;
   TcMaps maps;
   memset(&maps, 0, sizeof(maps));
-  rc = page_map(&maps.k, kv->k_pages, n_pages, n_kv_head, page_size, kv->k_page, kv->k_head, kv->k_row, box, q8,
-                what, err, errlen);
+  rc = page_map(&maps.k, kv->k_pages, n_pages, n_kv_head, page_size, kv->k_page, kv->k_head, kv->k_row, box, q8, what,
+                err, errlen);
   if (!rc)
-    rc = page_map(&maps.v, kv->v_pages, n_pages, n_kv_head, page_size, kv->v_page, kv->v_head, kv->v_row, box, q8,
-                  what, err, errlen);
+    rc = page_map(&maps.v, kv->v_pages, n_pages, n_kv_head, page_size, kv->v_page, kv->v_head, kv->v_row, box, q8, what,
+                  err, errlen);
   if (!rc && !few) rc = query_map(&maps.q, q, tokens, n_head, ld_q, n_rep, a.tpt, what, err, errlen);
   if (rc) return rc;
-  int sms = 148;
-  xb::sm_count(&sms);
-  const int ctas = few ? sms : 2 * sms;
   if (line_bound(a) >= 4e18) {
     set_err(err, errlen, "%s: %lld tokens of %lld sequences over %lld pages each are too many", what,
             (long long)tokens, (long long)batch, (long long)kv->max_pages);
     return XB_ERR_UNSUPPORTED;
   }
-  const bool wide = line_is_wide(a, ctas);
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
   if (few) {
@@ -2349,8 +2463,8 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
     pages.k = maps.k;
     pages.v = maps.v;
     e = !q8 ? launch_few<kBf16>(eight, wide, ctas, s, pages, a)
-            : q8->dtype == XB_DT_I8 ? launch_few<kInt8>(eight, wide, ctas, s, pages, a)
-                                    : launch_few<kE4m3>(eight, wide, ctas, s, pages, a);
+            : q8->dtype == XB_DT_I8 ? launch_few8<kInt8>(eight, wide, brief, ctas, s, pages, a)
+                                    : launch_few8<kE4m3>(eight, wide, brief, ctas, s, pages, a);
     if (e == cudaSuccess)
       e = launch_k(paged_attn_join_kernel<kFewRows, 4>, dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
   } else {

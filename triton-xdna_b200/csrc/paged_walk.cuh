@@ -32,7 +32,7 @@ struct Line {
 };
 
 constexpr int kFewTK = 32, kTcTK = 64;  // keys of a tile of the two kernels
-constexpr int kFewTK8 = 64;             // of the few-row kernel over 8-bit pages: the same bytes
+constexpr int kFewTK8 = 64;             // of the few-row kernel over 8-bit pages, where there are many keys a warp
 constexpr int kFewRows = 16;            // rows of a tile of the few-row kernel (at most)
 constexpr int kFewWarps = 8;            // its warps in a CTA, each with a piece of the line
 
