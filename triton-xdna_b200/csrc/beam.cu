@@ -17,7 +17,8 @@
 namespace xb {
 namespace beam {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kScan = 256, kPick = 256;  // threads of the two kernels
+constexpr int kResident = 4;             // CTAs of the first an SM
 constexpr int kMaxCount = 64, kMaxBeams = 64;
 constexpr int kLane = 16, kGroup = 32 * kLane;  // tokens that a lane and its warp take at a time
 constexpr int kBlocks = 8;      // runs of groups of which a lane keeps the maximum
@@ -57,10 +58,12 @@ __device__ __forceinline__ int shift_of(float top) {
 __device__ __forceinline__ float power(int n) { return n < -126 ? 0.0f : __int_as_float((n + 127) << 23); }
 
 // A number that at least `count` of the block's threads' `mine` reach, close to the
-// largest such one (-inf where none is known): the count-th of the count / 4 largest of
-// each warp.  `few` is shared and this call's own.  Every thread calls this.
+// largest such one (-inf where none is known): the count-th of the 2 count / warps largest
+// of each warp.  `few` is shared and this call's own.  Every thread calls this.
 constexpr int kFew = 2 * kMaxCount;
+template <int THREADS>
 __device__ __forceinline__ float reached_by(float mine, int count, float* few) {
+  constexpr int kWarps = THREADS / 32;
   const int part = (2 * count + kWarps - 1) / kWarps, lane = threadIdx.x & 31;
   float* to = few + (threadIdx.x >> 5) * part;
   for (int n = 0; n < part;) {
@@ -95,7 +98,7 @@ struct Ring {  // a warp's groups of tokens on their way from memory
   static constexpr int kBytes = kGroup * (int)sizeof(T);
   static constexpr int kStages = 8 / (int)sizeof(T);
   static constexpr int kStage = kBytes + 16;  // a row may start anywhere in a vector
-  static constexpr int kSmem = kWarps * kStages * kStage;
+  static constexpr int kSmem = kScan / 32 * kStages * kStage;
 };
 
 // One part of a row: groups of tokens, by turns to the CTA's warps, which run
@@ -111,14 +114,15 @@ struct Ring {  // a warp's groups of tokens on their way from memory
 // or in the L2: some 20 of 2048 for count = 16.  Keeping the candidates during the
 // stream took 44 instructions a token, mostly to find that there is none.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const T* __restrict__ logits, int64_t ld, int64_t vocab,
+__global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __restrict__ logits, int64_t ld, int64_t vocab,
                                                                 int count, int parts, uint64_t* __restrict__ lists,
                                                                 Stats* __restrict__ stats) {
   using R = Ring<T>;
+  constexpr int kWarps = kScan / 32;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t cand[kWarps][kHeld];
-  __shared__ float run_top[kBlocks][kThreads];
-  __shared__ uint16_t runs[kBlocks * kThreads];
+  __shared__ float run_top[kBlocks][kScan];
+  __shared__ uint16_t runs[kBlocks * kScan];
   __shared__ float few[kFew], warp_top[kWarps], warp_sum[kWarps];
   __shared__ int listed, total;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -236,17 +240,17 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const T* __restr
       held = count;
     }
   };
-  const float low = fmaxf(kLowest, reached_by(top, count, few));  // -inf is no candidate
+  const float low = fmaxf(kLowest, reached_by<kScan>(top, count, few));  // -inf is no candidate
   // the runs to look through
   if (top >= low)
     for (int b = 0; b < block; ++b)
-      if (run_top[b][threadIdx.x] >= low) runs[atomicAdd(&listed, 1)] = (uint16_t)(b * kThreads + threadIdx.x);
+      if (run_top[b][threadIdx.x] >= low) runs[atomicAdd(&listed, 1)] = (uint16_t)(b * kScan + threadIdx.x);
   __syncthreads();
   // a half-warp takes a run, a lane a token of each of its groups
   const int half = warp * 2 + (lane >> 4), inside = (lane & 15) * 32;
   for (int q0 = 0; q0 < listed; q0 += 2 * kWarps) {
     const int q = q0 + half, r = q < listed ? runs[q] : 0;
-    const int w = (r % kThreads) >> 5, within = (r & 31) + inside, it0 = r / kThreads * run;
+    const int w = (r % kScan) >> 5, within = (r & 31) + inside, it0 = r / kScan * run;
     const int64_t gw = p0 + w;
     const int nw = gw < g1 ? (int)((g1 - gw + kWarps - 1) / kWarps) : 0;  // that warp's groups
     const uint8_t* slots = ring + w * R::kStages * R::kStage + off + within * (int)sizeof(T);
@@ -296,13 +300,13 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const T* __restr
   // a key's place is the number of larger ones
   uint64_t* list = lists + (int64_t)blockIdx.x * count;
   const int found = total;
-  for (int i = threadIdx.x; i < found; i += kThreads) {
+  for (int i = threadIdx.x; i < found; i += kScan) {
     const uint64_t key = all[i];
     int place = 0;
     for (int j = 0; j < found; ++j) place += all[j] > key;
     if (place < count) list[place] = key;
   }
-  for (int i = found + threadIdx.x; i < count; i += kThreads) list[i] = 0;
+  for (int i = found + threadIdx.x; i < count; i += kScan) list[i] = 0;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < kWarps; ++i) s += warp_sum[i];
@@ -322,7 +326,7 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
 // lies below it (compared in fp32, which no rounding turns round) falls away.
 // Should more be left than fit, as where very many sums are equal, the choice
 // goes step by step, the best of all entries behind the last choice each time.
-__global__ void __launch_bounds__(kThreads) beam_pick_kernel(const float* __restrict__ scores, int64_t ld_scores,
+__global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restrict__ scores, int64_t ld_scores,
                                                              const uint64_t* __restrict__ lists,
                                                              const Stats* __restrict__ stats, int beams, int parts,
                                                              int count, float* __restrict__ values,
@@ -345,11 +349,11 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const float* __rest
   uint64_t ahead[kAhead];
 #pragma unroll
   for (int j = 0; j < kAhead; ++j) {
-    const int f = j * kThreads + threadIdx.x;
+    const int f = j * kPick + threadIdx.x;
     ahead[j] = f < entries ? lists[f] : 0;
   }
   if (threadIdx.x == 0) n = 0;
-  for (int k = warp; k < beams; k += kWarps) {
+  for (int k = warp; k < beams; k += kPick / 32) {
     const float score = scores[g * ld_scores + k];
     float top = -INFINITY;
     int shift = -0x40000000;
@@ -386,12 +390,12 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const float* __rest
   auto each = [&](auto&& take) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-      if (j * kThreads < entries) take(candidate(min(j * kThreads + (int)threadIdx.x, entries - 1), ahead[j]));
-    for (int f = kAhead * kThreads + threadIdx.x; f < entries; f += kThreads) take(candidate(f, lists[f]));
+      if (j * kPick < entries) take(candidate(min(j * kPick + (int)threadIdx.x, entries - 1), ahead[j]));
+    for (int f = kAhead * kPick + threadIdx.x; f < entries; f += kPick) take(candidate(f, lists[f]));
   };
   float best = -INFINITY;
   each([&](const Candidate& c) { best = fmaxf(best, (float)c.total); });
-  const float bound = reached_by(best, count, few);
+  const float bound = reached_by<kPick>(best, count, few);
   each([&](const Candidate& c) {
     if (c.total == -INFINITY || (float)c.total < bound) return;
     const int at = atomicAdd(&n, 1);
@@ -407,7 +411,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const float* __rest
   };
   const int left = n;
   if (left <= kPicked) {
-    for (int i0 = 0; i0 < left; i0 += kThreads / 4) {  // four lanes count those before a candidate
+    for (int i0 = 0; i0 < left; i0 += kPick / 4) {  // four lanes count those before a candidate
       const int i = i0 + threadIdx.x / 4;
       const Candidate mine = found[min(i, left - 1)];
       int place = 0;
@@ -417,7 +421,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const float* __rest
       place += __shfl_xor_sync(0xffffffffu, place, 2);
       if (i < left && place < count && (threadIdx.x & 3) == 0) put(place, mine);
     }
-    for (int i = left + threadIdx.x; i < count; i += kThreads) {  // fewer candidates than asked for
+    for (int i = left + threadIdx.x; i < count; i += kPick) {  // fewer candidates than asked for
       value[i] = -INFINITY;
       parent[i] = token[i] = -1;
     }
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(const float* __rest
     __syncthreads();
     found[threadIdx.x] = mine;
     __syncthreads();
-    for (int o = kThreads / 2; o > 0; o >>= 1) {
+    for (int o = kPick / 2; o > 0; o >>= 1) {
       if (threadIdx.x < o && before(found[threadIdx.x + o], found[threadIdx.x])) found[threadIdx.x] = found[threadIdx.x + o];
       __syncthreads();
     }
@@ -447,8 +451,8 @@ int parts_of(int64_t rows, int64_t vocab) {
   int sms = 148;
   sm_count(&sms);
   const int64_t groups = (vocab + kGroup - 1) / kGroup;
-  int64_t n = 4 * sms / rows;
-  if (n > groups / kWarps) n = groups / kWarps;  // a warp has a group at least
+  int64_t n = kResident * sms / rows;
+  if (n > groups / (kScan / 32)) n = groups / (kScan / 32);  // a warp has a group at least
   return (int)(n < 1 ? 1 : n);
 }
 
@@ -529,7 +533,7 @@ extern "C" int xb_beam_select(const void* logits, const float* scores, int64_t g
     cudaError_t e = xb::once_per_device(reinterpret_cast<const void*>(kernel), xb::kOnceSmem, [&](int*) {
       return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     });
-    return e != cudaSuccess ? e : launch_k(kernel, (unsigned)(rows * parts), kThreads, smem, s, x, ld, vocab,
+    return e != cudaSuccess ? e : launch_k(kernel, (unsigned)(rows * parts), kScan, smem, s, x, ld, vocab,
                                            (int)count, parts, lists, stats);
   };
   cudaError_t e = dtype == XB_DT_F32
@@ -537,7 +541,7 @@ extern "C" int xb_beam_select(const void* logits, const float* scores, int64_t g
                       : scan(beam_scan_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(logits),
                              Ring<__nv_bfloat16>::kSmem);
   if (e == cudaSuccess)
-    e = launch_k(beam_pick_kernel, (unsigned)groups, kThreads, 0, s, scores, ld_scores, lists, stats, (int)beams, parts,
+    e = launch_k(beam_pick_kernel, (unsigned)groups, kPick, 0, s, scores, ld_scores, lists, stats, (int)beams, parts,
                  (int)count, values, parents, tokens);
   if (e != cudaSuccess) {
     set_err(err, errlen, "%s: %s", what, cudaGetErrorString(e));

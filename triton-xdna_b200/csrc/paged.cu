@@ -394,28 +394,52 @@ __global__ void __launch_bounds__(256) paged_expand_kernel(const ExpandArgs a) {
     if (s0 == s1) continue;
     const int len = min(max(__ldg(a.kv_len + b), 0), a.max_pages * a.page_size);
     const int64_t parts = (int64_t)((len + 7) / 8) * a.KVH;
-    for (int64_t i = first; i < parts; i += step) {
-      const int head = (int)(i % a.KVH), p0 = (int)(i / a.KVH) * 8;
-      const int col = p0 / a.page_size, row = p0 - col * a.page_size + r;
-      const int id = __ldg(a.table + b * a.ld_table + col);
-      const bool ok = id >= 0 && id < a.n_pages;
-      const int64_t entry = (int64_t)b * a.max_pages + col;
-      const int64_t slot = a.compact ? entry : id;
-      if (head == 0 && row == 0 && lane == 0) a.slots[entry] = ok ? (int)slot : -1;
-      if (!ok) continue;
-      const int64_t to = ((slot * a.KVH + head) * a.page_size + row) * kRowDims + d;
+    constexpr int kAhead = 4;  // parts on their way
+    for (int64_t i0 = first; i0 < parts; i0 += (int64_t)step * kAhead) {
+      int id[kAhead], head[kAhead], col[kAhead], row[kAhead];
 #pragma unroll
-      for (int kind = 0; kind < 2; ++kind) {
-        const Pages& pg = kind ? a.v : a.k;
-        const Exponents& ex = kind ? a.ve : a.ke;
-        const uint4 c = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pg.p) + id * pg.page +
-                                                             head * pg.head + row * pg.row + d));
-        const float scale = byte_scale(__ldg(ex.p + id * ex.page + head * ex.head + row));
-        const uint2 x0 = decode4<F>(c.x, scale), x1 = decode4<F>(c.y, scale);
-        const uint2 x2 = decode4<F>(c.z, scale), x3 = decode4<F>(c.w, scale);
-        uint4* out = reinterpret_cast<uint4*>((kind ? a.v_out : a.k_out) + to);
-        out[0] = make_uint4(x0.x, x0.y, x1.x, x1.y);
-        out[1] = make_uint4(x2.x, x2.y, x3.x, x3.y);
+      for (int u = 0; u < kAhead; ++u) {
+        const int64_t i = i0 + (int64_t)u * step;
+        id[u] = -2;  // no part
+        if (i < parts) {
+          const int p0 = (int)(i / a.KVH) * 8;
+          head[u] = (int)(i - (int64_t)(p0 / 8) * a.KVH);
+          col[u] = p0 / a.page_size;
+          row[u] = p0 - col[u] * a.page_size + r;
+          id[u] = __ldg(a.table + b * a.ld_table + col[u]);
+          if (id[u] < 0 || id[u] >= a.n_pages) id[u] = -1;
+        }
+      }
+      uint4 c[kAhead][2];
+      uint32_t e[kAhead][2];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind)
+          if (id[u] >= 0) {
+            const Pages& pg = kind ? a.v : a.k;
+            const Exponents& ex = kind ? a.ve : a.ke;
+            c[u][kind] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pg.p) + id[u] * pg.page +
+                                                              head[u] * pg.head + row[u] * pg.row + d));
+            e[u][kind] = __ldg(ex.p + id[u] * ex.page + head[u] * ex.head + row[u]);
+          }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (id[u] == -2) continue;
+        const int64_t entry = (int64_t)b * a.max_pages + col[u], slot = a.compact ? entry : id[u];
+        if (head[u] == 0 && row[u] == 0 && lane == 0) a.slots[entry] = id[u] >= 0 ? (int)slot : -1;
+        if (id[u] < 0) continue;
+        const int64_t to = ((slot * a.KVH + head[u]) * a.page_size + row[u]) * kRowDims + d;
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind) {
+          const float scale = byte_scale((int)e[u][kind]);
+          const uint4 v = c[u][kind];
+          const uint2 x0 = decode4<F>(v.x, scale), x1 = decode4<F>(v.y, scale);
+          const uint2 x2 = decode4<F>(v.z, scale), x3 = decode4<F>(v.w, scale);
+          uint4* out = reinterpret_cast<uint4*>((kind ? a.v_out : a.k_out) + to);
+          out[0] = make_uint4(x0.x, x0.y, x1.x, x1.y);
+          out[1] = make_uint4(x2.x, x2.y, x3.x, x3.y);
+        }
       }
     }
   }
@@ -450,6 +474,7 @@ struct AttnArgs : Line {
   float* ws;  // [2 G] partials, then G Meta
   int64_t ld_q, ld_out, ld_table;
   int n_pages, box_rows;
+  bool expanded;  // the launch before this one is paged_expand_kernel
   uint32_t rep_magic;  // ceil(2^16 / n_rep)
   float scale_log2;
   int *bad, *status;
@@ -1374,8 +1399,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_sh;  // S / P buffers at columns 0, 64 and 128, O at 192
-  pdl_wait();
-  pdl_trigger();
+  // Behind paged_expand_kernel the lengths are there already: its CTAs let this
+  // kernel start after their own wait for all launches before.  So the search runs beside it.
+  if (!a.expanded) pdl_wait();
 
   auto fail = [&]() {
     atomicExch(a.status, XB_ERR_TIMEOUT);
@@ -1384,6 +1410,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
   Meta* meta = reinterpret_cast<Meta*>(a.ws + 2 * (int64_t)gridDim.x * part_floats(kTcRows));
   I total;
   const I share = find_pieces<kTcThreads, 1, I>(a, gridDim.x, blockIdx.x, sums, found, &total);
+  if (a.expanded) pdl_wait();
+  pdl_trigger();
   // A wait of a whole warp: the same answer in every lane (false: it ran out)
   auto wait_all = [&](uint64_t* bar, int phase) -> bool {
     if (__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, kWaitLimit, &abort_flag))) return true;
@@ -2386,9 +2414,10 @@ static int check_workspace(const void* workspace, size_t bytes, size_t need, con
   return XB_ERR_INVALID;
 }
 
-// xb_paged_attention_bf16 and, with `q8` (few rows), the attention over 8-bit pages.
+// xb_paged_attention_bf16 and, with `q8` (few rows), the attention over 8-bit pages;
+// `expanded`: over what paged_expand_kernel, launched just before, makes of them.
 static int attend(const char* what, const void* q, void* out, const xb_paged_kv* kv, const xb_paged_kv8* q8,
-                  int64_t tokens, int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
+                  bool expanded, int64_t tokens, int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
                   size_t workspace_bytes, void* stream, char* err, size_t errlen) {
   int rc = check_pages(kv, what, err, errlen);
   if (!rc) rc = check_attention(kv, tokens, n_head, scale, what, err, errlen);
@@ -2421,6 +2450,7 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
   a.max_pages = (int)kv->max_pages;
   a.n_pages = (int)n_pages;
   a.scale_log2 = scale_log2;
+  a.expanded = expanded;
   rc = status_words(&a.bad, &a.status, what, err, errlen);
   if (rc) return rc;
   const bool few = few_rows(tokens, batch, n_rep);
@@ -2483,7 +2513,7 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
 extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_kv* kv, int64_t tokens,
                                        int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
                                        size_t workspace_bytes, void* stream, char* err, size_t errlen) {
-  return attend("xb_paged_attention_bf16", q, out, kv, nullptr, tokens, n_head, ld_q, ld_out, scale, workspace,
+  return attend("xb_paged_attention_bf16", q, out, kv, nullptr, false, tokens, n_head, ld_q, ld_out, scale, workspace,
                 workspace_bytes, stream, err, errlen);
 }
 
@@ -2544,7 +2574,7 @@ extern "C" int xb_paged_attention_q8(const void* q, void* out, const xb_paged_kv
   if (!rc) rc = check_workspace(workspace, workspace_bytes, need, what, err, errlen);
   if (rc) return rc;
   if (few_rows(tokens, kv->batch, n_head / kv->n_kv_head))
-    return attend(what, q, out, kv, kv8, tokens, n_head, ld_q, ld_out, scale, workspace, workspace_bytes, stream, err,
+    return attend(what, q, out, kv, kv8, false, tokens, n_head, ld_q, ld_out, scale, workspace, workspace_bytes, stream, err,
                   errlen);
   ExpandArgs e;
   bool compact;
@@ -2589,7 +2619,7 @@ extern "C" int xb_paged_attention_q8(const void* q, void* out, const xb_paged_kv
   wide.k_row = wide.v_row = kHD;
   wide.k_head = wide.v_head = kv->page_size * kHD;
   wide.k_page = wide.v_page = kv->n_kv_head * kv->page_size * kHD;
-  return attend(what, q, out, &wide, nullptr, tokens, n_head, ld_q, ld_out, scale, workspace, own, stream, err, errlen);
+  return attend(what, q, out, &wide, nullptr, true, tokens, n_head, ld_q, ld_out, scale, workspace, own, stream, err, errlen);
 }
 
 extern "C" int xb_page_status(void* stream, int* status, char* err, size_t errlen) {
