@@ -146,13 +146,24 @@ def signatures() -> dict[str, tuple[str, list[str]]]:
     return dict(_sigs)
 
 
+class _Local(threading.local):
+    """A thread's error buffer, empty between calls."""
+
+    def __init__(self):
+        self.err = ctypes.create_string_buffer(1024)
+
+
+_local = _Local()
+
+
 def call(name: str, *args) -> None:
     """Call ``name(*args, err, errlen)`` and raise XbError on a negative status."""
-    lib = load()
-    err = ctypes.create_string_buffer(1024)
-    rc = getattr(lib, name)(*args, err, ctypes.sizeof(err))
+    err = _local.err
+    rc = getattr(_lib or load(), name)(*args, err, 1024)
     if rc != XB_OK:
-        raise XbError(name, rc, err.value.decode(errors="replace"))
+        message = err.value.decode(errors="replace")
+        err[0] = b"\0"
+        raise XbError(name, rc, message)
 
 
 def call_int(name: str, *args) -> int:

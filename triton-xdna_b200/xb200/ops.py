@@ -1072,7 +1072,17 @@ def beam_select(logits, scores, count):
 
 def _device_of(*ts) -> int:
     """Device index of CUDA tensors (None skipped), as _cuda checks them."""
-    dev = -1
+    try:
+        dev = ts[0].get_device()  # -1: a host tensor
+        for t in ts:
+            if t is not None and t.get_device() != dev:
+                break
+        else:
+            if dev >= 0:
+                return dev
+    except (AttributeError, RuntimeError):  # no tensor, or one of no device
+        pass
+    dev = -1  # one by one, for the error
     for t in ts:
         if t is not None:
             if not isinstance(t, torch.Tensor) or not t.is_cuda:
