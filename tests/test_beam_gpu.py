@@ -147,6 +147,26 @@ def test_masks_of_the_lowest_value_and_large_logits(dtype):
     check(logits, scores, 8, exactly=dtype is torch.float32)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_nothing_but_masks_and_logits_of_any_size(dtype):
+    """Whole rows at the type's lowest value (all tokens alike), rows far from zero, such parts among others."""
+    V = 40000
+    low = torch.finfo(dtype).min
+    logits, scores = make(1, 8, V, dtype, seed=31)
+    logits[0] = low
+    logits[1] = -low
+    logits[2, 1000:] = low
+    logits[3, :20000], logits[3, 20000:] = low, low / 2
+    logits[4] = logits[4] * 8 + 2.0 ** 22  # fp32: steps of a half; bf16: all alike
+    logits[5] = logits[5] - 2.0 ** 21
+    logits[6] = logits[6] * 1e6  # bf16: steps of thousands
+    logits[7, :100] = 1e30
+    for beams in range(8):  # one by one, and all together
+        check(logits[beams:beams + 1], scores[:, beams:beams + 1], 16)
+    scores = torch.zeros((1, 8), device="cuda") - torch.arange(8, device="cuda") / 3
+    check(logits, scores, 64)
+
+
 def test_scores_between_rows_of_a_wider_tensor():
     logits, scores = make(4, 3, 2500, seed=25)
     wide = torch.full((4, 9), 7.0, device="cuda")

@@ -43,19 +43,34 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t token) {
   return (uint64_t)ordered(x + 0.0f) << 32 | (0xffffffffu - token);
 }
 
-// Of a part: its maximum (-inf: none) and sum 2^shift, the sum of exp2(x kLog2e).
-// The shift is a whole number, so sums of different shifts are brought to one
-// without rounding, and x kLog2e - shift is one fused multiply-add, rounded in the size of
-// its result.
+// Of some tokens: their maximum (-inf: none) and sum 2^shift, the sum of exp2(x
+// kLog2e).  The shift is a whole number, so sums of different shifts are brought to
+// one without rounding, and x kLog2e - shift is one fused multiply-add, rounded in
+// the size of its result.  Where the maximum is 2^22 or more in size (a row of
+// masks of the lowest value) the shift is kFar and the sum that of exp(x - maximum).
+constexpr int kFar = 0x40000000;
 struct Stats {
   float top, sum;
   int shift, unused;
 };
 __device__ __forceinline__ int shift_of(float top) {
-  return top > -INFINITY && top < INFINITY ? (int)fminf(fmaxf(rintf(top * kLog2e), -1e9f), 1e9f) : 0;
+  return fabsf(top) < 4194304.0f ? (int)rintf(top * kLog2e) : kFar;
 }
 // 2^n, n <= 0
 __device__ __forceinline__ float power(int n) { return n < -126 ? 0.0f : __int_as_float((n + 127) << 23); }
+// The same sum with a larger maximum
+__device__ __forceinline__ void raise(Stats& s, float top) {
+  const int to = shift_of(top);
+  if (s.shift != kFar && to != kFar) {
+    s.sum *= power(min(s.shift - to, 0));  // a sum of nothing may have had any shift
+  } else if (s.top != -INFINITY) {
+    if (s.shift != kFar) s.sum *= ex2_approx(fmaf(-s.top, kLog2e, (float)s.shift));
+    s.sum *= ex2_approx((s.top - top) * kLog2e);
+    if (to != kFar) s.sum *= ex2_approx(fmaf(top, kLog2e, -(float)to));
+  }
+  s.top = top;
+  s.shift = to;
+}
 
 // A number that at least `count` of the block's threads' `mine` reach, close to the
 // largest such one (-inf where none is known): the count-th of the 2 count / warps largest
@@ -80,13 +95,20 @@ __device__ __forceinline__ float reached_by(float mine, int count, float* few) {
   __syncthreads();
   // the least of those that fewer than count are above
   const int all = part * kWarps;
-  float bound = INFINITY;
-  for (int i = lane; i < all; i += 32) {
-    int above = 0;
-    for (int j = 0; j < all; ++j) above += few[j] > few[i];
-    if (above < count) bound = fminf(bound, few[i]);
+  if (threadIdx.x < 32) {
+    float bound = INFINITY;
+    for (int i = lane; i < all; i += 32) {
+      const float mine_ = few[i];
+      int above = 0;
+#pragma unroll 8
+      for (int j = 0; j < all; ++j) above += few[j] > mine_;
+      if (above < count) bound = fminf(bound, mine_);
+    }
+    bound = unordered(__reduce_min_sync(0xffffffffu, ordered(bound)));
+    if (lane == 0) few[kFew] = bound;
   }
-  return unordered(__reduce_min_sync(0xffffffffu, ordered(bound)));
+  __syncthreads();
+  return few[kFew];
 }
 
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
@@ -123,7 +145,7 @@ __global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __
   __shared__ uint64_t cand[kWarps][kHeld];
   __shared__ float run_top[kBlocks][kScan];
   __shared__ uint16_t runs[kBlocks * kScan];
-  __shared__ float few[kFew], warp_top[kWarps], warp_sum[kWarps];
+  __shared__ float few[kFew + 1], warp_top[kWarps], warp_sum[kWarps];
   __shared__ int listed, total;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x / (uint32_t)parts;
@@ -169,8 +191,8 @@ __global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __
 #pragma unroll
   for (int i = 0; i < R::kStages; ++i) fill(i);
 
-  float top = -INFINITY, sum = 0.0f, here = -INFINITY;  // here: of the present run
-  int shift = 0;
+  Stats sums = {-INFINITY, 0.0f, 0, 0};
+  float here = -INFINITY;  // maximum of the present run
   int left = run, block = 0;
 #pragma unroll
   for (int i = 0; i < kBlocks; ++i) run_top[i][threadIdx.x] = -INFINITY;
@@ -194,17 +216,17 @@ __global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __
 #pragma unroll
     for (int i = 0; i < kLane; ++i) m = fmaxf(m, v[i]);
     here = fmaxf(here, m);
-    if (m > top) {
-      top = m;
-      const int to = shift_of(m);
-      sum *= power(min(shift - to, 0));  // a sum of nothing may have had any
-      shift = to;
-    }
-    const float base = -(float)shift;
-    float s[2] = {sum, 0.0f};
+    if (m > sums.top) raise(sums, m);
+    float s[2] = {sums.sum, 0.0f};
+    if (sums.shift != kFar) {
+      const float base = -(float)sums.shift;
 #pragma unroll
-    for (int i = 0; i < kLane; ++i) s[i & 1] += ex2_approx(fmaf(v[i], kLog2e, base));
-    sum = s[0] + s[1];
+      for (int i = 0; i < kLane; ++i) s[i & 1] += ex2_approx(fmaf(v[i], kLog2e, base));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLane; ++i) s[i & 1] += ex2_approx((v[i] - sums.top) * kLog2e);
+    }
+    sums.sum = s[0] + s[1];
     if (--left == 0 || it + 1 == n) {
       run_top[block++][threadIdx.x] = here;
       here = -INFINITY;
@@ -240,9 +262,9 @@ __global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __
       held = count;
     }
   };
-  const float low = fmaxf(kLowest, reached_by<kScan>(top, count, few));  // -inf is no candidate
+  const float low = fmaxf(kLowest, reached_by<kScan>(sums.top, count, few));  // -inf is no candidate
   // the runs to look through
-  if (top >= low)
+  if (sums.top >= low)
     for (int b = 0; b < block; ++b)
       if (run_top[b][threadIdx.x] >= low) runs[atomicAdd(&listed, 1)] = (uint16_t)(b * kScan + threadIdx.x);
   __syncthreads();
@@ -284,7 +306,7 @@ __global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __
   uint64_t* all = reinterpret_cast<uint64_t*>(ring);  // [kWarps * kHeld] at most
   for (int i = lane; i < held; i += 32) all[atomicAdd(&total, 1)] = own[i];
   // the part's maximum and sum
-  float m = top;
+  float m = sums.top;
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) warp_top[warp] = m;
@@ -292,8 +314,8 @@ __global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __
   m = warp_top[0];
 #pragma unroll
   for (int i = 1; i < kWarps; ++i) m = fmaxf(m, warp_top[i]);
-  const int to = shift_of(m);
-  float s = sum * power(min(shift - to, 0));
+  if (m > sums.top) raise(sums, m);
+  float s = sums.sum;
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) warp_sum[warp] = s;
@@ -310,7 +332,7 @@ __global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < kWarps; ++i) s += warp_sum[i];
-    stats[blockIdx.x] = Stats{m, s, to, 0};
+    stats[blockIdx.x] = Stats{m, s, sums.shift, 0};
   }
 }
 
@@ -334,7 +356,7 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
                                                              int64_t* __restrict__ tokens) {
   __shared__ Candidate found[kPicked];
   __shared__ double shifts[kMaxBeams];  // score - log sum; NaN: the beam is out
-  __shared__ float few[kFew];
+  __shared__ float few[kFew + 1];
   __shared__ int n;
   pdl_wait();
   pdl_trigger();
@@ -356,14 +378,17 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
   for (int k = warp; k < beams; k += kPick / 32) {
     const float score = scores[g * ld_scores + k];
     float top = -INFINITY;
-    int shift = -0x40000000;
+    int shift = -kFar;
     double sum = 0.0;
+    bool far = false;
     for (int i0 = 0; i0 < parts; i0 += 32) {
       const Stats s = i0 + lane < parts ? stats[k * parts + i0 + lane] : Stats{-INFINITY, 0.0f, 0, 0};
       const bool any = s.top != -INFINITY || s.sum != 0.0f;
       top = fmaxf(top, s.top);
-      const int to = max(shift, __reduce_max_sync(0xffffffffu, any ? s.shift : -0x40000000));
-      sum = scalbn(sum, max(shift - to, -2000)) + (any ? scalbn((double)s.sum, max(s.shift - to, -2000)) : 0.0);
+      far |= any && s.shift == kFar;
+      const int to = max(shift, __reduce_max_sync(0xffffffffu, any && s.shift != kFar ? s.shift : -kFar));
+      sum = scalbn(sum, max(shift - to, -2000)) +
+            (any && s.shift != kFar ? scalbn((double)s.sum, max(s.shift - to, -2000)) : 0.0);
       shift = to;
     }
 #pragma unroll
@@ -371,11 +396,22 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
-    if (lane == 0) {
-      // sum 2^shift = sum exp(x (1 + off)), which exp(top off) times the sum of exp(x) is but for off (x - top)
-      const double lse = log(sum) + 0.69314718055994530942 * shift - kLog2eOff * top;
-      shifts[k] = isfinite(score) && isfinite(lse) ? score - lse : __longlong_as_double(0x7ff8000000000000ll);
+    // sum 2^shift = sum exp(x (1 + off)), which exp(top off) times the sum of exp(x) is but for off (x - top)
+    double lse = log(sum) + 0.69314718055994530942 * shift - kLog2eOff * top;
+    if (__any_sync(0xffffffffu, far)) {  // all relative to the maximum
+      sum = 0.0;
+      for (int i = lane; i < parts; i += 32) {
+        const Stats s = stats[k * parts + i];
+        if (s.top != -INFINITY || s.sum != 0.0f)
+          sum += (double)s.sum * (s.shift == kFar ? exp((double)s.top - (double)top)
+                                                  : exp2(s.shift - (double)top * (double)kLog2e));
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      lse = (double)top + log(sum);
     }
+    if (lane == 0)
+      shifts[k] = isfinite(score) && isfinite(lse) ? score - lse : __longlong_as_double(0x7ff8000000000000ll);
   }
   __syncthreads();
   // entry f of the lists; total -inf: none
