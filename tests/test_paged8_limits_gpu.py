@@ -195,3 +195,24 @@ def test_write_attention_and_reading_back_in_one_graph(dtype):
         x.fill_(7)
     step()
     assert all(torch.equal(x, y) for x, y in zip(got, (q, out, k, v))) and ops.page_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,H,KVH", [([6, 4], 4, 4), ([12, 16], 4, 4), ([3, 2], 14, 2), ([40, 70], 14, 2)])
+def test_nan_of_a_new_token_leaves_the_earlier_ones(new, H, KVH, dtype):
+    """What a token writes, those before it in the same step do not see: 8 and 16 rows, and the expanded pages."""
+    b = Coded(dtype, new, [30, 75], H, KVH, 16, seed=72)
+    clean = b.attend().view(b.T, KVH, -1)
+    for pool, scale in ((b.kp, b.ks), (b.vp, b.vs)):
+        for i, at in ((0, new[0] - 1), (1, new[1] // 2), (1, 0)):
+            p = b.k[i].shape[0] - new[i] + at
+            page, row = int(b.table[i, p // 16]), p % 16
+            was = pool[page, 0, row].clone(), scale[page, 0, row].clone()
+            pool[page, 0, row], scale[page, 0, row] = 0, 255
+            out = b.attend().view(b.T, KVH, -1)
+            bad = torch.isnan(out)
+            sees = torch.zeros((b.T, KVH, 1), dtype=torch.bool, device="cuda")
+            sees[b.starts[i] + at:b.starts[i + 1], 0] = True
+            assert torch.equal(bad, sees.expand_as(bad))
+            b.check(torch.where(bad, clean, out).view(b.T, -1))  # a lost maximum may move the others' base
+            pool[page, 0, row], scale[page, 0, row] = was

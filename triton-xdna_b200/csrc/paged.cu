@@ -382,7 +382,9 @@ struct ExpandArgs {
 // The pages that a batch names as bf16, for the tcgen05 attention kernel, whose
 // operands are bf16 tiles in shared memory.  A warp takes 8 rows of a page and
 // head at a time: 16 codes a lane of K and of V.  Where pages go by their own
-// number and sequences share one, each writes the same values.
+// number and sequences share one, each writes the same values.  A value of NaN
+// becomes a key of NaN and a value of zeros: the same for rows that see it, and those
+// that do not are not reached by zero times NaN.
 template <Format F>
 __global__ void __launch_bounds__(256) paged_expand_kernel(const ExpandArgs a) {
   pdl_wait();
@@ -432,7 +434,7 @@ __global__ void __launch_bounds__(256) paged_expand_kernel(const ExpandArgs a) {
         const int64_t to = ((slot * a.KVH + head[u]) * a.page_size + row[u]) * kRowDims + d;
 #pragma unroll
         for (int kind = 0; kind < 2; ++kind) {
-          const float scale = byte_scale((int)e[u][kind]);
+          const float scale = e[u][1] != kNanByte ? byte_scale((int)e[u][kind]) : kind ? 0.0f : byte_scale(kNanByte);
           const uint4 v = c[u][kind];
           const uint2 x0 = decode4<F>(v.x, scale), x1 = decode4<F>(v.y, scale);
           const uint2 x2 = decode4<F>(v.z, scale), x3 = decode4<F>(v.w, scale);
@@ -977,13 +979,18 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT>::kThreads, 1) paged_att
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int key = k0 + (kCoded ? row_of(2 * mt + (e >> 1), g) : mt * 16 + g + (e >> 1) * 8);
+              for (int h = 0; h < 2; ++h) {
+                const int key = k0 + (kCoded ? row_of(2 * mt + h, g) : mt * 16 + g + h * 8);
+                // A value of NaN (2^-e_v is -infinity) goes by the scores here: a weight of zero times it would reach rows
+                // that do not see it.  What no row sees may have any exponent.
+                const bool nan = kCoded && fv[mt][h] == -INFINITY;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-                  if (key > pos[n][e & 1]) s[n][mt][e] = -INFINITY;
-                // what no row sees may have any exponent, also one that is NaN times a weight of zero
-                if (kCoded && key >= sc.keys) fv[mt][e >> 1] = 0.0f;
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                  for (int n = 0; n < NT; ++n)
+                    if (key > pos[n][e]) s[n][mt][2 * h + e] = -INFINITY;
+                    else if (nan) s[n][mt][2 * h + e] = __int_as_float(0x7fc00000);
+                if (kCoded && (nan || key >= sc.keys)) fv[mt][h] = 0.0f;
               }
           }
           uint32_t pb[NT][2 * MT];  // P as the B operand of O^T = V^T P^T, 8 keys each
