@@ -816,9 +816,9 @@ XB_API int xb_argmax_f32(const float* x, int64_t rows, int64_t cols,
  * [groups, beams] f32 (pitch ld_scores): of all beams k and tokens v of a
  * group the `count` largest of
  *   scores[k] + logits[k, v] - log(sum_u exp(logits[k, u])),
- * largest first, equal ones by the lowest (k, v): their sums (values f32),
- * beams (parents) and tokens, [groups, count] contiguous.  Sums are compared in 64
- * bits.  A beam with a score that is not finite (-inf: one that is out), with a
+ * largest first: their sums (values f32), beams (parents) and tokens, [groups,
+ * count] contiguous.  Sums are compared in 64 bits; equal ones go by the lowest k,
+ * those of one beam by the larger logit, then the lowest v.  A beam with a score that is not finite (-inf: one that is out), with a
  * NaN or +inf among its logits or with none above -inf has no continuation,
  * nor has a token whose logit is -inf; where fewer than `count` are left the rest
  * is -inf, -1, -1.  At most 64 beams, 64 continuations, 2^20 groups.  `workspace`

@@ -167,6 +167,17 @@ def test_rows_of_nothing_but_masks_and_logits_of_any_size(dtype):
     check(logits, scores, 64)
 
 
+def test_sums_that_64_bits_do_not_tell_apart():
+    """Scores so large that the logits are lost in the sums: the lowest beam first, its tokens as their logits."""
+    x, _ = make(2, 3, 5000, seed=40)
+    scores = torch.tensor([[-1e30, -1e30, -1e30], [-1e30, -1e29, -2e30]], device="cuda")
+    order = x.cpu().argsort(dim=1, descending=True, stable=True)
+    values, parents, tokens = (t.cpu() for t in ops.beam_select(x, scores, 40))
+    assert parents.tolist() == [[0] * 40, [1] * 40]
+    assert torch.equal(tokens[0], order[0, :40]) and torch.equal(tokens[1], order[4, :40])
+    assert torch.equal(values, torch.tensor([[-1e30] * 40, [-1e29] * 40]))
+
+
 def test_scores_between_rows_of_a_wider_tensor():
     logits, scores = make(4, 3, 2500, seed=25)
     wide = torch.full((4, 9), 7.0, device="cuda")

@@ -3,7 +3,8 @@
 //
 //   total[k, v] = score[k] + x[k, v] - log sum_u exp(x[k, u]),
 //
-// largest first, equal sums by the lowest (beam, token).  It stands beside the
+// largest first, equal sums by the lowest beam, then the larger logit, then the
+// lowest token.  It stands beside the
 // greedy choice (xb_argmax_f32, csrc/llm.cu; examples/qwen2_5/model.py:1134-1179
 // and examples/gpt2/model.py:1144-1206 take the argmax of the last position's logits).
 //
@@ -338,10 +339,14 @@ __global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __
 
 struct Candidate {
   double total;
-  uint64_t place;  // beam << 32 | token
+  uint64_t key;
+  int beam;
 };
+// Sums that 64 bits do not tell apart go by the beam, those of one beam by their
+// logits, as the lists do.
 __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
-  return a.total > b.total || (a.total == b.total && a.place < b.place);
+  if (a.total != b.total) return a.total > b.total;
+  return a.beam != b.beam ? a.beam < b.beam : a.key > b.key;
 }
 
 // One group: its beams' lists joined.  At least `count` entries reach a bound; what
@@ -420,7 +425,8 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
     const double t = shifts[k] + (double)unordered((uint32_t)(key >> 32));
     Candidate c;
     c.total = key != 0 && isfinite(t) ? t : -INFINITY;
-    c.place = (uint64_t)k << 32 | (0xffffffffu - (uint32_t)key);
+    c.key = key;
+    c.beam = k;
     return c;
   };
   auto each = [&](auto&& take) {
@@ -442,8 +448,8 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
   int64_t *parent = parents + g * count, *token = tokens + g * count;
   auto put = [&](int at, const Candidate& c) {
     value[at] = (float)c.total;
-    parent[at] = (int64_t)(c.place >> 32);
-    token[at] = (int64_t)(c.place & 0xffffffffu);
+    parent[at] = c.beam;
+    token[at] = (int64_t)(0xffffffffu - (uint32_t)c.key);
   };
   const int left = n;
   if (left <= kPicked) {
@@ -463,9 +469,9 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
     }
     return;
   }
-  Candidate last{INFINITY, 0};  // the candidate before
+  Candidate last{INFINITY, 0, 0};  // the candidate before
   for (int at = 0; at < count; ++at) {
-    Candidate mine{-INFINITY, ~0ull};
+    Candidate mine{-INFINITY, 0, kMaxBeams};
     each([&](const Candidate& c) {
       if ((at == 0 || before(last, c)) && before(c, mine)) mine = c;
     });
