@@ -349,16 +349,36 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
   return a.beam != b.beam ? a.beam < b.beam : a.key > b.key;
 }
 
+// 2^n, n <= 0, in 64 bits
+__device__ __forceinline__ double power64(int n) { return n < -1022 ? 0.0 : __hiloint2double((n + 1023) << 20, 0); }
+
+// log sum of a row one of whose parts is relative to its maximum: all of them, relative to the row's (rare, and kept out of
+// the way of what is fetched every time).
+__device__ __noinline__ double far_log_sum(const Stats* stats, int parts, float top) {
+  double sum = 0.0;
+  for (int i = threadIdx.x & 31; i < parts; i += 32) {
+    const Stats s = stats[i];
+    if (s.top != -INFINITY || s.sum != 0.0f)
+      sum += (double)s.sum * (s.shift == kFar ? exp((double)s.top - (double)top)
+                                              : exp2(s.shift - (double)top * (double)kLog2e));
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return (double)top + log(sum);
+}
+
 // One group: its beams' lists joined.  At least `count` entries reach a bound; what
 // lies below it (compared in fp32, which no rounding turns round) falls away.
 // Should more be left than fit, as where very many sums are equal, the choice
 // goes step by step, the best of all entries behind the last choice each time.
+// Latency bounds it, most of all that of fetching instructions, which are cold in
+// every launch: sums are formed once, and what is rare stays out of line.
 __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restrict__ scores, int64_t ld_scores,
-                                                             const uint64_t* __restrict__ lists,
-                                                             const Stats* __restrict__ stats, int beams, int parts,
-                                                             int count, float* __restrict__ values,
-                                                             int64_t* __restrict__ parents,
-                                                             int64_t* __restrict__ tokens) {
+                                                          const uint64_t* __restrict__ lists,
+                                                          const Stats* __restrict__ stats, int beams, int parts,
+                                                          uint64_t beam_magic, int count, float* __restrict__ values,
+                                                          int64_t* __restrict__ parents,
+                                                          int64_t* __restrict__ tokens) {
   __shared__ Candidate found[kPicked];
   __shared__ double shifts[kMaxBeams];  // score - log sum; NaN: the beam is out
   __shared__ float few[kFew + 1];
@@ -388,12 +408,11 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
     bool far = false;
     for (int i0 = 0; i0 < parts; i0 += 32) {
       const Stats s = i0 + lane < parts ? stats[k * parts + i0 + lane] : Stats{-INFINITY, 0.0f, 0, 0};
-      const bool any = s.top != -INFINITY || s.sum != 0.0f;
+      const bool any = s.top != -INFINITY || s.sum != 0.0f, near = any && s.shift != kFar;
       top = fmaxf(top, s.top);
-      far |= any && s.shift == kFar;
-      const int to = max(shift, __reduce_max_sync(0xffffffffu, any && s.shift != kFar ? s.shift : -kFar));
-      sum = scalbn(sum, max(shift - to, -2000)) +
-            (any && s.shift != kFar ? scalbn((double)s.sum, max(s.shift - to, -2000)) : 0.0);
+      far |= any && !near;
+      const int to = max(shift, __reduce_max_sync(0xffffffffu, near ? s.shift : -kFar));
+      sum = sum * power64(shift - to) + (near ? (double)s.sum * power64(s.shift - to) : 0.0);
       shift = to;
     }
 #pragma unroll
@@ -401,48 +420,54 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
-    // sum 2^shift = sum exp(x (1 + off)), which exp(top off) times the sum of exp(x) is but for off (x - top)
-    double lse = log(sum) + 0.69314718055994530942 * shift - kLog2eOff * top;
-    if (__any_sync(0xffffffffu, far)) {  // all relative to the maximum
-      sum = 0.0;
-      for (int i = lane; i < parts; i += 32) {
-        const Stats s = stats[k * parts + i];
-        if (s.top != -INFINITY || s.sum != 0.0f)
-          sum += (double)s.sum * (s.shift == kFar ? exp((double)s.top - (double)top)
-                                                  : exp2(s.shift - (double)top * (double)kLog2e));
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      lse = (double)top + log(sum);
+    // sum 2^shift = sum exp(x (1 + off)), which exp(top off) times the sum of exp(x) is but for off (x - top).  The logarithm
+    // of the sum's mantissa in 32 bits (off by 2^-24 as the sum is), the rest of it in 64.
+    const int hi = __double2hiint(sum);
+    const float mantissa = (float)__hiloint2double((hi & 0xfffff) | 0x3ff00000, __double2loint(sum));
+    double lse = (double)logf(mantissa) + 0.69314718055994530942 * ((hi >> 20) - 1023 + shift) - kLog2eOff * top;
+    bool out = !(sum > 0.0);  // NaN too
+    if (__any_sync(0xffffffffu, far)) {
+      lse = far_log_sum(stats + k * parts, parts, top);
+      out = !isfinite(lse);
     }
-    if (lane == 0)
-      shifts[k] = isfinite(score) && isfinite(lse) ? score - lse : __longlong_as_double(0x7ff8000000000000ll);
+    if (lane == 0) shifts[k] = isfinite(score) && !out ? score - lse : __longlong_as_double(0x7ff8000000000000ll);
   }
   __syncthreads();
   // entry f of the lists; total -inf: none
   auto candidate = [&](int f, uint64_t key) -> Candidate {
-    const int k = f / (parts * count);
-    const double t = shifts[k] + (double)unordered((uint32_t)(key >> 32));
     Candidate c;
-    c.total = key != 0 && isfinite(t) ? t : -INFINITY;
+    c.beam = (int)((uint64_t)f * beam_magic >> 32);  // f / (parts * count)
+    const double t = shifts[c.beam] + (double)unordered((uint32_t)(key >> 32));
+    c.total = key != 0 && t == t ? t : -INFINITY;
     c.key = key;
-    c.beam = k;
     return c;
   };
-  auto each = [&](auto&& take) {
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (j * kPick < entries) take(candidate(min(j * kPick + (int)threadIdx.x, entries - 1), ahead[j]));
-    for (int f = kAhead * kPick + threadIdx.x; f < entries; f += kPick) take(candidate(f, lists[f]));
-  };
+  double sums[kAhead];
   float best = -INFINITY;
-  each([&](const Candidate& c) { best = fmaxf(best, (float)c.total); });
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    if (j * kPick >= entries) break;
+    sums[j] = candidate(min(j * kPick + (int)threadIdx.x, entries - 1), ahead[j]).total;
+    best = fmaxf(best, (float)sums[j]);
+  }
+#pragma unroll 1
+  for (int f = kAhead * kPick + threadIdx.x; f < entries; f += kPick) best = fmaxf(best, (float)candidate(f, lists[f]).total);
   const float bound = reached_by<kPick>(best, count, few);
-  each([&](const Candidate& c) {
-    if (c.total == -INFINITY || (float)c.total < bound) return;
+  auto take = [&](double sum, int f, uint64_t key) {
+    if (sum == -INFINITY || (float)sum < bound) return;
     const int at = atomicAdd(&n, 1);
-    if (at < kPicked) found[at] = c;
-  });
+    if (at < kPicked) found[at] = candidate(f, key);
+  };
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    if (j * kPick >= entries) break;
+    take(sums[j], j * kPick + threadIdx.x, ahead[j]);
+  }
+#pragma unroll 1
+  for (int f = kAhead * kPick + threadIdx.x; f < entries; f += kPick) {
+    const uint64_t key = lists[f];
+    take(candidate(f, key).total, f, key);
+  }
   __syncthreads();
   float* value = values + g * count;
   int64_t *parent = parents + g * count, *token = tokens + g * count;
@@ -472,9 +497,11 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
   Candidate last{INFINITY, 0, 0};  // the candidate before
   for (int at = 0; at < count; ++at) {
     Candidate mine{-INFINITY, 0, kMaxBeams};
-    each([&](const Candidate& c) {
+#pragma unroll 1
+    for (int f = threadIdx.x; f < entries; f += kPick) {
+      const Candidate c = candidate(f, lists[f]);
       if ((at == 0 || before(last, c)) && before(c, mine)) mine = c;
-    });
+    }
     __syncthreads();
     found[threadIdx.x] = mine;
     __syncthreads();
@@ -584,7 +611,7 @@ extern "C" int xb_beam_select(const void* logits, const float* scores, int64_t g
                              Ring<__nv_bfloat16>::kSmem);
   if (e == cudaSuccess)
     e = launch_k(beam_pick_kernel, (unsigned)groups, kPick, 0, s, scores, ld_scores, lists, stats, (int)beams, parts,
-                 (int)count, values, parents, tokens);
+                 ((1ull << 32) + parts * count - 1) / (parts * count), (int)count, values, parents, tokens);
   if (e != cudaSuccess) {
     set_err(err, errlen, "%s: %s", what, cudaGetErrorString(e));
     return XB_ERR_CUDA;
