@@ -5,7 +5,9 @@ Every ``csrc/*.cu`` file is compiled for sm_100a only
 ``csrc/_build/`` and linked into ``xb200/libxb200.so`` next to this file.
 The CUDA runtime is linked statically, so the library depends on nothing but
 the driver; the tensor-map encoder is fetched through
-``cudaGetDriverEntryPoint`` instead of linking libcuda.
+``cudaGetDriverEntryPoint`` instead of linking libcuda.  ``csrc/calls.cpp``, the
+calls of some of its operators on torch tensors without the interpreter, is
+compiled with g++ against torch's headers into ``xb200/_calls.so``.
 
 Rebuilds are incremental on file modification times (any header change
 rebuilds everything).
@@ -19,6 +21,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)  # triton-xdna_b200/
@@ -26,6 +29,7 @@ CSRC = os.path.join(ROOT, "csrc")
 BUILD = os.path.join(CSRC, "_build")
 INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 LIB_PATH = os.path.join(PKG_DIR, "libxb200.so")
+CALLS_PATH = os.path.join(PKG_DIR, "_calls.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
@@ -69,13 +73,37 @@ def _compile(src: str, extra: list[str]) -> str:
     return obj
 
 
+def build_calls() -> str:
+    """Compile ``csrc/calls.cpp``; returns the path of ``_calls.so``."""
+    import torch
+
+    src, at = os.path.join(CSRC, "calls.cpp"), os.path.dirname(torch.__file__)
+    newest = max(os.path.getmtime(f) for f in (src, *_headers(), os.path.join(at, "version.py")))
+    if os.path.exists(CALLS_PATH) and os.path.getmtime(CALLS_PATH) >= newest:
+        return CALLS_PATH
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    include = [INCLUDE, os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    tmp = CALLS_PATH + ".tmp"
+    cmd = ["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *["-I" + p for p in include], src, "-o", tmp,
+           "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on calls.cpp:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, CALLS_PATH)
+    return CALLS_PATH
+
+
 def build(verbose: bool = False, extra_flags: list[str] | None = None) -> str:
     """Compile and link the library; returns the path of ``libxb200.so``."""
     os.makedirs(BUILD, exist_ok=True)
     extra = list(extra_flags or [])
     srcs = _sources()
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
+        calls = ex.submit(build_calls)
         objs = list(ex.map(lambda s: _compile(s, extra), srcs))
+        calls.result()
     if os.path.exists(LIB_PATH) and not extra:
         lib_m = os.path.getmtime(LIB_PATH)
         if all(os.path.getmtime(o) <= lib_m for o in objs):

@@ -13,6 +13,7 @@ import ctypes
 import functools
 import itertools
 import math
+import os
 import struct
 
 import torch
@@ -1024,6 +1025,28 @@ def argmax(x, out=None):
     return out
 
 
+_calls = None  # the module of the same name, once it has the library's addresses
+
+
+def _direct():
+    """csrc/calls.cpp: functions that make an ordinary call without the
+    interpreter, and leave any other alone."""
+    global _calls
+    if _calls is None:
+        lib = _lib.load()
+        if not os.path.exists(os.path.join(_lib.PKG_DIR, "_calls.so")):
+            raise RuntimeError("xb200/_calls.so is missing: build it with "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`")
+        from . import _calls as direct
+
+        direct.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "xb_paged_attention_workspace_size", "xb_paged_attention_bf16", "xb_paged_attention_q8_workspace_size",
+            "xb_paged_attention_q8", "xb_paged_rope_kv_bf16", "xb_paged_rope_kv_q8", "xb_paged_read_kv",
+            "xb_beam_select_workspace_size", "xb_beam_select")})
+        _calls = direct
+    return _calls
+
+
 @functools.lru_cache(maxsize=256)
 def _beam_select_bytes(dev, G, K, V, N) -> int:
     need = ctypes.c_size_t(0)
@@ -1039,6 +1062,9 @@ def beam_select(logits, scores, count):
     first, equal ones by the lowest k, then the logit, then the lowest v.  Returns (values [G, count] fp32,
     parents int64, tokens int64); a beam whose score is -inf is out, and places
     for which no continuation is left hold -inf, -1, -1."""
+    done = (_calls or _direct()).beam_select(logits, scores, count)
+    if done is not None:
+        return done
     dev = _device_of(logits, scores)
     dt = DT.get(logits.dtype)
     if logits.dtype not in FLOAT_DTYPES or scores.dtype is not torch.float32:
@@ -1195,6 +1221,9 @@ def paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_star
     8-bit pages (int8 or float8_e4m3fn, with k_scale and v_scale): the same bf16
     numbers are written as codes, with one exponent byte a position and KV head
     (include/xb200.h has the arithmetic)."""
+    if (_calls or _direct()).paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len,
+                                           k_scale, v_scale):
+        return q_out
     dev = _device_of(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
     if (cos_t is None) != (sin_t is None):
         raise ValueError("give both RoPE tables or neither")
@@ -1226,6 +1255,8 @@ def paged_read_kv(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k
     8-bit pages; what a code stands for is a bf16 number, so nothing is
     rounded.  Tokens outside the sequences are left alone; one without a page
     reads as zeros (page_status())."""
+    if (_calls or _direct()).paged_read_kv(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale):
+        return k_out, v_out
     dev = _device_of(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
     KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
     if k_scale is None:
@@ -1263,6 +1294,8 @@ def paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale
     sequences are left as they are; a token that sees no key gets zeros.
     8-bit pages (int8 or float8_e4m3fn, with k_scale and v_scale): the attention
     over what the codes stand for."""
+    if (_calls or _direct()).paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale, k_scale, v_scale):
+        return out
     dev = _device_of(q, k_pages, v_pages, out, page_table, q_start, kv_len, k_scale, v_scale)
     KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
     if q.dim() != 3 or q.shape[2] != D:
