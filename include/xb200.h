@@ -818,12 +818,13 @@ XB_API int xb_argmax_f32(const float* x, int64_t rows, int64_t cols,
  *   scores[k] + logits[k, v] - log(sum_u exp(logits[k, u])),
  * largest first: their sums (values f32), beams (parents) and tokens, [groups,
  * count] contiguous.  Sums are compared in 64 bits; equal ones go by the lowest k,
- * those of one beam by the larger logit, then the lowest v.  A beam with a score that is not finite (-inf: one that is out), with a
- * NaN or +inf among its logits or with none above -inf has no continuation,
- * nor has a token whose logit is -inf; where fewer than `count` are left the rest
- * is -inf, -1, -1.  At most 64 beams, 64 continuations, 2^20 groups.  `workspace`
- * (16-byte aligned, size from the query) belongs to the call.  Extends the greedy
- * choice of model.py:1155, 1171. */
+ * those of one beam by the larger logit, then the lowest v.  A beam with a score
+ * that is not finite (-inf: one that is out), with a NaN or +inf among its logits
+ * or with none above -inf has no continuation, nor has a token whose logit is
+ * -inf; where fewer than `count` are left the rest is -inf, -1, -1.  At most 64
+ * beams, 64 continuations, 2^20 groups.  `workspace` (16-byte aligned, size from
+ * the query) belongs to the call.  Extends the greedy choice of model.py:1155,
+ * 1171. */
 XB_API int xb_beam_select_workspace_size(int64_t groups, int64_t beams,
                                          int64_t vocab, int64_t count,
                                          size_t* bytes, char* err,

@@ -135,11 +135,23 @@ struct Ring {  // a warp's groups of tokens on their way from memory
 // least `count` lanes' maxima reach is one that the `count` best tokens reach, and
 // only the few runs whose maximum reaches it are looked through again, in the ring
 // or in the L2: some 20 of 2048 for count = 16.  Keeping the candidates during the
-// stream took 44 instructions a token, mostly to find that there is none.
+// stream took 44 instructions a token, mostly to find that there is none (94 us where
+// this takes 43).
+//
+// What bounds it: 256 rows of 151936 fp32 logits, 156 MB, take 43.2 us with the choice,
+// 3.6 TB/s.  The stream alone takes some 32: 14 instructions a token over all, memory
+// at 4.9 TB/s, and 512 CTAs for 592 places (busy 75 % of the time); behind it comes
+// what no CTA has other work for, the look through the runs and the lists (5), and the
+// choice (5).  240 rows of 50257 in bf16 take 18.8 us, 4 of 151936 8.8: start, one group a
+// warp, the bound, the lists and the second launch.  Measured (us of these three):
+// CTAs of 128 threads 48.9 / 19.0 / 11.8 where 256 took 44.8 / 19.5 / 9.5; rows divided
+// for 4, 6, 7, 8, 12 CTAs an SM 43.7 / 46.6 / 42.1 / 42.2 / 45.1 and 19.1 / 20.4 / 19.2 /
+// 19.4 / 23.4, but for 100 rows of 50257 4 13.5 and 7 16.7; 16 runs a lane, with maxima
+// of 16 bits, 42.8 / 19.8 / 10.1 where 8 take 43.9 / 19.6 / 9.9.
 template <typename T>
-__global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __restrict__ logits, int64_t ld, int64_t vocab,
-                                                                int count, int parts, uint64_t* __restrict__ lists,
-                                                                Stats* __restrict__ stats) {
+__global__ void __launch_bounds__(kScan, kResident)
+    beam_scan_kernel(const T* __restrict__ logits, int64_t ld, int64_t vocab, int count, int parts,
+                     uint64_t* __restrict__ lists, Stats* __restrict__ stats) {
   using R = Ring<T>;
   constexpr int kWarps = kScan / 32;
   extern __shared__ __align__(16) uint8_t ring[];
@@ -182,7 +194,8 @@ __global__ void __launch_bounds__(kScan, kResident) beam_scan_kernel(const T* __
           } else {  // vectors that reach out of the row: what of them lies in it
             for (int e = 0; e < 16; e += (int)sizeof(T))
               if (pos + e >= off && pos + e < end)
-                *reinterpret_cast<T*>(mine + it % R::kStages * R::kStage + k + e) = *reinterpret_cast<const T*>(src + e);
+                *reinterpret_cast<T*>(mine + it % R::kStages * R::kStage + k + e) =
+                    *reinterpret_cast<const T*>(src + e);
           }
         }
       }
@@ -352,8 +365,8 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
 // 2^n, n <= 0, in 64 bits
 __device__ __forceinline__ double power64(int n) { return n < -1022 ? 0.0 : __hiloint2double((n + 1023) << 20, 0); }
 
-// log sum of a row one of whose parts is relative to its maximum: all of them, relative to the row's (rare, and kept out of
-// the way of what is fetched every time).
+// log sum of a row one of whose parts is relative to its maximum: all of them, relative
+// to the row's (rare, and kept out of the way of what is fetched every time).
 __device__ __noinline__ double far_log_sum(const Stats* stats, int parts, float top) {
   double sum = 0.0;
   for (int i = threadIdx.x & 31; i < parts; i += 32) {
@@ -372,7 +385,9 @@ __device__ __noinline__ double far_log_sum(const Stats* stats, int parts, float 
 // Should more be left than fit, as where very many sums are equal, the choice
 // goes step by step, the best of all entries behind the last choice each time.
 // Latency bounds it, most of all that of fetching instructions, which are cold in
-// every launch: sums are formed once, and what is rare stays out of line.
+// every launch (3.4 of the 12 clocks between a warp's instructions): sums are formed
+// once, and what is rare stays out of line, which took 1 us off every call (1 x 4 beams
+// 9.8 -> 8.8).
 __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restrict__ scores, int64_t ld_scores,
                                                           const uint64_t* __restrict__ lists,
                                                           const Stats* __restrict__ stats, int beams, int parts,
@@ -420,8 +435,8 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
-    // sum 2^shift = sum exp(x (1 + off)), which exp(top off) times the sum of exp(x) is but for off (x - top).  The logarithm
-    // of the sum's mantissa in 32 bits (off by 2^-24 as the sum is), the rest of it in 64.
+    // sum 2^shift = sum exp(x (1 + off)), which exp(top off) times the sum of exp(x) is but for off (x - top).  The
+    // logarithm of the sum's mantissa in 32 bits (off by 2^-24 as the sum is), the rest of it in 64.
     const int hi = __double2hiint(sum);
     const float mantissa = (float)__hiloint2double((hi & 0xfffff) | 0x3ff00000, __double2loint(sum));
     double lse = (double)logf(mantissa) + 0.69314718055994530942 * ((hi >> 20) - 1023 + shift) - kLog2eOff * top;
@@ -451,7 +466,8 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
     best = fmaxf(best, (float)sums[j]);
   }
 #pragma unroll 1
-  for (int f = kAhead * kPick + threadIdx.x; f < entries; f += kPick) best = fmaxf(best, (float)candidate(f, lists[f]).total);
+  for (int f = kAhead * kPick + threadIdx.x; f < entries; f += kPick)
+    best = fmaxf(best, (float)candidate(f, lists[f]).total);
   const float bound = reached_by<kPick>(best, count, few);
   auto take = [&](double sum, int f, uint64_t key) {
     if (sum == -INFINITY || (float)sum < bound) return;
@@ -506,7 +522,8 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
     found[threadIdx.x] = mine;
     __syncthreads();
     for (int o = kPick / 2; o > 0; o >>= 1) {
-      if (threadIdx.x < o && before(found[threadIdx.x + o], found[threadIdx.x])) found[threadIdx.x] = found[threadIdx.x + o];
+      if (threadIdx.x < o && before(found[threadIdx.x + o], found[threadIdx.x]))
+        found[threadIdx.x] = found[threadIdx.x + o];
       __syncthreads();
     }
     last = found[0];

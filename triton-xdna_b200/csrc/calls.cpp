@@ -64,7 +64,6 @@ struct Args {
   PyObject* const* a;
   int device = -1;
   bool ok = true;
-  const at::Tensor* none = nullptr;
 
   const at::Tensor& operator()(int i) {
     static const at::Tensor nothing;
@@ -93,7 +92,8 @@ bool page_args(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table
       coded != (vs != nullptr) || table.scalar_type() != at::kInt || q_start.scalar_type() != at::kInt ||
       kv_len.scalar_type() != at::kInt)
     return false;
-  if (k.dim() != 4 || v.sizes() != k.sizes() || kv_len.dim() != 1 || table.dim() != 2 || q_start.dim() != 1) return false;
+  if (k.dim() != 4 || v.sizes() != k.sizes() || kv_len.dim() != 1 || table.dim() != 2 || q_start.dim() != 1)
+    return false;
   const int64_t n = k.size(0), h = k.size(1), p = k.size(2), d = k.size(3), B = table.size(0), cols = table.size(1);
   if (kv_len.size(0) != B || q_start.size(0) != B + 1 || cols == 0 || (table.stride(1) != 1 && cols > 1) ||
       !q_start.is_contiguous() || !kv_len.is_contiguous() || ((k.stride(3) != 1 || v.stride(3) != 1) && d > 1))
@@ -123,7 +123,8 @@ bool page_args(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table
   if (!coded) return true;
   kv8.dtype = type == at::kChar ? XB_DT_I8 : XB_DT_F8E4M3;
   for (const at::Tensor* t : {ks, vs})
-    if (t->scalar_type() != at::kByte || t->sizes() != k.sizes().slice(0, 3) || (t->stride(2) != 1 && p > 1)) return false;
+    if (t->scalar_type() != at::kByte || t->sizes() != k.sizes().slice(0, 3) || (t->stride(2) != 1 && p > 1))
+      return false;
   kv8.k_scale = static_cast<uint8_t*>(ks->data_ptr());
   kv8.v_scale = static_cast<uint8_t*>(vs->data_ptr());
   kv8.ks_page = n == 1 ? h * p : ks->stride(0);
@@ -137,7 +138,8 @@ bool page_args(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table
 int64_t token_rows(const at::Tensor& t, int64_t tokens, int64_t row) {
   if (t.scalar_type() != at::kBFloat16) return -1;
   const int64_t dims = t.dim();
-  if ((dims != 2 && dims != 3) || t.size(0) != tokens || (dims == 2 ? t.size(1) : t.size(1) * t.size(2)) != row) return -1;
+  if ((dims != 2 && dims != 3) || t.size(0) != tokens || (dims == 2 ? t.size(1) : t.size(1) * t.size(2)) != row)
+    return -1;
   if (tokens && (t.stride(-1) != 1 || (dims == 3 && t.size(1) > 1 && t.stride(1) != t.size(2)))) return -1;
   return tokens > 1 ? t.stride(0) : row;
 }
@@ -146,7 +148,8 @@ int64_t token_rows(const at::Tensor& t, int64_t tokens, int64_t row) {
 // of the same rows.
 bool apart(const void* p, int64_t ld_p, int64_t row_p, const void* q, int64_t ld_q, int64_t row_q, int64_t tokens) {
   const auto x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
-  if (tokens == 0 || x + 2 * ((tokens - 1) * ld_p + row_p) <= y || y + 2 * ((tokens - 1) * ld_q + row_q) <= x) return true;
+  if (tokens == 0 || x + 2 * ((tokens - 1) * ld_p + row_p) <= y || y + 2 * ((tokens - 1) * ld_q + row_q) <= x)
+    return true;
   if (ld_p != ld_q || ld_p <= 0) return false;
   int64_t off = (int64_t)(y - x) / 2 % ld_p;  // both are multiples of two
   if (off < 0) off += ld_p;
@@ -162,7 +165,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   if (!bound || count != 10 || !PyFloat_CheckExact(a[7])) Py_RETURN_FALSE;
   Args arg{a};
-  const at::Tensor &q = arg(0), &k = arg(1), &v = arg(2), &out = arg(3), &table = arg(4), &q_start = arg(5), &kv_len = arg(6);
+  const at::Tensor &q = arg(0), &k = arg(1), &v = arg(2), &out = arg(3), &table = arg(4), &q_start = arg(5),
+                   &kv_len = arg(6);
   const at::Tensor *ks = arg.optional(8), *vs = arg.optional(9);
   xb_paged_kv8 kv;
   if (!arg.here() || !page_args(k, v, table, q_start, kv_len, ks, vs, kv)) Py_RETURN_FALSE;
@@ -186,7 +190,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
   void* stream = c10::cuda::getCurrentCUDAStream(arg.device).stream();
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = coded ? entry.attention8(pq, po, &kv, T, H, ld_q, ld_out, scale, ws.get(), need, stream, err.text, sizeof(err.text))
+  rc = coded ? entry.attention8(pq, po, &kv, T, H, ld_q, ld_out, scale, ws.get(), need, stream, err.text,
+                                sizeof(err.text))
              : entry.attention(pq, po, &kv.kv, T, H, ld_q, ld_out, scale, ws.get(), need, stream, err.text,
                                sizeof(err.text));
   Py_END_ALLOW_THREADS
@@ -194,12 +199,13 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
-// paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale): whether it was done
+// paged_rope_kv(qkv, cos_t, sin_t, q_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale): the same
 PyObject* paged_rope_kv(PyObject*, PyObject* const* a, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   if (!bound || count != 11 || (a[1] == Py_None) != (a[2] == Py_None)) Py_RETURN_FALSE;
   Args arg{a};
-  const at::Tensor &qkv = arg(0), &q = arg(3), &k = arg(4), &v = arg(5), &table = arg(6), &q_start = arg(7), &kv_len = arg(8);
+  const at::Tensor &qkv = arg(0), &q = arg(3), &k = arg(4), &v = arg(5), &table = arg(6), &q_start = arg(7),
+                   &kv_len = arg(8);
   const at::Tensor *cos_t = arg.optional(1), *sin_t = arg.optional(2), *ks = arg.optional(9), *vs = arg.optional(10);
   xb_paged_kv8 kv;
   if (!arg.here() || !page_args(k, v, table, q_start, kv_len, ks, vs, kv)) Py_RETURN_FALSE;
@@ -233,7 +239,7 @@ PyObject* paged_rope_kv(PyObject*, PyObject* const* a, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
-// paged_read_kv(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale): whether it was done
+// paged_read_kv(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale): the same
 PyObject* paged_read_kv(PyObject*, PyObject* const* a, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   if (!bound || count != 9) Py_RETURN_FALSE;
@@ -286,7 +292,8 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t given) {
   const void* x = logits.data_ptr();
   const float* s = static_cast<const float*>(scores.data_ptr());
   float* to_values = static_cast<float*>(values.data_ptr());
-  int64_t *to_parents = static_cast<int64_t*>(parents.data_ptr()), *to_tokens = static_cast<int64_t*>(tokens.data_ptr());
+  int64_t* to_parents = static_cast<int64_t*>(parents.data_ptr());
+  int64_t* to_tokens = static_cast<int64_t*>(tokens.data_ptr());
   const int64_t ld = G * K > 1 ? logits.stride(0) : V, ld_scores = G > 1 ? scores.stride(0) : K;
   void* stream = c10::cuda::getCurrentCUDAStream(arg.device).stream();
   int rc;
@@ -310,16 +317,20 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t given) {
   END_HANDLE_TH_ERRORS
 }
 
+PyCFunction function(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
+  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
+}
+
 PyMethodDef methods[] = {
     {"bind", bind, METH_O, "Addresses of the library's entry points."},
-    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_attention)), METH_FASTCALL, ""},
-    {"paged_rope_kv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_rope_kv)), METH_FASTCALL, ""},
-    {"paged_read_kv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_read_kv)), METH_FASTCALL, ""},
-    {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(beam_select)), METH_FASTCALL, ""},
+    {"paged_attention", function(paged_attention), METH_FASTCALL, "Whether it made the call."},
+    {"paged_rope_kv", function(paged_rope_kv), METH_FASTCALL, "Whether it made the call."},
+    {"paged_read_kv", function(paged_read_kv), METH_FASTCALL, "Whether it made the call."},
+    {"beam_select", function(beam_select), METH_FASTCALL, "What it selected, None if it did not make the call."},
     {nullptr, nullptr, 0, nullptr},
 };
 
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Paged and beam operators without the interpreter.", -1, methods};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Calls of operators without the interpreter.", -1, methods};
 
 }  // namespace
 

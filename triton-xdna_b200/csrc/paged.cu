@@ -384,7 +384,11 @@ struct ExpandArgs {
 // head at a time: 16 codes a lane of K and of V.  Where pages go by their own
 // number and sequences share one, each writes the same values.  A value of NaN
 // becomes a key of NaN and a value of zeros: the same for rows that see it, and those
-// that do not are not reached by zero times NaN.
+// that do not are not reached by zero times NaN.  Alone it takes 5.3 us for 24 prompts
+// of 130-1021 tokens (the attention 64.9 with it, 56.5 over bf16 pages), 8.4 for 32768
+// positions (685), 12.4 for a mixed step of 50 sequences (39.2).  With one part a warp
+// on its way, and the attention's search for its work behind the expansion, 65.7 and
+// 41.3.
 template <Format F>
 __global__ void __launch_bounds__(256) paged_expand_kernel(const ExpandArgs a) {
   pdl_wait();
@@ -580,7 +584,14 @@ constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared m
 // 11.1, 64 of 513-640 12.3 / 12.4 / 13.9 / 14.9, 128 of them 16.2 / 15.8 / 15.8 /
 // 16.1, 160 of 200-30000 84.4 / 64.4 / 56.3 / 55.6 (e4m3), 85.4 / 67.1 / 57.4 / 57.6
 // (int8).  Either way 32 keys are computed at a time: code for 64 is fetched in more
-// time than it saves.
+// time than it saves.  Other warps x keys x buffers, 160 long ones (int8) and 100 beams
+// of 12 heads, where 12 x 64 x 2 takes 57.9 / 23.5: 16 x 32 x 2 65.8 / 24.5, 12 x 32 x 4
+// 72.3 / 25.0, 8 x 64 x 3 67.3 / 24.7, 12 x 96 x 1 57.6 / 23.8, 12 x 128 x 1 59.4 / 24.1,
+// 6 x 128 x 2 72.5 / 27.0.  What bounds them: the loads alone take 50.1 / 15.6 us (48.5 /
+// 14.6 without the exponents), so the long ones stand at 1.15 of their loads; a tile of
+// 64 keys is some 850 instructions, 3 warps a scheduler, a chain of products, maxima,
+// exponentials and products again, and with one query row of 8 in use (the beams) it
+// is the longer part.
 template <int ROWS, Format F, bool SHORT>
 struct FewCfg {
   static constexpr bool kLong = F != kBf16 && !SHORT;
@@ -690,8 +701,8 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int token, int kvh
 }
 
 template <int ROWS, typename I, Format F, bool SHORT>
-__global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT>::kThreads, 1) paged_attn_few_kernel(const __grid_constant__ KvMaps maps,
-                                                                        const AttnArgs a) {
+__global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT>::kThreads, 1)
+    paged_attn_few_kernel(const __grid_constant__ KvMaps maps, const AttnArgs a) {
   using C = FewCfg<ROWS, F, SHORT>;
   constexpr bool kCoded = F != kBf16;
   constexpr int kWarps = C::kWarps, kBufs = C::kBufs, TK = C::kTile, MT = kTK / 16;
@@ -2090,7 +2101,8 @@ cudaError_t launch_few(int ctas, cudaStream_t s, const KvMaps& maps, const AttnA
 }
 template <Format F>
 cudaError_t launch_few(bool eight, bool wide, int ctas, cudaStream_t s, const KvMaps& maps, const AttnArgs& a) {
-  return eight ? (wide ? launch_few<8, int64_t, F, false>(ctas, s, maps, a) : launch_few<8, int, F, false>(ctas, s, maps, a))
+  return eight ? (wide ? launch_few<8, int64_t, F, false>(ctas, s, maps, a)
+                       : launch_few<8, int, F, false>(ctas, s, maps, a))
                : (wide ? launch_few<16, int64_t, F, false>(ctas, s, maps, a)
                        : launch_few<16, int, F, false>(ctas, s, maps, a));
 }
@@ -2350,8 +2362,8 @@ extern "C" int xb_paged_read_kv(void* k_out, void* v_out, const xb_paged_kv8* kv
   if (rc) return rc;
   auto kernel = kv8->dtype == XB_DT_BF16 ? paged_read_kv_kernel<kBf16>
                 : kv8->dtype == XB_DT_I8 ? paged_read_kv_kernel<kInt8> : paged_read_kv_kernel<kE4m3>;
-  launch_k<false>(kernel, (unsigned)((tokens + 8 * kReadTokens - 1) / (8 * kReadTokens)), 256, 0, (cudaStream_t)stream, a,
-                  bad);
+  launch_k<false>(kernel, (unsigned)((tokens + 8 * kReadTokens - 1) / (8 * kReadTokens)), 256, 0,
+                  (cudaStream_t)stream, a, bad);
   return check_launch(what, err, errlen);
 }
 
@@ -2424,8 +2436,8 @@ static int check_workspace(const void* workspace, size_t bytes, size_t need, con
 // xb_paged_attention_bf16 and, with `q8` (few rows), the attention over 8-bit pages;
 // `expanded`: over what paged_expand_kernel, launched just before, makes of them.
 static int attend(const char* what, const void* q, void* out, const xb_paged_kv* kv, const xb_paged_kv8* q8,
-                  bool expanded, int64_t tokens, int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
-                  size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+                  bool expanded, int64_t tokens, int64_t n_head, int64_t ld_q, int64_t ld_out, float scale,
+                  void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen) {
   int rc = check_pages(kv, what, err, errlen);
   if (!rc) rc = check_attention(kv, tokens, n_head, scale, what, err, errlen);
   if (rc) return rc;
@@ -2581,8 +2593,8 @@ extern "C" int xb_paged_attention_q8(const void* q, void* out, const xb_paged_kv
   if (!rc) rc = check_workspace(workspace, workspace_bytes, need, what, err, errlen);
   if (rc) return rc;
   if (few_rows(tokens, kv->batch, n_head / kv->n_kv_head))
-    return attend(what, q, out, kv, kv8, false, tokens, n_head, ld_q, ld_out, scale, workspace, workspace_bytes, stream, err,
-                  errlen);
+    return attend(what, q, out, kv, kv8, false, tokens, n_head, ld_q, ld_out, scale, workspace, workspace_bytes, stream,
+                  err, errlen);
   ExpandArgs e;
   bool compact;
   const int64_t slots = expand_slots(kv->batch, kv->max_pages, kv->n_pages, &compact);
@@ -2626,7 +2638,8 @@ extern "C" int xb_paged_attention_q8(const void* q, void* out, const xb_paged_kv
   wide.k_row = wide.v_row = kHD;
   wide.k_head = wide.v_head = kv->page_size * kHD;
   wide.k_page = wide.v_page = kv->n_kv_head * kv->page_size * kHD;
-  return attend(what, q, out, &wide, nullptr, true, tokens, n_head, ld_q, ld_out, scale, workspace, own, stream, err, errlen);
+  return attend(what, q, out, &wide, nullptr, true, tokens, n_head, ld_q, ld_out, scale, workspace, own, stream, err,
+                errlen);
 }
 
 extern "C" int xb_page_status(void* stream, int* status, char* err, size_t errlen) {

@@ -73,7 +73,8 @@ class _Search:
 
     def result(self) -> list[Hypothesis]:
         """The best `beams`; unfinished ones count with the length that they have."""
-        more = [] if len(self.finished) == self.beams and self.done else [self._hypothesis(*x) for x in self.live if x[0]]
+        over = len(self.finished) == self.beams and self.done
+        more = [] if over else [self._hypothesis(*x) for x in self.live if x[0]]
         return sorted(self.finished + more, key=lambda h: -h.score)[:self.beams]
 
 

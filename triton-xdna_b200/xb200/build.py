@@ -86,8 +86,8 @@ def build_calls() -> str:
                sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
     tmp = CALLS_PATH + ".tmp"
     cmd = ["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *["-I" + p for p in include], src, "-o", tmp,
-           "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *["-I" + p for p in include], src,
+           "-o", tmp, "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on calls.cpp:\n{res.stdout}\n{res.stderr}")

@@ -1059,9 +1059,10 @@ def beam_select(logits, scores, count):
     """A beam search step's choice: logits [G * K, V] (fp32 or bf16) of G groups
     of K beams and their scores [G, K] (fp32); of each group's beams k and
     tokens v the `count` largest scores[k] + log_softmax(logits[k])[v], largest
-    first, equal ones by the lowest k, then the logit, then the lowest v.  Returns (values [G, count] fp32,
-    parents int64, tokens int64); a beam whose score is -inf is out, and places
-    for which no continuation is left hold -inf, -1, -1."""
+    first, equal ones by the lowest k, then the logit, then the lowest v.
+    Returns (values [G, count] fp32, parents int64, tokens int64); a beam whose
+    score is -inf is out, and places for which no continuation is left hold
+    -inf, -1, -1."""
     done = (_calls or _direct()).beam_select(logits, scores, count)
     if done is not None:
         return done
@@ -1255,7 +1256,8 @@ def paged_read_kv(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k
     8-bit pages; what a code stands for is a bf16 number, so nothing is
     rounded.  Tokens outside the sequences are left alone; one without a page
     reads as zeros (page_status())."""
-    if (_calls or _direct()).paged_read_kv(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale):
+    if (_calls or _direct()).paged_read_kv(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale,
+                                           v_scale):
         return k_out, v_out
     dev = _device_of(k_out, v_out, k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
     KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
@@ -1294,7 +1296,8 @@ def paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale
     sequences are left as they are; a token that sees no key gets zeros.
     8-bit pages (int8 or float8_e4m3fn, with k_scale and v_scale): the attention
     over what the codes stand for."""
-    if (_calls or _direct()).paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale, k_scale, v_scale):
+    if (_calls or _direct()).paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale, k_scale,
+                                             v_scale):
         return out
     dev = _device_of(q, k_pages, v_pages, out, page_table, q_start, kv_len, k_scale, v_scale)
     KVH, D, B, kv = _page_args(k_pages, v_pages, page_table, q_start, kv_len, k_scale, v_scale)
