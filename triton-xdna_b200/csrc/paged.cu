@@ -160,9 +160,9 @@ __device__ __forceinline__ int sequences_of(const int32_t* q_start, int B, int t
 // 8-bit pages: the lanes of a slot (a power of two of them, side by side) find its
 // largest magnitude by shuffles and store 8 codes each per half.  What is
 // quantised is the bf16 number that a bf16 page would hold.  Instructions bound it
-// (920 a token, 0.72 issued a clock), so that many tokens go to half a warp each,
-// which shares those of the search, the page and the tables: 36500 tokens 42.3 ->
-// 37.6 us (e4m3), 42.9 -> 38.1 (int8).  Few ones have a warp each (64 tokens 7.8
+// (920 a token with a warp each, 0.72 issued a clock), so that many tokens go to half a
+// warp each, which shares those of the search, the page and the tables (680, 0.63):
+// 36500 tokens 42.3 -> 37.6 us (e4m3), 42.9 -> 38.1 (int8).  Few ones have a warp each (64 tokens 7.8
 // against 9.0 with reading back).  Before that, rounding by an addition instead of
 // conversions 47.9 -> 42.9 (int8); 10 or 14 CTAs an SM instead of 12 39.0 / 39.5.
 template <Format F>
@@ -589,7 +589,7 @@ constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared m
 // 72.3 / 25.0, 8 x 64 x 3 67.3 / 24.7, 12 x 96 x 1 57.6 / 23.8, 12 x 128 x 1 59.4 / 24.1,
 // 6 x 128 x 2 72.5 / 27.0.  What bounds them: the loads alone take 50.1 / 15.6 us (48.5 /
 // 14.6 without the exponents), so the long ones stand at 1.15 of their loads; a tile of
-// 64 keys is some 850 instructions, 3 warps a scheduler, a chain of products, maxima,
+// 64 keys is some 950 instructions, 3 warps a scheduler, a chain of products, maxima,
 // exponentials and products again, and with one query row of 8 in use (the beams) it
 // is the longer part.
 template <int ROWS, Format F, bool SHORT>
