@@ -76,6 +76,26 @@ def test_where_the_two_tile_sizes_meet(H, KVH, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,H,KVH", [([1] * 11, 14, 2), ([1] * 12, 14, 2), ([1] * 74, 14, 2), ([1] * 75, 14, 2),
+                                       ([2, 0, 5, 1], 14, 2), ([1, 3, 2], 12, 12), ([16, 1, 9], 4, 4), ([1] * 148, 8, 1),
+                                       ([1], 16, 1)])
+def test_where_units_have_a_cta_each(new, H, KVH, dtype):
+    """Tables of 640 and 768 positions, and of one page more; lengths from none to all of them."""
+    g = torch.Generator().manual_seed(90)
+    for positions in (640, 656, 768, 784):
+        lens = [int(x) for x in torch.randint(0, positions, (len(new),), generator=g)]
+        lens[-1] = positions  # all of it
+        lens[0] = 1
+        b = Coded(dtype, new, [x - n for x, n in zip(lens, new)], H, KVH, 16, seed=91, pad=2)
+        table = torch.full((len(new), positions // 16), -1, dtype=torch.int32, device="cuda")
+        table[:, :b.table.shape[1]] = b.table_dev
+        b.table_dev = table
+        out = b.attend()
+        b.check(out)
+        assert bool((out[-2:] == 7).all()) and torch.equal(out, b.attend())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_many_sequences_without_a_key(dtype):
     b = Coded(dtype, [70] + [1] * 600 + [9] + [1] * 600, [100] + [-1] * 600 + [300] + [-1] * 600, 32, 1, 16, seed=63)
     out = b.attend()

@@ -551,6 +551,49 @@ __device__ __forceinline__ I find_pieces(const AttnArgs& a, int pieces, int firs
   return share;
 }
 
+// Unit number `unit` of the batch (its key tiles aside) into *g; b < 0: there are
+// fewer.  Every thread of the block calls this; sums and *g are shared.
+template <int THREADS>
+__device__ __forceinline__ void find_unit(const AttnArgs& a, int unit, int (*sums)[THREADS / 32], Segment* g) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) g->b = -1;
+  int run = 0;
+  for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+    const int b = b0 + threadIdx.x;
+    Seq<int> q;
+    q.nt = 0;
+    if (b < a.B) q = load_seq<int>(a, b);
+    const int c = q.nt * a.KVH;
+    int s = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += v;
+    }
+    const int buf = (b0 / THREADS) & 1;
+    if (lane == 31) sums[buf][warp] = s;
+    __syncthreads();
+    int start = run + s - c;  // this sequence's first unit
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) {
+      const int v = sums[buf][i];
+      if (i < warp) start += v;
+      run += v;
+    }
+    const int in = unit - start;
+    if (in >= 0 && in < c) {
+      const int kvh = in / q.nt, done = (in - kvh * q.nt) * a.tpt, tokens = min(a.tpt, q.n - done);
+      g->b = b;
+      g->kvh = kvh;
+      g->token = q.s0 + done;
+      g->rows = tokens * a.n_rep;
+      g->first_pos = q.base + done;
+      g->keys = max(q.base + done + tokens, 0);
+    }
+  }
+  __syncthreads();
+}
+
 // ----------------------------------------------------------------------------- attention: few rows (mma.sync)
 //
 // For batches whose sequences bring few tokens each (decoding, verification of
@@ -592,6 +635,13 @@ constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared m
 // 64 keys is some 950 instructions, 3 warps a scheduler, a chain of products, maxima,
 // exponentials and products again, and with one query row of 8 in use (the beams) it
 // is the longer part.
+// WHOLE (of SHORT): a unit a CTA, its keys divided among the warps by their number, and
+// no joining kernel.  The line's even cuts leave less to each warp but cost that launch:
+// units x positions, cut / whole: 2 x 60 6.9 / 5.4, 2 x 500 8.9 / 8.5, 2 x 740 8.8 / 10.0, 24 x
+// 250 9.5 / 7.1, 24 x 740 10.5 / 10.5, 64 x 1000 11.4 / 12.2, 128 x 60 10.1 / 6.2, 128 x
+// 500 11.5 / 9.2, 128 x 740 13.9 / 10.7.  So where an SM has at most one unit and a unit
+// at most 768 positions (kWholeKeys), 640 where the units are fewer than 24.
+constexpr int kWholeKeys = 768, kWholeKeysFew = 640, kWholeUnits = 24;
 template <int ROWS, Format F, bool SHORT>
 struct FewCfg {
   static constexpr bool kLong = F != kBf16 && !SHORT;
@@ -700,7 +750,7 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int token, int kvh
   *reinterpret_cast<uint2*>(op) = pk;
 }
 
-template <int ROWS, typename I, Format F, bool SHORT>
+template <int ROWS, typename I, Format F, bool SHORT, bool WHOLE>
 __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT>::kThreads, 1)
     paged_attn_few_kernel(const __grid_constant__ KvMaps maps, const AttnArgs a) {
   using C = FewCfg<ROWS, F, SHORT>;
@@ -741,15 +791,31 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT>::kThreads, 1)
   }
   pdl_wait();
   pdl_trigger();
-  I total;
-  const I share =
-      find_pieces<C::kThreads, kWarps, I>(a, gridDim.x * kWarps, blockIdx.x * kWarps, sums, found, &total);
+  I total = 0, share = 0;
   Meta* meta = reinterpret_cast<Meta*>(a.ws + 2 * (int64_t)gridDim.x * part_floats(kFewRows));
-  if (found[0].b < 0) {  // no warp of this CTA has work
-    if (threadIdx.x == 0) meta[blockIdx.x].last = -1;
-    return;
+  Segment own;  // WHOLE: this warp's part
+  bool busy;
+  if constexpr (WHOLE) {
+    find_unit<C::kThreads>(a, blockIdx.x, sums, &queue[0][0]);
+    own = queue[0][0];
+    __syncthreads();  // the queue is read
+    if (own.b < 0) return;
+    const int nk = (own.keys + TK - 1) / TK, parts = max(min(nk, kWarps), 1);
+    own.t0 = warp * nk / parts;
+    own.t1 = (warp + 1) * nk / parts;
+    own.starts = warp == 0;
+    own.ends = warp == parts - 1;
+    own.last = 0;
+    busy = warp < parts;
+  } else {
+    share = find_pieces<C::kThreads, kWarps, I>(a, gridDim.x * kWarps, blockIdx.x * kWarps, sums, found, &total);
+    if (found[0].b < 0) {  // no warp of this CTA has work
+      if (threadIdx.x == 0) meta[blockIdx.x].last = -1;
+      return;
+    }
+    busy = found[warp].b >= 0;
   }
-  if (found[warp].b >= 0) {
+  if (busy) {
     const bool leader = elect_one();
     // This thread's rows: 8 n + 2 t and the next one, and the tokens they belong to
     int tok[NT][2];
@@ -761,7 +827,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT>::kThreads, 1)
     // queue of segments.
     Walk<I> wi;
     Segment si, sc;
-    place(a, wi, (int)blockIdx.x * kWarps + warp, share, total, found[warp]);
+    if constexpr (!WHOLE) place(a, wi, (int)blockIdx.x * kWarps + warp, share, total, found[warp]);
     bool fresh = true, more_i = true;
     si.t1 = 0;
     sc.t1 = 0;
@@ -882,7 +948,12 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT>::kThreads, 1)
           request();
         } else {
           if (pushed - popped == kQueue) break;
-          more_i = (fresh || next_unit(a, wi)) && segment<TK>(a, wi, si);
+          if constexpr (WHOLE) {
+            more_i = fresh;
+            si = own;
+          } else {
+            more_i = (fresh || next_unit(a, wi)) && segment<TK>(a, wi, si);
+          }
           fresh = false;
           if (!more_i) break;
           if (lane == 0) queue[warp][pushed % kQueue] = si;
@@ -1251,7 +1322,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT>::kThreads, 1)
       }
     }
   }
-  if (!open_unit && threadIdx.x == 0) meta[blockIdx.x].last = -1;
+  if (!WHOLE && !open_unit && threadIdx.x == 0) meta[blockIdx.x].last = -1;
 }
 
 // ----------------------------------------------------------------------------- attention: many rows (tcgen05)
@@ -2094,10 +2165,10 @@ cudaError_t launch_main(void (*kernel)(M, AttnArgs), int ctas, int threads, int 
   return e != cudaSuccess ? e : launch_k(kernel, (unsigned)ctas, threads, smem, s, maps, a);
 }
 
-template <int ROWS, typename I, Format F, bool SHORT>
+template <int ROWS, typename I, Format F, bool SHORT, bool WHOLE = false>
 cudaError_t launch_few(int ctas, cudaStream_t s, const KvMaps& maps, const AttnArgs& a) {
   using C = FewCfg<ROWS, F, SHORT>;
-  return launch_main(paged_attn_few_kernel<ROWS, I, F, SHORT>, ctas, C::kThreads, C::kSmem, s, maps, a);
+  return launch_main(paged_attn_few_kernel<ROWS, I, F, SHORT, WHOLE>, ctas, C::kThreads, C::kSmem, s, maps, a);
 }
 template <Format F>
 cudaError_t launch_few(bool eight, bool wide, int ctas, cudaStream_t s, const KvMaps& maps, const AttnArgs& a) {
@@ -2106,9 +2177,13 @@ cudaError_t launch_few(bool eight, bool wide, int ctas, cudaStream_t s, const Kv
                : (wide ? launch_few<16, int64_t, F, false>(ctas, s, maps, a)
                        : launch_few<16, int, F, false>(ctas, s, maps, a));
 }
+// units: 0, or of WHOLE
 template <Format F>
-cudaError_t launch_few8(bool eight, bool wide, bool brief, int ctas, cudaStream_t s, const KvMaps& maps,
+cudaError_t launch_few8(bool eight, bool wide, bool brief, int units, int ctas, cudaStream_t s, const KvMaps& maps,
                         const AttnArgs& a) {
+  if (units > 0)
+    return eight ? launch_few<8, int, F, true, true>(units, s, maps, a)
+                 : launch_few<16, int, F, true, true>(units, s, maps, a);
   if (brief)
     return eight ? launch_few<8, int, F, true>(ctas, s, maps, a) : launch_few<16, int, F, true>(ctas, s, maps, a);
   return launch_few<F>(eight, wide, ctas, s, maps, a);
@@ -2482,7 +2557,10 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
   line_kernel(a, rows);
   const bool brief = q8 && (double)batch * n_kv_head * kv->max_pages * page_size <= 96.0 * kFewWarps * sms &&
                      !line_is_wide(a, ctas);
-  const int tile = !few ? kTcTK : q8 && !brief ? kFewTK8 : kFewTK;
+  // Every unit has a token of its own (where starts ascend), so that there are at most so many; see WHOLE.
+  const int64_t most = n_kv_head * tokens, positions = kv->max_pages * page_size;
+  const int units = few && q8 && most <= sms && positions <= (most < kWholeUnits ? kWholeKeysFew : kWholeKeys) ? (int)most : 0;
+  const int tile = !few ? kTcTK : q8 && !brief && units == 0 ? kFewTK8 : kFewTK;
   if (few) line_kernel(a, rows, tile);
   const bool wide = line_is_wide(a, ctas);
   a.ke = q8 ? Exponents{q8->k_scale, q8->ks_page, q8->ks_head} : Exponents{};
@@ -2512,9 +2590,9 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
     pages.k = maps.k;
     pages.v = maps.v;
     e = !q8 ? launch_few<kBf16>(eight, wide, ctas, s, pages, a)
-            : q8->dtype == XB_DT_I8 ? launch_few8<kInt8>(eight, wide, brief, ctas, s, pages, a)
-                                    : launch_few8<kE4m3>(eight, wide, brief, ctas, s, pages, a);
-    if (e == cudaSuccess)
+            : q8->dtype == XB_DT_I8 ? launch_few8<kInt8>(eight, wide, brief, units, ctas, s, pages, a)
+                                    : launch_few8<kE4m3>(eight, wide, brief, units, ctas, s, pages, a);
+    if (e == cudaSuccess && units == 0)
       e = launch_k(paged_attn_join_kernel<kFewRows, 4>, dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
   } else {
     e = wide ? launch_main(paged_attn_tc_kernel<int64_t>, ctas, kTcThreads, kTcSmem, s, maps, a)
