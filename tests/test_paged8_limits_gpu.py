@@ -80,9 +80,9 @@ def test_where_the_two_tile_sizes_meet(H, KVH, dtype):
                                        ([2, 0, 5, 1], 14, 2), ([1, 3, 2], 12, 12), ([16, 1, 9], 4, 4), ([1] * 148, 8, 1),
                                        ([1], 16, 1)])
 def test_where_units_have_a_cta_each(new, H, KVH, dtype):
-    """Tables of 640 and 768 positions, and of one page more; lengths from none to all of them."""
+    """Tables of two and three tiles a warp (8 or 12 of them), and of one page more; lengths from none to all of them."""
     g = torch.Generator().manual_seed(90)
-    for positions in (640, 656, 768, 784):
+    for positions in (512, 528, 768, 784, 1152, 1168):
         lens = [int(x) for x in torch.randint(0, positions, (len(new),), generator=g)]
         lens[-1] = positions  # all of it
         lens[0] = 1

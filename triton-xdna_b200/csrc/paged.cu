@@ -635,17 +635,21 @@ constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared m
 // 64 keys is some 950 instructions, 3 warps a scheduler, a chain of products, maxima,
 // exponentials and products again, and with one query row of 8 in use (the beams) it
 // is the longer part.
-// WHOLE (of SHORT): a unit a CTA, its keys divided among the warps by their number, and
-// no joining kernel.  The line's even cuts leave less to each warp but cost that launch:
-// units x positions, cut / whole: 2 x 60 6.9 / 5.4, 2 x 500 8.9 / 8.5, 2 x 740 8.8 / 10.0, 24 x
-// 250 9.5 / 7.1, 24 x 740 10.5 / 10.5, 64 x 1000 11.4 / 12.2, 128 x 60 10.1 / 6.2, 128 x
-// 500 11.5 / 9.2, 128 x 740 13.9 / 10.7.  So where an SM has at most one unit and a unit
-// at most 768 positions (kWholeKeys), 640 where the units are fewer than 24.
-constexpr int kWholeKeys = 768, kWholeKeysFew = 640, kWholeUnits = 24;
-template <int ROWS, Format F, bool SHORT>
+// WHOLE (of SHORT): a unit a CTA of 12 warps (16 rows: 8), its keys divided among them
+// by their number, and no joining kernel.  The line's even cuts leave less to each warp
+// but cost that launch.  Units x positions, cut / whole: 2 x 60 6.8 / 4.8, 2 x 500 8.8 /
+// 6.7, 2 x 740 8.7 / 7.3, 2 x 1000 8.7 / 9.1, 24 x 250 9.4 / 5.7, 24 x 1000 10.4 / 9.5, 24 x
+// 1250 10.7 / 11.3, 64 x 1000 11.3 / 9.6, 64 x 2000 14.3 / 15.6, 128 x 60 10.0 / 5.3, 128
+// x 500 11.4 / 7.4, 128 x 1000 14.0 / 9.8, 128 x 2000 19.1 / 16.6; 8 warps 7.1 at 128 x
+// 500, 10.6 at 128 x 1000, 14 warps 7.9 and 9.9.  So where an SM has at most one unit and a
+// warp at most three tiles of 32 keys by what the table can hold, two where there are fewer
+// than 24 units (the host knows no lengths: beyond that one long sequence among
+// short ones would set the time).
+constexpr int kWholeUnits = 24;
+template <int ROWS, Format F, bool SHORT, bool WHOLE>
 struct FewCfg {
   static constexpr bool kLong = F != kBf16 && !SHORT;
-  static constexpr int kWarps = kLong && ROWS == 8 ? 12 : kFewWarps, kBufs = 2;
+  static constexpr int kWarps = (kLong || WHOLE) && ROWS == 8 ? 12 : kFewWarps, kBufs = 2;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kTile = kLong ? kFewTK8 : kTK;  // keys
   static constexpr int kRowBytes = F == kBf16 ? kHD * 2 : kHD;
@@ -751,9 +755,9 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int token, int kvh
 }
 
 template <int ROWS, typename I, Format F, bool SHORT, bool WHOLE>
-__global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT>::kThreads, 1)
+__global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
     paged_attn_few_kernel(const __grid_constant__ KvMaps maps, const AttnArgs a) {
-  using C = FewCfg<ROWS, F, SHORT>;
+  using C = FewCfg<ROWS, F, SHORT, WHOLE>;
   constexpr bool kCoded = F != kBf16;
   constexpr int kWarps = C::kWarps, kBufs = C::kBufs, TK = C::kTile, MT = kTK / 16;
   extern __shared__ uint8_t smem_raw[];
@@ -2167,7 +2171,7 @@ cudaError_t launch_main(void (*kernel)(M, AttnArgs), int ctas, int threads, int 
 
 template <int ROWS, typename I, Format F, bool SHORT, bool WHOLE = false>
 cudaError_t launch_few(int ctas, cudaStream_t s, const KvMaps& maps, const AttnArgs& a) {
-  using C = FewCfg<ROWS, F, SHORT>;
+  using C = FewCfg<ROWS, F, SHORT, WHOLE>;
   return launch_main(paged_attn_few_kernel<ROWS, I, F, SHORT, WHOLE>, ctas, C::kThreads, C::kSmem, s, maps, a);
 }
 template <Format F>
@@ -2559,7 +2563,12 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
                      !line_is_wide(a, ctas);
   // Every unit has a token of its own (where starts ascend), so that there are at most so many; see WHOLE.
   const int64_t most = n_kv_head * tokens, positions = kv->max_pages * page_size;
-  const int units = few && q8 && most <= sms && positions <= (most < kWholeUnits ? kWholeKeysFew : kWholeKeys) ? (int)most : 0;
+  const int units = few && q8 && most <= sms &&
+                            positions <= (eight ? FewCfg<8, kInt8, true, true>::kWarps
+                                                : FewCfg<16, kInt8, true, true>::kWarps) *
+                                             kFewTK * (most < kWholeUnits ? 2 : 3)
+                        ? (int)most
+                        : 0;
   const int tile = !few ? kTcTK : q8 && !brief && units == 0 ? kFewTK8 : kFewTK;
   if (few) line_kernel(a, rows, tile);
   const bool wide = line_is_wide(a, ctas);
