@@ -138,11 +138,11 @@ struct Ring {  // a warp's groups of tokens on their way from memory
 // stream took 44 instructions a token, mostly to find that there is none (94 us where
 // this takes 43).
 //
-// What bounds it: 256 rows of 151936 fp32 logits, 156 MB, take 43.2 us with the choice,
-// 3.6 TB/s.  The stream alone takes some 32: 14 instructions a token over all, memory
+// What bounds it: 256 rows of 151936 fp32 logits, 156 MB, take 41.4 us with the choice,
+// 3.8 TB/s.  The stream alone takes some 32: 14 instructions a token over all, memory
 // at 4.9 TB/s, and 512 CTAs for 592 places (busy 75 % of the time); behind it comes
 // what no CTA has other work for, the look through the runs and the lists (5), and the
-// choice (5).  240 rows of 50257 in bf16 take 18.8 us, 4 of 151936 8.8: start, one group a
+// choice (4).  240 rows of 50257 in bf16 take 16.5 us, 4 of 151936 8.5: start, one group a
 // warp, the bound, the lists and the second launch.  Measured (us of these three):
 // CTAs of 128 threads 48.9 / 19.0 / 11.8 where 256 took 44.8 / 19.5 / 9.5; rows divided
 // for 4, 6, 7, 8, 12 CTAs an SM 43.7 / 46.6 / 42.1 / 42.2 / 45.1 and 19.1 / 20.4 / 19.2 /
@@ -356,10 +356,11 @@ struct Candidate {
   int beam;
 };
 // Sums that 64 bits do not tell apart go by the beam, those of one beam by their
-// logits, as the lists do.
+// logits, as the lists do.  Without branches: bf16 logits are equal often (48 x 5 beams
+// 18.6 us with them, 17.5 without).
 __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
-  if (a.total != b.total) return a.total > b.total;
-  return a.beam != b.beam ? a.beam < b.beam : a.key > b.key;
+  return (a.total > b.total) |
+         ((a.total == b.total) & ((a.beam < b.beam) | ((a.beam == b.beam) & (a.key > b.key))));
 }
 
 // 2^n, n <= 0, in 64 bits
@@ -405,13 +406,16 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
   const int total_lists = beams * parts;
   lists += g * total_lists * count;
   stats += g * total_lists;
-  // every entry of every list, a thread has every 256th: the first ones ahead of what they wait for
+  // every entry of every list, a thread has every 256th: the first ones ahead of what they wait for.  Where threads have
+  // one or none, every warp gets its part of them, which brings the bound close (48 x 5 beams 17.5 -> 16.5 us; of many
+  // entries it would scatter the loads: 1 x 4 8.5 -> 9.9).
   const int entries = total_lists * count;
   constexpr int kAhead = 8;
+  const int own = entries <= kPick ? lane * (kPick / 32) + warp : (int)threadIdx.x;
   uint64_t ahead[kAhead];
 #pragma unroll
   for (int j = 0; j < kAhead; ++j) {
-    const int f = j * kPick + threadIdx.x;
+    const int f = j * kPick + own;
     ahead[j] = f < entries ? lists[f] : 0;
   }
   if (threadIdx.x == 0) n = 0;
@@ -462,7 +466,7 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
 #pragma unroll
   for (int j = 0; j < kAhead; ++j) {
     if (j * kPick >= entries) break;
-    sums[j] = candidate(min(j * kPick + (int)threadIdx.x, entries - 1), ahead[j]).total;
+    sums[j] = candidate(min(j * kPick + own, entries - 1), ahead[j]).total;
     best = fmaxf(best, (float)sums[j]);
   }
 #pragma unroll 1
@@ -477,7 +481,7 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restric
 #pragma unroll
   for (int j = 0; j < kAhead; ++j) {
     if (j * kPick >= entries) break;
-    take(sums[j], j * kPick + threadIdx.x, ahead[j]);
+    take(sums[j], j * kPick + own, ahead[j]);
   }
 #pragma unroll 1
   for (int f = kAhead * kPick + threadIdx.x; f < entries; f += kPick) {
