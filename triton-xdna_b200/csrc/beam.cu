@@ -388,7 +388,8 @@ __device__ __noinline__ double far_log_sum(const Stats* stats, int parts, float 
 // Latency bounds it, most of all that of fetching instructions, which are cold in
 // every launch (3.4 of the 12 clocks between a warp's instructions): sums are formed
 // once, and what is rare stays out of line, which took 1 us off every call (1 x 4 beams
-// 9.8 -> 8.8).
+// 9.8 -> 8.8).  Of what it adds to a call (4 us) loads and log-sums take 1.3, the bound
+// 0.6.
 __global__ void __launch_bounds__(kPick) beam_pick_kernel(const float* __restrict__ scores, int64_t ld_scores,
                                                           const uint64_t* __restrict__ lists,
                                                           const Stats* __restrict__ stats, int beams, int parts,

@@ -2,7 +2,8 @@
 // bound by the host: of the 18 us between two calls of paged_attention from Python
 // the GPU worked 8, the two launches took 6, and looking at ten tensors through
 // the interpreter (shape, strides, type, address: some 50 attribute reads) with
-// ctypes' conversions the rest.  Here a call costs little more than its launches.
+// ctypes' conversions the rest.  Here a call costs little more than its launches: with
+// the same kernels 8.6 us (write and reading back 23.8 -> 8.4, select 21.4 -> 9.5).
 //
 // Each function takes a call if everything about it is as xb200/ops.py asks, makes
 // it through the same C entry point and says so; anything else (another type, a
