@@ -895,7 +895,9 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
       ++ni;
     };
     uint32_t qb[NT][4][2];
-    float cq[NT][2];  // 8-bit pages: what turns a row's products into scores, in log2 units
+    float cq[NT][2];  // 8-bit pages: what turns a row's products (below 2^30) into scores, in log2 units
+    constexpr float kHuge = 0x1p97f;
+    bool huge = false;  // some row's is that or more
     auto load_q = [&]() {
       if constexpr (kCoded) {
         // A dim's place in the product is K's: four in a row a lane, even and odd ones apart.  As fp16, scaled by a power
@@ -925,6 +927,10 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e) cq[n][e] = a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
         }
+        huge = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) huge |= fmaxf(cq[n][0], cq[n][1]) >= kHuge;
+        huge = __any_sync(0xffffffffu, huge);
       } else {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -1034,7 +1040,8 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
                 for (int n = 0; n < NT; ++n) mma_16816(s[n][mt], ka, qb[n][kk][0], qb[n][kk][1]);
               }
           }
-          // 8-bit pages: with K's exponent e_k and V's e_v a score is S c 2^e_k (c = cq), and e_v joins it: the weight
+          // 8-bit pages: with K's exponent e_k and V's e_v a score is (S c) 2^e_k (c = cq): c 2^e_k may pass fp32 where S is
+          // zero, S c only where the query is huge.  e_v joins the score: the weight
           // 2^(score + e_v - m) of a code of V is at most one and fits fp16 whatever the values' sizes; times 2^-e_v
           // it is the key's share of the denominator.
           float fv[kCoded ? MT : 1][2];  // 2^-e_v
@@ -1057,7 +1064,11 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                  for (int e = 0; e < 2; ++e) s[n][mt][2 * h + e] = fmaf(s[n][mt][2 * h + e], kf * cq[n][e], ev);
+                  for (int e = 0; e < 2; ++e) {
+                    float& x = s[n][mt][2 * h + e];
+                    if (!huge || cq[n][e] < kHuge) x = fmaf(x * cq[n][e], kf, ev);
+                    else x = fmaf(x, kf == INFINITY ? kf : fminf(kf * cq[n][e], 3.402823466e38f), ev);
+                  }
               }
           }
           const bool edge = k0 + kTK - 1 > first_pos;
