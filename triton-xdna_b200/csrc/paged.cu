@@ -697,6 +697,33 @@ __device__ __forceinline__ uint32_t pack2_half(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// Two fp32 at a time: one instruction for a pair, each rounded as on its own.
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n"
+      " mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return d;
+}
+
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n"
+      " mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return d;
+}
+
 // 8 bytes into shared memory, without a wait
 __device__ __forceinline__ void copy8_async(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
@@ -710,9 +737,26 @@ __device__ __forceinline__ uint32_t lds_u32(uint32_t addr) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-// What a sum of weights divides by: nothing seen gives zeros; a negative sum comes of a NaN among 8-bit values
+// 8-bit pages: weights of codes are held times 2^kUp (what fp16 holds most of), shares of the denominator times
+// 2^kShareUp.  With values' exponents of -80 .. 121 a share is up to 2^(kShareUp + 81), so that a CTA's sum is far inside
+// fp32, and the largest of a row at least 2^(kShareUp - 121), so that what is lost below 2^-126 is 2^-25 of it.
+constexpr float kUp = 14.0f, kShareUp = 20.0f;
+// What a sum of weights is multiplied by; nothing seen gives zeros
+template <bool CODED>
 __device__ __forceinline__ float inverse_of(float l) {
-  return l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : __int_as_float(0x7fc00000);
+  return l == 0.0f ? 0.0f : (CODED ? 64.0f : 1.0f) / l;  // 2^(kShareUp - kUp)
+}
+// l 2^by, for a base that is higher by -by.  8-bit pages: by halves, since exponents of values, which a base has in it
+// and a share has not, lie more than 126 apart.
+__device__ __forceinline__ float rebased(float l, float by) {
+  const float half = ex2_approx(0.5f * by);
+  return l * half * half;
+}
+// l 2^by + l1 2^by1, f = 2^by and f1 = 2^by1
+template <bool CODED>
+__device__ __forceinline__ float joined(float l, float by, float f, float l1, float by1, float f1) {
+  if constexpr (CODED) return rebased(l, by) + rebased(l1, by1);
+  else return l * f + l1 * f1;
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -895,9 +939,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
       ++ni;
     };
     uint32_t qb[NT][4][2];
-    float cq[NT][2];  // 8-bit pages: what turns a row's products (below 2^30) into scores, in log2 units
-    constexpr float kHuge = 0x1p97f;
-    bool huge = false;  // some row's is that or more
+    float2 c1[NT], c2[NT];  // 8-bit pages: what turns a row's products into scores, in log2 units
     auto load_q = [&]() {
       if constexpr (kCoded) {
         // A dim's place in the product is K's: four in a row a lane, even and odd ones apart.  As fp16, scaled by a power
@@ -924,13 +966,16 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
             qb[n][c][1] = pack2_half(__uint_as_float(x[c].x & 0xffff0000u) * mul,
                                      __uint_as_float(x[c].y & 0xffff0000u) * mul);
           }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) cq[n][e] = a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
+          // In two parts where it is large, so that neither times the products (below 2^30) nor times 2^e_k (up to 2^121) it
+          // passes fp32 where a score does not: one meets the products, the other, 1 for all but queries of some 2^112
+          // on, 2^e_k.  (From 2^118 on, where one key has all the weight, they stay at 2^103.)
+          auto split = [&](float c, float& p1, float& p2) {
+            p1 = fminf(c, 0x1p97f);
+            p2 = fminf(fmaxf(c * 0x1p-97f, 1.0f), 64.0f);
+          };
+          split(a.scale_log2 * __shfl_sync(0xffffffffu, back, 2 * t * 4), c1[n].x, c2[n].x);
+          split(a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + 1) * 4), c1[n].y, c2[n].y);
         }
-        huge = false;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) huge |= fmaxf(cq[n][0], cq[n][1]) >= kHuge;
-        huge = __any_sync(0xffffffffu, huge);
       } else {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -1040,54 +1085,49 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
                 for (int n = 0; n < NT; ++n) mma_16816(s[n][mt], ka, qb[n][kk][0], qb[n][kk][1]);
               }
           }
-          // 8-bit pages: with K's exponent e_k and V's e_v a score is (S c) 2^e_k (c = cq): c 2^e_k may pass fp32 where S is
-          // zero, S c only where the query is huge.  e_v joins the score: the weight
-          // 2^(score + e_v - m) of a code of V is at most one and fits fp16 whatever the values' sizes; times 2^-e_v
-          // it is the key's share of the denominator.
-          float fv[kCoded ? MT : 1][2];  // 2^-e_v
+          // 8-bit pages: with K's exponent e_k and V's e_v a score is (S c1) (2^e_k c2), and e_v joins it: the weight w =
+          // 2^(score + e_v - m) of a code of V fits fp16 whatever the values' sizes.  The key's share of the denominator, w
+          // 2^-e_v, is an exponential of its own: w vanishes below 2^-126, and exponents lie up to 201 apart (a vector of
+          // zeros has 2^-80).
+          float ev[kCoded ? MT : 1][2];
+          uint32_t nan = 0;
           if constexpr (kCoded) {
             // the bytes of this thread's keys, one of each group: the XOR of their order undone by a byte move
             const uint32_t at = smem_u32(&exps[warp][buf][0][part0 + 4 * g]), pick = 0x3210u ^ (uint32_t)(g >> 1) * 0x1111u;
             const uint32_t wk = __byte_perm(lds_u32(at), 0, pick), wv = __byte_perm(lds_u32(at + TK), 0, pick);
+            // bytes of 255: one more than the last seven bits reaches the eighth only where all are set
+            nan = ((wv & 0x7f7f7f7fu) + 0x01010101u) & wv & 0x80808080u;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const int j = 2 * mt + h, by = 8 * j;
-                auto exponent = [&](uint32_t w) { return (by == 24 ? w >> 1 : w << (23 - by)) & 0x7f800000u; };
                 // byte 255: an infinite factor, and the codes are zeros: NaN
-                const float kf = __uint_as_float(exponent(wk));
-                // the byte as a float: below 2^23's bits
-                const float ev = __uint_as_float(__byte_perm(wv, 0x4b000000u, 0x7650u | j)) - (8388608.0f + 127.0f);
-                // byte 255: -infinity, which turns the sum negative or NaN
-                fv[mt][h] = __uint_as_float(0x7f000000u - exponent(wv));
+                const float kf = __uint_as_float((by == 24 ? wk >> 1 : wk << (23 - by)) & 0x7f800000u);
+                // e_v - 6, from the byte as a float (below 2^23's bits): what all have less goes into the base
+                ev[mt][h] = __uint_as_float(__byte_perm(wv, 0x4b000000u, 0x7650u | j)) -
+                            (8388608.0f + 127.0f + (kShareUp - kUp));
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) {
-                    float& x = s[n][mt][2 * h + e];
-                    if (!huge || cq[n][e] < kHuge) x = fmaf(x * cq[n][e], kf, ev);
-                    else x = fmaf(x, kf == INFINITY ? kf : fminf(kf * cq[n][e], 3.402823466e38f), ev);
-                  }
+                for (int n = 0; n < NT; ++n) {
+                  const float2 x = fma2(mul2(make_float2(s[n][mt][2 * h], s[n][mt][2 * h + 1]), c1[n]),
+                                        mul2(make_float2(kf, kf), c2[n]), make_float2(ev[mt][h], ev[mt][h]));
+                  s[n][mt][2 * h] = x.x, s[n][mt][2 * h + 1] = x.y;
+                }
               }
           }
           const bool edge = k0 + kTK - 1 > first_pos;
-          if (edge) {  // some row does not see the whole tile
+          if (edge || (kCoded && nan != 0)) {  // some row does not see the whole tile; or a value is NaN
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const int key = k0 + (kCoded ? row_of(2 * mt + h, g) : mt * 16 + g + h * 8);
-                // A value of NaN (2^-e_v is -infinity) goes by the scores here: a weight of zero times it would reach rows
-                // that do not see it.  What no row sees may have any exponent.
-                const bool nan = kCoded && fv[mt][h] == -INFINITY;
+                const int j = 2 * mt + h, key = k0 + (kCoded ? row_of(j, g) : mt * 16 + g + h * 8);
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                   for (int n = 0; n < NT; ++n)
                     if (key > pos[n][e]) s[n][mt][2 * h + e] = -INFINITY;
-                    else if (nan) s[n][mt][2 * h + e] = __int_as_float(0x7fc00000);
-                if (kCoded && (nan || key >= sc.keys)) fv[mt][h] = 0.0f;
+                    else if (kCoded && (nan >> (8 * j) & 0x80u)) s[n][mt][2 * h + e] = __int_as_float(0x7fc00000);
               }
           }
           uint32_t pb[NT][2 * MT];  // P as the B operand of O^T = V^T P^T, 8 keys each
@@ -1102,7 +1142,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
             }
             // Over 8-bit pages a row's base moves only where a score is above it by more than one: fp16 has the room, and
             // most tiles need no exchange between lanes.
-            float base[2], al[2] = {1.0f, 1.0f};
+            float base[2], by[2] = {0.0f, 0.0f}, al[2] = {1.0f, 1.0f};
             bool moved = !kCoded || __any_sync(0xffffffffu, mx[0] > m[n][0] + 1.0f || mx[1] > m[n][1] + 1.0f);
             if (moved) {
               moved = false;
@@ -1113,13 +1153,14 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
                 for (int o_ = 4; o_ <= 16; o_ <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o_));
                 const float mn = fmaxf(m[n][e], kCoded ? mx[e] : mx[e] * a.scale_log2);
                 base[e] = mn == -INFINITY ? 0.0f : mn;
-                al[e] = ex2_approx(m[n][e] - base[e]);
+                by[e] = m[n][e] - base[e];
+                al[e] = ex2_approx(by[e]);
                 moved |= mn > m[n][e];
                 m[n][e] = mn;
               }
               if (__any_sync(0xffffffffu, moved)) {
-                l[n][0] *= al[0];
-                l[n][1] *= al[1];
+                l[n][0] = kCoded ? rebased(l[n][0], by[0]) : l[n][0] * al[0];
+                l[n][1] = kCoded ? rebased(l[n][1], by[1]) : l[n][1] * al[1];
 #pragma unroll
                 for (int mt = 0; mt < 4; ++mt) {
                   o[n][mt][0] *= al[0];
@@ -1134,19 +1175,23 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
               for (int e = 0; e < 2; ++e) base[e] = m[n][e] == -INFINITY ? 0.0f : m[n][e];
             }
             if constexpr (kCoded) {
-              // up to 2^15, the largest at least 2^14, so that fp16 holds weights from 2^-38 of it on; numerator and
-              // denominator alike
-              const float up[2] = {base[0] - 14.0f, base[1] - 14.0f};
+              // up to 2^15, the largest at least 2^14, so that fp16 holds weights from 2^-38 of it on
+              const float2 down = make_float2(kUp - base[0], kUp - base[1]);
+              float2 sum = make_float2(l[n][0], l[n][1]);
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) {
+                uint32_t p[2];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  s[n][mt][e] = ex2_approx(s[n][mt][e] - up[e & 1]);
-                  l[n][e & 1] = fmaf(s[n][mt][e], fv[mt][e >> 1], l[n][e & 1]);
+                for (int h = 0; h < 2; ++h) {
+                  const float2 x = add2(make_float2(s[n][mt][2 * h], s[n][mt][2 * h + 1]), down);
+                  const float2 y = fma2(make_float2(ev[mt][h], ev[mt][h]), make_float2(-1.0f, -1.0f), x);
+                  p[h] = pack2_half(ex2_approx(x.x), ex2_approx(x.y));
+                  sum = add2(sum, make_float2(ex2_approx(y.x), ex2_approx(y.y)));
                 }
-                pb[n][2 * mt] = transpose8(pack2_half(s[n][mt][0], s[n][mt][1]));
-                pb[n][2 * mt + 1] = transpose8(pack2_half(s[n][mt][2], s[n][mt][3]));
+                pb[n][2 * mt] = transpose8(p[0]);
+                pb[n][2 * mt + 1] = transpose8(p[1]);
               }
+              l[n][0] = sum.x, l[n][1] = sum.y;
             } else {
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) {
@@ -1231,7 +1276,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float inv = inverse_of(l[n][e]);
+            const float inv = inverse_of<true>(l[n][e]);
             const int r = 8 * n + 2 * t + e, tk = tok[n][e];
             bf16* p = a.out + (int64_t)(sc.token + tk) * a.ld_out + (sc.kvh * a.n_rep + r - tk * a.n_rep) * kHD + 2 * g;
 #pragma unroll
@@ -1320,11 +1365,11 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
         acc.y = acc.y * f0 + v.y * f;
         acc.z = acc.z * f0 + v.z * f;
         acc.w = acc.w * f0 + v.w * f;
-        l = l * f0 + part_l[k == c][k][r] * f;
+        l = joined<kCoded>(l, M - base, f0, part_l[k == c][k][r], m - base, f);
         M = mn;
       }
       if (whole) {
-        const float inv = inverse_of(l);
+        const float inv = inverse_of<kCoded>(l);
         store_out4(a, p.token, p.kvh, r, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
       } else {
         float* out_part = a.ws + (2 * (int64_t)blockIdx.x + (c >= 0)) * part_floats(kFewRows);
@@ -1423,33 +1468,6 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-
-// Two fp32 at a time: one instruction for a pair, each rounded as on its own.
-__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
-  float2 d;
-  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
-      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 x, float2 y) {
-  float2 d;
-  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n"
-      " mov.b64 {%0, %1}, d;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
-  return d;
-}
-
-__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
-  float2 d;
-  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n"
-      " mov.b64 {%0, %1}, d;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
-  return d;
 }
 
 template <typename I>
@@ -1911,7 +1929,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_attn_tc_kernel(const __gr
 // the next ones: o = sum_c o_c 2^(m_c - M), l likewise.  A CTA takes 256 / (16
 // LANES) rows; LANES threads share a row's 16-byte column, each with every
 // LANES-th partial, and meet by shuffles in a fixed order.
-template <int ROWS, int LANES>
+template <int ROWS, int LANES, bool CODED>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, int ctas) {
   pdl_wait();
   pdl_trigger();
@@ -1921,6 +1939,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
   const int r = blockIdx.y * kRows + threadIdx.x / (16 * LANES), d = col * 4;
   if (m.last < 0 || (int)blockIdx.y * kRows >= m.rows) return;
   const int c0 = blockIdx.x, n = min(m.last, ctas - 1) - c0 + 1;
+  constexpr float kDown = CODED ? 0x1p-8f : 1.0f;  // room for the shares of 2^31 keys whose values are zeros
   float M = -INFINITY, l = 0.0f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = ln; i0 < n; i0 += 4 * LANES) {  // four partials in flight
@@ -1932,14 +1951,14 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
       const float* p = a.ws + (2 * (int64_t)(c0 + i) + (i == 0)) * part_floats(ROWS);
       const bool in = i < n;
       pm[u] = in ? p[ROWS * kHD + r] : -INFINITY;
-      pl[u] = in ? p[ROWS * kHD + ROWS + r] : 0.0f;
+      pl[u] = in ? p[ROWS * kHD + ROWS + r] * kDown : 0.0f;
       v[u] = in ? *reinterpret_cast<const float4*>(p + r * kHD + d) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     const float mn = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), M);
     const float base = mn == -INFINITY ? 0.0f : mn;
     const float f0 = ex2_approx(M - base);
     acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
-    l *= f0;
+    l = CODED ? rebased(l, M - base) : l * f0;
     M = mn;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -1948,7 +1967,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
       acc.y += v[u].y * f;
       acc.z += v[u].z * f;
       acc.w += v[u].w * f;
-      l += pl[u] * f;
+      l += CODED ? rebased(pl[u], pm[u] - base) : pl[u] * f;
     }
   }
 #pragma unroll
@@ -1960,11 +1979,11 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
     acc.y = acc.y * f + __shfl_xor_sync(0xffffffffu, acc.y, o) * fo;
     acc.z = acc.z * f + __shfl_xor_sync(0xffffffffu, acc.z, o) * fo;
     acc.w = acc.w * f + __shfl_xor_sync(0xffffffffu, acc.w, o) * fo;
-    l = l * f + __shfl_xor_sync(0xffffffffu, l, o) * fo;
+    l = joined<CODED>(l, M - base, f, __shfl_xor_sync(0xffffffffu, l, o), om - base, fo);
     M = mn;
   }
   if (ln == 0 && r < m.rows) {
-    const float inv = inverse_of(l);
+    const float inv = inverse_of<CODED>(l) * kDown;
     store_out4(a, m.token, m.kvh, r, d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   }
 }
@@ -2613,12 +2632,13 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
             : q8->dtype == XB_DT_I8 ? launch_few8<kInt8>(eight, wide, brief, units, ctas, s, pages, a)
                                     : launch_few8<kE4m3>(eight, wide, brief, units, ctas, s, pages, a);
     if (e == cudaSuccess && units == 0)
-      e = launch_k(paged_attn_join_kernel<kFewRows, 4>, dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
+      e = launch_k(q8 ? paged_attn_join_kernel<kFewRows, 4, true> : paged_attn_join_kernel<kFewRows, 4, false>,
+                   dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
   } else {
     e = wide ? launch_main(paged_attn_tc_kernel<int64_t>, ctas, kTcThreads, kTcSmem, s, maps, a)
              : launch_main(paged_attn_tc_kernel<int>, ctas, kTcThreads, kTcSmem, s, maps, a);
     if (e == cudaSuccess)
-      e = launch_k(paged_attn_join_kernel<kTcRows, 1>, dim3((unsigned)ctas, kTcRows / 16), 256, 0, s, a, ctas);
+      e = launch_k(paged_attn_join_kernel<kTcRows, 1, false>, dim3((unsigned)ctas, kTcRows / 16), 256, 0, s, a, ctas);
   }
   if (e != cudaSuccess) {
     set_err(err, errlen, "%s: %s", what, cudaGetErrorString(e));
