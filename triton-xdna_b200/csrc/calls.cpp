@@ -7,9 +7,11 @@
 //
 // Each function takes a call if everything about it is as xb200/ops.py asks, makes
 // it through the same C entry point and says so; anything else (another type, a
-// wrong shape, tensors of another device than the current one, an error) it
-// leaves alone, before anything is launched, to the function of the same name there,
-// which has the checks one by one and their messages.
+// wrong shape, tensors of another device than the current one, arguments that the
+// library refuses) it leaves alone, before anything is launched, to the function of
+// the same name there, which has the checks one by one and their messages.  An
+// error of CUDA's, which may come after a launch, is raised here: the call is not
+// made again.
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
@@ -36,6 +38,7 @@ struct Entries {
   decltype(&xb_beam_select_workspace_size) beam_size;
   decltype(&xb_beam_select) beam;
 } entry = {};
+PyObject* error_type = nullptr;  // xb200/_lib.py's XbError
 bool bound = false;
 
 PyObject* bind(PyObject*, PyObject* addresses) {
@@ -50,6 +53,13 @@ PyObject* bind(PyObject*, PyObject* addresses) {
     PyErr_SetString(PyExc_TypeError, "bind takes a dict");
     return nullptr;
   }
+  PyObject* type = PyDict_GetItemString(addresses, "error");
+  if (!type || !PyExceptionClass_Check(type)) {
+    PyErr_SetString(PyExc_RuntimeError, "no type of errors");
+    return nullptr;
+  }
+  Py_INCREF(type);
+  Py_XSETREF(error_type, type);
   bound = get(entry.attention_size, "xb_paged_attention_workspace_size") &&
           get(entry.attention, "xb_paged_attention_bf16") &&
           get(entry.attention8_size, "xb_paged_attention_q8_workspace_size") &&
@@ -158,8 +168,20 @@ bool apart(const void* p, int64_t ld_p, int64_t row_p, const void* q, int64_t ld
 }
 
 struct Error {
-  char text[256];
+  char text[256] = "";
 };
+
+// Whether an entry point's answer is that it made the call; false: it refused its arguments, and has launched nothing.
+// Anything else raises XbError.
+bool made(const char* name, int rc, const Error& err) {
+  if (rc == XB_OK) return true;
+  if (rc == XB_ERR_INVALID || rc == XB_ERR_UNSUPPORTED) return false;
+  if (PyObject* e = PyObject_CallFunction(error_type, "sis", name, rc, err.text)) {
+    PyErr_SetObject(error_type, e);
+    Py_DECREF(e);
+  }
+  throw python_error();
+}
 
 // paged_attention(q, k_pages, v_pages, out, page_table, q_start, kv_len, scale, k_scale, v_scale): whether it was done
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
@@ -181,22 +203,22 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
   const bool coded = kv.dtype != XB_DT_BF16;
   Error err;
   size_t need = 0;
-  if ((coded ? entry.attention8_size(T, kv.kv.batch, H, kv.kv.n_kv_head, kv.kv.n_pages, kv.kv.page_size,
-                                     kv.kv.max_pages, &need, err.text, sizeof(err.text))
-             : entry.attention_size(T, kv.kv.batch, H, kv.kv.n_kv_head, &need, err.text, sizeof(err.text))) != XB_OK)
+  int rc = coded ? entry.attention8_size(T, kv.kv.batch, H, kv.kv.n_kv_head, kv.kv.n_pages, kv.kv.page_size,
+                                         kv.kv.max_pages, &need, err.text, sizeof(err.text))
+                 : entry.attention_size(T, kv.kv.batch, H, kv.kv.n_kv_head, &need, err.text, sizeof(err.text));
+  if (!made(coded ? "xb_paged_attention_q8_workspace_size" : "xb_paged_attention_workspace_size", rc, err))
     Py_RETURN_FALSE;
   const float scale = (float)PyFloat_AS_DOUBLE(a[7]);
   // of this call alone: the caching allocator orders its reuse on the stream, and a captured graph keeps its own
   c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(need);
   void* stream = c10::cuda::getCurrentCUDAStream(arg.device).stream();
-  int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = coded ? entry.attention8(pq, po, &kv, T, H, ld_q, ld_out, scale, ws.get(), need, stream, err.text,
                                 sizeof(err.text))
              : entry.attention(pq, po, &kv.kv, T, H, ld_q, ld_out, scale, ws.get(), need, stream, err.text,
                                sizeof(err.text));
   Py_END_ALLOW_THREADS
-  return PyBool_FromLong(rc == XB_OK);
+  return PyBool_FromLong(made(coded ? "xb_paged_attention_q8" : "xb_paged_attention_bf16", rc, err));
   END_HANDLE_TH_ERRORS
 }
 
@@ -236,7 +258,7 @@ PyObject* paged_rope_kv(PyObject*, PyObject* const* a, Py_ssize_t count) {
            ? entry.rope_kv8(px, c, s, pq, &kv, T, H, rows, ld_qkv, ld_q, stream, err.text, sizeof(err.text))
            : entry.rope_kv(px, c, s, pq, &kv.kv, T, H, rows, ld_qkv, ld_q, stream, err.text, sizeof(err.text));
   Py_END_ALLOW_THREADS
-  return PyBool_FromLong(rc == XB_OK);
+  return PyBool_FromLong(made(kv.dtype != XB_DT_BF16 ? "xb_paged_rope_kv_q8" : "xb_paged_rope_kv_bf16", rc, err));
   END_HANDLE_TH_ERRORS
 }
 
@@ -261,7 +283,7 @@ PyObject* paged_read_kv(PyObject*, PyObject* const* a, Py_ssize_t count) {
   Py_BEGIN_ALLOW_THREADS
   rc = entry.read_kv(pk, pv, &kv, T, ld_k, ld_v, stream, err.text, sizeof(err.text));
   Py_END_ALLOW_THREADS
-  return PyBool_FromLong(rc == XB_OK);
+  return PyBool_FromLong(made("xb_paged_read_kv", rc, err));
   END_HANDLE_TH_ERRORS
 }
 
@@ -285,7 +307,8 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t given) {
   if ((logits.stride(1) != 1 && V > 1) || (scores.stride(1) != 1 && K > 1)) Py_RETURN_NONE;
   Error err;
   size_t need = 0;
-  if (entry.beam_size(G, K, V, count, &need, err.text, sizeof(err.text)) != XB_OK) Py_RETURN_NONE;
+  int rc = entry.beam_size(G, K, V, count, &need, err.text, sizeof(err.text));
+  if (!made("xb_beam_select_workspace_size", rc, err)) Py_RETURN_NONE;
   const at::TensorOptions on = at::TensorOptions().device(logits.device());
   at::Tensor values = at::empty({G, count}, on.dtype(at::kFloat));
   at::Tensor parents = at::empty({G, count}, on.dtype(at::kLong)), tokens = at::empty({G, count}, on.dtype(at::kLong));
@@ -297,17 +320,16 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t given) {
   int64_t* to_tokens = static_cast<int64_t*>(tokens.data_ptr());
   const int64_t ld = G * K > 1 ? logits.stride(0) : V, ld_scores = G > 1 ? scores.stride(0) : K;
   void* stream = c10::cuda::getCurrentCUDAStream(arg.device).stream();
-  int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = entry.beam(x, s, G, K, V, ld, ld_scores, count, type == at::kFloat ? XB_DT_F32 : XB_DT_BF16, to_values,
                   to_parents, to_tokens, ws.get(), need, stream, err.text, sizeof(err.text));
   Py_END_ALLOW_THREADS
-  if (rc != XB_OK) Py_RETURN_NONE;
+  if (!made("xb_beam_select", rc, err)) Py_RETURN_NONE;
   PyObject* out = PyTuple_New(3);
   if (!out) return nullptr;
-  at::Tensor* made[3] = {&values, &parents, &tokens};
+  at::Tensor* results[3] = {&values, &parents, &tokens};
   for (int i = 0; i < 3; ++i) {
-    PyObject* t = THPVariable_Wrap(std::move(*made[i]));
+    PyObject* t = THPVariable_Wrap(std::move(*results[i]));
     if (!t) {
       Py_DECREF(out);
       return nullptr;
@@ -323,7 +345,7 @@ PyCFunction function(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
 }
 
 PyMethodDef methods[] = {
-    {"bind", bind, METH_O, "Addresses of the library's entry points."},
+    {"bind", bind, METH_O, "Addresses of the library's entry points, and the type of its errors (error)."},
     {"paged_attention", function(paged_attention), METH_FASTCALL, "Whether it made the call."},
     {"paged_rope_kv", function(paged_rope_kv), METH_FASTCALL, "Whether it made the call."},
     {"paged_read_kv", function(paged_read_kv), METH_FASTCALL, "Whether it made the call."},

@@ -1039,10 +1039,11 @@ def _direct():
                                "`python -c 'import __graft_entry__ as g; g.build()'`")
         from . import _calls as direct
 
-        direct.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+        addresses = {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "xb_paged_attention_workspace_size", "xb_paged_attention_bf16", "xb_paged_attention_q8_workspace_size",
             "xb_paged_attention_q8", "xb_paged_rope_kv_bf16", "xb_paged_rope_kv_q8", "xb_paged_read_kv",
-            "xb_beam_select_workspace_size", "xb_beam_select")})
+            "xb_beam_select_workspace_size", "xb_beam_select")}
+        direct.bind({**addresses, "error": _lib.XbError})
         _calls = direct
     return _calls
 
