@@ -2542,11 +2542,26 @@ static int check_workspace(const void* workspace, size_t bytes, size_t need, con
   return XB_ERR_INVALID;
 }
 
+// paged_expand_kernel over the pages that `e` names.
+static cudaError_t launch_expand(const ExpandArgs& e, int dtype, cudaStream_t s) {
+  int sms = 148;
+  xb::sm_count(&sms);
+  // CTAs of 8 warps for each sequence: as many as its longest could use, 8 per SM over all of them
+  const int64_t most = ((int64_t)e.max_pages * e.page_size / 8 * e.KVH + 7) / 8;
+  const int64_t rows = e.B < 65535 ? e.B : 65535;
+  int64_t x = (8 * sms + rows - 1) / rows;
+  x = x < most ? x : most;
+  return launch_k<false>(dtype == XB_DT_I8 ? paged_expand_kernel<kInt8> : paged_expand_kernel<kE4m3>,
+                         dim3((unsigned)x, (unsigned)rows), 256, 0, s, e);
+}
+
 // xb_paged_attention_bf16 and, with `q8` (few rows), the attention over 8-bit pages;
-// `expanded`: over what paged_expand_kernel, launched just before, makes of them.
+// `expand`: over what that launch, made when nothing can be refused any more, makes of
+// pages of `expand_dtype`.
 static int attend(const char* what, const void* q, void* out, const xb_paged_kv* kv, const xb_paged_kv8* q8,
-                  bool expanded, int64_t tokens, int64_t n_head, int64_t ld_q, int64_t ld_out, float scale,
-                  void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+                  const ExpandArgs* expand, int expand_dtype, int64_t tokens, int64_t n_head, int64_t ld_q,
+                  int64_t ld_out, float scale, void* workspace, size_t workspace_bytes, void* stream, char* err,
+                  size_t errlen) {
   int rc = check_pages(kv, what, err, errlen);
   if (!rc) rc = check_attention(kv, tokens, n_head, scale, what, err, errlen);
   if (rc) return rc;
@@ -2578,9 +2593,7 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
   a.max_pages = (int)kv->max_pages;
   a.n_pages = (int)n_pages;
   a.scale_log2 = scale_log2;
-  a.expanded = expanded;
-  rc = status_words(&a.bad, &a.status, what, err, errlen);
-  if (rc) return rc;
+  a.expanded = expand != nullptr;
   const bool few = few_rows(tokens, batch, n_rep);
   const bool eight = few && n_rep <= 8 && tokens * n_rep <= 8 * batch;  // the same rule for half a tile
   int sms = 148;
@@ -2601,6 +2614,13 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
                         : 0;
   const int tile = !few ? kTcTK : q8 && !brief && units == 0 ? kFewTK8 : kFewTK;
   if (few) line_kernel(a, rows, tile);
+  if (line_bound(a) >= 4e18) {
+    set_err(err, errlen, "%s: %lld tokens of %lld sequences over %lld pages each are too many", what,
+            (long long)tokens, (long long)batch, (long long)kv->max_pages);
+    return XB_ERR_UNSUPPORTED;
+  }
+  rc = status_words(&a.bad, &a.status, what, err, errlen);
+  if (rc) return rc;
   const bool wide = line_is_wide(a, ctas);
   a.ke = q8 ? Exponents{q8->k_scale, q8->ks_page, q8->ks_head} : Exponents{};
   a.ve = q8 ? Exponents{q8->v_scale, q8->vs_page, q8->vs_head} : Exponents{};
@@ -2617,14 +2637,9 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
                   err, errlen);
   if (!rc && !few) rc = query_map(&maps.q, q, tokens, n_head, ld_q, n_rep, a.tpt, what, err, errlen);
   if (rc) return rc;
-  if (line_bound(a) >= 4e18) {
-    set_err(err, errlen, "%s: %lld tokens of %lld sequences over %lld pages each are too many", what,
-            (long long)tokens, (long long)batch, (long long)kv->max_pages);
-    return XB_ERR_UNSUPPORTED;
-  }
   cudaStream_t s = (cudaStream_t)stream;
-  cudaError_t e;
-  if (few) {
+  cudaError_t e = expand ? launch_expand(*expand, expand_dtype, s) : cudaSuccess;
+  if (e == cudaSuccess && few) {
     KvMaps pages;
     pages.k = maps.k;
     pages.v = maps.v;
@@ -2634,7 +2649,7 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
     if (e == cudaSuccess && units == 0)
       e = launch_k(q8 ? paged_attn_join_kernel<kFewRows, 4, true> : paged_attn_join_kernel<kFewRows, 4, false>,
                    dim3((unsigned)ctas, kFewRows / 4), 256, 0, s, a, ctas);
-  } else {
+  } else if (e == cudaSuccess) {
     e = wide ? launch_main(paged_attn_tc_kernel<int64_t>, ctas, kTcThreads, kTcSmem, s, maps, a)
              : launch_main(paged_attn_tc_kernel<int>, ctas, kTcThreads, kTcSmem, s, maps, a);
     if (e == cudaSuccess)
@@ -2650,8 +2665,8 @@ static int attend(const char* what, const void* q, void* out, const xb_paged_kv*
 extern "C" int xb_paged_attention_bf16(const void* q, void* out, const xb_paged_kv* kv, int64_t tokens,
                                        int64_t n_head, int64_t ld_q, int64_t ld_out, float scale, void* workspace,
                                        size_t workspace_bytes, void* stream, char* err, size_t errlen) {
-  return attend("xb_paged_attention_bf16", q, out, kv, nullptr, false, tokens, n_head, ld_q, ld_out, scale, workspace,
-                workspace_bytes, stream, err, errlen);
+  return attend("xb_paged_attention_bf16", q, out, kv, nullptr, nullptr, 0, tokens, n_head, ld_q, ld_out, scale,
+                workspace, workspace_bytes, stream, err, errlen);
 }
 
 // Where an 8-bit call's pages go as bf16: a slot for each table entry, or for
@@ -2711,8 +2726,8 @@ extern "C" int xb_paged_attention_q8(const void* q, void* out, const xb_paged_kv
   if (!rc) rc = check_workspace(workspace, workspace_bytes, need, what, err, errlen);
   if (rc) return rc;
   if (few_rows(tokens, kv->batch, n_head / kv->n_kv_head))
-    return attend(what, q, out, kv, kv8, false, tokens, n_head, ld_q, ld_out, scale, workspace, workspace_bytes, stream,
-                  err, errlen);
+    return attend(what, q, out, kv, kv8, nullptr, 0, tokens, n_head, ld_q, ld_out, scale, workspace, workspace_bytes,
+                  stream, err, errlen);
   ExpandArgs e;
   bool compact;
   const int64_t slots = expand_slots(kv->batch, kv->max_pages, kv->n_pages, &compact);
@@ -2736,17 +2751,6 @@ extern "C" int xb_paged_attention_q8(const void* q, void* out, const xb_paged_kv
   e.max_pages = (int)kv->max_pages;
   e.n_pages = (int)kv->n_pages;
   e.compact = compact;
-  int sms = 148;
-  xb::sm_count(&sms);
-  // CTAs of 8 warps for each sequence: as many as its longest could use, 8 per SM over all of them
-  const int64_t most = (kv->max_pages * kv->page_size / 8 * kv->n_kv_head + 7) / 8;
-  const int64_t rows = kv->batch < 65535 ? kv->batch : 65535;
-  int64_t x = (8 * sms + rows - 1) / rows;
-  x = x < most ? x : most;
-  launch_k<false>(kv8->dtype == XB_DT_I8 ? paged_expand_kernel<kInt8> : paged_expand_kernel<kE4m3>,
-                  dim3((unsigned)x, (unsigned)rows), 256, 0, (cudaStream_t)stream, e);
-  rc = check_launch(what, err, errlen);
-  if (rc) return rc;
   xb_paged_kv wide = *kv;
   wide.k_pages = e.k_out;
   wide.v_pages = e.v_out;
@@ -2756,8 +2760,8 @@ extern "C" int xb_paged_attention_q8(const void* q, void* out, const xb_paged_kv
   wide.k_row = wide.v_row = kHD;
   wide.k_head = wide.v_head = kv->page_size * kHD;
   wide.k_page = wide.v_page = kv->n_kv_head * kv->page_size * kHD;
-  return attend(what, q, out, &wide, nullptr, true, tokens, n_head, ld_q, ld_out, scale, workspace, own, stream, err,
-                errlen);
+  return attend(what, q, out, &wide, nullptr, &e, (int)kv8->dtype, tokens, n_head, ld_q, ld_out, scale, workspace, own,
+                stream, err, errlen);
 }
 
 extern "C" int xb_page_status(void* stream, int* status, char* err, size_t errlen) {
