@@ -357,4 +357,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Calls of operators witho
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", XB_TORCH_VERSION) != 0) Py_CLEAR(m);
+  return m;
+}

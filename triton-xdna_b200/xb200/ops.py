@@ -13,8 +13,8 @@ import ctypes
 import functools
 import itertools
 import math
-import os
 import struct
+import warnings
 
 import torch
 
@@ -1028,17 +1028,31 @@ def argmax(x, out=None):
 _calls = None  # the module of the same name, once it has the library's addresses
 
 
+class _LeftAlone:
+    """In the place of csrc/calls.cpp where it is missing: it takes no call."""
+
+    paged_attention = paged_rope_kv = paged_read_kv = staticmethod(lambda *args: False)
+    beam_select = staticmethod(lambda *args: None)
+
+
 def _direct():
     """csrc/calls.cpp: functions that make an ordinary call without the
-    interpreter, and leave any other alone."""
+    interpreter, and leave any other alone.  The library does without it (no C++
+    compiler when it was built, another torch since): the same kernels, after
+    checks that take some 10 us a call."""
     global _calls
     if _calls is None:
         lib = _lib.load()
-        if not os.path.exists(os.path.join(_lib.PKG_DIR, "_calls.so")):
-            raise RuntimeError("xb200/_calls.so is missing: build it with "
-                               "`python -c 'import __graft_entry__ as g; g.build()'`")
-        from . import _calls as direct
+        try:
+            from . import _calls as direct
 
+            if direct.torch_version != torch.__version__:
+                raise ImportError(f"it was built with torch {direct.torch_version}, this is {torch.__version__}")
+        except ImportError as e:
+            warnings.warn(f"xb200/_calls.so is not used, so paged and beam operators take longer to call: {e}.  "
+                          "`python -c 'import __graft_entry__ as g; g.build()'` builds it", RuntimeWarning)
+            _calls = _LeftAlone
+            return _calls
         addresses = {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "xb_paged_attention_workspace_size", "xb_paged_attention_bf16", "xb_paged_attention_q8_workspace_size",
             "xb_paged_attention_q8", "xb_paged_rope_kv_bf16", "xb_paged_rope_kv_q8", "xb_paged_read_kv",
