@@ -716,7 +716,8 @@ XB_API int xb_paged_rope_kv_bf16(const void* qkv, const float* cos_t,
  * token at position p sees keys 0 .. p.  q [tokens, n_head, 64] (token pitch
  * ld_q), out [tokens, n_head * 64] (pitch ld_out), head_dim 64, n_head /
  * n_kv_head at most 128, scale > 0 and scale * log2(e) finite.  Online softmax
- * in fp32, P rounded to bf16 before P V, as xb_attention_bf16.  A token with a
+ * in fp32, P rounded to bf16 before P V, as xb_attention_bf16; scores (q k scale
+ * log2(e)) have to stay below 2^30 in size.  A token with a
  * negative position (kv_len[b] < n) sees nothing: its row is zero.  Lengths
  * beyond the table count as max_pages * page_size; a page id outside the pool
  * reads as zeros (flagged).  What lies behind a sequence's last key may be
@@ -786,7 +787,14 @@ XB_API int xb_paged_read_kv(void* k_out, void* v_out, const xb_paged_kv8* kv,
                             void* stream, char* err, size_t errlen);
 
 /* xb_paged_attention_bf16 over 8-bit pages: the attention over what the codes
- * stand for. */
+ * stand for.  Calls of few rows (at most 16 a sequence and KV head on average)
+ * run on the codes: weights are rounded to fp16 relative to the largest product
+ * of a weight and its value's 2^e, and vanish 2^-38 below it; the sum of weights
+ * is in fp32, for exponents of values any distance apart.  Calls of more rows
+ * expand every page that the batch's sequences with new tokens name to bf16 in the
+ * workspace (at most twice the bytes of the pool's codes) and go on as
+ * xb_paged_attention_bf16, so a step in which a long chunk stands beside many
+ * single tokens over long contexts costs more than over bf16 pages. */
 XB_API int xb_paged_attention_q8_workspace_size(
     int64_t tokens, int64_t batch, int64_t n_head, int64_t n_kv_head,
     int64_t n_pages, int64_t page_size, int64_t max_pages, size_t* bytes,
@@ -817,8 +825,12 @@ XB_API int xb_argmax_f32(const float* x, int64_t rows, int64_t cols,
  * group the `count` largest of
  *   scores[k] + logits[k, v] - log(sum_u exp(logits[k, u])),
  * largest first: their sums (values f32), beams (parents) and tokens, [groups,
- * count] contiguous.  Sums are compared in 64 bits; equal ones go by the lowest k,
- * those of one beam by the larger logit, then the lowest v.  A beam with a score
+ * count] contiguous.  A row's log-sum is formed in 32 bits, off by at most 2^-17
+ * (rows that are alike: alike to the bit); the sums are formed with it and
+ * compared in 64.  So the order within a beam, and among rows that are alike, is
+ * exact, while sums of different beams that lie closer than that may change places.
+ * Equal ones go by the lowest k, those of one beam by the larger logit, then the
+ * lowest v.  A beam with a score
  * that is not finite (-inf: one that is out), with a NaN or +inf among its logits
  * or with none above -inf has no continuation, nor has a token whose logit is
  * -inf; where fewer than `count` are left the rest is -inf, -1, -1.  At most 64

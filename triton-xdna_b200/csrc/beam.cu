@@ -11,8 +11,11 @@
 // A row's order of tokens is that of its logits, so the first kernel reads each
 // logit once, keeps the running maximum and sum of the log-sum and the `count`
 // best (logit, token) of a part of a row; the second adds the scores (in 64 bits:
-// sums of two beams may lie closer than 32 tell apart) and picks among the parts'
+// two sums of a beam may lie closer than 32 tell apart) and picks among the parts'
 // lists.
+// What the log-sum itself is off by decides between beams whose sums lie closer
+// than that: exponentials to 2^-22, added in fp32, measured at most 2^-21.7 for 64
+// rows each of 1000 to 151936 logits of spread 1 to 8 (the bound is 2^-17).
 #include "common.cuh"
 
 namespace xb {

@@ -5,8 +5,8 @@
 // what a code stands for is a bf16 number: reading back rounds nothing, and a
 // matrix product sees exactly what is stored.  It costs int8 up to one of its
 // seven bits (a scale of a / 127 would use them all) and e4m3 nothing.
-// Bytes: 47 (so that sums of weights 2^-e stay far inside fp32; smaller vectors
-// round to zeros) to 248 / 246 (what the largest codes stand for is finite;
+// Bytes: 47 (so that sums of 2^-e stay inside fp32, see kShareUp in paged.cu;
+// smaller vectors round to zeros, and zeros have it) to 248 / 246 (what the largest codes stand for is finite;
 // vectors beyond saturate), and 255: an infinity or NaN in the vector, which
 // reads as NaN throughout.
 #pragma once

@@ -386,9 +386,11 @@ struct ExpandArgs {
 // becomes a key of NaN and a value of zeros: the same for rows that see it, and those
 // that do not are not reached by zero times NaN.  Alone it takes 5.3 us for 24 prompts
 // of 130-1021 tokens (the attention 64.9 with it, 56.5 over bf16 pages), 8.4 for 32768
-// positions (685), 12.4 for a mixed step of 50 sequences (39.2).  With one part a warp
-// on its way, and the attention's search for its work behind the expansion, 65.7 and
-// 41.3.
+// positions (685), 12.4 for a mixed step of 50 sequences (39.2; over bf16 pages 26.2).  With
+// one part a warp on its way, and the attention's search for its work behind the
+// expansion, 65.7 and 41.3.  It takes in every sequence that has a new token, whole, single
+// tokens' contexts too: 160 sequences of 200-30000 keys beside a chunk of 512 take 373 us
+// where bf16 pages take 145.
 template <Format F>
 __global__ void __launch_bounds__(256) paged_expand_kernel(const ExpandArgs a) {
   pdl_wait();
@@ -644,7 +646,9 @@ constexpr int kPartLd = kHD + 4;           // row pitch of a partial in shared m
 // 500, 10.6 at 128 x 1000, 14 warps 7.9 and 9.9.  So where an SM has at most one unit and a
 // warp at most three tiles of 32 keys by what the table can hold, two where there are fewer
 // than 24 units (the host knows no lengths: beyond that one long sequence among
-// short ones would set the time).
+// short ones would set the time).  Short sequences behind a wide table so take the other
+// way: 2 x 512 with room for 1152 or more 8.2 (7.3 with its own table), 128 x 513-640 with
+// room for 2048 14.0 (8.0).
 constexpr int kWholeUnits = 24;
 template <int ROWS, Format F, bool SHORT, bool WHOLE>
 struct FewCfg {
@@ -1088,7 +1092,8 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
           // 8-bit pages: with K's exponent e_k and V's e_v a score is (S c1) (2^e_k c2), and e_v joins it: the weight w =
           // 2^(score + e_v - m) of a code of V fits fp16 whatever the values' sizes.  The key's share of the denominator, w
           // 2^-e_v, is an exponential of its own: w vanishes below 2^-126, and exponents lie up to 201 apart (a vector of
-          // zeros has 2^-80).
+          // zeros has 2^-80).  With the pairs of fp32 that costs the 160 long sequences 0.2 of 57.6 us; only where exponents lie
+          // that far apart, behind a vote, 63.0, as the branches part what the scheduler mixes.
           float ev[kCoded ? MT : 1][2];
           uint32_t nan = 0;
           if constexpr (kCoded) {

@@ -1074,7 +1074,9 @@ def beam_select(logits, scores, count):
     """A beam search step's choice: logits [G * K, V] (fp32 or bf16) of G groups
     of K beams and their scores [G, K] (fp32); of each group's beams k and
     tokens v the `count` largest scores[k] + log_softmax(logits[k])[v], largest
-    first, equal ones by the lowest k, then the logit, then the lowest v.
+    first, equal ones by the lowest k, then the logit, then the lowest v.  A row's
+    log-sum is off by up to 2^-17 (rows that are alike: alike to the bit), so sums of
+    different beams that lie closer than that may change places.
     Returns (values [G, count] fp32, parents int64, tokens int64); a beam whose
     score is -inf is out, and places for which no continuation is left hold
     -inf, -1, -1."""

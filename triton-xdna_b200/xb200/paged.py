@@ -19,7 +19,9 @@ tables that the kernels read are on the device.
 With ``dtype=torch.int8`` or ``torch.float8_e4m3fn`` the pool holds codes and an
 exponent byte for each position and KV head: half the bytes, so twice the
 positions in the same memory and half the reading of a decode step over long
-contexts.  Nothing else changes for the caller.
+contexts.  Steps of many tokens a sequence (prompts, chunks, also beside single
+tokens) expand their sequences' pages to bf16 first and take longer than over bf16
+pages.  Nothing else changes for the caller.
 """
 
 from __future__ import annotations
