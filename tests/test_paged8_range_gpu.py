@@ -7,6 +7,8 @@ times a code of 448 is not bounded by the values themselves, but by 2^-39 2^-80 
 2^-110 a key.
 """
 
+import math
+
 import pytest
 import torch
 from test_paged8_gpu import DTYPES, Coded
@@ -21,9 +23,9 @@ VARIANTS = [([1] * 3, [90, 700, 300], 0), ([2] * 3, [90, 400, 300], 0), ([1] * 3
             ([40, 1, 70], [90, 700, 300], 0)]
 
 
-def _check(b, out):
-    o, a, lost = b.exact()
-    got = out.cpu().double().reshape(b.T, b.H, b.D)
+def _check(b, out, rows=slice(None)):
+    o, a, lost = (x[rows] for x in b.exact())
+    got = out.cpu().double().reshape(b.T, b.H, b.D)[rows]
     assert bool(torch.isfinite(got).all())
     tiny = 2.0 ** -134 + max(v.shape[0] for v in b.v) * 2.0 ** -110
     over = (got - o).abs() - (2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -12) * a + lost + tiny)
@@ -117,3 +119,34 @@ def test_values_of_all_sizes_at_once(new, past, cols, dtype):
             _shift(b.vs, v, b.table[i], [p for p in range(v.shape[0]) if (p % 5 == at if at < 5 else p % 5 == 2 and
                                                                           p // 100 % 2 == at - 40)], step)
     _check(b, b.attend())
+
+
+def _determined(b, limit):
+    """Rows [T, H] whose result fp32 scores settle: all but those in which some other key's score is so close to the
+    largest that the sums' rounding decides.  The 64 products of a score are exact, their sum is off by at most 2^-23 of A =
+    sum |q k| an addition (a tensor core cuts off), so two scores by 64 x 2 x 2^-23 A = 2^-16 A, and where they are 40
+    further apart than that the other weights are lost below 2^-40.  Scores have to stay below `limit`."""
+    ok = torch.zeros((b.T, b.H), dtype=torch.bool)
+    for i, n in enumerate(b.new):
+        t, L = b.starts[i], b.k[i].shape[0]
+        k = b.k[i].double().repeat_interleave(b.H // b.KVH, 1).transpose(0, 1)  # [H, L, D]
+        q = b.q[t:t + n].double().transpose(0, 1) * (0.125 / math.log(2.0))
+        hidden = torch.arange(L)[None, :] > L - n + torch.arange(n)[:, None]
+        s, a = ((x @ y.transpose(1, 2)).masked_fill(hidden, -math.inf) for x, y in ((q, k), (q.abs(), k.abs())))
+        top = s.topk(min(2, L), -1).values
+        gap = top[..., 0] - top[..., -1] if L > 1 else torch.full((b.H, n), math.inf, dtype=torch.float64)
+        one = (torch.isfinite(s).sum(-1) == 1) | (gap > 2.0 ** -16 * a.amax(-1) + 40)
+        ok[t:t + n] = (one & (s.masked_fill(hidden, 0).abs().amax(-1) < limit)).t()
+    return ok
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,past,cols", VARIANTS)
+@pytest.mark.parametrize("step", range(17, 25))
+def test_scores_whose_neighbours_are_more_than_one_apart(step, new, past, cols, dtype):
+    """Scores of 2^22 to 2^30: fp32 there has steps of 0.5 to 128, and fp16 ends at 2^16."""
+    b = Coded(dtype, new, past, 14, 2, 16, seed=95, extra_cols=cols)
+    b.q = torch.ldexp(b.q.float(), torch.tensor(step)).to(torch.bfloat16)
+    ok = _determined(b, math.inf if max(new) < 3 else 2.0 ** 30)
+    assert step > 21 or ok.float().mean() > 0.9
+    _check(b, b.attend(), ok)

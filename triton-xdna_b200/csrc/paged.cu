@@ -1146,9 +1146,9 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
               for (int mt = 2; mt < MT; ++mt) mx[e] = fmaxf(mx[e], fmaxf(s[n][mt][e], s[n][mt][e + 2]));
             }
             // Over 8-bit pages a row's base moves only where a score is above it by more than one: fp16 has the room, and
-            // most tiles need no exchange between lanes.
+            // most tiles need no exchange between lanes.  (Their difference: one more than a base of 2^24 may round to two.)
             float base[2], by[2] = {0.0f, 0.0f}, al[2] = {1.0f, 1.0f};
-            bool moved = !kCoded || __any_sync(0xffffffffu, mx[0] > m[n][0] + 1.0f || mx[1] > m[n][1] + 1.0f);
+            bool moved = !kCoded || __any_sync(0xffffffffu, mx[0] - m[n][0] > 1.0f || mx[1] - m[n][1] > 1.0f);
             if (moved) {
               moved = false;
 #pragma unroll
@@ -1180,8 +1180,9 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
               for (int e = 0; e < 2; ++e) base[e] = m[n][e] == -INFINITY ? 0.0f : m[n][e];
             }
             if constexpr (kCoded) {
-              // up to 2^15, the largest at least 2^14, so that fp16 holds weights from 2^-38 of it on
-              const float2 down = make_float2(kUp - base[0], kUp - base[1]);
+              // up to 2^15, the largest at least 2^14, so that fp16 holds weights from 2^-38 of it on (from bases of 2^25 on
+              // kUp falls to what fp32 has room for: rounded to nearest it could rise, past fp16's end)
+              const float2 down = make_float2(__fsub_rd(kUp, base[0]), __fsub_rd(kUp, base[1]));
               float2 sum = make_float2(l[n][0], l[n][1]);
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) {
