@@ -1092,7 +1092,7 @@ __global__ void __launch_bounds__(FewCfg<ROWS, F, SHORT, WHOLE>::kThreads, 1)
           // 8-bit pages: with K's exponent e_k and V's e_v a score is (S c1) (2^e_k c2), and e_v joins it: the weight w =
           // 2^(score + e_v - m) of a code of V fits fp16 whatever the values' sizes.  The key's share of the denominator, w
           // 2^-e_v, is an exponential of its own: w vanishes below 2^-126, and exponents lie up to 201 apart (a vector of
-          // zeros has 2^-80).  With the pairs of fp32 that costs the 160 long sequences 0.2 of 57.6 us; only where exponents lie
+          // zeros has 2^-80).  With the pairs of fp32 that costs the 160 long sequences 0.3 of 57.8 us; only where exponents lie
           // that far apart, behind a vote, 63.0, as the branches part what the scheduler mixes.
           float ev[kCoded ? MT : 1][2];
           uint32_t nan = 0;
